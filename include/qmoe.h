@@ -654,6 +654,131 @@ int qmoe_gr_mix(qmoe_gr_ctx *ctx, int slot, const float *hyper, int n, float *mi
 int qmoe_gr_inject(qmoe_gr_ctx *ctx, const float *inject, const float *out, int n, float *hyper,
                    void *stream, qmoe_err *err);
 
+/* ------------------------------------------------------- paged cache
+ * k and v of MANY sequences in pages of a pool, and the attention that reads
+ * them: what a server of batches needs beside qmoe_attn_*, whose cache holds
+ * one sequence per layer.  No counterpart in the reference (one sequence,
+ * contiguous caches).
+ *
+ * A cache is the caller's device memory, described by this struct: pages of
+ * k and v, a table of page numbers per slot (a sequence's place), the slots'
+ * cached rows, and how many table entries hold each page.  Row j of slot s
+ * is row j % page_rows of page table[s][j / page_rows] in every layer.  The
+ * calls keep these rules and expect them at their start: the entries of a
+ * slot's rows are pages of the pool or -1 (released), the entries after them
+ * -1, refs counts the entries that hold a page, and a page with refs 0 is
+ * free.  An entry that is no page of the pool is never followed: its rows
+ * are not seen, not written and not counted.
+ *
+ * All calls are asynchronous on `stream`, read lengths and tables on the
+ * device when they run, allocate nothing and make no host round trip, so
+ * they can be captured in a graph.  The current device must be the
+ * pointers'.  Calls that need a workspace take the caller's, of at least
+ * qmoe_paged_ws_bytes bytes, 16-byte aligned, its contents undefined; calls
+ * that may overlap in time need workspaces of their own, and calls that
+ * change a cache must not overlap with other calls on it. */
+typedef struct {
+    void *k, *v;            /* pages: layer l, page p, row r, head j, dim i at
+                             * l*layer_stride + p*page_stride + r*row_stride + j*head_stride + i;
+                             * 16-byte aligned, elements do not overlap */
+    int64_t layer_stride, page_stride, row_stride, head_stride; /* elements, the same for k and v;
+                             * multiples of 16 bytes */
+    int dtype;              /* QMOE_F32 or QMOE_BF16 */
+    int n_layers;
+    int n_pages;            /* 1 .. 2^20 */
+    int page_rows;          /* 1 .. 4096, any */
+    int n_kv_heads;
+    int head_dim;           /* 64, 128, 192 or 256 */
+    int32_t *table;         /* [n_slots, max_pages] device */
+    int64_t table_stride;   /* >= max_pages */
+    int32_t *lens;          /* [n_slots] device: cached rows */
+    int32_t *refs;          /* [n_pages] device */
+    int n_slots, max_pages; /* max_pages * page_rows <= 2^30 */
+} qmoe_paged_cache;
+
+/* A ragged batch: sequence i owns rows starts[i] .. starts[i+1] of the call
+ * and slot slots[i] (slots NULL: slot i), and its rows are the LAST ones of
+ * that slot's lens: row t has position lens - (starts[i+1] - t).  Values out
+ * of range are clamped on the device (starts into [0, n], lens into [0, table
+ * rows]); a slot out of range has no rows.  Rows of the call outside every
+ * sequence are left alone. */
+typedef struct {
+    const int32_t *starts;  /* [n_seqs + 1] device, ascending */
+    const int32_t *slots;   /* [n_seqs] device, or NULL (n_seqs <= n_slots) */
+    int n;                  /* rows of the call */
+    int n_seqs;             /* <= 65536 */
+} qmoe_paged_batch;
+
+/* workspace bytes of a call; 0 for arguments that the call refuses.  n and
+ * n_heads count for QMOE_PAGED_ATTN only, n_seqs not for QMOE_PAGED_COMPACT. */
+enum { QMOE_PAGED_ATTN = 0, QMOE_PAGED_RESERVE = 1, QMOE_PAGED_FORK = 2, QMOE_PAGED_COMPACT = 3 };
+size_t qmoe_paged_ws_bytes(const qmoe_paged_cache *c, int call, int n, int n_seqs, int n_heads);
+
+/* Writes the batch's new rows k, v [n, n_kv_heads, head_dim] into the pages
+ * of `layer`.  src_dtype is the pages', or QMOE_F32 for bf16 pages (rounded
+ * to nearest even).  Strides in elements, multiples of 16 bytes, dims
+ * contiguous, k and v 16-byte aligned.  A row with no page, or at a negative
+ * position (more new rows than cached ones), is not written.  A batch names
+ * a slot once. */
+int qmoe_paged_append(const qmoe_paged_cache *c, int layer, const qmoe_paged_batch *b, const void *k, const void *v,
+                      int src_dtype, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                      int64_t v_head_stride, void *stream, qmoe_err *err);
+
+/* Attention of the batch's rows over `layer`: out = softmax(scale q.k) v over
+ * the cached rows j that the query at position p sees,
+ *   j <= p, with a page, and (window == 0 or p - j < window or j < sinks).
+ * A query that sees no row gives zeros; rows outside its sight never reach
+ * its output, whatever they hold.  q and out [n, n_heads, head_dim] have the
+ * pages' type; scores, softmax statistics and sums are fp32, and with bf16
+ * the softmax weights are rounded to bf16 for the product with v.  Results
+ * are the same from call to call. */
+typedef struct {
+    const void *q;
+    void *out;              /* not overlapping q or the cache */
+    int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride; /* elements, multiples of 16 bytes */
+    int n_heads;            /* a multiple of n_kv_heads; n * n_heads <= 2^30 */
+    int window;             /* 0: none */
+    int sinks;              /* first rows that stay visible behind the window */
+    int grouped;            /* 0: head h reads kv head h % n_kv_heads, as qmoe_attn_*;
+                             * 1: kv head h / (n_heads / n_kv_heads) */
+    float scale;            /* 0: 1 / sqrt(head_dim) */
+} qmoe_paged_query;
+int qmoe_paged_attn(const qmoe_paged_cache *c, int layer, const qmoe_paged_batch *b, const qmoe_paged_query *q,
+                    void *ws, size_t ws_bytes, void *stream, qmoe_err *err);
+
+/* Makes room for n_new[i] more rows in slot slots[i] (NULL: slot i) and adds
+ * them to lens.  Free pages go to the batch in order, lowest first.  Where a
+ * slot's last page is partly filled and held by others too, the slot gets a
+ * copy of it in every layer; of several slots of the batch that alone hold
+ * it, the last keeps it.  *status (device): 0; or the pages lacking; or -1
+ * for a slot out of range or named twice, a negative n_new, a length or a
+ * sum past the table, or a partly filled last page that was released.
+ * Unless 0, nothing is changed.  n_seqs <= 1024. */
+int qmoe_paged_reserve(const qmoe_paged_cache *c, const int32_t *slots, const int32_t *n_new, int n_seqs,
+                       int32_t *status, void *ws, size_t ws_bytes, void *stream, qmoe_err *err);
+
+/* Makes slot dst[i] a copy of the first rows[i] (NULL: all; clamped to the
+ * length) rows of slot src[i] by sharing its pages; what dst held is
+ * released.  All sources are read before any slot is written, so slots may
+ * trade places; src[i] == dst[i] cuts a slot short (rows 0 frees it).
+ * *status (device): 0, or -1 with nothing changed for a slot out of range or
+ * a dst named twice.  n_seqs <= 1024. */
+int qmoe_paged_fork(const qmoe_paged_cache *c, const int32_t *src, const int32_t *dst, const int32_t *rows, int n_seqs,
+                    int32_t *status, void *ws, size_t ws_bytes, void *stream, qmoe_err *err);
+
+/* Releases the pages of the slots (NULL: slots 0 .. n_seqs - 1) that no later
+ * query sees under this window (>= 1) and sinks: all rows behind the window
+ * of a query at position lens, none of them a sink.  Slots out of range are
+ * passed over. */
+int qmoe_paged_evict(const qmoe_paged_cache *c, const int32_t *slots, int n_seqs, int window, int sinks, void *stream,
+                     qmoe_err *err);
+
+/* Moves the used pages to the front of the pool: with U used pages, those
+ * numbered U and above go, in order, to the free numbers below U, in order;
+ * contents (every layer), all tables and refs follow.  *used (device) = U. */
+int qmoe_paged_compact(const qmoe_paged_cache *c, int32_t *used, void *ws, size_t ws_bytes, void *stream,
+                       qmoe_err *err);
+
 #ifdef __cplusplus
 }
 #endif

@@ -446,6 +446,55 @@ uint64_t qk_tensor_key(uint64_t seed, uint32_t layer, uint32_t tag);
 #define QK_NOALLOC_SCRATCH_BYTES ((size_t)64 << 20)
 int qk_noalloc_scratch(void **ptr);
 
+/* ------------------------------------------------------------ paged cache
+ * (paged_pages.hip, paged_attn.hip, qmoe_paged.c) */
+
+/* division by a fixed d (paged_parts.h) */
+typedef struct {
+    uint32_t mul, shift, d;
+} pg_div;
+
+/* a paged cache as the kernels take it; strides in elements */
+typedef struct {
+    void *k, *v;           /* of layer 0, or of the call's layer */
+    int64_t layer_stride, page_stride, row_stride, head_stride, table_stride;
+    int32_t *table, *lens, *refs;
+    pg_div page_rows;
+    int dtype, n_layers, n_pages, kvh, hd, n_slots, max_pages;
+    int cap;               /* rows of a full table: max_pages * page_rows */
+} pg_cache;
+
+/* limits (checked by qmoe_paged.c) */
+#define PG_MAX_ROWS (1 << 30)  /* rows of a table, rows of a call times heads */
+#define PG_MAX_BATCH 1024      /* sequences of a reserve or fork call */
+#define PG_MAX_PAGES (1 << 20) /* pages of a pool: a batch's needs sum in 32 bits */
+#define PG_MAX_SEQS (1 << 16)  /* sequences of an append, attention or evict call */
+
+typedef struct {
+    const void *q;
+    void *out;
+    int64_t q_token, q_head, o_token, o_head; /* strides, elements */
+    const int32_t *starts, *slots;
+    int n, n_seqs, h, window, sinks, grouped;
+    float scale;           /* score * this, log2 units: softmax scale * log2(e) */
+} pg_attn;
+
+/* workspace bytes and launches; 0 or a hipError_t */
+size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h);
+int qk_launch_pg_attn(const pg_cache *c, const pg_attn *a, void *ws, void *stream);
+int qk_launch_pg_append(const pg_cache *c, const void *k, const void *v, int src_dtype, int64_t k_token, int64_t k_head,
+                        int64_t v_token, int64_t v_head, const int32_t *starts, const int32_t *slots, int n, int n_seqs,
+                        void *stream);
+size_t qk_pg_reserve_ws(const pg_cache *c, int n_seqs);
+int qk_launch_pg_reserve(const pg_cache *c, const int32_t *slots, const int32_t *n_new, int n_seqs, int32_t *status,
+                         void *ws, void *stream);
+size_t qk_pg_fork_ws(const pg_cache *c, int n_seqs);
+int qk_launch_pg_fork(const pg_cache *c, const int32_t *src, const int32_t *dst, const int32_t *rows, int n_seqs,
+                      int32_t *status, void *ws, void *stream);
+int qk_launch_pg_evict(const pg_cache *c, const int32_t *slots, int n_seqs, int window, int sinks, void *stream);
+size_t qk_pg_compact_ws(const pg_cache *c);
+int qk_launch_pg_compact(const pg_cache *c, int32_t *used, void *ws, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

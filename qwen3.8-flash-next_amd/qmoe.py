@@ -107,6 +107,27 @@ class QmoeGrConfig(ctypes.Structure):
     _fields_ = [(f, ctypes.c_int) for f in ("hidden", "hc_count", "hc_lowrank", "n_slots", "max_tokens")]
 
 
+class QmoePagedCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+               [(f, ctypes.c_int64) for f in ("layer_stride", "page_stride", "row_stride", "head_stride")] + \
+               [(f, ctypes.c_int) for f in ("dtype", "n_layers", "n_pages", "page_rows", "n_kv_heads", "head_dim")] + \
+               [("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("lens", ctypes.c_void_p),
+                ("refs", ctypes.c_void_p), ("n_slots", ctypes.c_int), ("max_pages", ctypes.c_int)]
+
+
+class QmoePagedBatch(ctypes.Structure):
+    _fields_ = [("starts", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("n", ctypes.c_int), ("n_seqs", ctypes.c_int)]
+
+
+class QmoePagedQuery(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p)] + \
+               [(f, ctypes.c_int64) for f in ("q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride")] + \
+               [(f, ctypes.c_int) for f in ("n_heads", "window", "sinks", "grouped")] + [("scale", ctypes.c_float)]
+
+
+PAGED_ATTN, PAGED_RESERVE, PAGED_FORK, PAGED_COMPACT = 0, 1, 2, 3
+
+
 class QmoeStTensor(ctypes.Structure):
     _fields_ = [("dtype", ctypes.c_int), ("ndim", ctypes.c_int), ("shape", ctypes.c_int64 * 8),
                 ("file", ctypes.c_int), ("offset", ctypes.c_uint64), ("nbytes", ctypes.c_uint64)]
@@ -155,6 +176,18 @@ SIGNATURES = {
     "qmoe_gr_upload_slot": (_I, [_P, _I, ctypes.POINTER(QmoeHcWeights), ctypes.POINTER(QmoeErr)]),
     "qmoe_gr_mix": (_I, [_P, _I, _P, _I, _P, _P, _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_gr_inject": (_I, [_P, _P, _P, _I, _P, _P, ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_ws_bytes": (ctypes.c_size_t, [ctypes.POINTER(QmoePagedCache), _I, _I, _I, _I]),
+    "qmoe_paged_append": (_I, [ctypes.POINTER(QmoePagedCache), _I, ctypes.POINTER(QmoePagedBatch), _P, _P, _I,
+                               ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _P,
+                               ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_attn": (_I, [ctypes.POINTER(QmoePagedCache), _I, ctypes.POINTER(QmoePagedBatch),
+                             ctypes.POINTER(QmoePagedQuery), _P, ctypes.c_size_t, _P, ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_reserve": (_I, [ctypes.POINTER(QmoePagedCache), _P, _P, _I, _P, _P, ctypes.c_size_t, _P,
+                                ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_fork": (_I, [ctypes.POINTER(QmoePagedCache), _P, _P, _P, _I, _P, _P, ctypes.c_size_t, _P,
+                             ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_evict": (_I, [ctypes.POINTER(QmoePagedCache), _P, _I, _I, _I, _P, ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_compact": (_I, [ctypes.POINTER(QmoePagedCache), _P, _P, ctypes.c_size_t, _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_dn_create": (_I, [ctypes.POINTER(_P), ctypes.POINTER(QmoeDnConfig), ctypes.POINTER(QmoeErr)]),
     "qmoe_dn_destroy": (None, [_P]),
     "qmoe_dn_upload_layer": (_I, [_P, _I, ctypes.POINTER(QmoeDnWeights), ctypes.POINTER(QmoeErr)]),
@@ -989,6 +1022,208 @@ class GatedResidualContext:
         _check(lib().qmoe_gr_inject(self._h, _ptr(inject), _ptr(out), hyper.shape[0], _ptr(hyper),
                                     _stream(stream), ctypes.byref(err)), err, "qmoe_gr_inject")
         return hyper
+
+
+class PagedCache:
+    """k and v of many sequences in pages of a pool (qmoe_paged_*), on the
+    caller's tensors:
+
+      k, v   [n_layers, n_pages, page_rows, n_kv_heads, head_dim] f32 or bf16,
+             head_dim contiguous, the same strides
+      table  [n_slots, max_pages] int32: the page of every page_rows rows, -1 none
+      lens   [n_slots] int32: cached rows
+      refs   [n_pages] int32: table entries that hold the page
+
+    Batches are ragged: starts [n_seqs + 1] int32 cuts the rows of a call
+    into sequences, slots [n_seqs] int32 names their slots (None: sequence i
+    is slot i), and a sequence's rows are the last ones of its lens.  One
+    serving step is reserve (room for the new rows), then per layer append
+    and attend.  Calls return without waiting and may be captured in a HIP
+    graph; a call's workspace comes from torch's allocator on the call's
+    stream."""
+
+    def __init__(self, k, v, table, lens, refs):
+        import torch
+        if k.dim() != 5 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+            raise QmoeError("k and v must be [layers, pages, rows, kv heads, head dim] with one shape, type and strides")
+        if k.stride(4) != 1:
+            raise QmoeError("the head dim of k and v must be contiguous")
+        self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
+        self.device, self.dtype = k.device, k.dtype
+        for nm, t, shape in (("v", v, v.shape), ("table", table, (lens.numel(), table.shape[-1])),
+                             ("lens", lens, (lens.numel(),)), ("refs", refs, (k.shape[1],))):
+            if t.device != self.device or tuple(t.shape) != tuple(shape):
+                raise QmoeError(f"{nm} must be {list(shape)} on {self.device}")
+            if nm != "v" and (t.dtype != torch.int32 or t.stride(-1) != 1 and t.shape[-1] > 1):
+                raise QmoeError(f"{nm} must be int32 with contiguous rows")
+        L, P, R, kvh, hd = k.shape
+        self.kvh, self.hd = kvh, hd
+        self._c = QmoePagedCache(k.data_ptr(), v.data_ptr(), *k.stride()[:4], _dtype_code(k), L, P, R, kvh, hd,
+                                 table.data_ptr(), max(table.stride(0), table.shape[1]) if table.shape[0] == 1 else table.stride(0),
+                                 lens.data_ptr(), refs.data_ptr(), table.shape[0], table.shape[1])
+        self._cp = ctypes.byref(self._c)
+        if self.device.type != "cuda":
+            raise QmoeError(f"a paged cache lives on the GPU, not on {self.device}")
+
+    @classmethod
+    def allocate(cls, n_layers, n_pages, page_rows, n_kv_heads, head_dim, n_slots, max_pages, dtype=None, device="cuda"):
+        """an empty cache of its own tensors (bf16 pages unless dtype says f32)"""
+        import torch
+        shape = (n_layers, n_pages, page_rows, n_kv_heads, head_dim)
+        k, v = (torch.empty(shape, dtype=dtype or torch.bfloat16, device=device) for _ in range(2))
+        return cls(k, v, torch.full((n_slots, max_pages), -1, dtype=torch.int32, device=device),
+                   torch.zeros(n_slots, dtype=torch.int32, device=device),
+                   torch.zeros(n_pages, dtype=torch.int32, device=device))
+
+    # -- the call's device, stream and small arguments
+    def _stream(self, stream):
+        import torch
+        if stream is None:
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return stream if isinstance(stream, int) else stream.cuda_stream
+
+    def _place(self, stream):
+        """the cache's device as the current one, and the call's stream as
+        torch's, so that what the call allocates belongs to that stream"""
+        import contextlib
+        import torch
+        if stream is None and self.device.index == torch.cuda.current_device():
+            return contextlib.nullcontext()
+        st = contextlib.ExitStack()
+        st.enter_context(torch.cuda.device(self.device))
+        if stream is not None:
+            if isinstance(stream, int):
+                stream = torch.cuda.ExternalStream(stream, device=self.device)
+            st.enter_context(torch.cuda.stream(stream))
+        return st
+
+    def _ints(self, t, n, what):
+        """device address of an int32 vector of n (or None)"""
+        import torch
+        if t is None:
+            return None
+        if t.dtype != torch.int32 or t.device != self.device or t.dim() != 1 or (n is not None and t.shape[0] != n) or \
+                (t.shape[0] > 1 and t.stride(0) != 1):
+            raise QmoeError(f"{what} must be a contiguous int32 vector" + (f" of {n}" if n is not None else "") +
+                            f" on {self.device}")
+        return t.data_ptr()
+
+    def _rows(self, t, heads, dtypes, what):
+        if t.device != self.device or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.hd or \
+                t.dtype not in dtypes or t.stride(2) != 1:
+            raise QmoeError(f"{what} must be [n, {heads}, {self.hd}] {' or '.join(str(d) for d in dtypes)} with the head "
+                            f"dim contiguous on {self.device}")
+
+    def _batch(self, n, starts, slots):
+        p = self._ints(starts, None, "starts")
+        if p is None or starts.shape[0] < 1:
+            raise QmoeError("starts must hold one number more than there are sequences")
+        m = starts.shape[0] - 1
+        return QmoePagedBatch(p, self._ints(slots, m, "slots"), n, m)
+
+    def _work(self, call, n=0, n_seqs=0, heads=0):
+        import torch
+        need = lib().qmoe_paged_ws_bytes(self._cp, call, n, n_seqs, heads)
+        return torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
+
+    # -- rows
+    def append(self, layer, k, v, starts, slots=None, stream=None):
+        """new rows k, v [n, n_kv_heads, head_dim] into the pages of `layer`
+        (the pages' type, or f32 rounded into bf16 pages)"""
+        import torch
+        dtypes = (self.dtype,) if self.dtype == torch.float32 else (self.dtype, torch.float32)
+        self._rows(k, self.kvh, dtypes, "k")
+        self._rows(v, self.kvh, dtypes, "v")
+        if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
+            raise QmoeError("k and v must have the same rows and type")
+        b = self._batch(k.shape[0], starts, slots)
+        err = QmoeErr()
+        with self._place(stream):
+            _check(lib().qmoe_paged_append(self._cp, layer, ctypes.byref(b), k.data_ptr(), v.data_ptr(), _dtype_code(k),
+                                           k.stride(0), k.stride(1), v.stride(0), v.stride(1), self._stream(stream),
+                                           ctypes.byref(err)), err, "qmoe_paged_append")
+
+    def attend(self, layer, q, starts, slots=None, window=0, sinks=0, scale=None, grouped=False, out=None, stream=None):
+        """q [n, n_heads, head_dim] of the pages' type -> softmax(scale q.k) v
+        over the rows each query sees, [n, n_heads, head_dim]: those up to its
+        own, with a window only the last `window` and the first `sinks`.
+        Head h reads kv head h % n_kv_heads as the attention mixer's, with
+        `grouped` h // (n_heads / n_kv_heads); scale None is
+        1 / sqrt(head_dim).  Rows of no sequence are left as out has them."""
+        import torch
+        heads = q.shape[1] if q.dim() == 3 else 0
+        self._rows(q, heads, (self.dtype,), "q")
+        n = q.shape[0]
+        b = self._batch(n, starts, slots)
+        err = QmoeErr()
+        with self._place(stream):
+            if out is None:
+                out = torch.empty((n, heads, self.hd), dtype=self.dtype, device=self.device)
+            else:
+                self._rows(out, heads, (self.dtype,), "out")
+                if out.shape[0] != n:
+                    raise QmoeError(f"out has {out.shape[0]} rows, q {n}")
+            a = QmoePagedQuery(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), heads,
+                               window, sinks, 1 if grouped else 0, 0.0 if scale is None else scale)
+            ws = self._work(PAGED_ATTN, n, b.n_seqs, heads)
+            _check(lib().qmoe_paged_attn(self._cp, layer, ctypes.byref(b), ctypes.byref(a), ws.data_ptr(), ws.numel(),
+                                         self._stream(stream), ctypes.byref(err)), err, "qmoe_paged_attn")
+        return out
+
+    # -- pages
+    def reserve(self, n_new, slots=None, stream=None):
+        """room for n_new[i] more rows in every slot of the batch, lens
+        advanced; a shared, partly filled last page is copied.  Returns an
+        int32 [1] on the device: 0, the pages lacking, or -1 for a batch that
+        is refused (nothing is changed unless 0)."""
+        import torch
+        p = self._ints(n_new, None, "n_new")
+        m = n_new.shape[0]
+        sl = self._ints(slots, m, "slots")
+        err = QmoeErr()
+        with self._place(stream):
+            status, ws = torch.empty(1, dtype=torch.int32, device=self.device), self._work(PAGED_RESERVE, n_seqs=m)
+            _check(lib().qmoe_paged_reserve(self._cp, sl, p, m, status.data_ptr(), ws.data_ptr(), ws.numel(),
+                                            self._stream(stream), ctypes.byref(err)), err, "qmoe_paged_reserve")
+        return status
+
+    def fork(self, src, dst, rows=None, stream=None):
+        """slot dst[i] becomes the first rows[i] (None: all) rows of slot
+        src[i] by sharing pages; all sources are read first.  Returns an int32
+        [1] on the device: 0, or -1 (refused, nothing changed)."""
+        import torch
+        s = self._ints(src, None, "src")
+        m = src.shape[0]
+        d, r = self._ints(dst, m, "dst"), self._ints(rows, m, "rows")
+        err = QmoeErr()
+        with self._place(stream):
+            status, ws = torch.empty(1, dtype=torch.int32, device=self.device), self._work(PAGED_FORK, n_seqs=m)
+            _check(lib().qmoe_paged_fork(self._cp, s, d, r, m, status.data_ptr(), ws.data_ptr(), ws.numel(),
+                                         self._stream(stream), ctypes.byref(err)), err, "qmoe_paged_fork")
+        return status
+
+    def trim(self, slots, rows, stream=None):
+        """cuts slots to their first rows[i] rows (0 frees a slot)"""
+        return self.fork(slots, slots, rows, stream)
+
+    def evict(self, window, sinks=0, slots=None, stream=None):
+        """releases the pages that no later query sees under this window and sinks"""
+        sl = self._ints(slots, None, "slots")
+        m = self.table.shape[0] if slots is None else slots.shape[0]
+        err = QmoeErr()
+        with self._place(stream):
+            _check(lib().qmoe_paged_evict(self._cp, sl, m, window, sinks, self._stream(stream), ctypes.byref(err)), err,
+                   "qmoe_paged_evict")
+
+    def compact(self, stream=None):
+        """moves the used pages to the front of the pool; returns their number, an int32 [1] on the device"""
+        import torch
+        err = QmoeErr()
+        with self._place(stream):
+            used, ws = torch.empty(1, dtype=torch.int32, device=self.device), self._work(PAGED_COMPACT)
+            _check(lib().qmoe_paged_compact(self._cp, used.data_ptr(), ws.data_ptr(), ws.numel(), self._stream(stream),
+                                            ctypes.byref(err)), err, "qmoe_paged_compact")
+        return used
 
 
 def decoder_layer_types(n_layers, full_attention_interval=4):
