@@ -2,14 +2,33 @@
  * paged_attn.hip -- attention of a ragged batch of new tokens over a paged
  * cache: softmax(scale q.k) v over the rows that a token sees (causal, a
  * sliding window, sinks), a group of query heads per kv head.
+ *
+ * The (token, head) rows of a sequence that read one kv head are one matrix
+ * of queries: row r is token r / G, member r % G of the group, so a page is
+ * read once for all heads of its group.  Rows are cut into tiles, the keys of
+ * a row tile into parts where there are too few tiles to fill the card; a
+ * unit of work is (sequence, row tile, part, kv head), numbered on the device
+ * from the lengths it finds (pa_find), and a second launch joins the parts.
+ *
+ * Products are transposed: S^T = K Q^T leaves each lane the scores of one
+ * row, for keys 8 a + 4 (lane / 32) + b of a tile of 32, and those registers
+ * are the B operand of O^T = V^T P^T as they are, if V^T's operand takes its
+ * keys in that order.  Maximum, sum and O stay with the lane (fp32).
  */
 #include "qk_device.h"
+#include "mfma_parts.h"
 #include "paged_parts.h"
 
+typedef float qm_f32x16 __attribute__((ext_vector_type(16)));
+
 struct PaArgs {
-    pg_cache c; /* k and v of the call's layer */
+    pg_cache c;   /* k and v of the call's layer */
     pg_attn a;
-    int G;      /* query heads per kv head */
+    int G;        /* query heads per kv head */
+    int units;    /* units that the call is cut into, about */
+    int least;    /* key tiles of a part at the least */
+    float *po;    /* partial O [slot, RT, HD], unscaled */
+    float2 *pml;  /* [slot, RT]: maximum (log2 units), sum */
 };
 
 /* query head of member g of kv head kh's group: heads kh, kh + kvh, ... (the
@@ -37,103 +56,553 @@ __device__ __forceinline__ void pa_get8(const T *p, float x[8]) {
         x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
     }
 }
+/* 4 consecutive elements of the output type */
 template <typename T>
-__device__ __forceinline__ void pa_put(T *p, float x) {
-    if constexpr (sizeof(T) == 2) qk_st((uint16_t *)p, (uint16_t)qk_cvt_pk_bf16(x, x));
-    else qk_st((float *)p, x);
+__device__ __forceinline__ void pa_put4(T *p, float a, float b, float c, float d) {
+    if constexpr (sizeof(T) == 2) {
+        qk_u32x2 w = {qk_cvt_pk_bf16(a, b), qk_cvt_pk_bf16(c, d)};
+        *(QK_GLOBAL qk_u32x2 *)p = w;
+    } else {
+        qk_st((float4 *)p, make_float4(a, b, c, d));
+    }
 }
 
 /* what a row's maximum and sum give: the factor on its sum of p v, NaN for a
  * row whose scores are all -inf (0/0, as the formula), 0 for a row that sees
- * nothing */
-__device__ __forceinline__ float pa_norm(float m, float l, bool seen) {
-    return m == -INFINITY && !seen ? 0.0f : 1.0f / l;
+ * nothing.  A part that sees only scores of -inf has the sum 1 beside the
+ * maximum -inf, so that the join tells the two apart. */
+__device__ __forceinline__ float pa_sum(float m, float l, bool seen) { return m == -INFINITY && seen ? 1.0f : l; }
+__device__ __forceinline__ float pa_norm(float m, float l) {
+    return m == -INFINITY ? (l > 0.0f ? NAN : 0.0f) : 1.0f / l;
 }
 
-/*
- * One wave per (token, query head): lane = key for the scores, lane = dims
- * for the sum of p v, 64 keys at a time under a running maximum.
- */
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void k_pa_rows(PaArgs p) {
-    const int lane = threadIdx.x & 63;
-    const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int t = r / p.a.h, hh = r - t * p.a.h;
-    if (t >= p.a.n) return;
-    int lo = 0, hi = p.a.n_seqs;
-    if (t < qk_ld(p.a.starts) || t >= qk_ld(p.a.starts + hi)) return;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (qk_ld(p.a.starts + mid) <= t) lo = mid;
-        else hi = mid;
-    }
-    const pg_seq s = pg_seq_at(&p.c, p.a.starts, p.a.slots, p.a.n, lo);
-    if (t < s.start || t >= s.start + s.count) return;
-    const int pos = s.len - s.count + t - s.start;
-    const int kh = p.a.grouped ? hh / p.G : hh % p.c.kvh;
-    const T *kp = (const T *)p.c.k + (int64_t)kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)kh * p.c.head_stride;
-    const T *q = (const T *)p.a.q + t * p.a.q_token + hh * p.a.q_head;
-    const int32_t *row = p.c.table + (int64_t)s.slot * p.c.table_stride;
-    const pg_tiles tl = pg_tiles_of(pos, pos, p.a.window, p.a.sinks, 64);
-    float m = -INFINITY, l = 0.0f, acc[HD / 64];
-    bool seen = false;
-#pragma unroll
-    for (int e = 0; e < HD / 64; e++) acc[e] = 0.0f;
-    for (int i = 0; i < tl.nt && s.slot >= 0; i++) {
-        const int j = pg_tile(tl, i) * 64 + lane;
-        const int64_t at = pg_sees(pos, j, p.a.window, p.a.sinks) ? pg_row_at(&p.c, row, j) : -1;
-        float sc = -INFINITY;
-        if (at >= 0) {
-            float d = 0.0f;
-            for (int c = 0; c < HD; c += 8) {
-                float x[8], y[8];
-                pa_get8(kp + at + c, x);
-                pa_get8(q + c, y);
-#pragma unroll
-                for (int u = 0; u < 8; u++) d = fmaf(x[u], y[u], d);
-            }
-            sc = d * p.a.scale;
+/* ------------------------------------------------------------ units */
+
+struct PaUnit {
+    pg_seq s;
+    int rtile, part, parts, kh;
+    int slot; /* of the part's partial results */
+};
+
+/* exclusive prefix sums of two values over the workgroup's 256 threads */
+__device__ __forceinline__ int2 pa_scan(int2 v, int2 *lds, int2 &total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int2 x = v;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int a = __shfl_up(x.x, o, QK_WAVE), b = __shfl_up(x.y, o, QK_WAVE);
+        if (lane >= o) {
+            x.x += a;
+            x.y += b;
         }
-        float mx = sc;
-        for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, QK_WAVE));
-        const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.0f : exp2f(m - mn);
-        seen |= __any(at >= 0);
+    }
+    if (lane == 63) lds[wave] = x;
+    __syncthreads();
+    int2 before = make_int2(0, 0);
+    total = make_int2(0, 0);
+    for (int w = 0; w < 4; w++) {
+        const int2 t = lds[w];
+        if (w < wave) {
+            before.x += t.x;
+            before.y += t.y;
+        }
+        total.x += t.x;
+        total.y += t.y;
+    }
+    __syncthreads();
+    return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
+}
+
+/* Unit `want` of the call (JOIN: the want-th (sequence, row tile, kv head)
+ * that has parts to join); false past the last.  256 threads, every one of
+ * which looks at its share of the sequences. */
+template <int RT, int KT, bool JOIN>
+__device__ bool pa_find(const PaArgs &p, int want, PaUnit &u) {
+    __shared__ int2 tmp[4];
+    __shared__ long long sums[4];
+    __shared__ int found[4];
+    const int tid = threadIdx.x, n = p.a.n_seqs;
+    auto load = [&](int i) {
+        pg_load l = {0, 0};
+        if (i < n)
+            l = pg_load_of(pg_seq_at(&p.c, p.a.starts, p.a.slots, p.a.n, i), p.G, RT, p.a.window, p.a.sinks, KT);
+        return l;
+    };
+    const pg_load l0 = load(tid);
+    long long t = (long long)l0.row_tiles * l0.key_tiles;
+    for (int i = tid + 256; i < n; i += 256) {
+        const pg_load l = load(i);
+        t += (long long)l.row_tiles * l.key_tiles;
+    }
+    for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o, QK_WAVE);
+    if ((tid & 63) == 0) sums[tid >> 6] = t;
+    if (tid == 0) found[0] = -1;
+    __syncthreads();
+    const int share = pg_share((sums[0] + sums[1] + sums[2] + sums[3]) * p.c.kvh, p.units, p.least);
+    int2 base = make_int2(0, 0); /* units (tasks to join), split units before the chunk */
+    for (int c = 0; c < n; c += 256) {
+        const pg_load l = c ? load(c + tid) : l0;
+        const int parts = pg_parts(l.key_tiles, share), tasks = l.row_tiles * p.c.kvh;
+        const int split = parts > 1 ? tasks * parts : 0;
+        const int mine = JOIN ? (parts > 1 ? tasks : 0) : tasks * parts;
+        int2 total;
+        const int2 at = pa_scan(make_int2(mine, split), tmp, total);
+        if (want >= base.x + at.x && want < base.x + at.x + mine) {
+            found[0] = c + tid;
+            found[1] = want - base.x - at.x;
+            found[2] = base.y + at.y;
+            found[3] = parts;
+        }
+        base.x += total.x;
+        base.y += total.y;
+        if (want < base.x) break;
+    }
+    __syncthreads();
+    const int i = __builtin_amdgcn_readfirstlane(found[0]);
+    if (i < 0) return false;
+    const int local = __builtin_amdgcn_readfirstlane(found[1]);
+    u.parts = __builtin_amdgcn_readfirstlane(found[3]);
+    u.s = pg_seq_at(&p.c, p.a.starts, p.a.slots, p.a.n, i);
+    const int rtiles = (u.s.count * p.G + RT - 1) / RT, q = local / p.c.kvh;
+    u.kh = local - q * p.c.kvh;
+    const int back = JOIN ? q : q / u.parts;
+    u.part = JOIN ? 0 : q - back * u.parts;
+    u.rtile = rtiles - 1 - back;
+    u.slot = __builtin_amdgcn_readfirstlane(found[2]) + (back * u.parts + u.part) * p.c.kvh + u.kh;
+    return true;
+}
+
+/* ------------------------------------------------------------ masks */
+
+/* bits j = 0..31 with base + j <= x */
+__device__ __forceinline__ uint32_t pa_upto(int x, int base) {
+    const int d = x - base;
+    return d >= 31 ? 0xFFFFFFFFu : (d < 0 ? 0u : (2u << d) - 1u);
+}
+/* the keys base..base+31 that the query at position p sees */
+__device__ __forceinline__ uint32_t pa_mask(const PaArgs &p, int pos, int base) {
+    uint32_t w = pa_upto(pos, base);
+    if (p.a.window > 0) w &= ~pa_upto(pg_lo(pos, p.a.window) - 1, base) | pa_upto(p.a.sinks - 1, base);
+    return w;
+}
+/* all of them are seen at all positions p0..p1 */
+__device__ __forceinline__ bool pa_full(const PaArgs &p, int p0, int p1, int base) {
+    return base + 31 <= p0 && (p.a.window == 0 || base >= pg_lo(p1, p.a.window) || base + 31 < p.a.sinks);
+}
+
+/* ------------------------------------------------- one row at a time
+ * fp32 on the vector ALU, keys of the unit's part only: for units in which a
+ * row that some query does not see holds an infinity or NaN (or, f32 on
+ * MFMA, a value that the bf16 parts cannot carry): a masked key is never
+ * multiplied here.  Waves take the unit's rows in turn. */
+template <typename T, int HD, int RT, int KT>
+__device__ __noinline__ void pa_slow(const PaArgs &p, const PaUnit &u, int kt0, int kt1, pg_tiles tl, int waves) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
+    const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
+    const int rows = u.s.count * p.G;
+    for (int r = u.rtile * RT + wave; r < min(u.rtile * RT + RT, rows); r += waves) {
+        const int t = r / p.G, hh = pa_head(p, u.kh, r - t * p.G), pos = u.s.len - u.s.count + t;
+        const T *q = (const T *)p.a.q + (int64_t)(u.s.start + t) * p.a.q_token + (int64_t)hh * p.a.q_head;
+        float m = -INFINITY, l = 0.0f, acc[HD / 16];
+        bool seen = false;
+#pragma unroll
+        for (int e = 0; e < HD / 16; e++) acc[e] = 0.0f;
+        for (int b = kt0 * KT; b < kt1 * KT; b += 64) { /* the part's tiles in runs of 64 keys */
+            const int i = (b + lane) / KT;
+            const int j = i < kt1 ? pg_tile(tl, i) * KT + (b + lane) % KT : 0x7FFFFFFF;
+            const int64_t at = pg_sees(pos, j, p.a.window, p.a.sinks) ? pg_row_at(&p.c, row, j) : -1;
+            float sc = -INFINITY;
+            if (at >= 0) {
+                float d = 0.0f;
+                for (int c = 0; c < HD; c += 8) {
+                    float x[8], y[8];
+                    pa_get8(kp + at + c, x);
+                    pa_get8(q + c, y);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) d = fmaf(x[k], y[k], d);
+                }
+                sc = d * p.a.scale;
+            }
+            float mx = sc;
+            for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, QK_WAVE));
+            const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            seen |= __any(at >= 0);
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < HD / 16; e++) acc[e] *= f;
+            m = mn;
+            const float pr = at < 0 ? 0.0f : __builtin_amdgcn_exp2f(sc - (m == -INFINITY ? 0.0f : m));
+            l += pr;
+            for (uint64_t todo = __ballot(at >= 0); todo; todo &= todo - 1) {
+                const int k = __builtin_ctzll(todo);
+                const float pj = __shfl(pr, k, QK_WAVE);
+                const int64_t aj = ((int64_t)__shfl((int)(at >> 32), k, QK_WAVE) << 32) | (uint32_t)__shfl((int)at, k, QK_WAVE);
+                /* dims 4 (lane % 16) .. of every 64, the four quarters of the wave alike */
+#pragma unroll
+                for (int e = 0; e < HD / 64; e++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        acc[4 * e + x] = fmaf(pj, pa_get(vp + aj + 64 * e + 4 * (lane & 15) + x), acc[4 * e + x]);
+            }
+        }
+        for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o, QK_WAVE);
+        l = pa_sum(m, l, seen);
+        const float f = pa_norm(m, l);
+        if (lane < 16) {
+#pragma unroll
+            for (int e = 0; e < HD / 64; e++) {
+                const int d = 64 * e + 4 * lane;
+                const float *o = acc + 4 * e;
+                if (u.parts > 1)
+                    qk_st((float4 *)(p.po + ((int64_t)u.slot * RT + r - u.rtile * RT) * HD + d), make_float4(o[0], o[1], o[2], o[3]));
+                else
+                    pa_put4((T *)p.a.out + (int64_t)(u.s.start + t) * p.a.o_token + (int64_t)hh * p.a.o_head + d, o[0] * f, o[1] * f,
+                            o[2] * f, o[3] * f);
+            }
+            if (u.parts > 1 && lane == 0) p.pml[(int64_t)u.slot * RT + r - u.rtile * RT] = make_float2(m, l);
+        }
+    }
+}
+
+/* running maximum and sum of a row over 32 more scores (log2 units, masked
+ * ones -inf), held by lanes l and l + 32; leaves the weights in st and
+ * rescales the sums so far */
+template <int NO>
+__device__ __forceinline__ void pa_softmax(qm_f32x16 &st, float &m, float &l, qm_f32x16 (&o)[NO]) {
+    float mx = st[0];
+#pragma unroll
+    for (int i = 1; i < 16; i++) mx = fmaxf(mx, st[i]);
+    mx = fmaxf(mx, __uint_as_float(qk_xor32_u(__float_as_uint(mx))));
+    const float mn = fmaxf(m, mx);
+    if (__any(mn > m)) {
+        const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
         l *= f;
 #pragma unroll
-        for (int e = 0; e < HD / 64; e++) acc[e] *= f;
-        m = mn;
-        const float pr = at < 0 ? 0.0f : exp2f(sc - (m == -INFINITY ? 0.0f : m));
-        l += pr;
-        for (uint64_t todo = __ballot(at >= 0); todo; todo &= todo - 1) {
-            const int b = __builtin_ctzll(todo);
-            const float pj = __shfl(pr, b, QK_WAVE);
-            const int64_t aj = ((int64_t)__shfl((int)(at >> 32), b, QK_WAVE) << 32) | (uint32_t)__shfl((int)at, b, QK_WAVE);
+        for (int d = 0; d < NO; d++)
 #pragma unroll
-            for (int e = 0; e < HD / 64; e++) acc[e] = fmaf(pj, pa_get(vp + aj + lane + 64 * e), acc[e]);
+            for (int i = 0; i < 16; i++) o[d][i] *= f;
+        m = mn;
+    }
+    const float ms = m == -INFINITY ? 0.0f : m; /* no finite score yet */
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        st[i] = __builtin_amdgcn_exp2f(st[i] - ms);
+        l += st[i];
+    }
+}
+
+__device__ __forceinline__ bool pa_bad_bf16(uint32_t w) {
+    return (w & 0x7F800000u) == 0x7F800000u || (w & 0x7F80u) == 0x7F80u;
+}
+__device__ __forceinline__ bool pa_bad_f32(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
+
+/* ------------------------------------------------------------ few rows
+ * Decode: a unit is 32 rows (a group's heads of one to a few tokens) and a
+ * part of the keys; its four waves take the part's tiles of 32 keys in turn
+ * and join through LDS at the end.  K and V go straight from the pages to
+ * registers in operand order, so the main loop has no barrier and the loads
+ * of eight waves per CU are in flight.  K: lane = key.  V: a lane takes
+ * HD / 32 dims of the keys its half of P^T has, and the bf16 pairs are turned
+ * in registers (two keys' words, one byte permute); O^T's row r is dim
+ * (HD / 32) r + e of tile e.  f32 runs on the fp32 matrix instructions, whose
+ * operands are single elements.
+ * Bound: HBM, the visible pages read once. */
+#define PD_RT 32
+#define PD_KT 32
+template <typename T, int HD>
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_few(PaArgs p) {
+    constexpr int E = HD / 32;  /* dims per lane of V = tiles of O */
+    constexpr bool B16 = sizeof(T) == 2;
+    constexpr int QN = B16 ? HD / 16 : HD / 8; /* 16-byte operand pieces of a row half */
+    constexpr int LD = HD + 4;  /* floats per row in LDS: 16-byte pieces of 8 rows on different banks */
+    __shared__ __attribute__((aligned(16))) float sum[PD_RT * LD];
+    __shared__ float2 ml[4][PD_RT];
+    PaUnit u;
+    if (!pa_find<PD_RT, PD_KT, false>(p, blockIdx.x, u)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
+    const int row0 = u.rtile * PD_RT, nrow = min(PD_RT, u.s.count * p.G - row0);
+    const int first = u.s.len - u.s.count;
+    const int p0 = first + row0 / p.G, p1 = first + (row0 + nrow - 1) / p.G;
+    const pg_tiles tl = pg_tiles_of(p0, p1, p.a.window, p.a.sinks, PD_KT);
+    const int kt0 = pg_part(tl.nt, u.part, u.parts), kt1 = pg_part(tl.nt, u.part + 1, u.parts);
+    const int r = row0 + min(c, nrow - 1), t = r / p.G, pos = first + t;
+    const int hh = pa_head(p, u.kh, r - t * p.G);
+    const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
+    const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
+
+    uint4 q[QN];
+    {
+        const T *src = (const T *)p.a.q + (int64_t)(u.s.start + t) * p.a.q_token + (int64_t)hh * p.a.q_head + h * (B16 ? 8 : 4);
+#pragma unroll
+        for (int s = 0; s < QN; s++) q[s] = qk_ld((const uint4 *)(src + s * (B16 ? 16 : 8)));
+    }
+    float m = -INFINITY, l = 0.0f;
+    bool seen = false, bad = false;
+    qm_f32x16 o[E];
+#pragma unroll
+    for (int d = 0; d < E; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+
+    auto where = [&](int i) { /* this lane's key of tile i: row offset or -1 */
+        const int j = i < kt1 ? pg_tile(tl, i) * PD_KT + c : -1;
+        return j <= p1 ? pg_row_at(&p.c, row, j) : -1;
+    };
+    int64_t next = kt0 + wave < kt1 ? where(kt0 + wave) : -1;
+    for (int i = kt0 + wave; i < kt1; i += 4) {
+        const int base = pg_tile(tl, i) * PD_KT;
+        const int64_t at = next;
+        const uint32_t valid = (uint32_t)__ballot(at >= 0);
+        const int64_t safe = at < 0 ? 0 : at; /* the pool's first row; its scores are masked, its v zeroed */
+        uint4 kx[QN];
+#pragma unroll
+        for (int s = 0; s < QN; s++) kx[s] = qk_ld((const uint4 *)(kp + safe + h * (B16 ? 8 : 4) + s * (B16 ? 16 : 8)));
+        /* v of the keys 8 a + 4 h + b, in that order */
+        struct alignas(E * sizeof(T) >= 16 ? 16 : E * sizeof(T) >= 8 ? 8 : 4) VRow { uint32_t w[E * sizeof(T) / 4]; };
+        VRow vx[16];
+#pragma unroll
+        for (int k = 0; k < 16; k++) {
+            const int key = 8 * (k >> 2) + 4 * h + (k & 3);
+            const int64_t av = ((int64_t)__shfl((int)(safe >> 32), key, QK_WAVE) << 32) | (uint32_t)__shfl((int)safe, key, QK_WAVE);
+            const uint32_t *src = (const uint32_t *)(vp + av + c * E);
+            if constexpr (sizeof(VRow) == 16) *(uint4 *)vx[k].w = qk_ld((const uint4 *)src);
+            else if constexpr (sizeof(VRow) == 8) *(uint2 *)vx[k].w = qk_ld((const uint2 *)src);
+            else {
+#pragma unroll
+                for (int x = 0; x < (int)(sizeof(VRow) / 4); x++) vx[k].w[x] = qk_ld(src + x);
+            }
+        }
+        next = where(i + 4);
+
+        qm_f32x16 st;
+#pragma unroll
+        for (int x = 0; x < 16; x++) st[x] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < QN; s++) {
+            if constexpr (B16) {
+                st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(qm_bf16x8, kx[s]), __builtin_bit_cast(qm_bf16x8, q[s]), st, 0, 0, 0);
+            } else {
+                const float4 kf = __builtin_bit_cast(float4, kx[s]), qf = __builtin_bit_cast(float4, q[s]);
+                st = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.x, qf.x, st, 0, 0, 0);
+                st = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.y, qf.y, st, 0, 0, 0);
+                st = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.z, qf.z, st, 0, 0, 0);
+                st = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.w, qf.w, st, 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 16; x++) st[x] *= p.a.scale;
+        if (valid != 0xFFFFFFFFu || !pa_full(p, p0, p1, base)) {
+            uint32_t mw = pa_mask(p, pos, base) & valid;
+            seen |= mw != 0;
+            mw >>= 4 * h;
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const int key = 8 * (k >> 2) + (k & 3);
+                st[k] = (mw >> key) & 1u ? st[k] : -INFINITY;
+                const bool dead = !((valid >> (key + 4 * h)) & 1u);
+#pragma unroll
+                for (int x = 0; x < (int)(sizeof(VRow) / 4); x++) {
+                    vx[k].w[x] = dead ? 0u : vx[k].w[x];
+                    bad |= B16 ? pa_bad_bf16(vx[k].w[x]) : pa_bad_f32(__uint_as_float(vx[k].w[x]));
+                }
+            }
+        } else {
+            seen = true;
+        }
+        pa_softmax(st, m, l, o);
+        if constexpr (B16) {
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const uint4 pw = make_uint4(qk_cvt_pk_bf16(st[8 * s], st[8 * s + 1]), qk_cvt_pk_bf16(st[8 * s + 2], st[8 * s + 3]),
+                                            qk_cvt_pk_bf16(st[8 * s + 4], st[8 * s + 5]), qk_cvt_pk_bf16(st[8 * s + 6], st[8 * s + 7]));
+#pragma unroll
+                for (int d = 0; d < E; d++) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        w[x] = __builtin_amdgcn_perm(vx[8 * s + 2 * x + 1].w[d >> 1], vx[8 * s + 2 * x].w[d >> 1],
+                                                     d & 1 ? 0x07060302u : 0x05040100u);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(qm_bf16x8, make_uint4(w[0], w[1], w[2], w[3])),
+                                                                   __builtin_bit_cast(qm_bf16x8, pw), o[d], 0, 0, 0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+#pragma unroll
+                for (int d = 0; d < E; d++)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(vx[k].w[d]), st[k], o[d], 0, 0, 0);
         }
     }
-    for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o, QK_WAVE);
-    const float f = pa_norm(m, l, seen);
-    T *out = (T *)p.a.out + t * p.a.o_token + hh * p.a.o_head;
+    l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
+    l = pa_sum(m, l, seen);
+    if (h == 0) ml[wave][c] = make_float2(m, l);
+    if (__syncthreads_or(bad)) {
+        pa_slow<T, HD, PD_RT, PD_KT>(p, u, kt0, kt1, tl, 4);
+        return;
+    }
+    float M = -INFINITY, L = 0.0f;
 #pragma unroll
-    for (int e = 0; e < HD / 64; e++) pa_put(out + lane + 64 * e, acc[e] * f);
+    for (int w = 0; w < 4; w++) M = fmaxf(M, ml[w][c].x);
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        const float2 x = ml[w][c];
+        L += x.x == M ? x.y : x.y * __builtin_amdgcn_exp2f(x.x - M);
+    }
+    const float f = m == M ? 1.0f : __builtin_amdgcn_exp2f(m - M);
+    for (int w = 0; w < 4; w++) { /* in order, so the sum is the same every time */
+        if (wave == w && c < nrow) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                float *dst = sum + c * LD + (8 * g + 4 * h) * E;
+                float x[4 * E];
+#pragma unroll
+                for (int b = 0; b < 4; b++)
+#pragma unroll
+                    for (int d = 0; d < E; d++) x[b * E + d] = o[d][4 * g + b] * f;
+#pragma unroll
+                for (int b = 0; b < E; b++) {
+                    float4 *d4 = (float4 *)dst + b;
+                    float4 y = make_float4(x[4 * b], x[4 * b + 1], x[4 * b + 2], x[4 * b + 3]);
+                    if (w) {
+                        const float4 z = *d4;
+                        y = make_float4(z.x + y.x, z.y + y.y, z.z + y.z, z.w + y.w);
+                    }
+                    *d4 = y;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    /* rows of the unit, 4 dims per thread */
+    if (wave == 0 && h == 0) ml[0][c] = make_float2(M, L);
+    __syncthreads();
+    for (int i = tid; i < nrow * (HD / 4); i += 256) {
+        const int rr = i / (HD / 4), d = 4 * (i - rr * (HD / 4));
+        const float4 x = *(const float4 *)(sum + rr * LD + d);
+        if (u.parts > 1) {
+            qk_st((float4 *)(p.po + ((int64_t)u.slot * PD_RT + rr) * HD + d), x);
+        } else {
+            const int tt = (row0 + rr) / p.G, oh = pa_head(p, u.kh, row0 + rr - tt * p.G);
+            const float g = pa_norm(ml[0][rr].x, ml[0][rr].y);
+            pa_put4((T *)p.a.out + (int64_t)(u.s.start + tt) * p.a.o_token + (int64_t)oh * p.a.o_head + d, x.x * g, x.y * g, x.z * g, x.w * g);
+        }
+    }
+    if (u.parts > 1 && tid < nrow) p.pml[(int64_t)u.slot * PD_RT + tid] = ml[0][tid];
+}
+
+/* ------------------------------------------------------------ join
+ * A workgroup takes rows of a task: its four waves the parts in turn, lane =
+ * dims, then a sum in wave order.  Bound: the parts read once, and for few
+ * rows the latency of the loads. */
+template <typename T, int HD, int RT, int KT>
+__global__ __launch_bounds__(256) void k_pa_join(PaArgs p) {
+    constexpr int E = HD / 64;
+    __shared__ float acc[4][HD];
+    __shared__ float lsum[4];
+    PaUnit u;
+    if (!pa_find<RT, KT, true>(p, blockIdx.x, u)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int rr = blockIdx.y; rr < min(RT, u.s.count * p.G - u.rtile * RT); rr += gridDim.y) {
+        auto at = [&](int i) { return (int64_t)(u.slot + i * p.c.kvh) * RT + rr; };
+        float M = -INFINITY;
+        for (int i = lane; i < u.parts; i += 64) M = fmaxf(M, qk_ld((const float *)(p.pml + at(i))));
+        for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, QK_WAVE));
+        float L = 0.0f, x[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) x[e] = 0.0f;
+#pragma unroll 4
+        for (int i = wave; i < u.parts; i += 4) {
+            const float pm = qk_ld((const float *)(p.pml + at(i))), pl = qk_ld((const float *)(p.pml + at(i)) + 1);
+            const float f = pm == M ? 1.0f : __builtin_amdgcn_exp2f(pm - M);
+            L = fmaf(pl, f, L);
+#pragma unroll
+            for (int e = 0; e < E; e++) x[e] = fmaf(qk_ld(p.po + at(i) * HD + lane + 64 * e), f, x[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) acc[wave][lane + 64 * e] = x[e];
+        if (lane == 0) lsum[wave] = L;
+        __syncthreads();
+        if (tid < HD / 4) {
+            const float f = pa_norm(M, lsum[0] + lsum[1] + lsum[2] + lsum[3]);
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float4 z = *(const float4 *)(acc[w] + 4 * tid);
+                y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+            }
+            const int r = u.rtile * RT + rr, t = r / p.G, hh = pa_head(p, u.kh, r - t * p.G);
+            pa_put4((T *)p.a.out + (int64_t)(u.s.start + t) * p.a.o_token + (int64_t)hh * p.a.o_head + 4 * tid, y.x * f, y.y * f,
+                    y.z * f, y.w * f);
+        }
+        __syncthreads();
+    }
 }
 
 /* ------------------------------------------------------------ host side */
 
-extern "C" size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h) { return 256; }
+/* how a call is cut: units asked for, the grid that holds them whatever the
+ * lengths, tasks that can need a join, and the slots of partial results */
+struct PaPlan {
+    int units, least;
+    int64_t grid, join, slots;
+};
+
+static PaPlan pa_plan(const pg_cache *c, int n, int n_seqs, int h, int rt, int kt, int units, int least) {
+    PaPlan q;
+    const int G = h / c->kvh;
+    q.units = units;
+    q.least = least;
+    /* sum of ceil(rows / rt) over the sequences that have rows */
+    const int64_t rows = (int64_t)n * G, seqs = n_seqs < n ? n_seqs : n;
+    const int64_t per_head = rows / rt + seqs < rows ? rows / rt + seqs : rows;
+    const int64_t tasks = per_head * c->kvh;
+    const int64_t key_tiles = ((int64_t)c->cap + kt - 1) / kt + 1;
+    const int64_t parts = key_tiles <= least ? 1 : (key_tiles + least - 1) / least;
+    q.grid = tasks * parts < units + tasks ? tasks * parts : units + tasks;
+    q.slots = parts == 1 ? 0 : tasks * parts < 2 * (int64_t)units ? tasks * parts : 2 * (int64_t)units;
+    q.join = parts == 1 ? 0 : tasks < units ? tasks : units; /* a split task has two units at least */
+    return q;
+}
+
+/* workgroups that share a task's rows: about 1024 in all, where the tasks are
+ * few every row has its own */
+static unsigned pa_join_rows(int64_t tasks, int rt) {
+    const int64_t r = 1024 / tasks;
+    return (unsigned)(r < 1 ? 1 : r > rt ? rt : r);
+}
+
+static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h) { return pa_plan(c, n, n_seqs, h, PD_RT, PD_KT, 1024, 8); }
+
+static size_t pa_up(size_t v) { return (v + 255) / 256 * 256; }
+extern "C" size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h) {
+    const PaPlan q = pa_plan_of(c, n, n_seqs, h);
+    return 256 + pa_up((size_t)q.slots * PD_RT * 8) + pa_up((size_t)q.slots * PD_RT * c->hd * 4);
+}
+
+template <typename T, int HD>
+static int pa_launch(PaArgs p, void *ws, hipStream_t st) {
+    const PaPlan q = pa_plan_of(&p.c, p.a.n, p.a.n_seqs, p.a.h);
+    p.units = q.units;
+    p.least = q.least;
+    p.pml = (float2 *)ws;
+    p.po = (float *)((char *)ws + pa_up((size_t)q.slots * PD_RT * 8));
+    hipLaunchKernelGGL((k_pa_few<T, HD>), dim3((unsigned)q.grid), dim3(256), 0, st, p);
+    const int rc = QK_CHECK_LAUNCH();
+    if (rc || q.join == 0) return rc;
+    hipLaunchKernelGGL((k_pa_join<T, HD, PD_RT, PD_KT>), dim3((unsigned)q.join, pa_join_rows(q.join, PD_RT)), dim3(256), 0, st, p);
+    return QK_CHECK_LAUNCH();
+}
 
 template <typename T>
-static int pa_launch(const PaArgs &p, hipStream_t st) {
-    const dim3 grid((unsigned)(((int64_t)p.a.n * p.a.h + 3) / 4));
+static int pa_launch_hd(const PaArgs &p, void *ws, hipStream_t st) {
     switch (p.c.hd) {
-    case 64: hipLaunchKernelGGL((k_pa_rows<T, 64>), grid, dim3(256), 0, st, p); break;
-    case 128: hipLaunchKernelGGL((k_pa_rows<T, 128>), grid, dim3(256), 0, st, p); break;
-    case 192: hipLaunchKernelGGL((k_pa_rows<T, 192>), grid, dim3(256), 0, st, p); break;
-    case 256: hipLaunchKernelGGL((k_pa_rows<T, 256>), grid, dim3(256), 0, st, p); break;
+    case 64: return pa_launch<T, 64>(p, ws, st);
+    case 128: return pa_launch<T, 128>(p, ws, st);
+    case 192: return pa_launch<T, 192>(p, ws, st);
+    case 256: return pa_launch<T, 256>(p, ws, st);
     default: return (int)hipErrorInvalidValue;
     }
-    return QK_CHECK_LAUNCH();
 }
 
 extern "C" int qk_launch_pg_attn(const pg_cache *c, const pg_attn *a, void *ws, void *stream) {
@@ -141,5 +610,8 @@ extern "C" int qk_launch_pg_attn(const pg_cache *c, const pg_attn *a, void *ws, 
     p.c = *c;
     p.a = *a;
     p.G = a->h / c->kvh;
-    return c->dtype == QMOE_BF16 ? pa_launch<uint16_t>(p, (hipStream_t)stream) : pa_launch<float>(p, (hipStream_t)stream);
+    p.po = NULL;
+    p.pml = NULL;
+    return c->dtype == QMOE_BF16 ? pa_launch_hd<uint16_t>(p, ws, (hipStream_t)stream)
+                                 : pa_launch_hd<float>(p, ws, (hipStream_t)stream);
 }
