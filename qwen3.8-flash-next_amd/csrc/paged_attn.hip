@@ -195,7 +195,7 @@ __device__ __forceinline__ bool pa_full(const PaArgs &p, int p0, int p1, int bas
  * MFMA, a value that the bf16 parts cannot carry): a masked key is never
  * multiplied here.  Waves take the unit's rows in turn. */
 template <typename T, int HD, int RT, int KT>
-__device__ __noinline__ void pa_slow(const PaArgs &p, const PaUnit &u, int kt0, int kt1, pg_tiles tl, int waves) {
+__device__ __forceinline__ void pa_slow(const PaArgs &p, const PaUnit &u, int kt0, int kt1, pg_tiles tl, int waves) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
     const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
@@ -264,18 +264,21 @@ __device__ __noinline__ void pa_slow(const PaArgs &p, const PaUnit &u, int kt0, 
     }
 }
 
-/* running maximum and sum of a row over 32 more scores (log2 units, masked
- * ones -inf), held by lanes l and l + 32; leaves the weights in st and
- * rescales the sums so far */
-template <int NO>
-__device__ __forceinline__ void pa_softmax(qm_f32x16 &st, float &m, float &l, qm_f32x16 (&o)[NO]) {
-    float mx = st[0];
+/* running maximum and sum of a row over 32 NS more scores (log2 units, masked
+ * ones -inf), held by lanes l and l + 32; leaves the weights in st.  The sums
+ * so far are rescaled only when a maximum has grown by more than 8: weights
+ * reach 256 then, which costs no accuracy (fp32 sums, bf16 weights are
+ * relative), and most rescalings of a long row are saved. */
+template <int NS, int NO>
+__device__ __forceinline__ void pa_softmax(qm_f32x16 (&st)[NS], float &m, float &l, qm_f32x16 (&o)[NO]) {
+    float mx = st[0][0];
 #pragma unroll
-    for (int i = 1; i < 16; i++) mx = fmaxf(mx, st[i]);
+    for (int t = 0; t < NS; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) mx = fmaxf(mx, st[t][i]);
     mx = fmaxf(mx, __uint_as_float(qk_xor32_u(__float_as_uint(mx))));
-    const float mn = fmaxf(m, mx);
-    if (__any(mn > m)) {
-        const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+    if (__any(mx > m + 8.0f)) {
+        const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
         l *= f;
 #pragma unroll
         for (int d = 0; d < NO; d++)
@@ -285,10 +288,18 @@ __device__ __forceinline__ void pa_softmax(qm_f32x16 &st, float &m, float &l, qm
     }
     const float ms = m == -INFINITY ? 0.0f : m; /* no finite score yet */
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        st[i] = __builtin_amdgcn_exp2f(st[i] - ms);
-        l += st[i];
-    }
+    for (int t = 0; t < NS; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            st[t][i] = __builtin_amdgcn_exp2f(st[t][i] - ms);
+            l += st[t][i];
+        }
+}
+
+/* eight weights of a row as a B operand */
+__device__ __forceinline__ qm_bf16x8 pa_pack(const qm_f32x16 &st, int s) {
+    return __builtin_bit_cast(qm_bf16x8, make_uint4(qk_cvt_pk_bf16(st[8 * s], st[8 * s + 1]), qk_cvt_pk_bf16(st[8 * s + 2], st[8 * s + 3]),
+                                                    qk_cvt_pk_bf16(st[8 * s + 4], st[8 * s + 5]), qk_cvt_pk_bf16(st[8 * s + 6], st[8 * s + 7])));
 }
 
 __device__ __forceinline__ bool pa_bad_bf16(uint32_t w) {
@@ -374,7 +385,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_few(PaArgs p) {
         }
         next = where(i + 4);
 
-        qm_f32x16 st;
+        qm_f32x16 sts[1];
+        qm_f32x16 &st = sts[0];
 #pragma unroll
         for (int x = 0; x < 16; x++) st[x] = 0.0f;
 #pragma unroll
@@ -409,12 +421,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_few(PaArgs p) {
         } else {
             seen = true;
         }
-        pa_softmax(st, m, l, o);
+        pa_softmax(sts, m, l, o);
         if constexpr (B16) {
 #pragma unroll
             for (int s = 0; s < 2; s++) {
-                const uint4 pw = make_uint4(qk_cvt_pk_bf16(st[8 * s], st[8 * s + 1]), qk_cvt_pk_bf16(st[8 * s + 2], st[8 * s + 3]),
-                                            qk_cvt_pk_bf16(st[8 * s + 4], st[8 * s + 5]), qk_cvt_pk_bf16(st[8 * s + 6], st[8 * s + 7]));
+                const qm_bf16x8 pw = pa_pack(st, s);
 #pragma unroll
                 for (int d = 0; d < E; d++) {
                     uint32_t w[4];
@@ -423,7 +434,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_few(PaArgs p) {
                         w[x] = __builtin_amdgcn_perm(vx[8 * s + 2 * x + 1].w[d >> 1], vx[8 * s + 2 * x].w[d >> 1],
                                                      d & 1 ? 0x07060302u : 0x05040100u);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(qm_bf16x8, make_uint4(w[0], w[1], w[2], w[3])),
-                                                                   __builtin_bit_cast(qm_bf16x8, pw), o[d], 0, 0, 0);
+                                                                   pw, o[d], 0, 0, 0);
                 }
             }
         } else {
@@ -489,6 +500,180 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_few(PaArgs p) {
         }
     }
     if (u.parts > 1 && tid < nrow) p.pml[(int64_t)u.slot * PD_RT + tid] = ml[0][tid];
+}
+
+/* ------------------------------------------------------------ many rows
+ * Prompts, bf16: a unit is 128 rows, 32 per wave, and a part of the keys.
+ * Tiles of KT keys of K and V are copied straight from the pages to LDS, two
+ * buffers, one barrier per tile.  The copies' lanes pick the 16-byte pieces,
+ * so a tile lies in rows with its pieces exchanged by the row's number (an
+ * xor): K's operand reads (a lane per row) and V's transposing reads (a lane
+ * per dim, four keys) then meet no bank twice.  Where a tile's rows lie is
+ * looked up for 1024 keys at a time; a row without a page or after the last
+ * query is copied from a piece of zeros.
+ * Bound: matrix cores and, next to them, LDS (each wave reads the whole tile
+ * for 32 rows) and the exponentials. */
+#define PM_RT 128
+#define PM_CHUNK 1024
+__device__ const uint4 pa_zero = {0, 0, 0, 0};
+typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) pa_s16x4 *pa_tptr;
+
+constexpr int pm_kt(int hd) { return hd <= 128 ? 64 : 32; }
+
+template <int HD>
+__global__ __launch_bounds__(256, 2) void k_pa_many(PaArgs p) {
+    typedef uint16_t T;
+    constexpr int KT = pm_kt(HD), CR = HD / 8, NB = KT * CR / 256, NS = KT / 32, E = HD / 32, KS = HD / 16;
+    __shared__ __attribute__((aligned(16))) uint4 kv[2][2][KT * CR];
+    __shared__ int64_t where[PM_CHUNK];
+    PaUnit u;
+    if (!pa_find<PM_RT, KT, false>(p, blockIdx.x, u)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, h = lane >> 5;
+    const int row0 = u.rtile * PM_RT, rows = u.s.count * p.G, nrow = min(PM_RT, rows - row0);
+    const int first = u.s.len - u.s.count;
+    const int p0 = first + row0 / p.G, p1 = first + (row0 + nrow - 1) / p.G;
+    const pg_tiles tl = pg_tiles_of(p0, p1, p.a.window, p.a.sinks, KT);
+    const int kt0 = pg_part(tl.nt, u.part, u.parts), kt1 = pg_part(tl.nt, u.part + 1, u.parts), nt = kt1 - kt0;
+    /* this wave's rows; a wave past the last row copies and waits only */
+    const int w0 = row0 + 32 * wave, wn = min(32, rows - w0);
+    const int pw0 = first + w0 / p.G, pw1 = first + (w0 + wn - 1) / p.G;
+    const int r = min(w0 + c, rows - 1), t = r / p.G, pos = first + t;
+    const int hh = pa_head(p, u.kh, r - t * p.G);
+    const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
+    const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
+
+    auto look = [&](int i0) { /* rows of the tiles i0.. of the part */
+        for (int k = tid; k < PM_CHUNK; k += 256) {
+            const int i = kt0 + i0 + k / KT;
+            const int j = i < kt1 ? pg_tile(tl, i) * KT + k % KT : -1;
+            where[k] = j >= 0 && j <= p1 ? pg_row_at(&p.c, row, j) : -1;
+        }
+        __syncthreads();
+    };
+    /* piece x of this thread: row and piece of the tile in LDS order */
+    uint32_t lds0[2][2];
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+            lds0[b][x] = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(qm_lptr)&kv[b][x][0] + 1024 * wave);
+    uint64_t vnext = 0;
+    auto copy = [&](int i) {
+        const int64_t *wh = where + i % (PM_CHUNK / KT) * KT;
+        const int b = i & 1;
+#pragma unroll
+        for (int x = 0; x < NB; x++) {
+            const int L = x * 256 + wave * 64 + lane, rr = L / CR, pc = L - rr * CR;
+            const int64_t at = wh[rr];
+            const T *ks = kp + at + 8 * (pc ^ (rr & 7)), *vs = vp + at + 8 * (pc ^ (((rr & 3) << 1) | ((rr >> 2) & 1)));
+            qm_copy<0>(at < 0 ? &pa_zero : (const uint4 *)ks, lds0[b][0] + 4096 * x);
+            qm_copy<0>(at < 0 ? &pa_zero : (const uint4 *)vs, lds0[b][1] + 4096 * x);
+        }
+        vnext = __ballot(wh[lane & (KT - 1)] >= 0);
+    };
+    if (nt > 0) {
+        look(0);
+        copy(0);
+    }
+    uint4 q[KS];
+    {
+        const T *src = (const T *)p.a.q + (int64_t)(u.s.start + t) * p.a.q_token + (int64_t)hh * p.a.q_head + h * 8;
+#pragma unroll
+        for (int s = 0; s < KS; s++) q[s] = qk_ld((const uint4 *)(src + s * 16));
+    }
+    float m = -INFINITY, l = 0.0f;
+    bool seen = false, bad = false;
+    qm_f32x16 o[E];
+#pragma unroll
+    for (int d = 0; d < E; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    /* V: lane j of 16 reads 4 dims of key j / 4 and receives 4 keys of dim j */
+    const int j = lane & 15, g16 = (lane >> 4) & 1, fv = ((j >> 2) << 1) | h;
+
+    for (int i = 0; i < nt; i++) {
+        qm_sync<0>(); /* tile i is in LDS; every wave is done with tile i - 1 */
+        const uint64_t valid = vnext;
+        if (i + 1 < nt) {
+            if ((i + 1) % (PM_CHUNK / KT) == 0) look(i + 1);
+            copy(i + 1);
+        }
+        const int base = pg_tile(tl, kt0 + i) * KT;
+        /* nothing of the tile is seen by this wave */
+        if (wn <= 0 || base > pw1 || (p.a.window > 0 && base + KT <= pg_lo(pw0, p.a.window) && base >= p.a.sinks)) continue;
+        const uint4 *kb = kv[i & 1][0], *vb = kv[i & 1][1];
+        qm_f32x16 st[NS];
+#pragma unroll
+        for (int n = 0; n < NS; n++) {
+#pragma unroll
+            for (int x = 0; x < 16; x++) st[n][x] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+                st[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    __builtin_bit_cast(qm_bf16x8, kb[(32 * n + c) * CR + 8 * (s >> 2) + ((2 * (s & 3) + h) ^ (c & 7))]),
+                    __builtin_bit_cast(qm_bf16x8, q[s]), st[n], 0, 0, 0);
+#pragma unroll
+            for (int x = 0; x < 16; x++) st[n][x] *= p.a.scale;
+        }
+#pragma unroll
+        for (int n = 0; n < NS; n++) {
+            const uint32_t v32 = (uint32_t)(valid >> (32 * n));
+            if (v32 == 0xFFFFFFFFu && pa_full(p, pw0, pw1, base + 32 * n)) {
+                seen = true;
+                continue;
+            }
+            uint32_t mw = pa_mask(p, pos, base + 32 * n) & v32;
+            seen |= mw != 0;
+            mw >>= 4 * h;
+#pragma unroll
+            for (int x = 0; x < 16; x++) st[n][x] = (mw >> (8 * (x >> 2) + (x & 3))) & 1u ? st[n][x] : -INFINITY;
+            for (int x = 0; x < CR / 2; x++) {
+                const uint4 w = vb[32 * n * CR + 64 * x + lane];
+                bad |= pa_bad_bf16(w.x) || pa_bad_bf16(w.y) || pa_bad_bf16(w.z) || pa_bad_bf16(w.w);
+            }
+        }
+        pa_softmax(st, m, l, o);
+#pragma unroll
+        for (int n = 0; n < NS; n++)
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const qm_bf16x8 pw = pa_pack(st[n], s);
+                const int key = 32 * n + 16 * s + 4 * h + (j >> 2);
+#pragma unroll
+                for (int d = 0; d < E; d++) {
+                    const int pc = 8 * (d >> 1) + ((4 * (d & 1) + 2 * g16 + ((j & 3) >> 1)) ^ fv);
+                    const pa_s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_tptr)((const short *)(vb + key * CR + pc) + 4 * (j & 1)));
+                    const pa_s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_tptr)((const short *)(vb + (key + 8) * CR + pc) + 4 * (j & 1)));
+                    const uint2 aw = __builtin_bit_cast(uint2, a), bw = __builtin_bit_cast(uint2, b);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(qm_bf16x8, make_uint4(aw.x, aw.y, bw.x, bw.y)), pw, o[d], 0, 0, 0);
+                }
+            }
+    }
+    if (__syncthreads_or(bad)) {
+        pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 4);
+        return;
+    }
+    l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
+    l = pa_sum(m, l, seen);
+    if (c >= wn) return;
+    if (u.parts > 1) {
+        const int64_t at = (int64_t)u.slot * PM_RT + 32 * wave + c;
+#pragma unroll
+        for (int d = 0; d < E; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+                qk_st((float4 *)(p.po + at * HD + 32 * d + 8 * g + 4 * h), make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]));
+        if (h == 0) p.pml[at] = make_float2(m, l);
+        return;
+    }
+    const float f = pa_norm(m, l);
+    T *out = (T *)p.a.out + (int64_t)(u.s.start + t) * p.a.o_token + (int64_t)hh * p.a.o_head;
+#pragma unroll
+    for (int d = 0; d < E; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            pa_put4(out + 32 * d + 8 * g + 4 * h, o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f);
 }
 
 /* ------------------------------------------------------------ join
@@ -572,26 +757,43 @@ static unsigned pa_join_rows(int64_t tasks, int rt) {
     return (unsigned)(r < 1 ? 1 : r > rt ? rt : r);
 }
 
-static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h) { return pa_plan(c, n, n_seqs, h, PD_RT, PD_KT, 1024, 8); }
+/* which kernel: rows per sequence past one unit of the few-row kernel, on
+ * average, go to the many-row one */
+static bool pa_many(const pg_cache *c, int n, int n_seqs, int h) {
+    return c->dtype == QMOE_BF16 && (int64_t)n * (h / c->kvh) > (int64_t)PD_RT * n_seqs;
+}
+static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h) {
+    if (pa_many(c, n, n_seqs, h)) return pa_plan(c, n, n_seqs, h, PM_RT, pm_kt(c->hd), 512, 512 / pm_kt(c->hd));
+    return pa_plan(c, n, n_seqs, h, PD_RT, PD_KT, 1024, 8);
+}
 
 static size_t pa_up(size_t v) { return (v + 255) / 256 * 256; }
 extern "C" size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h) {
     const PaPlan q = pa_plan_of(c, n, n_seqs, h);
-    return 256 + pa_up((size_t)q.slots * PD_RT * 8) + pa_up((size_t)q.slots * PD_RT * c->hd * 4);
+    const int rt = pa_many(c, n, n_seqs, h) ? PM_RT : PD_RT;
+    return 256 + pa_up((size_t)q.slots * rt * 8) + pa_up((size_t)q.slots * rt * c->hd * 4);
 }
 
-template <typename T, int HD>
-static int pa_launch(PaArgs p, void *ws, hipStream_t st) {
+template <typename T, int HD, int RT, int KT>
+static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), void *ws, hipStream_t st) {
     const PaPlan q = pa_plan_of(&p.c, p.a.n, p.a.n_seqs, p.a.h);
     p.units = q.units;
     p.least = q.least;
     p.pml = (float2 *)ws;
-    p.po = (float *)((char *)ws + pa_up((size_t)q.slots * PD_RT * 8));
-    hipLaunchKernelGGL((k_pa_few<T, HD>), dim3((unsigned)q.grid), dim3(256), 0, st, p);
+    p.po = (float *)((char *)ws + pa_up((size_t)q.slots * RT * 8));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)q.grid), dim3(256), 0, st, p);
     const int rc = QK_CHECK_LAUNCH();
     if (rc || q.join == 0) return rc;
-    hipLaunchKernelGGL((k_pa_join<T, HD, PD_RT, PD_KT>), dim3((unsigned)q.join, pa_join_rows(q.join, PD_RT)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((k_pa_join<T, HD, RT, KT>), dim3((unsigned)q.join, pa_join_rows(q.join, RT)), dim3(256), 0, st, p);
     return QK_CHECK_LAUNCH();
+}
+
+template <typename T, int HD>
+static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
+    if constexpr (sizeof(T) == 2)
+        if (pa_many(&p.c, p.a.n, p.a.n_seqs, p.a.h))
+            return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD>, ws, st);
+    return pa_launch_rt<T, HD, PD_RT, PD_KT>(p, k_pa_few<T, HD>, ws, st);
 }
 
 template <typename T>
