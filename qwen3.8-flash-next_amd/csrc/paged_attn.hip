@@ -264,9 +264,10 @@ __device__ __forceinline__ void pa_slow(const PaArgs &p, const PaUnit &u, int kt
     }
 }
 
+#define PA_GROW 8.0f
 /* running maximum and sum of a row over 32 NS more scores (log2 units, masked
  * ones -inf), held by lanes l and l + 32; leaves the weights in st.  The sums
- * so far are rescaled only when a maximum has grown by more than 8: weights
+ * so far are rescaled only when a maximum has grown by more than PA_GROW: weights
  * reach 256 then, which costs no accuracy (fp32 sums, bf16 weights are
  * relative), and most rescalings of a long row are saved. */
 template <int NS, int NO>
@@ -277,7 +278,7 @@ __device__ __forceinline__ void pa_softmax(qm_f32x16 (&st)[NS], float &m, float 
 #pragma unroll
         for (int i = 0; i < 16; i++) mx = fmaxf(mx, st[t][i]);
     mx = fmaxf(mx, __uint_as_float(qk_xor32_u(__float_as_uint(mx))));
-    if (__any(mx > m + 8.0f)) {
+    if (__any(mx > m + PA_GROW)) {
         const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
         l *= f;
 #pragma unroll
@@ -308,198 +309,256 @@ __device__ __forceinline__ bool pa_bad_bf16(uint32_t w) {
 __device__ __forceinline__ bool pa_bad_f32(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
 /* ------------------------------------------------------------ few rows
- * Decode: a unit is 32 rows (a group's heads of one to a few tokens) and a
+ * Decode: a unit is 16 NC rows (a group's heads of one to a few tokens) and a
  * part of the keys; its four waves take the part's tiles of 32 keys in turn
  * and join through LDS at the end.  K and V go straight from the pages to
  * registers in operand order, so the main loop has no barrier and the loads
- * of eight waves per CU are in flight.  K: lane = key.  V: a lane takes
- * HD / 32 dims of the keys its half of P^T has, and the bf16 pairs are turned
- * in registers (two keys' words, one byte permute); O^T's row r is dim
- * (HD / 32) r + e of tile e.  f32 runs on the fp32 matrix instructions, whose
- * operands are single elements.
+ * of eight or more waves per CU are in flight.  16-wide instructions: lane =
+ * (row or key c = lane % 16, quarter g = lane / 16); the scores of a tile
+ * leave lane (c, g) the keys 16 n + 4 g + b of row c.  K: lane c = key, a
+ * quarter has every fourth piece of 16 bytes.  V: a lane takes HD / 16 dims of
+ * the eight keys its quarter of P^T has; bf16 pairs are turned in registers
+ * (two keys' words, one byte permute), and O^T's row x of tile e is dim
+ * (HD / 16) x + e.  f32 runs on the fp32 matrix instructions, whose operands
+ * are single elements.
  * Bound: HBM, the visible pages read once. */
-#define PD_RT 32
 #define PD_KT 32
-template <typename T, int HD>
-__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_few(PaArgs p) {
-    constexpr int E = HD / 32;  /* dims per lane of V = tiles of O */
+typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T, int HD, int NC>
+constexpr int pd_occ() { return NC * HD * (int)sizeof(T) <= 512 ? 2 : 1; }
+
+template <typename T, int HD, int NC>
+__global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p) {
+    constexpr int RT = 16 * NC;
+    constexpr int E = HD / 16;  /* dims per lane of V = tiles of O */
     constexpr bool B16 = sizeof(T) == 2;
-    constexpr int QN = B16 ? HD / 16 : HD / 8; /* 16-byte operand pieces of a row half */
+    constexpr int PE = 16 / (int)sizeof(T);   /* elements of a 16-byte piece */
+    constexpr int QN = HD / (4 * PE);         /* pieces of a quarter of a row */
     constexpr int LD = HD + 4;  /* floats per row in LDS: 16-byte pieces of 8 rows on different banks */
-    __shared__ __attribute__((aligned(16))) float sum[PD_RT * LD];
-    __shared__ float2 ml[4][PD_RT];
+    constexpr int VW = E * (int)sizeof(T) / 4; /* words of a lane's dims of one key */
+    __shared__ __attribute__((aligned(16))) float sum[RT * LD];
+    __shared__ float2 ml[4][RT];
+    __shared__ __attribute__((aligned(16))) int64_t where[4][32];
     PaUnit u;
-    if (!pa_find<PD_RT, PD_KT, false>(p, blockIdx.x, u)) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
-    const int row0 = u.rtile * PD_RT, nrow = min(PD_RT, u.s.count * p.G - row0);
+    if (!pa_find<RT, PD_KT, false>(p, blockIdx.x, u)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int row0 = u.rtile * RT, nrow = min(RT, u.s.count * p.G - row0);
     const int first = u.s.len - u.s.count;
     const int p0 = first + row0 / p.G, p1 = first + (row0 + nrow - 1) / p.G;
     const pg_tiles tl = pg_tiles_of(p0, p1, p.a.window, p.a.sinks, PD_KT);
     const int kt0 = pg_part(tl.nt, u.part, u.parts), kt1 = pg_part(tl.nt, u.part + 1, u.parts);
-    const int r = row0 + min(c, nrow - 1), t = r / p.G, pos = first + t;
-    const int hh = pa_head(p, u.kh, r - t * p.G);
     const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
     const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
 
-    uint4 q[QN];
-    {
-        const T *src = (const T *)p.a.q + (int64_t)(u.s.start + t) * p.a.q_token + (int64_t)hh * p.a.q_head + h * (B16 ? 8 : 4);
-#pragma unroll
-        for (int s = 0; s < QN; s++) q[s] = qk_ld((const uint4 *)(src + s * (B16 ? 16 : 8)));
-    }
-    float m = -INFINITY, l = 0.0f;
-    bool seen = false, bad = false;
-    qm_f32x16 o[E];
-#pragma unroll
-    for (int d = 0; d < E; d++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-
-    auto where = [&](int i) { /* this lane's key of tile i: row offset or -1 */
-        const int j = i < kt1 ? pg_tile(tl, i) * PD_KT + c : -1;
+    auto find = [&](int i) { /* key lane % 32 of tile i: row offset or -1 */
+        const int j = i < kt1 ? pg_tile(tl, i) * PD_KT + (lane & 31) : -1;
         return j <= p1 ? pg_row_at(&p.c, row, j) : -1;
     };
-    int64_t next = kt0 + wave < kt1 ? where(kt0 + wave) : -1;
+    int64_t next = find(kt0 + wave);
+    uint4 q[NC][QN];
+    int pos[NC];
+    float m[NC], l[NC];
+    bool seen[NC], bad = false;
+    pa_f32x4 o[NC][E];
+#pragma unroll
+    for (int x = 0; x < NC; x++) {
+        const int r = row0 + min(16 * x + c, nrow - 1), t = r / p.G;
+        pos[x] = first + t;
+        const T *src = (const T *)p.a.q + (int64_t)(u.s.start + t) * p.a.q_token + (int64_t)pa_head(p, u.kh, r - t * p.G) * p.a.q_head + g * PE;
+#pragma unroll
+        for (int s = 0; s < QN; s++) q[x][s] = qk_ld((const uint4 *)(src + s * 4 * PE));
+        m[x] = -INFINITY;
+        l[x] = 0.0f;
+        seen[x] = false;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[x][e] = pa_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
     for (int i = kt0 + wave; i < kt1; i += 4) {
         const int base = pg_tile(tl, i) * PD_KT;
-        const int64_t at = next;
-        const uint32_t valid = (uint32_t)__ballot(at >= 0);
-        const int64_t safe = at < 0 ? 0 : at; /* the pool's first row; its scores are masked, its v zeroed */
-        uint4 kx[QN];
+        const uint32_t valid = (uint32_t)__ballot(next >= 0);
+        /* a row without a page reads the pool's first one; its scores are masked, its v zeroed */
+        if (lane < 32) where[wave][lane] = next < 0 ? 0 : next;
+        __builtin_amdgcn_wave_barrier();
+        uint4 kx[2][QN];
 #pragma unroll
-        for (int s = 0; s < QN; s++) kx[s] = qk_ld((const uint4 *)(kp + safe + h * (B16 ? 8 : 4) + s * (B16 ? 16 : 8)));
-        /* v of the keys 8 a + 4 h + b, in that order */
-        struct alignas(E * sizeof(T) >= 16 ? 16 : E * sizeof(T) >= 8 ? 8 : 4) VRow { uint32_t w[E * sizeof(T) / 4]; };
-        VRow vx[16];
+        for (int n = 0; n < 2; n++) {
+            const T *src = kp + where[wave][16 * n + c] + g * PE;
 #pragma unroll
-        for (int k = 0; k < 16; k++) {
-            const int key = 8 * (k >> 2) + 4 * h + (k & 3);
-            const int64_t av = ((int64_t)__shfl((int)(safe >> 32), key, QK_WAVE) << 32) | (uint32_t)__shfl((int)safe, key, QK_WAVE);
-            const uint32_t *src = (const uint32_t *)(vp + av + c * E);
-            if constexpr (sizeof(VRow) == 16) *(uint4 *)vx[k].w = qk_ld((const uint4 *)src);
-            else if constexpr (sizeof(VRow) == 8) *(uint2 *)vx[k].w = qk_ld((const uint2 *)src);
-            else {
-#pragma unroll
-                for (int x = 0; x < (int)(sizeof(VRow) / 4); x++) vx[k].w[x] = qk_ld(src + x);
-            }
+            for (int s = 0; s < QN; s++) kx[n][s] = qk_ld((const uint4 *)(src + s * 4 * PE));
         }
-        next = where(i + 4);
-
-        qm_f32x16 sts[1];
-        qm_f32x16 &st = sts[0];
+        uint32_t vx[8][VW]; /* key 16 (k / 4) + 4 g + k % 4 */
 #pragma unroll
-        for (int x = 0; x < 16; x++) st[x] = 0.0f;
+        for (int k = 0; k < 8; k++) {
+            const uint32_t *src = (const uint32_t *)(vp + where[wave][16 * (k >> 2) + 4 * g + (k & 3)] + c * E);
+            if constexpr (VW % 4 == 0) {
 #pragma unroll
-        for (int s = 0; s < QN; s++) {
-            if constexpr (B16) {
-                st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(qm_bf16x8, kx[s]), __builtin_bit_cast(qm_bf16x8, q[s]), st, 0, 0, 0);
+                for (int x = 0; x < VW; x += 4) {
+                    const uint4 w = qk_ld((const uint4 *)(src + x));
+                    vx[k][x] = w.x; vx[k][x + 1] = w.y; vx[k][x + 2] = w.z; vx[k][x + 3] = w.w;
+                }
             } else {
-                const float4 kf = __builtin_bit_cast(float4, kx[s]), qf = __builtin_bit_cast(float4, q[s]);
-                st = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.x, qf.x, st, 0, 0, 0);
-                st = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.y, qf.y, st, 0, 0, 0);
-                st = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.z, qf.z, st, 0, 0, 0);
-                st = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.w, qf.w, st, 0, 0, 0);
+#pragma unroll
+                for (int x = 0; x < VW; x += 2) {
+                    const uint2 w = qk_ld((const uint2 *)(src + x));
+                    vx[k][x] = w.x; vx[k][x + 1] = w.y;
+                }
             }
         }
+        next = find(i + 4);
+
+        pa_f32x4 st[NC][2];
 #pragma unroll
-        for (int x = 0; x < 16; x++) st[x] *= p.a.scale;
+        for (int x = 0; x < NC; x++)
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                pa_f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int s = 0; s < QN; s++) {
+                    if constexpr (B16) {
+                        a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qm_bf16x8, kx[n][s]), __builtin_bit_cast(qm_bf16x8, q[x][s]), a, 0, 0, 0);
+                    } else {
+                        const float4 kf = __builtin_bit_cast(float4, kx[n][s]), qf = __builtin_bit_cast(float4, q[x][s]);
+                        a = __builtin_amdgcn_mfma_f32_16x16x4f32(kf.x, qf.x, a, 0, 0, 0);
+                        a = __builtin_amdgcn_mfma_f32_16x16x4f32(kf.y, qf.y, a, 0, 0, 0);
+                        a = __builtin_amdgcn_mfma_f32_16x16x4f32(kf.z, qf.z, a, 0, 0, 0);
+                        a = __builtin_amdgcn_mfma_f32_16x16x4f32(kf.w, qf.w, a, 0, 0, 0);
+                    }
+                }
+                st[x][n] = a * p.a.scale;
+            }
         if (valid != 0xFFFFFFFFu || !pa_full(p, p0, p1, base)) {
-            uint32_t mw = pa_mask(p, pos, base) & valid;
-            seen |= mw != 0;
-            mw >>= 4 * h;
 #pragma unroll
-            for (int k = 0; k < 16; k++) {
-                const int key = 8 * (k >> 2) + (k & 3);
-                st[k] = (mw >> key) & 1u ? st[k] : -INFINITY;
-                const bool dead = !((valid >> (key + 4 * h)) & 1u);
+            for (int x = 0; x < NC; x++) {
+                uint32_t mw = pa_mask(p, pos[x], base) & valid;
+                seen[x] |= mw != 0;
+                mw >>= 4 * g;
 #pragma unroll
-                for (int x = 0; x < (int)(sizeof(VRow) / 4); x++) {
-                    vx[k].w[x] = dead ? 0u : vx[k].w[x];
-                    bad |= B16 ? pa_bad_bf16(vx[k].w[x]) : pa_bad_f32(__uint_as_float(vx[k].w[x]));
+                for (int k = 0; k < 8; k++) st[x][k >> 2][k & 3] = (mw >> (16 * (k >> 2) + (k & 3))) & 1u ? st[x][k >> 2][k & 3] : -INFINITY;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const bool dead = !((valid >> (16 * (k >> 2) + 4 * g + (k & 3))) & 1u);
+#pragma unroll
+                for (int x = 0; x < VW; x++) {
+                    vx[k][x] = dead ? 0u : vx[k][x];
+                    bad |= B16 ? pa_bad_bf16(vx[k][x]) : pa_bad_f32(__uint_as_float(vx[k][x]));
                 }
             }
         } else {
-            seen = true;
+#pragma unroll
+            for (int x = 0; x < NC; x++) seen[x] = true;
         }
-        pa_softmax(sts, m, l, o);
+#pragma unroll
+        for (int x = 0; x < NC; x++) {
+            float mx = st[x][0][0];
+#pragma unroll
+            for (int k = 1; k < 8; k++) mx = fmaxf(mx, st[x][k >> 2][k & 3]);
+            mx = fmaxf(mx, __uint_as_float(qk_xor16_u(__float_as_uint(mx))));
+            mx = fmaxf(mx, __uint_as_float(qk_xor32_u(__float_as_uint(mx))));
+            if (__any(mx > m[x] + PA_GROW)) {
+                const float mn = fmaxf(m[x], mx), f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[x] - mn);
+                l[x] *= f;
+#pragma unroll
+                for (int e = 0; e < E; e++) o[x][e] *= f;
+                m[x] = mn;
+            }
+            const float ms = m[x] == -INFINITY ? 0.0f : m[x];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float w = __builtin_amdgcn_exp2f(st[x][k >> 2][k & 3] - ms);
+                st[x][k >> 2][k & 3] = w;
+                l[x] += w;
+            }
+        }
         if constexpr (B16) {
+            qm_bf16x8 pw[NC];
 #pragma unroll
-            for (int s = 0; s < 2; s++) {
-                const qm_bf16x8 pw = pa_pack(st, s);
+            for (int x = 0; x < NC; x++)
+                pw[x] = __builtin_bit_cast(qm_bf16x8, make_uint4(qk_cvt_pk_bf16(st[x][0][0], st[x][0][1]), qk_cvt_pk_bf16(st[x][0][2], st[x][0][3]),
+                                                                 qk_cvt_pk_bf16(st[x][1][0], st[x][1][1]), qk_cvt_pk_bf16(st[x][1][2], st[x][1][3])));
 #pragma unroll
-                for (int d = 0; d < E; d++) {
-                    uint32_t w[4];
+            for (int e = 0; e < E; e++) {
+                uint32_t w[4];
 #pragma unroll
-                    for (int x = 0; x < 4; x++)
-                        w[x] = __builtin_amdgcn_perm(vx[8 * s + 2 * x + 1].w[d >> 1], vx[8 * s + 2 * x].w[d >> 1],
-                                                     d & 1 ? 0x07060302u : 0x05040100u);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(qm_bf16x8, make_uint4(w[0], w[1], w[2], w[3])),
-                                                                   pw, o[d], 0, 0, 0);
-                }
+                for (int x = 0; x < 4; x++)
+                    w[x] = __builtin_amdgcn_perm(vx[2 * x + 1][e >> 1], vx[2 * x][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+                const qm_bf16x8 a = __builtin_bit_cast(qm_bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+                for (int x = 0; x < NC; x++) o[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pw[x], o[x][e], 0, 0, 0);
             }
         } else {
 #pragma unroll
-            for (int k = 0; k < 16; k++)
+            for (int k = 0; k < 8; k++)
 #pragma unroll
-                for (int d = 0; d < E; d++)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(vx[k].w[d]), st[k], o[d], 0, 0, 0);
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int x = 0; x < NC; x++)
+                        o[x][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vx[k][e]), st[x][k >> 2][k & 3], o[x][e], 0, 0, 0);
         }
     }
-    l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
-    l = pa_sum(m, l, seen);
-    if (h == 0) ml[wave][c] = make_float2(m, l);
+#pragma unroll
+    for (int x = 0; x < NC; x++) {
+        l[x] += __uint_as_float(qk_xor16_u(__float_as_uint(l[x])));
+        l[x] += __uint_as_float(qk_xor32_u(__float_as_uint(l[x])));
+        l[x] = pa_sum(m[x], l[x], seen[x]);
+        if (g == 0) ml[wave][16 * x + c] = make_float2(m[x], l[x]);
+    }
     if (__syncthreads_or(bad)) {
-        pa_slow<T, HD, PD_RT, PD_KT>(p, u, kt0, kt1, tl, 4);
+        pa_slow<T, HD, RT, PD_KT>(p, u, kt0, kt1, tl, 4);
         return;
     }
-    float M = -INFINITY, L = 0.0f;
+    float M[NC], L[NC], f[NC];
 #pragma unroll
-    for (int w = 0; w < 4; w++) M = fmaxf(M, ml[w][c].x);
+    for (int x = 0; x < NC; x++) {
+        M[x] = -INFINITY;
+        L[x] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
-        const float2 x = ml[w][c];
-        L += x.x == M ? x.y : x.y * __builtin_amdgcn_exp2f(x.x - M);
+        for (int w = 0; w < 4; w++) M[x] = fmaxf(M[x], ml[w][16 * x + c].x);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float2 y = ml[w][16 * x + c];
+            L[x] += y.x == M[x] ? y.y : y.y * __builtin_amdgcn_exp2f(y.x - M[x]);
+        }
+        f[x] = m[x] == M[x] ? 1.0f : __builtin_amdgcn_exp2f(m[x] - M[x]);
     }
-    const float f = m == M ? 1.0f : __builtin_amdgcn_exp2f(m - M);
     for (int w = 0; w < 4; w++) { /* in order, so the sum is the same every time */
-        if (wave == w && c < nrow) {
+        if (wave == w)
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                float *dst = sum + c * LD + (8 * g + 4 * h) * E;
-                float x[4 * E];
+            for (int x = 0; x < NC; x++) {
+                if (16 * x + c >= nrow) continue;
+                float4 *dst = (float4 *)(sum + (16 * x + c) * LD + 4 * g * E);
 #pragma unroll
-                for (int b = 0; b < 4; b++)
-#pragma unroll
-                    for (int d = 0; d < E; d++) x[b * E + d] = o[d][4 * g + b] * f;
-#pragma unroll
-                for (int b = 0; b < E; b++) {
-                    float4 *d4 = (float4 *)dst + b;
-                    float4 y = make_float4(x[4 * b], x[4 * b + 1], x[4 * b + 2], x[4 * b + 3]);
+                for (int k = 0; k < E; k++) { /* dims 4 g E + 4 k ..: element y of tile e at y E + e */
+                    float4 y = make_float4(o[x][(4 * k) % E][4 * k / E] * f[x], o[x][(4 * k + 1) % E][(4 * k + 1) / E] * f[x],
+                                           o[x][(4 * k + 2) % E][(4 * k + 2) / E] * f[x], o[x][(4 * k + 3) % E][(4 * k + 3) / E] * f[x]);
                     if (w) {
-                        const float4 z = *d4;
+                        const float4 z = dst[k];
                         y = make_float4(z.x + y.x, z.y + y.y, z.z + y.z, z.w + y.w);
                     }
-                    *d4 = y;
+                    dst[k] = y;
                 }
             }
-        }
         __syncthreads();
     }
     /* rows of the unit, 4 dims per thread */
-    if (wave == 0 && h == 0) ml[0][c] = make_float2(M, L);
+    if (wave == 0 && g == 0)
+#pragma unroll
+        for (int x = 0; x < NC; x++) ml[0][16 * x + c] = make_float2(M[x], L[x]);
     __syncthreads();
     for (int i = tid; i < nrow * (HD / 4); i += 256) {
         const int rr = i / (HD / 4), d = 4 * (i - rr * (HD / 4));
         const float4 x = *(const float4 *)(sum + rr * LD + d);
         if (u.parts > 1) {
-            qk_st((float4 *)(p.po + ((int64_t)u.slot * PD_RT + rr) * HD + d), x);
+            qk_st((float4 *)(p.po + ((int64_t)u.slot * RT + rr) * HD + d), x);
         } else {
             const int tt = (row0 + rr) / p.G, oh = pa_head(p, u.kh, row0 + rr - tt * p.G);
-            const float g = pa_norm(ml[0][rr].x, ml[0][rr].y);
-            pa_put4((T *)p.a.out + (int64_t)(u.s.start + tt) * p.a.o_token + (int64_t)oh * p.a.o_head + d, x.x * g, x.y * g, x.z * g, x.w * g);
+            const float n = pa_norm(ml[0][rr].x, ml[0][rr].y);
+            pa_put4((T *)p.a.out + (int64_t)(u.s.start + tt) * p.a.o_token + (int64_t)oh * p.a.o_head + d, x.x * n, x.y * n, x.z * n, x.w * n);
         }
     }
-    if (u.parts > 1 && tid < nrow) p.pml[(int64_t)u.slot * PD_RT + tid] = ml[0][tid];
+    if (u.parts > 1 && tid < nrow) p.pml[(int64_t)u.slot * RT + tid] = ml[0][tid];
 }
 
 /* ------------------------------------------------------------ many rows
@@ -757,20 +816,23 @@ static unsigned pa_join_rows(int64_t tasks, int rt) {
     return (unsigned)(r < 1 ? 1 : r > rt ? rt : r);
 }
 
-/* which kernel: rows per sequence past one unit of the few-row kernel, on
- * average, go to the many-row one */
-static bool pa_many(const pg_cache *c, int n, int n_seqs, int h) {
-    return c->dtype == QMOE_BF16 && (int64_t)n * (h / c->kvh) > (int64_t)PD_RT * n_seqs;
+/* Row tile of the few-row kernel (16 or 32), or PM_RT for the many-row one,
+ * by the rows that a sequence has on average. */
+static int pa_rows(const pg_cache *c, int n, int n_seqs, int h) {
+    const int64_t rows = (int64_t)n * (h / c->kvh);
+    if (rows <= (int64_t)16 * n_seqs) return 16;
+    return rows <= (int64_t)32 * n_seqs || c->dtype != QMOE_BF16 ? 32 : PM_RT;
 }
 static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h) {
-    if (pa_many(c, n, n_seqs, h)) return pa_plan(c, n, n_seqs, h, PM_RT, pm_kt(c->hd), 512, 512 / pm_kt(c->hd));
-    return pa_plan(c, n, n_seqs, h, PD_RT, PD_KT, 1024, 8);
+    const int rt = pa_rows(c, n, n_seqs, h);
+    if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, pm_kt(c->hd), 512, 512 / pm_kt(c->hd));
+    return pa_plan(c, n, n_seqs, h, rt, PD_KT, 1024, 8);
 }
 
 static size_t pa_up(size_t v) { return (v + 255) / 256 * 256; }
 extern "C" size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h) {
     const PaPlan q = pa_plan_of(c, n, n_seqs, h);
-    const int rt = pa_many(c, n, n_seqs, h) ? PM_RT : PD_RT;
+    const int rt = pa_rows(c, n, n_seqs, h);
     return 256 + pa_up((size_t)q.slots * rt * 8) + pa_up((size_t)q.slots * rt * c->hd * 4);
 }
 
@@ -790,10 +852,11 @@ static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), void *ws, hipStream_t 
 
 template <typename T, int HD>
 static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
+    const int rt = pa_rows(&p.c, p.a.n, p.a.n_seqs, p.a.h);
     if constexpr (sizeof(T) == 2)
-        if (pa_many(&p.c, p.a.n, p.a.n_seqs, p.a.h))
-            return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD>, ws, st);
-    return pa_launch_rt<T, HD, PD_RT, PD_KT>(p, k_pa_few<T, HD>, ws, st);
+        if (rt == PM_RT) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD>, ws, st);
+    if (rt == 16) return pa_launch_rt<T, HD, 16, PD_KT>(p, k_pa_few<T, HD, 1>, ws, st);
+    return pa_launch_rt<T, HD, 32, PD_KT>(p, k_pa_few<T, HD, 2>, ws, st);
 }
 
 template <typename T>
