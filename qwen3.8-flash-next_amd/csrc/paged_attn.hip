@@ -25,7 +25,7 @@ struct PaArgs {
     pg_cache c;   /* k and v of the call's layer */
     pg_attn a;
     int G;        /* query heads per kv head */
-    int units;    /* units that the call is cut into, about */
+    float per_unit; /* kv heads / units that the call is cut into, rounded up */
     int least;    /* key tiles of a part at the least */
     float *po;    /* partial O [slot, RT, HD], unscaled */
     float2 *pml;  /* [slot, RT]: maximum (log2 units), sum */
@@ -84,90 +84,92 @@ struct PaUnit {
     int slot; /* of the part's partial results */
 };
 
-/* exclusive prefix sums of two values over the workgroup's 256 threads */
-__device__ __forceinline__ int2 pa_scan(int2 v, int2 *lds, int2 &total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int2 x = v;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int a = __shfl_up(x.x, o, QK_WAVE), b = __shfl_up(x.y, o, QK_WAVE);
-        if (lane >= o) {
-            x.x += a;
-            x.y += b;
-        }
-    }
-    if (lane == 63) lds[wave] = x;
-    __syncthreads();
-    int2 before = make_int2(0, 0);
-    total = make_int2(0, 0);
-    for (int w = 0; w < 4; w++) {
-        const int2 t = lds[w];
-        if (w < wave) {
-            before.x += t.x;
-            before.y += t.y;
-        }
-        total.x += t.x;
-        total.y += t.y;
-    }
-    __syncthreads();
-    return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
+/* inclusive prefix sum over the wave */
+__device__ __forceinline__ int pa_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false); /* row_shr:1, 2, 4, 8 within 16 lanes */
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, QK_DPP_ROW_BCAST15, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, QK_DPP_ROW_BCAST31, 0xC, 0xF, false);
+    return v;
 }
 
 /* Unit `want` of the call (JOIN: the want-th (sequence, row tile, kv head)
- * that has parts to join); false past the last.  256 threads, every one of
- * which looks at its share of the sequences. */
+ * that has parts to join); false past the last.  Every wave finds it by
+ * itself, a lane per run of sequences, without LDS or barriers: this stands
+ * before the first load of a page, and a decode call is a few microseconds
+ * long.  The total is summed in fp32, in a fixed order. */
 template <int RT, int KT, bool JOIN>
-__device__ bool pa_find(const PaArgs &p, int want, PaUnit &u) {
-    __shared__ int2 tmp[4];
-    __shared__ long long sums[4];
-    __shared__ int found[4];
-    const int tid = threadIdx.x, n = p.a.n_seqs;
-    auto load = [&](int i) {
-        pg_load l = {0, 0};
-        if (i < n)
-            l = pg_load_of(pg_seq_at(&p.c, p.a.starts, p.a.slots, p.a.n, i), p.G, RT, p.a.window, p.a.sinks, KT);
-        return l;
-    };
-    const pg_load l0 = load(tid);
-    long long t = (long long)l0.row_tiles * l0.key_tiles;
-    for (int i = tid + 256; i < n; i += 256) {
-        const pg_load l = load(i);
-        t += (long long)l.row_tiles * l.key_tiles;
-    }
-    for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o, QK_WAVE);
-    if ((tid & 63) == 0) sums[tid >> 6] = t;
-    if (tid == 0) found[0] = -1;
-    __syncthreads();
-    const int share = pg_share((sums[0] + sums[1] + sums[2] + sums[3]) * p.c.kvh, p.units, p.least);
-    int2 base = make_int2(0, 0); /* units (tasks to join), split units before the chunk */
-    for (int c = 0; c < n; c += 256) {
-        const pg_load l = c ? load(c + tid) : l0;
-        const int parts = pg_parts(l.key_tiles, share), tasks = l.row_tiles * p.c.kvh;
-        const int split = parts > 1 ? tasks * parts : 0;
-        const int mine = JOIN ? (parts > 1 ? tasks : 0) : tasks * parts;
-        int2 total;
-        const int2 at = pa_scan(make_int2(mine, split), tmp, total);
-        if (want >= base.x + at.x && want < base.x + at.x + mine) {
-            found[0] = c + tid;
-            found[1] = want - base.x - at.x;
-            found[2] = base.y + at.y;
-            found[3] = parts;
+__device__ __forceinline__ bool pa_find(const PaArgs &p, int want, PaUnit &u) {
+    const int lane = threadIdx.x & 63, n = p.a.n_seqs, per = (n + 63) >> 6;
+    auto seq = [&](int i) { return pg_seq_at(&p.c, p.a.starts, p.a.slots, p.a.n, i); };
+    auto load = [&](const pg_seq &s) { return pg_load_of(s, p.G, RT, p.a.window, p.a.sinks, KT); };
+    pg_seq s0 = {-1, 0, 0, 0};
+    pg_load l0 = {0, 0};
+    float t = 0.0f;
+    for (int k = 0; k < per; k++) {
+        const int i = lane * per + k;
+        if (i < n) {
+            s0 = seq(i);
+            l0 = load(s0);
+            t += (float)l0.row_tiles * (float)l0.key_tiles;
         }
-        base.x += total.x;
-        base.y += total.y;
-        if (want < base.x) break;
     }
-    __syncthreads();
-    const int i = __builtin_amdgcn_readfirstlane(found[0]);
-    if (i < 0) return false;
-    const int local = __builtin_amdgcn_readfirstlane(found[1]);
-    u.parts = __builtin_amdgcn_readfirstlane(found[3]);
-    u.s = pg_seq_at(&p.c, p.a.starts, p.a.slots, p.a.n, i);
-    const int rtiles = (u.s.count * p.G + RT - 1) / RT, q = local / p.c.kvh;
-    u.kh = local - q * p.c.kvh;
+    t = qk_group_sum<64>(t);
+    const int share = pg_share(t, p.per_unit, p.least);
+    auto count = [&](const pg_load &l, int &parts, int &units, int &split) {
+        parts = pg_parts(l.key_tiles, share);
+        const int tasks = l.row_tiles * p.c.kvh;
+        split = parts > 1 ? tasks * parts : 0;
+        units = JOIN ? (parts > 1 ? tasks : 0) : tasks * parts;
+    };
+    int parts = 1, units = 0, split = 0;
+    if (per == 1) {
+        count(l0, parts, units, split);
+    } else {
+        for (int k = 0; k < per; k++) {
+            const int i = lane * per + k;
+            if (i < n) {
+                int a, b, c;
+                count(load(seq(i)), a, b, c);
+                units += b;
+                split += c;
+            }
+        }
+    }
+    const int ue = pa_scan(units) - units, se = pa_scan(split) - split;
+    const uint64_t here = __ballot(want >= ue && want < ue + units);
+    if (!here) return false;
+    const int at = __builtin_ctzll(here);
+    int ubase = __builtin_amdgcn_readlane(ue, at), sbase = __builtin_amdgcn_readlane(se, at);
+    if (per == 1) {
+        u.parts = __builtin_amdgcn_readlane(parts, at);
+        u.s.slot = __builtin_amdgcn_readlane(s0.slot, at);
+        u.s.start = __builtin_amdgcn_readlane(s0.start, at);
+        u.s.count = __builtin_amdgcn_readlane(s0.count, at);
+        u.s.len = __builtin_amdgcn_readlane(s0.len, at);
+    } else {
+        for (int k = 0; k < per; k++) {
+            const pg_seq s = seq(min(at * per + k, n - 1));
+            count(load(s), parts, units, split);
+            u.parts = __builtin_amdgcn_readfirstlane(parts);
+            u.s.slot = __builtin_amdgcn_readfirstlane(s.slot);
+            u.s.start = __builtin_amdgcn_readfirstlane(s.start);
+            u.s.count = __builtin_amdgcn_readfirstlane(s.count);
+            u.s.len = __builtin_amdgcn_readfirstlane(s.len);
+            const int nu = __builtin_amdgcn_readfirstlane(units);
+            if (want < ubase + nu) break;
+            ubase += nu;
+            sbase += __builtin_amdgcn_readfirstlane(split);
+        }
+    }
+    const int rtiles = (u.s.count * p.G + RT - 1) / RT, q = (want - ubase) / p.c.kvh;
+    u.kh = want - ubase - q * p.c.kvh;
     const int back = JOIN ? q : q / u.parts;
     u.part = JOIN ? 0 : q - back * u.parts;
     u.rtile = rtiles - 1 - back;
-    u.slot = __builtin_amdgcn_readfirstlane(found[2]) + (back * u.parts + u.part) * p.c.kvh + u.kh;
+    u.slot = sbase + (back * u.parts + u.part) * p.c.kvh + u.kh;
     return true;
 }
 
@@ -561,6 +563,29 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
     if (u.parts > 1 && tid < nrow) p.pml[(int64_t)u.slot * RT + tid] = ml[0][tid];
 }
 
+/* a row of a 32-wide unit, held by lanes l and l + 32: the output, or the
+ * part's results */
+#define PM_RT 128
+template <typename T, int HD>
+__device__ __forceinline__ void pa_store(const PaArgs &p, const PaUnit &u, const qm_f32x16 (&o)[HD / 32], float m, float l, bool seen, int rr,
+                                         int t, int hh) {
+    const int h = (threadIdx.x >> 5) & 1;
+    l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
+    l = pa_sum(m, l, seen);
+    const float f = u.parts > 1 ? 1.0f : pa_norm(m, l);
+    T *out = (T *)p.a.out + (int64_t)(u.s.start + t) * p.a.o_token + (int64_t)hh * p.a.o_head + 4 * h;
+    float *po = p.po + ((int64_t)u.slot * PM_RT + rr) * HD + 4 * h;
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const float4 y = make_float4(o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f);
+            if (u.parts > 1) qk_st((float4 *)(po + 32 * d + 8 * g), y);
+            else pa_put4(out + 32 * d + 8 * g, y.x, y.y, y.z, y.w);
+        }
+    if (u.parts > 1 && h == 0) p.pml[(int64_t)u.slot * PM_RT + rr] = make_float2(m, l);
+}
+
 /* ------------------------------------------------------------ many rows
  * Prompts, bf16: a unit is 128 rows, 32 per wave, and a part of the keys.
  * Tiles of KT keys of K and V are copied straight from the pages to LDS, two
@@ -572,13 +597,12 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
  * query is copied from a piece of zeros.
  * Bound: matrix cores and, next to them, LDS (each wave reads the whole tile
  * for 32 rows) and the exponentials. */
-#define PM_RT 128
 #define PM_CHUNK 1024
 __device__ const uint4 pa_zero = {0, 0, 0, 0};
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pa_s16x4 *pa_tptr;
 
-constexpr int pm_kt(int hd) { return hd <= 128 ? 64 : 32; }
+constexpr int pm_kt(int hd, bool f32 = false) { return hd <= 128 && !f32 ? 64 : 32; }
 
 template <int HD>
 __global__ __launch_bounds__(256, 2) void k_pa_many(PaArgs p) {
@@ -603,7 +627,7 @@ __global__ __launch_bounds__(256, 2) void k_pa_many(PaArgs p) {
     const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
 
     auto look = [&](int i0) { /* rows of the tiles i0.. of the part */
-        for (int k = tid; k < PM_CHUNK; k += 256) {
+        for (int k = tid; k < min(PM_CHUNK, (nt - i0) * KT); k += 256) {
             const int i = kt0 + i0 + k / KT;
             const int j = i < kt1 ? pg_tile(tl, i) * KT + k % KT : -1;
             where[k] = j >= 0 && j <= p1 ? pg_row_at(&p.c, row, j) : -1;
@@ -713,71 +737,261 @@ __global__ __launch_bounds__(256, 2) void k_pa_many(PaArgs p) {
         pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 4);
         return;
     }
-    l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
-    l = pa_sum(m, l, seen);
-    if (c >= wn) return;
-    if (u.parts > 1) {
-        const int64_t at = (int64_t)u.slot * PM_RT + 32 * wave + c;
+    if (c < wn) pa_store<T, HD>(p, u, o, m, l, seen, 32 * wave + c, t, hh);
+}
+
+/* ------------------------------------------------------------ many rows, f32
+ * The same unit at fp32 precision: K, V, Q and the weights as three bf16
+ * parts each (hi + mid + lo, 24 bits) and six of the nine partial products
+ * (the others are below 2^-24 of them), which run at 417 TFLOP/s against 157
+ * of the fp32 instructions.  A tile is 32 keys; its rows come through
+ * registers, where the workgroup splits them once for its four waves, into
+ * one LDS buffer for K and one for V: V is written while the scores are
+ * formed, the next tile's K while V is multiplied, one barrier after each.  Values past PA_BIG, infinities and NaN have no parts; their
+ * units take the one-row path.
+ * Bound: matrix cores, six products per tile. */
+#define PA_BIG 1e15f /* parts, products and sums of values up to this stay finite */
+
+/* eight fp32 -> three bf16 parts */
+__device__ __forceinline__ void pa_split8(const float x[8], uint4 w[3]) {
+    float r[8];
 #pragma unroll
-        for (int d = 0; d < E; d++)
+    for (int j = 0; j < 8; j++) r[j] = x[j];
 #pragma unroll
-            for (int g = 0; g < 4; g++)
-                qk_st((float4 *)(p.po + at * HD + 32 * d + 8 * g + 4 * h), make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]));
-        if (h == 0) p.pml[at] = make_float2(m, l);
-        return;
+    for (int i = 0; i < 3; i++) {
+        uint32_t v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            v[j] = qk_cvt_pk_bf16(r[2 * j], r[2 * j + 1]);
+            r[2 * j] -= qk_bf16_lo(v[j]);
+            r[2 * j + 1] -= qk_bf16_hi(v[j]);
+        }
+        w[i] = make_uint4(v[0], v[1], v[2], v[3]);
     }
-    const float f = pa_norm(m, l);
-    T *out = (T *)p.a.out + (int64_t)(u.s.start + t) * p.a.o_token + (int64_t)hh * p.a.o_head;
+}
+__device__ __forceinline__ bool pa_big8(const float x[8]) {
+    bool b = false;
+#pragma unroll
+    for (int j = 0; j < 8; j++) b |= !(fabsf(x[j]) <= PA_BIG);
+    return b;
+}
+/* sum of a * b over the parts, the smallest products first */
+__device__ __forceinline__ qm_f32x16 pa_mfma6(const uint4 a[3], const uint4 b[3], qm_f32x16 c) {
+    constexpr int ia[6] = {2, 1, 0, 1, 0, 0}, ib[6] = {0, 1, 2, 0, 1, 0};
+#pragma unroll
+    for (int i = 0; i < 6; i++)
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(qm_bf16x8, a[ia[i]]), __builtin_bit_cast(qm_bf16x8, b[ib[i]]), c, 0, 0, 0);
+    return c;
+}
+
+template <int HD>
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_many32(PaArgs p) {
+    typedef float T;
+    constexpr int KT = 32, CR = HD / 8, NB = KT * CR / 256, E = HD / 32, KS = HD / 16;
+    __shared__ __attribute__((aligned(16))) uint4 kv[2][3][KT * CR];
+    __shared__ int64_t where[PM_CHUNK];
+    PaUnit u;
+    if (!pa_find<PM_RT, KT, false>(p, blockIdx.x, u)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, h = lane >> 5;
+    const int row0 = u.rtile * PM_RT, rows = u.s.count * p.G, nrow = min(PM_RT, rows - row0);
+    const int first = u.s.len - u.s.count;
+    const int p0 = first + row0 / p.G, p1 = first + (row0 + nrow - 1) / p.G;
+    const pg_tiles tl = pg_tiles_of(p0, p1, p.a.window, p.a.sinks, KT);
+    const int kt0 = pg_part(tl.nt, u.part, u.parts), kt1 = pg_part(tl.nt, u.part + 1, u.parts), nt = kt1 - kt0;
+    /* this wave's rows; a wave past the last row loads and waits only */
+    const int w0 = row0 + 32 * wave, wn = min(32, rows - w0);
+    const int pw0 = first + w0 / p.G, pw1 = first + (w0 + wn - 1) / p.G;
+    const int r = min(w0 + c, rows - 1), t = r / p.G, pos = first + t;
+    const int hh = pa_head(p, u.kh, r - t * p.G);
+    const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
+    const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
+    auto look = [&](int i0) { /* rows of the tiles i0.. of the part */
+        for (int k = tid; k < min(PM_CHUNK, (nt - i0) * KT); k += 256) {
+            const int i = kt0 + i0 + k / KT;
+            const int j = i < kt1 ? pg_tile(tl, i) * KT + k % KT : -1;
+            where[k] = j >= 0 && j <= p1 ? pg_row_at(&p.c, row, j) : -1;
+        }
+        __syncthreads();
+    };
+    float4 kx[NB][2], vx[NB][2];
+    uint32_t vnext = 0;
+    bool bad = false;
+    auto load = [&](int i) { /* tile i into registers; rows without a page as zeros */
+        const int64_t *wh = where + i % (PM_CHUNK / KT) * KT;
+#pragma unroll
+        for (int x = 0; x < NB; x++) {
+            const int L = x * 256 + tid, rr = L / CR, pc = L - rr * CR;
+            const int64_t at = wh[rr], safe = at < 0 ? 0 : at;
+            const float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                const float4 a = qk_ld((const float4 *)(kp + safe + 8 * pc) + y), b = qk_ld((const float4 *)(vp + safe + 8 * pc) + y);
+                kx[x][y] = at < 0 ? z : a;
+                vx[x][y] = at < 0 ? z : b;
+            }
+        }
+        vnext = (uint32_t)__ballot(wh[lane & 31] >= 0);
+    };
+    auto put = [&](int which, const float4 (&src)[NB][2]) {
+#pragma unroll
+        for (int x = 0; x < NB; x++) {
+            const int L = x * 256 + tid, rr = L / CR, pc = L - rr * CR;
+            const int at = rr * CR + (pc ^ (which ? ((rr & 3) << 1) | ((rr >> 2) & 1) : rr & 7));
+            const float v[8] = {src[x][0].x, src[x][0].y, src[x][0].z, src[x][0].w, src[x][1].x, src[x][1].y, src[x][1].z, src[x][1].w};
+            uint4 w[3];
+            bad |= pa_big8(v);
+            pa_split8(v, w);
+#pragma unroll
+            for (int y = 0; y < 3; y++) kv[which][y][at] = w[y];
+        }
+    };
+    if (nt > 0) {
+        look(0);
+        load(0);
+    }
+    uint4 q[KS][3];
+    {
+        const T *src = (const T *)p.a.q + (int64_t)(u.s.start + t) * p.a.q_token + (int64_t)hh * p.a.q_head + h * 8;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            float x[8];
+            pa_get8(src + s * 16, x);
+            bad |= pa_big8(x);
+            pa_split8(x, q[s]);
+        }
+    }
+    float m = -INFINITY, l = 0.0f;
+    bool seen = false;
+    qm_f32x16 o[E];
 #pragma unroll
     for (int d = 0; d < E; d++)
 #pragma unroll
-        for (int g = 0; g < 4; g++)
-            pa_put4(out + 32 * d + 8 * g + 4 * h, o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f);
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    const int j = lane & 15, g16 = (lane >> 4) & 1, fv = ((j >> 2) << 1) | h;
+    if (nt > 0) put(0, kx);
+    qk_lds_barrier();
+    for (int i = 0; i < nt; i++) {
+        const uint32_t valid = vnext;
+        /* K of tile i is in LDS, and every wave is done with V of tile i - 1 */
+        put(1, vx);
+        if (i + 1 < nt) {
+            if ((i + 1) % (PM_CHUNK / KT) == 0) look(i + 1);
+            load(i + 1);
+        }
+        const int base = pg_tile(tl, kt0 + i) * KT;
+        const bool act = wn > 0 && base <= pw1 && !(p.a.window > 0 && base + KT <= pg_lo(pw0, p.a.window) && base >= p.a.sinks);
+        qm_f32x16 st[1];
+        if (act) {
+            const uint4 *kb = kv[0][0];
+#pragma unroll
+            for (int x = 0; x < 16; x++) st[0][x] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                uint4 a[3];
+#pragma unroll
+                for (int y = 0; y < 3; y++) a[y] = kb[y * KT * CR + c * CR + 8 * (s >> 2) + ((2 * (s & 3) + h) ^ (c & 7))];
+                st[0] = pa_mfma6(a, q[s], st[0]);
+            }
+#pragma unroll
+            for (int x = 0; x < 16; x++) st[0][x] *= p.a.scale;
+            if (valid == 0xFFFFFFFFu && pa_full(p, pw0, pw1, base)) {
+                seen = true;
+            } else {
+                uint32_t mw = pa_mask(p, pos, base) & valid;
+                seen |= mw != 0;
+                mw >>= 4 * h;
+#pragma unroll
+                for (int x = 0; x < 16; x++) st[0][x] = (mw >> (8 * (x >> 2) + (x & 3))) & 1u ? st[0][x] : -INFINITY;
+            }
+            pa_softmax(st, m, l, o);
+        }
+        qk_lds_barrier(); /* V is in LDS, and every wave has its scores */
+        if (i + 1 < nt) put(0, kx);
+        if (act) {
+            const uint4 *vb = kv[1][0];
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const float x[8] = {st[0][8 * s], st[0][8 * s + 1], st[0][8 * s + 2], st[0][8 * s + 3],
+                                    st[0][8 * s + 4], st[0][8 * s + 5], st[0][8 * s + 6], st[0][8 * s + 7]};
+                uint4 pw[3];
+                pa_split8(x, pw);
+                const int key = 16 * s + 4 * h + (j >> 2);
+#pragma unroll
+                for (int d = 0; d < E; d++) {
+                    const int pc = 8 * (d >> 1) + ((4 * (d & 1) + 2 * g16 + ((j & 3) >> 1)) ^ fv);
+                    uint4 a[3];
+#pragma unroll
+                    for (int y = 0; y < 3; y++) {
+                        const pa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_tptr)((const short *)(vb + y * KT * CR + key * CR + pc) + 4 * (j & 1)));
+                        const pa_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_tptr)((const short *)(vb + y * KT * CR + (key + 8) * CR + pc) + 4 * (j & 1)));
+                        const uint2 aw = __builtin_bit_cast(uint2, lo), bw = __builtin_bit_cast(uint2, hi);
+                        a[y] = make_uint4(aw.x, aw.y, bw.x, bw.y);
+                    }
+                    o[d] = pa_mfma6(a, pw, o[d]);
+                }
+            }
+        }
+        qk_lds_barrier();
+    }
+    if (__syncthreads_or(bad)) {
+        pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 4);
+        return;
+    }
+    if (c < wn) pa_store<T, HD>(p, u, o, m, l, seen, 32 * wave + c, t, hh);
 }
 
 /* ------------------------------------------------------------ join
- * A workgroup takes rows of a task: its four waves the parts in turn, lane =
- * dims, then a sum in wave order.  Bound: the parts read once, and for few
- * rows the latency of the loads. */
+ * Rows of a task whose keys were cut into parts: lane = dims, up to PJ_FEW
+ * parts a wave per row, more the four waves on one row, the parts in turn,
+ * then a sum in wave order.  Bound: the parts read once, and for few rows the
+ * latency of the loads. */
+#define PJ_FEW 16
+template <typename T, int HD>
+__device__ __forceinline__ void pa_join_out(const PaArgs &p, const PaUnit &u, int r, int d, float4 y, float f) {
+    const int t = r / p.G, hh = pa_head(p, u.kh, r - t * p.G);
+    pa_put4((T *)p.a.out + (int64_t)(u.s.start + t) * p.a.o_token + (int64_t)hh * p.a.o_head + d, y.x * f, y.y * f, y.z * f, y.w * f);
+}
+
 template <typename T, int HD, int RT, int KT>
 __global__ __launch_bounds__(256) void k_pa_join(PaArgs p) {
-    constexpr int E = HD / 64;
-    __shared__ float acc[4][HD];
+    constexpr int Q = HD / 4; /* lanes of 4 dims */
+    __shared__ __attribute__((aligned(16))) float acc[4][HD];
     __shared__ float lsum[4];
     PaUnit u;
     if (!pa_find<RT, KT, true>(p, blockIdx.x, u)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int rr = blockIdx.y; rr < min(RT, u.s.count * p.G - u.rtile * RT); rr += gridDim.y) {
+    const bool few = u.parts <= PJ_FEW;
+    const int step = few ? 1 : 4, i0 = few ? 0 : wave;
+    for (int rr = few ? blockIdx.y * 4 + wave : blockIdx.y; rr < min(RT, u.s.count * p.G - u.rtile * RT); rr += gridDim.y * (few ? 4 : 1)) {
         auto at = [&](int i) { return (int64_t)(u.slot + i * p.c.kvh) * RT + rr; };
         float M = -INFINITY;
         for (int i = lane; i < u.parts; i += 64) M = fmaxf(M, qk_ld((const float *)(p.pml + at(i))));
         for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, QK_WAVE));
-        float L = 0.0f, x[E];
-#pragma unroll
-        for (int e = 0; e < E; e++) x[e] = 0.0f;
-#pragma unroll 4
-        for (int i = wave; i < u.parts; i += 4) {
+        float L = 0.0f;
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+        for (int i = i0; i < u.parts; i += step) {
             const float pm = qk_ld((const float *)(p.pml + at(i))), pl = qk_ld((const float *)(p.pml + at(i)) + 1);
+            const float4 x = qk_ld((const float4 *)(p.po + at(i) * HD + 4 * (lane % Q)));
             const float f = pm == M ? 1.0f : __builtin_amdgcn_exp2f(pm - M);
             L = fmaf(pl, f, L);
-#pragma unroll
-            for (int e = 0; e < E; e++) x[e] = fmaf(qk_ld(p.po + at(i) * HD + lane + 64 * e), f, x[e]);
+            y = make_float4(fmaf(x.x, f, y.x), fmaf(x.y, f, y.y), fmaf(x.z, f, y.z), fmaf(x.w, f, y.w));
         }
-#pragma unroll
-        for (int e = 0; e < E; e++) acc[wave][lane + 64 * e] = x[e];
+        if (few) {
+            if (lane < Q) pa_join_out<T, HD>(p, u, u.rtile * RT + rr, 4 * lane, y, pa_norm(M, L));
+            continue;
+        }
+        if (lane < Q) *(float4 *)(acc[wave] + 4 * lane) = y;
         if (lane == 0) lsum[wave] = L;
         __syncthreads();
-        if (tid < HD / 4) {
-            const float f = pa_norm(M, lsum[0] + lsum[1] + lsum[2] + lsum[3]);
-            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (tid < Q) {
+            y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < 4; w++) {
                 const float4 z = *(const float4 *)(acc[w] + 4 * tid);
                 y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
             }
-            const int r = u.rtile * RT + rr, t = r / p.G, hh = pa_head(p, u.kh, r - t * p.G);
-            pa_put4((T *)p.a.out + (int64_t)(u.s.start + t) * p.a.o_token + (int64_t)hh * p.a.o_head + 4 * tid, y.x * f, y.y * f,
-                    y.z * f, y.w * f);
+            pa_join_out<T, HD>(p, u, u.rtile * RT + rr, 4 * tid, y, pa_norm(M, lsum[0] + lsum[1] + lsum[2] + lsum[3]));
         }
         __syncthreads();
     }
@@ -809,10 +1023,10 @@ static PaPlan pa_plan(const pg_cache *c, int n, int n_seqs, int h, int rt, int k
     return q;
 }
 
-/* workgroups that share a task's rows: about 1024 in all, where the tasks are
+/* workgroups that share a task's rows: about 2048 in all, where the tasks are
  * few every row has its own */
 static unsigned pa_join_rows(int64_t tasks, int rt) {
-    const int64_t r = 1024 / tasks;
+    const int64_t r = 2048 / tasks;
     return (unsigned)(r < 1 ? 1 : r > rt ? rt : r);
 }
 
@@ -821,11 +1035,12 @@ static unsigned pa_join_rows(int64_t tasks, int rt) {
 static int pa_rows(const pg_cache *c, int n, int n_seqs, int h) {
     const int64_t rows = (int64_t)n * (h / c->kvh);
     if (rows <= (int64_t)16 * n_seqs) return 16;
-    return rows <= (int64_t)32 * n_seqs || c->dtype != QMOE_BF16 ? 32 : PM_RT;
+    return rows <= (int64_t)32 * n_seqs ? 32 : PM_RT;
 }
 static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h) {
     const int rt = pa_rows(c, n, n_seqs, h);
-    if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, pm_kt(c->hd), 512, 512 / pm_kt(c->hd));
+    const int kt = pm_kt(c->hd, c->dtype == QMOE_F32);
+    if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, kt, 512, 512 / kt);
     return pa_plan(c, n, n_seqs, h, rt, PD_KT, 1024, 8);
 }
 
@@ -839,7 +1054,7 @@ extern "C" size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h) {
 template <typename T, int HD, int RT, int KT>
 static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), void *ws, hipStream_t st) {
     const PaPlan q = pa_plan_of(&p.c, p.a.n, p.a.n_seqs, p.a.h);
-    p.units = q.units;
+    p.per_unit = pg_per_unit(p.c.kvh, q.units);
     p.least = q.least;
     p.pml = (float2 *)ws;
     p.po = (float *)((char *)ws + pa_up((size_t)q.slots * RT * 8));
@@ -853,8 +1068,10 @@ static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), void *ws, hipStream_t 
 template <typename T, int HD>
 static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
     const int rt = pa_rows(&p.c, p.a.n, p.a.n_seqs, p.a.h);
-    if constexpr (sizeof(T) == 2)
-        if (rt == PM_RT) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD>, ws, st);
+    if (rt == PM_RT) {
+        if constexpr (sizeof(T) == 2) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD>, ws, st);
+        else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD>, ws, st);
+    }
     if (rt == 16) return pa_launch_rt<T, HD, 16, PD_KT>(p, k_pa_few<T, HD, 1>, ws, st);
     return pa_launch_rt<T, HD, 32, PD_KT>(p, k_pa_few<T, HD, 2>, ws, st);
 }

@@ -109,10 +109,15 @@ QK_HD static inline pg_load pg_load_of(pg_seq s, int G, int rt, int window, int 
     }
     return l;
 }
-/* key tiles per unit, such that about `units` of them cover the call */
-QK_HD static inline int pg_share(int64_t total, int units, int least) {
-    const int64_t s = (total + units - 1) / units;
-    return s < least ? least : s > 0x7FFFFFFF ? 0x7FFFFFFF : (int)s;
+/* Key tiles per part, such that the parts of all tasks number at most `units`
+ * + tasks: total = the sum of row_tiles * key_tiles over the sequences and
+ * per_unit = pg_per_unit(kv heads, units).  fp32 sums of 1024 terms and a tree
+ * are off by less than 2^-13.9, which the factor in per_unit covers. */
+QK_HD static inline float pg_per_unit(int kvh, int units) { return 1.0001f * (float)kvh / (float)units; }
+QK_HD static inline int pg_share(float total, float per_unit, int least) {
+    const float s = total * per_unit;
+    const int n = (s < 1e9f ? (int)s : 1000000000) + 1;
+    return n < least ? least : n;
 }
 QK_HD static inline int pg_parts(int key_tiles, int share) {
     return key_tiles <= share ? 1 : (key_tiles + share - 1) / share;

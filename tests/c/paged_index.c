@@ -113,7 +113,8 @@ static void units(void) {
         const int G = 1 + rnd() % 12, rt = rnd() % 2 ? 32 : 128, kt = 64, window = rnd() % 2 ? 100 : 0, sinks = rnd() % 20;
         const int n_seqs = 1 + rnd() % 6, want = 1 + rnd() % 600;
         pg_seq s[6];
-        int64_t total = 0, n_units = 0, tasks = 0, split = 0, rows = 0;
+        float total = 0.0f;
+        int64_t n_units = 0, tasks = 0, split = 0, rows = 0;
         for (int i = 0; i < n_seqs; i++) {
             s[i].slot = s[i].start = 0;
             s[i].count = rnd() % 300;
@@ -121,9 +122,9 @@ static void units(void) {
             rows += s[i].count;
             const pg_load l = pg_load_of(s[i], G, rt, window, sinks, kt);
             CHECK(l.row_tiles == (s[i].count * G + rt - 1) / rt, "row tiles");
-            total += (int64_t)l.row_tiles * l.key_tiles;
+            total += (float)l.row_tiles * (float)l.key_tiles;
         }
-        const int share = pg_share(total, want, 1 + rnd() % 8);
+        const int share = pg_share(total, pg_per_unit(1, want), 1 + rnd() % 8);
         for (int i = 0; i < n_seqs; i++) {
             const pg_load l = pg_load_of(s[i], G, rt, window, sinks, kt);
             const int parts = pg_parts(l.key_tiles, share);
