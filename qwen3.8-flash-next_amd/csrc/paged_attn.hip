@@ -1041,7 +1041,9 @@ static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h) {
     const int rt = pa_rows(c, n, n_seqs, h);
     const int kt = pm_kt(c->hd, c->dtype == QMOE_F32);
     if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, kt, 512, 512 / kt);
-    return pa_plan(c, n, n_seqs, h, rt, PD_KT, 1024, 8);
+    /* tables of up to 16 tiles (512 rows) are not cut: the join's launch costs
+     * more than the shorter run of tiles gives */
+    return pa_plan(c, n, n_seqs, h, rt, PD_KT, 1024, c->cap <= 16 * PD_KT ? 17 : 8);
 }
 
 static size_t pa_up(size_t v) { return (v + 255) / 256 * 256; }

@@ -194,7 +194,8 @@ __device__ __forceinline__ void pg_refuse(const PgReserve &a, int status) {
 }
 
 __global__ __launch_bounds__(1024) void k_pg_reserve(PgReserve a) {
-    __shared__ int slot_of[PG_MAX_BATCH], part_of[PG_MAX_BATCH], base_of[PG_MAX_BATCH], first_of[PG_MAX_BATCH];
+    __shared__ __attribute__((aligned(16))) int slot_of[PG_MAX_BATCH], part_of[PG_MAX_BATCH];
+    __shared__ int base_of[PG_MAX_BATCH], first_of[PG_MAX_BATCH];
     __shared__ int tmp[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int R = (int)a.c.page_rows.d;
@@ -222,16 +223,25 @@ __global__ __launch_bounds__(1024) void k_pg_reserve(PgReserve a) {
     part_of[tid] = part;
     __syncthreads();
     /* the same slot twice; how many of the batch write to this page, and
-     * whether a later one does */
-    int writers = 0;
-    bool later = false;
-    if (live)
-        for (int j = 0; j < a.n; j++) {
-            bad |= j != tid && slot_of[j] == slot;
-            const bool same = part >= 0 && part_of[j] == part;
-            writers += same;
-            later |= same && j > tid;
+     * whether a later one does.  Four of the batch per LDS read, counts in
+     * place of truth values: 256 sequences one at a time made the kernel 39 us
+     * long instead of 13. */
+    int named = 0, writers = 0, last = 0;
+    if (live) {
+#pragma unroll 4
+        for (int j = 0; j < a.n; j += 4) {
+            const int4 sl = *(const int4 *)(slot_of + j), pt = *(const int4 *)(part_of + j);
+            const int s4[4] = {sl.x, sl.y, sl.z, sl.w}, p4[4] = {pt.x, pt.y, pt.z, pt.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                named += s4[k] == slot;
+                writers += p4[k] == part;
+                last = p4[k] == part ? j + k : last;
+            }
         }
+        bad |= named != 1;
+    }
+    const bool later = last > tid;
     if (__syncthreads_or(bad)) {
         pg_refuse(a, -1);
         return;
@@ -381,6 +391,48 @@ __global__ __launch_bounds__(256) void k_pg_fork_write(PgFork a) {
     if (tid == 0) a.c.lens[d] = len;
 }
 
+/* The same in one launch, one workgroup, for batches whose entries fit LDS:
+ * four branches of a short prompt. */
+#define PG_FORK_SMALL 12288
+__global__ __launch_bounds__(1024) void k_pg_fork_small(PgFork a) {
+    __shared__ int32_t entries[PG_FORK_SMALL];
+    __shared__ int dst[PG_MAX_BATCH], len_of[PG_MAX_BATCH];
+    const int tid = threadIdx.x, W = a.c.max_pages, R = (int)a.c.page_rows.d;
+    bool bad = false;
+    if (tid < a.n) {
+        const int s = qk_ld(a.src + tid), d = qk_ld(a.dst + tid);
+        bad = s < 0 || s >= a.c.n_slots || d < 0 || d >= a.c.n_slots;
+        int len = bad ? 0 : min(max(qk_ld(a.c.lens + s), 0), a.c.cap);
+        if (a.rows) len = min(max(qk_ld(a.rows + tid), 0), len);
+        dst[tid] = d;
+        len_of[tid] = len;
+    }
+    __syncthreads();
+    if (tid < a.n)
+        for (int j = 0; j < a.n; j++) bad |= j != tid && dst[j] == dst[tid];
+    if (__syncthreads_or(bad)) {
+        if (tid == 0) *a.status = -1;
+        return;
+    }
+    for (int x = tid; x < a.n * W; x += 1024) {
+        const int i = x / W, e = x - i * W;
+        const bool keep = e < (int)pg_div_of(a.c.page_rows, (uint32_t)(len_of[i] + R - 1));
+        entries[x] = keep ? qk_ld(a.c.table + qk_ld(a.src + i) * a.c.table_stride + e) : -1;
+    }
+    __syncthreads();
+    for (int x = tid; x < a.n * W; x += 1024) {
+        const int i = x / W, e = x - i * W;
+        int32_t *at = a.c.table + dst[i] * a.c.table_stride + e;
+        const int was = qk_ld(at), now = entries[x];
+        if (was == now) continue;
+        if (was >= 0 && was < a.c.n_pages) atomicSub(a.c.refs + was, 1);
+        if (now >= 0 && now < a.c.n_pages) atomicAdd(a.c.refs + now, 1);
+        *at = now;
+    }
+    if (tid < a.n) a.c.lens[dst[tid]] = len_of[tid];
+    if (tid == 0) *a.status = 0;
+}
+
 extern "C" size_t qk_pg_fork_ws(const pg_cache *c, int n_seqs) {
     return pg_up((size_t)n_seqs * 8) + pg_up((size_t)n_seqs * c->max_pages * 4);
 }
@@ -393,6 +445,10 @@ extern "C" int qk_launch_pg_fork(const pg_cache *c, const int32_t *src, const in
     a.src = src; a.dst = dst; a.rows = rows; a.n = n_seqs; a.status = status;
     a.head = (int2 *)ws;
     a.entries = (int32_t *)((char *)ws + pg_up((size_t)n_seqs * 8));
+    if ((int64_t)n_seqs * c->max_pages <= PG_FORK_SMALL) {
+        hipLaunchKernelGGL(k_pg_fork_small, dim3(1), dim3(1024), 0, st, a);
+        return QK_CHECK_LAUNCH();
+    }
     if (n_seqs > 0) {
         hipLaunchKernelGGL(k_pg_fork_read, dim3(n_seqs), dim3(256), 0, st, a);
         const int rc = QK_CHECK_LAUNCH();

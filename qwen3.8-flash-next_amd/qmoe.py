@@ -1050,6 +1050,9 @@ class PagedCache:
             raise QmoeError("the head dim of k and v must be contiguous")
         self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
         self.device, self.dtype = k.device, k.dtype
+        self._torch, self._i32, self._u8 = torch, torch.int32, torch.uint8
+        self._own = (k.dtype,)  # types of q and out, and of appended rows
+        self._src = (k.dtype,) if k.dtype == torch.float32 else (k.dtype, torch.float32)
         for nm, t, shape in (("v", v, v.shape), ("table", table, (lens.numel(), table.shape[-1])),
                              ("lens", lens, (lens.numel(),)), ("refs", refs, (k.shape[1],))):
             if t.device != self.device or tuple(t.shape) != tuple(shape):
@@ -1076,41 +1079,34 @@ class PagedCache:
                    torch.zeros(n_pages, dtype=torch.int32, device=device))
 
     # -- the call's device, stream and small arguments
-    def _stream(self, stream):
-        import torch
-        if stream is None:
-            return torch.cuda.current_stream(self.device).cuda_stream
-        return stream if isinstance(stream, int) else stream.cuda_stream
-
-    def _place(self, stream):
-        """the cache's device as the current one, and the call's stream as
-        torch's, so that what the call allocates belongs to that stream"""
-        import contextlib
-        import torch
+    def _on(self, stream, call):
+        """call(stream handle) with the cache's device as the current one and
+        the call's stream as torch's, so that what the call allocates belongs
+        to that stream"""
+        torch = self._torch
         if stream is None and self.device.index == torch.cuda.current_device():
-            return contextlib.nullcontext()
-        st = contextlib.ExitStack()
-        st.enter_context(torch.cuda.device(self.device))
-        if stream is not None:
+            return call(torch._C._cuda_getCurrentRawStream(self.device.index))
+        with torch.cuda.device(self.device):
+            if stream is None:
+                return call(torch._C._cuda_getCurrentRawStream(self.device.index))
             if isinstance(stream, int):
                 stream = torch.cuda.ExternalStream(stream, device=self.device)
-            st.enter_context(torch.cuda.stream(stream))
-        return st
+            with torch.cuda.stream(stream):
+                return call(stream.cuda_stream)
 
     def _ints(self, t, n, what):
         """device address of an int32 vector of n (or None)"""
-        import torch
         if t is None:
             return None
-        if t.dtype != torch.int32 or t.device != self.device or t.dim() != 1 or (n is not None and t.shape[0] != n) or \
-                (t.shape[0] > 1 and t.stride(0) != 1):
+        if t.dtype != self._i32 or t.device != self.device or t.dim() != 1 or (n is not None and t.shape[0] != n) or \
+                not t.is_contiguous():
             raise QmoeError(f"{what} must be a contiguous int32 vector" + (f" of {n}" if n is not None else "") +
                             f" on {self.device}")
         return t.data_ptr()
 
     def _rows(self, t, heads, dtypes, what):
-        if t.device != self.device or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.hd or \
-                t.dtype not in dtypes or t.stride(2) != 1:
+        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.hd or t.dtype not in dtypes or t.stride(2) != 1 or \
+                t.device != self.device:
             raise QmoeError(f"{what} must be [n, {heads}, {self.hd}] {' or '.join(str(d) for d in dtypes)} with the head "
                             f"dim contiguous on {self.device}")
 
@@ -1119,29 +1115,31 @@ class PagedCache:
         if p is None or starts.shape[0] < 1:
             raise QmoeError("starts must hold one number more than there are sequences")
         m = starts.shape[0] - 1
-        return QmoePagedBatch(p, self._ints(slots, m, "slots"), n, m)
+        return QmoePagedBatch(p, None if slots is None else self._ints(slots, m, "slots"), n, m)
 
     def _work(self, call, n=0, n_seqs=0, heads=0):
-        import torch
+        """the call's workspace; a call that the library refuses gets 16 bytes"""
         need = lib().qmoe_paged_ws_bytes(self._cp, call, n, n_seqs, heads)
-        return torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
+        return self._torch.empty(max(need, 16), dtype=self._u8, device=self.device)
+
+    def _status(self):
+        return self._torch.empty(1, dtype=self._i32, device=self.device)
 
     # -- rows
     def append(self, layer, k, v, starts, slots=None, stream=None):
         """new rows k, v [n, n_kv_heads, head_dim] into the pages of `layer`
         (the pages' type, or f32 rounded into bf16 pages)"""
-        import torch
-        dtypes = (self.dtype,) if self.dtype == torch.float32 else (self.dtype, torch.float32)
-        self._rows(k, self.kvh, dtypes, "k")
-        self._rows(v, self.kvh, dtypes, "v")
+        self._rows(k, self.kvh, self._src, "k")
+        self._rows(v, self.kvh, self._src, "v")
         if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
             raise QmoeError("k and v must have the same rows and type")
-        b = self._batch(k.shape[0], starts, slots)
-        err = QmoeErr()
-        with self._place(stream):
+        b, err = self._batch(k.shape[0], starts, slots), QmoeErr()
+
+        def call(st):
             _check(lib().qmoe_paged_append(self._cp, layer, ctypes.byref(b), k.data_ptr(), v.data_ptr(), _dtype_code(k),
-                                           k.stride(0), k.stride(1), v.stride(0), v.stride(1), self._stream(stream),
-                                           ctypes.byref(err)), err, "qmoe_paged_append")
+                                           k.stride(0), k.stride(1), v.stride(0), v.stride(1), st, ctypes.byref(err)), err,
+                   "qmoe_paged_append")
+        self._on(stream, call)
 
     def attend(self, layer, q, starts, slots=None, window=0, sinks=0, scale=None, grouped=False, out=None, stream=None):
         """q [n, n_heads, head_dim] of the pages' type -> softmax(scale q.k) v
@@ -1150,25 +1148,24 @@ class PagedCache:
         Head h reads kv head h % n_kv_heads as the attention mixer's, with
         `grouped` h // (n_heads / n_kv_heads); scale None is
         1 / sqrt(head_dim).  Rows of no sequence are left as out has them."""
-        import torch
         heads = q.shape[1] if q.dim() == 3 else 0
-        self._rows(q, heads, (self.dtype,), "q")
+        self._rows(q, heads, self._own, "q")
         n = q.shape[0]
-        b = self._batch(n, starts, slots)
-        err = QmoeErr()
-        with self._place(stream):
-            if out is None:
-                out = torch.empty((n, heads, self.hd), dtype=self.dtype, device=self.device)
-            else:
-                self._rows(out, heads, (self.dtype,), "out")
-                if out.shape[0] != n:
-                    raise QmoeError(f"out has {out.shape[0]} rows, q {n}")
-            a = QmoePagedQuery(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), heads,
-                               window, sinks, 1 if grouped else 0, 0.0 if scale is None else scale)
+        b, err = self._batch(n, starts, slots), QmoeErr()
+        if out is not None:
+            self._rows(out, heads, self._own, "out")
+            if out.shape[0] != n:
+                raise QmoeError(f"out has {out.shape[0]} rows, q {n}")
+
+        def call(st):
+            o = self._torch.empty((n, heads, self.hd), dtype=self.dtype, device=self.device) if out is None else out
+            a = QmoePagedQuery(q.data_ptr(), o.data_ptr(), q.stride(0), q.stride(1), o.stride(0), o.stride(1), heads, window,
+                               sinks, 1 if grouped else 0, 0.0 if scale is None else scale)
             ws = self._work(PAGED_ATTN, n, b.n_seqs, heads)
-            _check(lib().qmoe_paged_attn(self._cp, layer, ctypes.byref(b), ctypes.byref(a), ws.data_ptr(), ws.numel(),
-                                         self._stream(stream), ctypes.byref(err)), err, "qmoe_paged_attn")
-        return out
+            _check(lib().qmoe_paged_attn(self._cp, layer, ctypes.byref(b), ctypes.byref(a), ws.data_ptr(), ws.numel(), st,
+                                         ctypes.byref(err)), err, "qmoe_paged_attn")
+            return o
+        return self._on(stream, call)
 
     # -- pages
     def reserve(self, n_new, slots=None, stream=None):
@@ -1176,31 +1173,33 @@ class PagedCache:
         advanced; a shared, partly filled last page is copied.  Returns an
         int32 [1] on the device: 0, the pages lacking, or -1 for a batch that
         is refused (nothing is changed unless 0)."""
-        import torch
-        p = self._ints(n_new, None, "n_new")
-        m = n_new.shape[0]
-        sl = self._ints(slots, m, "slots")
-        err = QmoeErr()
-        with self._place(stream):
-            status, ws = torch.empty(1, dtype=torch.int32, device=self.device), self._work(PAGED_RESERVE, n_seqs=m)
-            _check(lib().qmoe_paged_reserve(self._cp, sl, p, m, status.data_ptr(), ws.data_ptr(), ws.numel(),
-                                            self._stream(stream), ctypes.byref(err)), err, "qmoe_paged_reserve")
-        return status
+        if n_new is None:
+            raise QmoeError("n_new must be given")
+        p, m = self._ints(n_new, None, "n_new"), n_new.shape[0]
+        sl, err = self._ints(slots, m, "slots"), QmoeErr()
+
+        def call(st):
+            status, ws = self._status(), self._work(PAGED_RESERVE, 0, m)
+            _check(lib().qmoe_paged_reserve(self._cp, sl, p, m, status.data_ptr(), ws.data_ptr(), ws.numel(), st,
+                                            ctypes.byref(err)), err, "qmoe_paged_reserve")
+            return status
+        return self._on(stream, call)
 
     def fork(self, src, dst, rows=None, stream=None):
         """slot dst[i] becomes the first rows[i] (None: all) rows of slot
         src[i] by sharing pages; all sources are read first.  Returns an int32
         [1] on the device: 0, or -1 (refused, nothing changed)."""
-        import torch
-        s = self._ints(src, None, "src")
-        m = src.shape[0]
-        d, r = self._ints(dst, m, "dst"), self._ints(rows, m, "rows")
-        err = QmoeErr()
-        with self._place(stream):
-            status, ws = torch.empty(1, dtype=torch.int32, device=self.device), self._work(PAGED_FORK, n_seqs=m)
-            _check(lib().qmoe_paged_fork(self._cp, s, d, r, m, status.data_ptr(), ws.data_ptr(), ws.numel(),
-                                         self._stream(stream), ctypes.byref(err)), err, "qmoe_paged_fork")
-        return status
+        if src is None or dst is None:
+            raise QmoeError("src and dst must be given")
+        s, m = self._ints(src, None, "src"), src.shape[0]
+        d, r, err = self._ints(dst, m, "dst"), self._ints(rows, m, "rows"), QmoeErr()
+
+        def call(st):
+            status, ws = self._status(), self._work(PAGED_FORK, 0, m)
+            _check(lib().qmoe_paged_fork(self._cp, s, d, r, m, status.data_ptr(), ws.data_ptr(), ws.numel(), st,
+                                         ctypes.byref(err)), err, "qmoe_paged_fork")
+            return status
+        return self._on(stream, call)
 
     def trim(self, slots, rows, stream=None):
         """cuts slots to their first rows[i] rows (0 frees a slot)"""
@@ -1208,22 +1207,23 @@ class PagedCache:
 
     def evict(self, window, sinks=0, slots=None, stream=None):
         """releases the pages that no later query sees under this window and sinks"""
-        sl = self._ints(slots, None, "slots")
+        sl, err = self._ints(slots, None, "slots"), QmoeErr()
         m = self.table.shape[0] if slots is None else slots.shape[0]
-        err = QmoeErr()
-        with self._place(stream):
-            _check(lib().qmoe_paged_evict(self._cp, sl, m, window, sinks, self._stream(stream), ctypes.byref(err)), err,
-                   "qmoe_paged_evict")
+
+        def call(st):
+            _check(lib().qmoe_paged_evict(self._cp, sl, m, window, sinks, st, ctypes.byref(err)), err, "qmoe_paged_evict")
+        self._on(stream, call)
 
     def compact(self, stream=None):
         """moves the used pages to the front of the pool; returns their number, an int32 [1] on the device"""
-        import torch
         err = QmoeErr()
-        with self._place(stream):
-            used, ws = torch.empty(1, dtype=torch.int32, device=self.device), self._work(PAGED_COMPACT)
-            _check(lib().qmoe_paged_compact(self._cp, used.data_ptr(), ws.data_ptr(), ws.numel(), self._stream(stream),
-                                            ctypes.byref(err)), err, "qmoe_paged_compact")
-        return used
+
+        def call(st):
+            used, ws = self._status(), self._work(PAGED_COMPACT)
+            _check(lib().qmoe_paged_compact(self._cp, used.data_ptr(), ws.data_ptr(), ws.numel(), st, ctypes.byref(err)), err,
+                   "qmoe_paged_compact")
+            return used
+        return self._on(stream, call)
 
 
 def decoder_layer_types(n_layers, full_attention_interval=4):
