@@ -21,12 +21,14 @@
 
 typedef float qm_f32x16 __attribute__((ext_vector_type(16)));
 
+#define PM_RT 128 /* rows of a unit of the many-row kernels */
+
 struct PaArgs {
     pg_cache c;   /* k and v of the call's layer */
     pg_attn a;
     int G;        /* query heads per kv head */
     float per_unit; /* kv heads / units that the call is cut into, rounded up */
-    int least;    /* key tiles of a part at the least */
+    int extra;    /* key tiles that a join is worth (pg_share) */
     float *po;    /* partial O [slot, RT, HD], unscaled */
     float2 *pml;  /* [slot, RT]: maximum (log2 units), sum */
 };
@@ -106,18 +108,18 @@ __device__ __forceinline__ bool pa_find(const PaArgs &p, int want, PaUnit &u) {
     auto seq = [&](int i) { return pg_seq_at(&p.c, p.a.starts, p.a.slots, p.a.n, i); };
     auto load = [&](const pg_seq &s) { return pg_load_of(s, p.G, RT, p.a.window, p.a.sinks, KT); };
     pg_seq s0 = {-1, 0, 0, 0};
-    pg_load l0 = {0, 0};
+    pg_load l0 = {0, 0, 0.0f};
     float t = 0.0f;
     for (int k = 0; k < per; k++) {
         const int i = lane * per + k;
         if (i < n) {
             s0 = seq(i);
             l0 = load(s0);
-            t += (float)l0.row_tiles * (float)l0.key_tiles;
+            t += l0.work;
         }
     }
     t = qk_group_sum<64>(t);
-    const int share = pg_share(t, p.per_unit, p.least);
+    const int share = pg_share(t, p.per_unit, p.extra);
     auto count = [&](const pg_load &l, int &parts, int &units, int &split) {
         parts = pg_parts(l.key_tiles, share);
         const int tasks = l.row_tiles * p.c.kvh;
@@ -138,7 +140,22 @@ __device__ __forceinline__ bool pa_find(const PaArgs &p, int want, PaUnit &u) {
             }
         }
     }
-    const int ue = pa_scan(units) - units, se = pa_scan(split) - split;
+    int ue, se; /* units and split units before this lane's */
+    if (RT == PM_RT && per == 1) {
+        /* the sequences with the longest parts come first, so that the last
+         * units to start are short ones */
+        const int len = units ? (l0.key_tiles + parts - 1) / parts : 0;
+        ue = se = 0;
+        for (int k = 0; k < n; k++) {
+            const int lk = __builtin_amdgcn_readlane(len, k);
+            const bool before = lk > len || (lk == len && k < lane);
+            ue += before ? __builtin_amdgcn_readlane(units, k) : 0;
+            se += before ? __builtin_amdgcn_readlane(split, k) : 0;
+        }
+    } else {
+        ue = pa_scan(units) - units;
+        se = pa_scan(split) - split;
+    }
     const uint64_t here = __ballot(want >= ue && want < ue + units);
     if (!here) return false;
     const int at = __builtin_ctzll(here);
@@ -192,10 +209,9 @@ __device__ __forceinline__ bool pa_full(const PaArgs &p, int p0, int p1, int bas
 }
 
 /* ------------------------------------------------- one row at a time
- * fp32 on the vector ALU, keys of the unit's part only: for units in which a
- * row that some query does not see holds an infinity or NaN (or, f32 on
- * MFMA, a value that the bf16 parts cannot carry): a masked key is never
- * multiplied here.  Waves take the unit's rows in turn. */
+ * fp32 on the vector ALU, keys of the unit's part only, for units with
+ * results that are not finite (pa_again): a masked key is never multiplied
+ * here.  Waves take the unit's rows in turn. */
 template <typename T, int HD, int RT, int KT>
 __device__ __forceinline__ void pa_slow(const PaArgs &p, const PaUnit &u, int kt0, int kt1, pg_tiles tl, int waves) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -266,20 +282,29 @@ __device__ __forceinline__ void pa_slow(const PaArgs &p, const PaUnit &u, int kt
     }
 }
 
+/* maximum of three, a NaN passed over; without the canonicalising moves that
+ * fmaxf of a matrix result brings */
+__device__ __forceinline__ float pa_max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 #define PA_GROW 8.0f
-/* running maximum and sum of a row over 32 NS more scores (log2 units, masked
- * ones -inf), held by lanes l and l + 32; leaves the weights in st.  The sums
- * so far are rescaled only when a maximum has grown by more than PA_GROW: weights
+/* running maximum and sum of a row over 32 NS more scores (unscaled, masked
+ * ones -inf), held by lanes l and l + 32; leaves the weights in st.  m is in
+ * log2 units; the scale is positive (a negative one is in q).  The sums so
+ * far are rescaled only when a maximum has grown by more than PA_GROW: weights
  * reach 256 then, which costs no accuracy (fp32 sums, bf16 weights are
  * relative), and most rescalings of a long row are saved. */
 template <int NS, int NO>
-__device__ __forceinline__ void pa_softmax(qm_f32x16 (&st)[NS], float &m, float &l, qm_f32x16 (&o)[NO]) {
-    float mx = st[0][0];
+__device__ __forceinline__ void pa_softmax(qm_f32x16 (&st)[NS], float scale, float &m, float &l, qm_f32x16 (&o)[NO]) {
+    float mx = -INFINITY;
 #pragma unroll
     for (int t = 0; t < NS; t++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) mx = fmaxf(mx, st[t][i]);
-    mx = fmaxf(mx, __uint_as_float(qk_xor32_u(__float_as_uint(mx))));
+        for (int i = 0; i < 16; i += 2) mx = pa_max3(st[t][i], st[t][i + 1], mx);
+    mx = fmaxf(mx, __uint_as_float(qk_xor32_u(__float_as_uint(mx)))) * scale;
     if (__any(mx > m + PA_GROW)) {
         const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
         l *= f;
@@ -293,22 +318,44 @@ __device__ __forceinline__ void pa_softmax(qm_f32x16 (&st)[NS], float &m, float 
 #pragma unroll
     for (int t = 0; t < NS; t++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            st[t][i] = __builtin_amdgcn_exp2f(st[t][i] - ms);
-            l += st[t][i];
-        }
+        for (int i = 0; i < 16; i++) st[t][i] = __builtin_amdgcn_exp2f(fmaf(st[t][i], scale, -ms));
 }
 
-/* eight weights of a row as a B operand */
-__device__ __forceinline__ qm_bf16x8 pa_pack(const qm_f32x16 &st, int s) {
-    return __builtin_bit_cast(qm_bf16x8, make_uint4(qk_cvt_pk_bf16(st[8 * s], st[8 * s + 1]), qk_cvt_pk_bf16(st[8 * s + 2], st[8 * s + 3]),
-                                                    qk_cvt_pk_bf16(st[8 * s + 4], st[8 * s + 5]), qk_cvt_pk_bf16(st[8 * s + 6], st[8 * s + 7])));
+/* eight weights of a row as a B operand; l takes the sum of the rounded
+ * weights, so that they add up to one again */
+__device__ __forceinline__ qm_bf16x8 pa_pack(const qm_f32x16 &st, int s, float &l) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        w[i] = qk_cvt_pk_bf16(st[8 * s + 2 * i], st[8 * s + 2 * i + 1]);
+        l = qk_dot2(w[i], QK_BF16_ONES, l);
+    }
+    return __builtin_bit_cast(qm_bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
 }
 
-__device__ __forceinline__ bool pa_bad_bf16(uint32_t w) {
-    return (w & 0x7F800000u) == 0x7F800000u || (w & 0x7F80u) == 0x7F80u;
+/* Where piece pc (16 bytes) of row rr of a tile lies in LDS: the pieces of a
+ * row are exchanged by an xor, so that the 16 rows of K that a quarter of a
+ * wave reads at once lie on all 64 banks (rows of 128 and 384 bytes start on
+ * alternating halves of them), and for V the 4 pieces of each of 4 rows. */
+template <int CR>
+__device__ __forceinline__ int pa_kswz(int rr) { return CR % 16 == 0 ? rr & 15 : (rr >> 1) & 7; }
+template <int CR>
+__device__ __forceinline__ int pa_vswz(int rr) { return CR % 16 == 0 ? (rr & 3) << 2 : ((rr >> 1) & 1) << 2; }
+
+/* A row that some query of the unit does not see may hold an infinity or NaN,
+ * and weight 0 times that is NaN: such a unit is computed again one row at a
+ * time.  It shows in the sums themselves, so the loops need no test: O or the
+ * sum of weights is not finite (also where that is the right result), or
+ * every score seen was -inf. */
+template <int N, int W, typename V>
+__device__ __forceinline__ bool pa_again(const V (&o)[N], float m, float l, bool seen) {
+    float x = l == l ? fabsf(l) : INFINITY;
+#pragma unroll
+    for (int d = 0; d < N; d++)
+#pragma unroll
+        for (int i = 0; i < W; i++) x = fmaxf(x, o[d][i] == o[d][i] ? fabsf(o[d][i]) : INFINITY);
+    return !(x < INFINITY) || (m == -INFINITY && seen);
 }
-__device__ __forceinline__ bool pa_bad_f32(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
 /* ------------------------------------------------------------ few rows
  * Decode: a unit is 16 NC rows (a group's heads of one to a few tokens) and a
@@ -358,10 +405,13 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
         return j <= p1 ? pg_row_at(&p.c, row, j) : -1;
     };
     int64_t next = find(kt0 + wave);
+    /* a negative scale is turned into the sign of q */
+    const float scale = fabsf(p.a.scale);
+    const uint32_t flip = p.a.scale < 0.0f ? (B16 ? 0x80008000u : 0x80000000u) : 0u;
     uint4 q[NC][QN];
     int pos[NC];
     float m[NC], l[NC];
-    bool seen[NC], bad = false;
+    bool seen[NC];
     pa_f32x4 o[NC][E];
 #pragma unroll
     for (int x = 0; x < NC; x++) {
@@ -369,7 +419,10 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
         pos[x] = first + t;
         const T *src = (const T *)p.a.q + (int64_t)(u.s.start + t) * p.a.q_token + (int64_t)pa_head(p, u.kh, r - t * p.G) * p.a.q_head + g * PE;
 #pragma unroll
-        for (int s = 0; s < QN; s++) q[x][s] = qk_ld((const uint4 *)(src + s * 4 * PE));
+        for (int s = 0; s < QN; s++) {
+            const uint4 w = qk_ld((const uint4 *)(src + s * 4 * PE));
+            q[x][s] = make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip);
+        }
         m[x] = -INFINITY;
         l[x] = 0.0f;
         seen[x] = false;
@@ -428,7 +481,7 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
                         a = __builtin_amdgcn_mfma_f32_16x16x4f32(kf.w, qf.w, a, 0, 0, 0);
                     }
                 }
-                st[x][n] = a * p.a.scale;
+                st[x][n] = a;
             }
         if (valid != 0xFFFFFFFFu || !pa_full(p, p0, p1, base)) {
 #pragma unroll
@@ -443,10 +496,7 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
             for (int k = 0; k < 8; k++) {
                 const bool dead = !((valid >> (16 * (k >> 2) + 4 * g + (k & 3))) & 1u);
 #pragma unroll
-                for (int x = 0; x < VW; x++) {
-                    vx[k][x] = dead ? 0u : vx[k][x];
-                    bad |= B16 ? pa_bad_bf16(vx[k][x]) : pa_bad_f32(__uint_as_float(vx[k][x]));
-                }
+                for (int x = 0; x < VW; x++) vx[k][x] = dead ? 0u : vx[k][x];
             }
         } else {
 #pragma unroll
@@ -454,12 +504,13 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
         }
 #pragma unroll
         for (int x = 0; x < NC; x++) {
-            float mx = st[x][0][0];
-#pragma unroll
-            for (int k = 1; k < 8; k++) mx = fmaxf(mx, st[x][k >> 2][k & 3]);
+            float mx = pa_max3(st[x][0][0], st[x][0][1], st[x][0][2]);
+            mx = pa_max3(st[x][0][3], st[x][1][0], mx);
+            mx = pa_max3(st[x][1][1], st[x][1][2], mx);
+            mx = fmaxf(mx, st[x][1][3]);
             mx = fmaxf(mx, __uint_as_float(qk_xor16_u(__float_as_uint(mx))));
-            mx = fmaxf(mx, __uint_as_float(qk_xor32_u(__float_as_uint(mx))));
-            if (__any(mx > m[x] + PA_GROW)) {
+            mx = fmaxf(mx, __uint_as_float(qk_xor32_u(__float_as_uint(mx)))) * scale;
+            if (__any(mx > m[x] + PA_GROW)) { /* as pa_softmax */
                 const float mn = fmaxf(m[x], mx), f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[x] - mn);
                 l[x] *= f;
 #pragma unroll
@@ -469,17 +520,23 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
             const float ms = m[x] == -INFINITY ? 0.0f : m[x];
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const float w = __builtin_amdgcn_exp2f(st[x][k >> 2][k & 3] - ms);
+                const float w = __builtin_amdgcn_exp2f(fmaf(st[x][k >> 2][k & 3], scale, -ms));
                 st[x][k >> 2][k & 3] = w;
-                l[x] += w;
+                if constexpr (!B16) l[x] += w;
             }
         }
         if constexpr (B16) {
             qm_bf16x8 pw[NC];
 #pragma unroll
-            for (int x = 0; x < NC; x++)
-                pw[x] = __builtin_bit_cast(qm_bf16x8, make_uint4(qk_cvt_pk_bf16(st[x][0][0], st[x][0][1]), qk_cvt_pk_bf16(st[x][0][2], st[x][0][3]),
-                                                                 qk_cvt_pk_bf16(st[x][1][0], st[x][1][1]), qk_cvt_pk_bf16(st[x][1][2], st[x][1][3])));
+            for (int x = 0; x < NC; x++) { /* l: the sum of the rounded weights, as pa_pack */
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    w[k] = qk_cvt_pk_bf16(st[x][k >> 1][2 * (k & 1)], st[x][k >> 1][2 * (k & 1) + 1]);
+                    l[x] = qk_dot2(w[k], QK_BF16_ONES, l[x]);
+                }
+                pw[x] = __builtin_bit_cast(qm_bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+            }
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 uint32_t w[4];
@@ -500,14 +557,16 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
                         o[x][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vx[k][e]), st[x][k >> 2][k & 3], o[x][e], 0, 0, 0);
         }
     }
+    bool again = false;
 #pragma unroll
     for (int x = 0; x < NC; x++) {
+        again |= pa_again<E, 4>(o[x], m[x], l[x], seen[x]);
         l[x] += __uint_as_float(qk_xor16_u(__float_as_uint(l[x])));
         l[x] += __uint_as_float(qk_xor32_u(__float_as_uint(l[x])));
         l[x] = pa_sum(m[x], l[x], seen[x]);
         if (g == 0) ml[wave][16 * x + c] = make_float2(m[x], l[x]);
     }
-    if (__syncthreads_or(bad)) {
+    if (__syncthreads_or(again)) {
         pa_slow<T, HD, RT, PD_KT>(p, u, kt0, kt1, tl, 4);
         return;
     }
@@ -565,13 +624,10 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
 
 /* a row of a 32-wide unit, held by lanes l and l + 32: the output, or the
  * part's results */
-#define PM_RT 128
 template <typename T, int HD>
-__device__ __forceinline__ void pa_store(const PaArgs &p, const PaUnit &u, const qm_f32x16 (&o)[HD / 32], float m, float l, bool seen, int rr,
-                                         int t, int hh) {
+__device__ __forceinline__ void pa_store(const PaArgs &p, const PaUnit &u, const qm_f32x16 (&o)[HD / 32], float m, float l, int rr, int t,
+                                         int hh) {
     const int h = (threadIdx.x >> 5) & 1;
-    l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
-    l = pa_sum(m, l, seen);
     const float f = u.parts > 1 ? 1.0f : pa_norm(m, l);
     T *out = (T *)p.a.out + (int64_t)(u.s.start + t) * p.a.o_token + (int64_t)hh * p.a.o_head + 4 * h;
     float *po = p.po + ((int64_t)u.slot * PM_RT + rr) * HD + 4 * h;
@@ -604,15 +660,51 @@ typedef __attribute__((address_space(3))) pa_s16x4 *pa_tptr;
 
 constexpr int pm_kt(int hd, bool f32 = false) { return hd <= 128 && !f32 ? 64 : 32; }
 
+/* the rows' results of the second four waves into the first four's, through
+ * `ex` (HD / 8 pieces of 64 float4 per wave) and `ml`; true for the first */
+template <int E>
+__device__ __forceinline__ bool pa_merge(qm_f32x16 (&o)[E], float &m, float &l, float4 *ex, float2 *ml) {
+    const int tid = threadIdx.x & 255;
+    float4 *x = ex + (tid >> 6) * (E * 4 * 64) + (tid & 63);
+    const bool second = threadIdx.x >= 256;
+    if (second) {
+#pragma unroll
+        for (int d = 0; d < E; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) x[(4 * d + g) * 64] = make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+        ml[tid] = make_float2(m, l);
+    }
+    __syncthreads();
+    if (second) return false;
+    const float2 y = ml[tid];
+    const float M = fmaxf(m, y.x);
+    const float f0 = m == M ? 1.0f : __builtin_amdgcn_exp2f(m - M), f1 = y.x == M ? 1.0f : __builtin_amdgcn_exp2f(y.x - M);
+    l = l * f0 + y.y * f1;
+    m = M;
+#pragma unroll
+    for (int d = 0; d < E; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const float4 z = x[(4 * d + g) * 64];
+            o[d][4 * g] = o[d][4 * g] * f0 + z.x * f1;
+            o[d][4 * g + 1] = o[d][4 * g + 1] * f0 + z.y * f1;
+            o[d][4 * g + 2] = o[d][4 * g + 2] * f0 + z.z * f1;
+            o[d][4 * g + 3] = o[d][4 * g + 3] * f0 + z.w * f1;
+        }
+    return true;
+}
+
 template <int HD>
-__global__ __launch_bounds__(256, 2) void k_pa_many(PaArgs p) {
+__global__ __launch_bounds__(512, 1) void k_pa_many(PaArgs p) {
     typedef uint16_t T;
     constexpr int KT = pm_kt(HD), CR = HD / 8, NB = KT * CR / 256, NS = KT / 32, E = HD / 32, KS = HD / 16;
-    __shared__ __attribute__((aligned(16))) uint4 kv[2][2][KT * CR];
-    __shared__ int64_t where[PM_CHUNK];
+    constexpr int CH = PM_CHUNK / KT / 2; /* steps per look-up */
+    __shared__ __attribute__((aligned(16))) uint4 kv[2][2][2][KT * CR]; /* buffer, even / odd tile, k / v */
+    __shared__ __attribute__((aligned(16))) int64_t where[PM_CHUNK];
     PaUnit u;
     if (!pa_find<PM_RT, KT, false>(p, blockIdx.x, u)) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), c = lane & 31, h = lane >> 5;
+    const int odd = __builtin_amdgcn_readfirstlane(tid >> 8);
     const int row0 = u.rtile * PM_RT, rows = u.s.count * p.G, nrow = min(PM_RT, rows - row0);
     const int first = u.s.len - u.s.count;
     const int p0 = first + row0 / p.G, p1 = first + (row0 + nrow - 1) / p.G;
@@ -627,29 +719,29 @@ __global__ __launch_bounds__(256, 2) void k_pa_many(PaArgs p) {
     const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
 
     auto look = [&](int i0) { /* rows of the tiles i0.. of the part */
-        for (int k = tid; k < min(PM_CHUNK, (nt - i0) * KT); k += 256) {
-            const int i = kt0 + i0 + k / KT;
-            const int j = i < kt1 ? pg_tile(tl, i) * KT + k % KT : -1;
-            where[k] = j >= 0 && j <= p1 ? pg_row_at(&p.c, row, j) : -1;
+        for (int k = tid; k < min(PM_CHUNK, (nt - i0) * KT); k += 512) {
+            const int j = pg_tile(tl, kt0 + i0 + k / KT) * KT + k % KT;
+            where[k] = j <= p1 ? pg_row_at(&p.c, row, j) : -1;
         }
         __syncthreads();
     };
-    /* piece x of this thread: row and piece of the tile in LDS order */
-    uint32_t lds0[2][2];
+    uint32_t lds0[2][2]; /* this wave's place in its tile's K and V, per buffer */
 #pragma unroll
     for (int b = 0; b < 2; b++)
 #pragma unroll
         for (int x = 0; x < 2; x++)
-            lds0[b][x] = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(qm_lptr)&kv[b][x][0] + 1024 * wave);
+            lds0[b][x] = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(qm_lptr)&kv[b][odd][x][0] + 1024 * wave);
     uint64_t vnext = 0;
-    auto copy = [&](int i) {
-        const int64_t *wh = where + i % (PM_CHUNK / KT) * KT;
+    auto copy = [&](int i) { /* step i: this half's tile, 2 i + odd */
+        vnext = 0;
+        if (2 * i + odd >= nt) return;
+        const int64_t *wh = where + (2 * (i % CH) + odd) * KT;
         const int b = i & 1;
 #pragma unroll
         for (int x = 0; x < NB; x++) {
             const int L = x * 256 + wave * 64 + lane, rr = L / CR, pc = L - rr * CR;
             const int64_t at = wh[rr];
-            const T *ks = kp + at + 8 * (pc ^ (rr & 7)), *vs = vp + at + 8 * (pc ^ (((rr & 3) << 1) | ((rr >> 2) & 1)));
+            const T *ks = kp + at + 8 * (pc ^ pa_kswz<CR>(rr)), *vs = vp + at + 8 * (pc ^ pa_vswz<CR>(rr));
             qm_copy<0>(at < 0 ? &pa_zero : (const uint4 *)ks, lds0[b][0] + 4096 * x);
             qm_copy<0>(at < 0 ? &pa_zero : (const uint4 *)vs, lds0[b][1] + 4096 * x);
         }
@@ -659,33 +751,38 @@ __global__ __launch_bounds__(256, 2) void k_pa_many(PaArgs p) {
         look(0);
         copy(0);
     }
+    const float scale = fabsf(p.a.scale);
     uint4 q[KS];
     {
+        const uint32_t flip = p.a.scale < 0.0f ? 0x80008000u : 0u;
         const T *src = (const T *)p.a.q + (int64_t)(u.s.start + t) * p.a.q_token + (int64_t)hh * p.a.q_head + h * 8;
 #pragma unroll
-        for (int s = 0; s < KS; s++) q[s] = qk_ld((const uint4 *)(src + s * 16));
+        for (int s = 0; s < KS; s++) {
+            const uint4 w = qk_ld((const uint4 *)(src + s * 16));
+            q[s] = make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip);
+        }
     }
     float m = -INFINITY, l = 0.0f;
-    bool seen = false, bad = false;
+    bool seen = false;
     qm_f32x16 o[E];
 #pragma unroll
     for (int d = 0; d < E; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
     /* V: lane j of 16 reads 4 dims of key j / 4 and receives 4 keys of dim j */
-    const int j = lane & 15, g16 = (lane >> 4) & 1, fv = ((j >> 2) << 1) | h;
+    const int j = lane & 15, g16 = (lane >> 4) & 1, fv = pa_vswz<CR>(j >> 2);
 
-    for (int i = 0; i < nt; i++) {
-        qm_sync<0>(); /* tile i is in LDS; every wave is done with tile i - 1 */
+    for (int i = 0; i < (nt + 1) / 2; i++) {
+        qm_sync<0>(); /* the step's tiles are in LDS; every wave is done with the last step's */
         const uint64_t valid = vnext;
-        if (i + 1 < nt) {
-            if ((i + 1) % (PM_CHUNK / KT) == 0) look(i + 1);
+        if (2 * (i + 1) < nt) {
+            if ((i + 1) % CH == 0) look(2 * (i + 1));
             copy(i + 1);
         }
-        const int base = pg_tile(tl, kt0 + i) * KT;
+        const int base = pg_tile(tl, kt0 + 2 * i + odd) * KT;
         /* nothing of the tile is seen by this wave */
-        if (wn <= 0 || base > pw1 || (p.a.window > 0 && base + KT <= pg_lo(pw0, p.a.window) && base >= p.a.sinks)) continue;
-        const uint4 *kb = kv[i & 1][0], *vb = kv[i & 1][1];
+        if (wn <= 0 || 2 * i + odd >= nt || base > pw1 || (p.a.window > 0 && base + KT <= pg_lo(pw0, p.a.window) && base >= p.a.sinks)) continue;
+        const uint4 *kb = kv[i & 1][odd][0], *vb = kv[i & 1][odd][1];
         qm_f32x16 st[NS];
 #pragma unroll
         for (int n = 0; n < NS; n++) {
@@ -694,10 +791,8 @@ __global__ __launch_bounds__(256, 2) void k_pa_many(PaArgs p) {
 #pragma unroll
             for (int s = 0; s < KS; s++)
                 st[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                    __builtin_bit_cast(qm_bf16x8, kb[(32 * n + c) * CR + 8 * (s >> 2) + ((2 * (s & 3) + h) ^ (c & 7))]),
+                    __builtin_bit_cast(qm_bf16x8, kb[(32 * n + c) * CR + ((2 * s + h) ^ pa_kswz<CR>(c))]),
                     __builtin_bit_cast(qm_bf16x8, q[s]), st[n], 0, 0, 0);
-#pragma unroll
-            for (int x = 0; x < 16; x++) st[n][x] *= p.a.scale;
         }
 #pragma unroll
         for (int n = 0; n < NS; n++) {
@@ -711,21 +806,17 @@ __global__ __launch_bounds__(256, 2) void k_pa_many(PaArgs p) {
             mw >>= 4 * h;
 #pragma unroll
             for (int x = 0; x < 16; x++) st[n][x] = (mw >> (8 * (x >> 2) + (x & 3))) & 1u ? st[n][x] : -INFINITY;
-            for (int x = 0; x < CR / 2; x++) {
-                const uint4 w = vb[32 * n * CR + 64 * x + lane];
-                bad |= pa_bad_bf16(w.x) || pa_bad_bf16(w.y) || pa_bad_bf16(w.z) || pa_bad_bf16(w.w);
-            }
         }
-        pa_softmax(st, m, l, o);
+        pa_softmax(st, scale, m, l, o);
 #pragma unroll
         for (int n = 0; n < NS; n++)
 #pragma unroll
             for (int s = 0; s < 2; s++) {
-                const qm_bf16x8 pw = pa_pack(st[n], s);
+                const qm_bf16x8 pw = pa_pack(st[n], s, l);
                 const int key = 32 * n + 16 * s + 4 * h + (j >> 2);
 #pragma unroll
                 for (int d = 0; d < E; d++) {
-                    const int pc = 8 * (d >> 1) + ((4 * (d & 1) + 2 * g16 + ((j & 3) >> 1)) ^ fv);
+                    const int pc = (4 * d + 2 * g16 + ((j & 3) >> 1)) ^ fv;
                     const pa_s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_tptr)((const short *)(vb + key * CR + pc) + 4 * (j & 1)));
                     const pa_s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_tptr)((const short *)(vb + (key + 8) * CR + pc) + 4 * (j & 1)));
                     const uint2 aw = __builtin_bit_cast(uint2, a), bw = __builtin_bit_cast(uint2, b);
@@ -733,11 +824,13 @@ __global__ __launch_bounds__(256, 2) void k_pa_many(PaArgs p) {
                 }
             }
     }
-    if (__syncthreads_or(bad)) {
-        pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 4);
+    if (__syncthreads_or(wn > 0 && pa_again<E, 16>(o, m, l, seen))) {
+        pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 8);
         return;
     }
-    if (c < wn) pa_store<T, HD>(p, u, o, m, l, seen, 32 * wave + c, t, hh);
+    l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
+    if (!pa_merge<E>(o, m, l, (float4 *)kv, (float2 *)where)) return;
+    if (c < wn) pa_store<T, HD>(p, u, o, m, l, 32 * wave + c, t, hh);
 }
 
 /* ------------------------------------------------------------ many rows, f32
@@ -747,10 +840,9 @@ __global__ __launch_bounds__(256, 2) void k_pa_many(PaArgs p) {
  * of the fp32 instructions.  A tile is 32 keys; its rows come through
  * registers, where the workgroup splits them once for its four waves, into
  * one LDS buffer for K and one for V: V is written while the scores are
- * formed, the next tile's K while V is multiplied, one barrier after each.  Values past PA_BIG, infinities and NaN have no parts; their
- * units take the one-row path.
+ * formed, the next tile's K while V is multiplied, one barrier after each.  Infinities, NaN and values that round to a bf16 infinity have no
+ * parts: their differences are NaN, and the unit is computed again (pa_again).
  * Bound: matrix cores, six products per tile. */
-#define PA_BIG 1e15f /* parts, products and sums of values up to this stay finite */
 
 /* eight fp32 -> three bf16 parts */
 __device__ __forceinline__ void pa_split8(const float x[8], uint4 w[3]) {
@@ -769,12 +861,6 @@ __device__ __forceinline__ void pa_split8(const float x[8], uint4 w[3]) {
         w[i] = make_uint4(v[0], v[1], v[2], v[3]);
     }
 }
-__device__ __forceinline__ bool pa_big8(const float x[8]) {
-    bool b = false;
-#pragma unroll
-    for (int j = 0; j < 8; j++) b |= !(fabsf(x[j]) <= PA_BIG);
-    return b;
-}
 /* sum of a * b over the parts, the smallest products first */
 __device__ __forceinline__ qm_f32x16 pa_mfma6(const uint4 a[3], const uint4 b[3], qm_f32x16 c) {
     constexpr int ia[6] = {2, 1, 0, 1, 0, 0}, ib[6] = {0, 1, 2, 0, 1, 0};
@@ -784,15 +870,20 @@ __device__ __forceinline__ qm_f32x16 pa_mfma6(const uint4 a[3], const uint4 b[3]
     return c;
 }
 
+/* head dims past 128: four waves, whose registers and LDS are full */
+constexpr int pm_halves32(int hd) { return hd <= 128 ? 2 : 1; }
+
 template <int HD>
-__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_many32(PaArgs p) {
+__global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p) {
     typedef float T;
-    constexpr int KT = 32, CR = HD / 8, NB = KT * CR / 256, E = HD / 32, KS = HD / 16;
-    __shared__ __attribute__((aligned(16))) uint4 kv[2][3][KT * CR];
-    __shared__ int64_t where[PM_CHUNK];
+    constexpr int KT = 32, CR = HD / 8, NB = KT * CR / 256, E = HD / 32, KS = HD / 16, NG = pm_halves32(HD);
+    constexpr int CH = PM_CHUNK / KT / NG; /* steps per look-up */
+    __shared__ __attribute__((aligned(16))) uint4 kv[NG][2][3][KT * CR]; /* even / odd tile, k / v, part */
+    __shared__ __attribute__((aligned(16))) int64_t where[PM_CHUNK];
     PaUnit u;
     if (!pa_find<PM_RT, KT, false>(p, blockIdx.x, u)) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, h = lane >> 5;
+    const int odd = NG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int row0 = u.rtile * PM_RT, rows = u.s.count * p.G, nrow = min(PM_RT, rows - row0);
     const int first = u.s.len - u.s.count;
     const int p0 = first + row0 / p.G, p1 = first + (row0 + nrow - 1) / p.G;
@@ -806,18 +897,18 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_many32(PaArgs p) 
     const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
     const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
     auto look = [&](int i0) { /* rows of the tiles i0.. of the part */
-        for (int k = tid; k < min(PM_CHUNK, (nt - i0) * KT); k += 256) {
-            const int i = kt0 + i0 + k / KT;
-            const int j = i < kt1 ? pg_tile(tl, i) * KT + k % KT : -1;
-            where[k] = j >= 0 && j <= p1 ? pg_row_at(&p.c, row, j) : -1;
+        for (int k = threadIdx.x; k < min(PM_CHUNK, (nt - i0) * KT); k += 256 * NG) {
+            const int j = pg_tile(tl, kt0 + i0 + k / KT) * KT + k % KT;
+            where[k] = j <= p1 ? pg_row_at(&p.c, row, j) : -1;
         }
         __syncthreads();
     };
     float4 kx[NB][2], vx[NB][2];
     uint32_t vnext = 0;
-    bool bad = false;
-    auto load = [&](int i) { /* tile i into registers; rows without a page as zeros */
-        const int64_t *wh = where + i % (PM_CHUNK / KT) * KT;
+    auto load = [&](int i) { /* step i, this half's tile 2 i + odd, into registers; rows without a page as zeros */
+        vnext = 0;
+        if (NG * i + odd >= nt) return;
+        const int64_t *wh = where + (NG * (i % CH) + odd) * KT;
 #pragma unroll
         for (int x = 0; x < NB; x++) {
             const int L = x * 256 + tid, rr = L / CR, pc = L - rr * CR;
@@ -836,19 +927,19 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_many32(PaArgs p) 
 #pragma unroll
         for (int x = 0; x < NB; x++) {
             const int L = x * 256 + tid, rr = L / CR, pc = L - rr * CR;
-            const int at = rr * CR + (pc ^ (which ? ((rr & 3) << 1) | ((rr >> 2) & 1) : rr & 7));
+            const int at = rr * CR + (pc ^ (which ? pa_vswz<CR>(rr) : pa_kswz<CR>(rr)));
             const float v[8] = {src[x][0].x, src[x][0].y, src[x][0].z, src[x][0].w, src[x][1].x, src[x][1].y, src[x][1].z, src[x][1].w};
             uint4 w[3];
-            bad |= pa_big8(v);
             pa_split8(v, w);
 #pragma unroll
-            for (int y = 0; y < 3; y++) kv[which][y][at] = w[y];
+            for (int y = 0; y < 3; y++) kv[odd][which][y][at] = w[y];
         }
     };
     if (nt > 0) {
         look(0);
         load(0);
     }
+    const float scale = fabsf(p.a.scale), sign = p.a.scale < 0.0f ? -1.0f : 1.0f;
     uint4 q[KS][3];
     {
         const T *src = (const T *)p.a.q + (int64_t)(u.s.start + t) * p.a.q_token + (int64_t)hh * p.a.q_head + h * 8;
@@ -856,7 +947,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_many32(PaArgs p) 
         for (int s = 0; s < KS; s++) {
             float x[8];
             pa_get8(src + s * 16, x);
-            bad |= pa_big8(x);
+#pragma unroll
+            for (int y = 0; y < 8; y++) x[y] *= sign;
             pa_split8(x, q[s]);
         }
     }
@@ -867,33 +959,32 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_many32(PaArgs p) 
     for (int d = 0; d < E; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-    const int j = lane & 15, g16 = (lane >> 4) & 1, fv = ((j >> 2) << 1) | h;
-    if (nt > 0) put(0, kx);
+    const int j = lane & 15, g16 = (lane >> 4) & 1, fv = pa_vswz<CR>(j >> 2);
+    if (odd < nt) put(0, kx);
     qk_lds_barrier();
-    for (int i = 0; i < nt; i++) {
+    for (int i = 0; i < (nt + NG - 1) / NG; i++) {
         const uint32_t valid = vnext;
-        /* K of tile i is in LDS, and every wave is done with V of tile i - 1 */
-        put(1, vx);
-        if (i + 1 < nt) {
-            if ((i + 1) % (PM_CHUNK / KT) == 0) look(i + 1);
+        const bool mine = NG * i + odd < nt;
+        /* K of the step is in LDS, and every wave is done with V of the last */
+        if (mine) put(1, vx);
+        if (NG * (i + 1) < nt) {
+            if ((i + 1) % CH == 0) look(NG * (i + 1));
             load(i + 1);
         }
-        const int base = pg_tile(tl, kt0 + i) * KT;
-        const bool act = wn > 0 && base <= pw1 && !(p.a.window > 0 && base + KT <= pg_lo(pw0, p.a.window) && base >= p.a.sinks);
+        const int base = pg_tile(tl, kt0 + NG * i + odd) * KT;
+        const bool act = mine && wn > 0 && base <= pw1 && !(p.a.window > 0 && base + KT <= pg_lo(pw0, p.a.window) && base >= p.a.sinks);
         qm_f32x16 st[1];
         if (act) {
-            const uint4 *kb = kv[0][0];
+            const uint4 *kb = kv[odd][0][0];
 #pragma unroll
             for (int x = 0; x < 16; x++) st[0][x] = 0.0f;
 #pragma unroll
             for (int s = 0; s < KS; s++) {
                 uint4 a[3];
 #pragma unroll
-                for (int y = 0; y < 3; y++) a[y] = kb[y * KT * CR + c * CR + 8 * (s >> 2) + ((2 * (s & 3) + h) ^ (c & 7))];
+                for (int y = 0; y < 3; y++) a[y] = kb[y * KT * CR + c * CR + ((2 * s + h) ^ pa_kswz<CR>(c))];
                 st[0] = pa_mfma6(a, q[s], st[0]);
             }
-#pragma unroll
-            for (int x = 0; x < 16; x++) st[0][x] *= p.a.scale;
             if (valid == 0xFFFFFFFFu && pa_full(p, pw0, pw1, base)) {
                 seen = true;
             } else {
@@ -903,12 +994,14 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_many32(PaArgs p) 
 #pragma unroll
                 for (int x = 0; x < 16; x++) st[0][x] = (mw >> (8 * (x >> 2) + (x & 3))) & 1u ? st[0][x] : -INFINITY;
             }
-            pa_softmax(st, m, l, o);
+            pa_softmax(st, scale, m, l, o);
+#pragma unroll
+            for (int x = 0; x < 16; x++) l += st[0][x];
         }
         qk_lds_barrier(); /* V is in LDS, and every wave has its scores */
-        if (i + 1 < nt) put(0, kx);
+        if (NG * (i + 1) + odd < nt) put(0, kx);
         if (act) {
-            const uint4 *vb = kv[1][0];
+            const uint4 *vb = kv[odd][1][0];
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 const float x[8] = {st[0][8 * s], st[0][8 * s + 1], st[0][8 * s + 2], st[0][8 * s + 3],
@@ -918,7 +1011,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_many32(PaArgs p) 
                 const int key = 16 * s + 4 * h + (j >> 2);
 #pragma unroll
                 for (int d = 0; d < E; d++) {
-                    const int pc = 8 * (d >> 1) + ((4 * (d & 1) + 2 * g16 + ((j & 3) >> 1)) ^ fv);
+                    const int pc = (4 * d + 2 * g16 + ((j & 3) >> 1)) ^ fv;
                     uint4 a[3];
 #pragma unroll
                     for (int y = 0; y < 3; y++) {
@@ -933,11 +1026,14 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pa_many32(PaArgs p) 
         }
         qk_lds_barrier();
     }
-    if (__syncthreads_or(bad)) {
-        pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 4);
+    if (__syncthreads_or(wn > 0 && pa_again<E, 16>(o, m, l, seen))) {
+        pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 4 * NG);
         return;
     }
-    if (c < wn) pa_store<T, HD>(p, u, o, m, l, seen, 32 * wave + c, t, hh);
+    l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
+    if constexpr (NG == 2)
+        if (!pa_merge<E>(o, m, l, (float4 *)kv, (float2 *)where)) return;
+    if (c < wn) pa_store<T, HD>(p, u, o, m, l, 32 * wave + c, t, hh);
 }
 
 /* ------------------------------------------------------------ join
@@ -1002,24 +1098,24 @@ __global__ __launch_bounds__(256) void k_pa_join(PaArgs p) {
 /* how a call is cut: units asked for, the grid that holds them whatever the
  * lengths, tasks that can need a join, and the slots of partial results */
 struct PaPlan {
-    int units, least;
+    int units, extra;
     int64_t grid, join, slots;
 };
 
-static PaPlan pa_plan(const pg_cache *c, int n, int n_seqs, int h, int rt, int kt, int units, int least) {
+static PaPlan pa_plan(const pg_cache *c, int n, int n_seqs, int h, int rt, int kt, int units, int extra) {
     PaPlan q;
     const int G = h / c->kvh;
     q.units = units;
-    q.least = least;
+    q.extra = extra;
     /* sum of ceil(rows / rt) over the sequences that have rows */
     const int64_t rows = (int64_t)n * G, seqs = n_seqs < n ? n_seqs : n;
     const int64_t per_head = rows / rt + seqs < rows ? rows / rt + seqs : rows;
     const int64_t tasks = per_head * c->kvh;
-    const int64_t key_tiles = ((int64_t)c->cap + kt - 1) / kt + 1;
-    const int64_t parts = key_tiles <= least ? 1 : (key_tiles + least - 1) / least;
-    q.grid = tasks * parts < units + tasks ? tasks * parts : units + tasks;
-    q.slots = parts == 1 ? 0 : tasks * parts < 2 * (int64_t)units ? tasks * parts : 2 * (int64_t)units;
-    q.join = parts == 1 ? 0 : tasks < units ? tasks : units; /* a split task has two units at least */
+    /* parts of the longest task, then the bounds that pg_share gives */
+    const int64_t parts = pg_parts(c->cap / kt + 2, extra + 1), most = tasks * parts;
+    q.grid = most < 2 * (int64_t)units + tasks ? most : 2 * (int64_t)units + tasks;
+    q.slots = parts == 1 ? 0 : most < 3 * (int64_t)units ? most : 3 * (int64_t)units;
+    q.join = parts == 1 ? 0 : tasks < 3 * (int64_t)units / 2 ? tasks : 3 * (int64_t)units / 2; /* two parts at least */
     return q;
 }
 
@@ -1040,7 +1136,7 @@ static int pa_rows(const pg_cache *c, int n, int n_seqs, int h) {
 static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h) {
     const int rt = pa_rows(c, n, n_seqs, h);
     const int kt = pm_kt(c->hd, c->dtype == QMOE_F32);
-    if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, kt, 512, 512 / kt);
+    if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, kt, 256, c->dtype == QMOE_BF16 ? 12 : 2);
     /* tables of up to 16 tiles (512 rows) are not cut: the join's launch costs
      * more than the shorter run of tiles gives */
     return pa_plan(c, n, n_seqs, h, rt, PD_KT, 1024, c->cap <= 16 * PD_KT ? 17 : 8);
@@ -1054,13 +1150,13 @@ extern "C" size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h) {
 }
 
 template <typename T, int HD, int RT, int KT>
-static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), void *ws, hipStream_t st) {
+static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), int threads, void *ws, hipStream_t st) {
     const PaPlan q = pa_plan_of(&p.c, p.a.n, p.a.n_seqs, p.a.h);
     p.per_unit = pg_per_unit(p.c.kvh, q.units);
-    p.least = q.least;
+    p.extra = q.extra;
     p.pml = (float2 *)ws;
     p.po = (float *)((char *)ws + pa_up((size_t)q.slots * RT * 8));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)q.grid), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)q.grid), dim3(threads), 0, st, p);
     const int rc = QK_CHECK_LAUNCH();
     if (rc || q.join == 0) return rc;
     hipLaunchKernelGGL((k_pa_join<T, HD, RT, KT>), dim3((unsigned)q.join, pa_join_rows(q.join, RT)), dim3(256), 0, st, p);
@@ -1071,11 +1167,11 @@ template <typename T, int HD>
 static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
     const int rt = pa_rows(&p.c, p.a.n, p.a.n_seqs, p.a.h);
     if (rt == PM_RT) {
-        if constexpr (sizeof(T) == 2) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD>, ws, st);
-        else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD>, ws, st);
+        if constexpr (sizeof(T) == 2) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD>, 512, ws, st);
+        else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD>, 256 * pm_halves32(HD), ws, st);
     }
-    if (rt == 16) return pa_launch_rt<T, HD, 16, PD_KT>(p, k_pa_few<T, HD, 1>, ws, st);
-    return pa_launch_rt<T, HD, 32, PD_KT>(p, k_pa_few<T, HD, 2>, ws, st);
+    if (rt == 16) return pa_launch_rt<T, HD, 16, PD_KT>(p, k_pa_few<T, HD, 1>, 256, ws, st);
+    return pa_launch_rt<T, HD, 32, PD_KT>(p, k_pa_few<T, HD, 2>, 256, ws, st);
 }
 
 template <typename T>

@@ -97,32 +97,42 @@ QK_HD static inline int pg_tile(pg_tiles t, int i) { return i < t.st ? i : t.ms 
  * (sequence, row tile, kv head). */
 typedef struct {
     int row_tiles, key_tiles; /* key tiles of the last row tile, the longest of the sequence (to one tile) */
+    float work;               /* row_tiles times the mean of the first and last row tile's key tiles */
 } pg_load;
 QK_HD static inline pg_load pg_load_of(pg_seq s, int G, int rt, int window, int sinks, int kt) {
     pg_load l;
     const int rows = s.count * G;
     l.row_tiles = (rows + rt - 1) / rt;
     l.key_tiles = 0;
+    l.work = 0.0f;
     if (l.row_tiles > 0) {
-        const int t0 = (l.row_tiles - 1) * rt / G;
-        l.key_tiles = pg_tiles_of(s.len - s.count + t0, s.len - 1, window, sinks, kt).nt;
+        const int p = s.len - s.count, t0 = (l.row_tiles - 1) * rt / G;
+        l.key_tiles = pg_tiles_of(p + t0, s.len - 1, window, sinks, kt).nt;
+        l.work = (float)l.key_tiles;
+        if (l.row_tiles > 1)
+            l.work = (float)l.row_tiles * 0.5f *
+                     ((float)l.key_tiles + (float)pg_tiles_of(p, p + pg_min((rt - 1) / G, s.count - 1), window, sinks, kt).nt);
     }
     return l;
 }
-/* Key tiles per part, such that the parts of all tasks number at most `units`
- * + tasks: total = the sum of row_tiles * key_tiles over the sequences and
- * per_unit = pg_per_unit(kv heads, units).  fp32 sums of 1024 terms and a tree
- * are off by less than 2^-13.9, which the factor in per_unit covers. */
+/* Key tiles per part, from the units that fill the card: a run of total / units
+ * tiles, and `extra` tiles more, what storing and joining a part costs in
+ * time.  total = the sum of `work` over the sequences, per_unit =
+ * pg_per_unit(kv heads, units).  total is at least half of the sum of
+ * row_tiles * key_tiles, so there are at most 2 units + tasks parts; a task of
+ * parts > 1 has 1.5 shares at least, so at most 3 units of them belong to
+ * such.  fp32 sums of 1024 terms and a tree are off by less than 2^-13.9, which the
+ * factor in per_unit covers. */
 QK_HD static inline float pg_per_unit(int kvh, int units) { return 1.0001f * (float)kvh / (float)units; }
-QK_HD static inline int pg_share(float total, float per_unit, int least) {
+QK_HD static inline int pg_share(float total, float per_unit, int extra) {
     const float s = total * per_unit;
-    const int n = (s < 1e9f ? (int)s : 1000000000) + 1;
-    return n < least ? least : n;
+    return (s < 1e9f ? (int)s : 1000000000) + 1 + extra;
 }
+/* to the nearest: a task of 1.4 shares is not worth a join */
 QK_HD static inline int pg_parts(int key_tiles, int share) {
-    return key_tiles <= share ? 1 : (key_tiles + share - 1) / share;
+    const int n = (int)(((int64_t)key_tiles + share / 2) / share);
+    return n < 1 ? 1 : n;
 }
-
 /* first of nt key tiles of part i */
 QK_HD static inline int pg_part(int nt, int i, int parts) { return (int)((int64_t)nt * i / parts); }
 

@@ -114,7 +114,7 @@ static void units(void) {
         const int n_seqs = 1 + rnd() % 6, want = 1 + rnd() % 600;
         pg_seq s[6];
         float total = 0.0f;
-        int64_t n_units = 0, tasks = 0, split = 0, rows = 0;
+        int64_t most = 0, n_units = 0, tasks = 0, split = 0, rows = 0;
         for (int i = 0; i < n_seqs; i++) {
             s[i].slot = s[i].start = 0;
             s[i].count = rnd() % 300;
@@ -122,7 +122,8 @@ static void units(void) {
             rows += s[i].count;
             const pg_load l = pg_load_of(s[i], G, rt, window, sinks, kt);
             CHECK(l.row_tiles == (s[i].count * G + rt - 1) / rt, "row tiles");
-            total += (float)l.row_tiles * (float)l.key_tiles;
+            total += l.work;
+            most += (int64_t)l.row_tiles * l.key_tiles;
         }
         const int share = pg_share(total, pg_per_unit(1, want), 1 + rnd() % 8);
         for (int i = 0; i < n_seqs; i++) {
@@ -141,8 +142,9 @@ static void units(void) {
                           l.key_tiles + 2 + rt / kt, "row tile %d", r);
             }
         }
-        CHECK(n_units <= want + tasks, "%lld units of %d + %lld", (long long)n_units, want, (long long)tasks);
-        CHECK(split <= 2 * (int64_t)want, "%lld split units of %d", (long long)split, want);
+        CHECK(2 * (double)total >= (double)most, "%g of %lld", (double)total, (long long)most);
+        CHECK(n_units <= 2 * (int64_t)want + tasks, "%lld units of %d + %lld", (long long)n_units, want, (long long)tasks);
+        CHECK(split <= 3 * (int64_t)want, "%lld split units of %d", (long long)split, want);
         CHECK(tasks <= rows * G / rt + n_seqs, "tasks");
     }
 }
