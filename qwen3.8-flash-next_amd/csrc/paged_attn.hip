@@ -654,57 +654,63 @@ __device__ __forceinline__ void pa_store(const PaArgs &p, const PaUnit &u, const
  * Bound: matrix cores and, next to them, LDS (each wave reads the whole tile
  * for 32 rows) and the exponentials. */
 #define PM_CHUNK 1024
-__device__ const uint4 pa_zero = {0, 0, 0, 0};
+__device__ const uint4 pa_zero[32] = {}; /* a row of zeros */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pa_s16x4 *pa_tptr;
 
+/* keys of a tile, and groups of four waves that take tiles in turn */
+constexpr int pm_groups(int hd) { return 2; }
 constexpr int pm_kt(int hd, bool f32 = false) { return hd <= 128 && !f32 ? 64 : 32; }
 
-/* the rows' results of the second four waves into the first four's, through
- * `ex` (HD / 8 pieces of 64 float4 per wave) and `ml`; true for the first */
-template <int E>
+/* the rows' results of the other groups of four waves into the first one's,
+ * through `ex` (HD / 8 pieces of 64 float4 per wave) and `ml`, in order; true
+ * for the first */
+template <int E, int NG>
 __device__ __forceinline__ bool pa_merge(qm_f32x16 (&o)[E], float &m, float &l, float4 *ex, float2 *ml) {
-    const int tid = threadIdx.x & 255;
+    const int tid = threadIdx.x & 255, group = threadIdx.x >> 8;
     float4 *x = ex + (tid >> 6) * (E * 4 * 64) + (tid & 63);
-    const bool second = threadIdx.x >= 256;
-    if (second) {
+    for (int k = 1; k < NG; k++) {
+        if (group == k) {
 #pragma unroll
-        for (int d = 0; d < E; d++)
+            for (int d = 0; d < E; d++)
 #pragma unroll
-            for (int g = 0; g < 4; g++) x[(4 * d + g) * 64] = make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
-        ml[tid] = make_float2(m, l);
-    }
-    __syncthreads();
-    if (second) return false;
-    const float2 y = ml[tid];
-    const float M = fmaxf(m, y.x);
-    const float f0 = m == M ? 1.0f : __builtin_amdgcn_exp2f(m - M), f1 = y.x == M ? 1.0f : __builtin_amdgcn_exp2f(y.x - M);
-    l = l * f0 + y.y * f1;
-    m = M;
-#pragma unroll
-    for (int d = 0; d < E; d++)
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const float4 z = x[(4 * d + g) * 64];
-            o[d][4 * g] = o[d][4 * g] * f0 + z.x * f1;
-            o[d][4 * g + 1] = o[d][4 * g + 1] * f0 + z.y * f1;
-            o[d][4 * g + 2] = o[d][4 * g + 2] * f0 + z.z * f1;
-            o[d][4 * g + 3] = o[d][4 * g + 3] * f0 + z.w * f1;
+                for (int g = 0; g < 4; g++) x[(4 * d + g) * 64] = make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+            ml[tid] = make_float2(m, l);
         }
-    return true;
+        __syncthreads();
+        if (group == 0) {
+            const float2 y = ml[tid];
+            const float M = fmaxf(m, y.x);
+            const float f0 = m == M ? 1.0f : __builtin_amdgcn_exp2f(m - M), f1 = y.x == M ? 1.0f : __builtin_amdgcn_exp2f(y.x - M);
+            l = l * f0 + y.y * f1;
+            m = M;
+#pragma unroll
+            for (int d = 0; d < E; d++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const float4 z = x[(4 * d + g) * 64];
+                    o[d][4 * g] = o[d][4 * g] * f0 + z.x * f1;
+                    o[d][4 * g + 1] = o[d][4 * g + 1] * f0 + z.y * f1;
+                    o[d][4 * g + 2] = o[d][4 * g + 2] * f0 + z.z * f1;
+                    o[d][4 * g + 3] = o[d][4 * g + 3] * f0 + z.w * f1;
+                }
+        }
+        if (k + 1 < NG) __syncthreads();
+    }
+    return group == 0;
 }
 
 template <int HD>
-__global__ __launch_bounds__(512, 1) void k_pa_many(PaArgs p) {
+__global__ __launch_bounds__(256 * pm_groups(HD), 1) void k_pa_many(PaArgs p) {
     typedef uint16_t T;
-    constexpr int KT = pm_kt(HD), CR = HD / 8, NB = KT * CR / 256, NS = KT / 32, E = HD / 32, KS = HD / 16;
-    constexpr int CH = PM_CHUNK / KT / 2; /* steps per look-up */
-    __shared__ __attribute__((aligned(16))) uint4 kv[2][2][2][KT * CR]; /* buffer, even / odd tile, k / v */
-    __shared__ __attribute__((aligned(16))) int64_t where[PM_CHUNK];
+    constexpr int KT = pm_kt(HD), CR = HD / 8, NB = KT * CR / 256, NS = KT / 32, E = HD / 32, KS = HD / 16, NG = pm_groups(HD);
+    constexpr int CH = PM_CHUNK / KT / NG; /* steps per look-up */
+    __shared__ __attribute__((aligned(16))) uint4 kv[2][NG][2][KT * CR]; /* buffer, group's tile, k / v */
+    __shared__ __attribute__((aligned(16))) ulonglong2 where[PM_CHUNK]; /* addresses of a key's k and v */
     PaUnit u;
     if (!pa_find<PM_RT, KT, false>(p, blockIdx.x, u)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), c = lane & 31, h = lane >> 5;
-    const int odd = __builtin_amdgcn_readfirstlane(tid >> 8);
+    const int group = __builtin_amdgcn_readfirstlane(tid >> 8);
     const int row0 = u.rtile * PM_RT, rows = u.s.count * p.G, nrow = min(PM_RT, rows - row0);
     const int first = u.s.len - u.s.count;
     const int p0 = first + row0 / p.G, p1 = first + (row0 + nrow - 1) / p.G;
@@ -718,34 +724,34 @@ __global__ __launch_bounds__(512, 1) void k_pa_many(PaArgs p) {
     const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
     const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
 
+    const uint64_t zero = (uint64_t)pa_zero;
     auto look = [&](int i0) { /* rows of the tiles i0.. of the part */
-        for (int k = tid; k < min(PM_CHUNK, (nt - i0) * KT); k += 512) {
+        for (int k = tid; k < min(CH * NG, nt - i0) * KT; k += 256 * NG) {
             const int j = pg_tile(tl, kt0 + i0 + k / KT) * KT + k % KT;
-            where[k] = j <= p1 ? pg_row_at(&p.c, row, j) : -1;
+            const int64_t at = j <= p1 ? pg_row_at(&p.c, row, j) : -1;
+            ulonglong2 w;
+            w.x = at < 0 ? zero : (uint64_t)(kp + at);
+            w.y = at < 0 ? zero : (uint64_t)(vp + at);
+            where[k] = w;
         }
         __syncthreads();
     };
-    uint32_t lds0[2][2]; /* this wave's place in its tile's K and V, per buffer */
-#pragma unroll
-    for (int b = 0; b < 2; b++)
-#pragma unroll
-        for (int x = 0; x < 2; x++)
-            lds0[b][x] = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(qm_lptr)&kv[b][odd][x][0] + 1024 * wave);
+    /* this wave's place in its tile's K; V and the other buffer lie behind */
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(qm_lptr)&kv[0][group][0][0] + 1024 * wave);
     uint64_t vnext = 0;
-    auto copy = [&](int i) { /* step i: this half's tile, 2 i + odd */
+    auto copy = [&](int i) { /* step i: this group's tile, NG i + group */
         vnext = 0;
-        if (2 * i + odd >= nt) return;
-        const int64_t *wh = where + (2 * (i % CH) + odd) * KT;
-        const int b = i & 1;
+        if (NG * i + group >= nt) return;
+        const ulonglong2 *wh = where + (NG * (i % CH) + group) * KT;
+        const uint32_t dst = lds0 + (i & 1) * (NG * 2 * KT * CR * 16);
 #pragma unroll
         for (int x = 0; x < NB; x++) {
             const int L = x * 256 + wave * 64 + lane, rr = L / CR, pc = L - rr * CR;
-            const int64_t at = wh[rr];
-            const T *ks = kp + at + 8 * (pc ^ pa_kswz<CR>(rr)), *vs = vp + at + 8 * (pc ^ pa_vswz<CR>(rr));
-            qm_copy<0>(at < 0 ? &pa_zero : (const uint4 *)ks, lds0[b][0] + 4096 * x);
-            qm_copy<0>(at < 0 ? &pa_zero : (const uint4 *)vs, lds0[b][1] + 4096 * x);
+            const ulonglong2 w = wh[rr];
+            qm_copy<0>((const uint4 *)(w.x + 16 * (pc ^ pa_kswz<CR>(rr))), dst + 4096 * x);
+            qm_copy<0>((const uint4 *)(w.y + 16 * (pc ^ pa_vswz<CR>(rr))), dst + KT * CR * 16 + 4096 * x);
         }
-        vnext = __ballot(wh[lane & (KT - 1)] >= 0);
+        vnext = __ballot(wh[lane & (KT - 1)].x != zero);
     };
     if (nt > 0) {
         look(0);
@@ -772,17 +778,17 @@ __global__ __launch_bounds__(512, 1) void k_pa_many(PaArgs p) {
     /* V: lane j of 16 reads 4 dims of key j / 4 and receives 4 keys of dim j */
     const int j = lane & 15, g16 = (lane >> 4) & 1, fv = pa_vswz<CR>(j >> 2);
 
-    for (int i = 0; i < (nt + 1) / 2; i++) {
+    for (int i = 0; i < (nt + NG - 1) / NG; i++) {
         qm_sync<0>(); /* the step's tiles are in LDS; every wave is done with the last step's */
         const uint64_t valid = vnext;
-        if (2 * (i + 1) < nt) {
-            if ((i + 1) % CH == 0) look(2 * (i + 1));
+        if (NG * (i + 1) < nt) {
+            if ((i + 1) % CH == 0) look(NG * (i + 1));
             copy(i + 1);
         }
-        const int base = pg_tile(tl, kt0 + 2 * i + odd) * KT;
+        const int base = pg_tile(tl, kt0 + NG * i + group) * KT;
         /* nothing of the tile is seen by this wave */
-        if (wn <= 0 || 2 * i + odd >= nt || base > pw1 || (p.a.window > 0 && base + KT <= pg_lo(pw0, p.a.window) && base >= p.a.sinks)) continue;
-        const uint4 *kb = kv[i & 1][odd][0], *vb = kv[i & 1][odd][1];
+        if (wn <= 0 || NG * i + group >= nt || base > pw1 || (p.a.window > 0 && base + KT <= pg_lo(pw0, p.a.window) && base >= p.a.sinks)) continue;
+        const uint4 *kb = kv[i & 1][group][0], *vb = kv[i & 1][group][1];
         qm_f32x16 st[NS];
 #pragma unroll
         for (int n = 0; n < NS; n++) {
@@ -825,11 +831,11 @@ __global__ __launch_bounds__(512, 1) void k_pa_many(PaArgs p) {
             }
     }
     if (__syncthreads_or(wn > 0 && pa_again<E, 16>(o, m, l, seen))) {
-        pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 8);
+        pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 4 * NG);
         return;
     }
     l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
-    if (!pa_merge<E>(o, m, l, (float4 *)kv, (float2 *)where)) return;
+    if (!pa_merge<E, NG>(o, m, l, (float4 *)kv, (float2 *)where)) return;
     if (c < wn) pa_store<T, HD>(p, u, o, m, l, 32 * wave + c, t, hh);
 }
 
@@ -897,7 +903,7 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
     const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
     const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
     auto look = [&](int i0) { /* rows of the tiles i0.. of the part */
-        for (int k = threadIdx.x; k < min(PM_CHUNK, (nt - i0) * KT); k += 256 * NG) {
+        for (int k = threadIdx.x; k < min(CH * NG, nt - i0) * KT; k += 256 * NG) {
             const int j = pg_tile(tl, kt0 + i0 + k / KT) * KT + k % KT;
             where[k] = j <= p1 ? pg_row_at(&p.c, row, j) : -1;
         }
@@ -1032,7 +1038,7 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
     }
     l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
     if constexpr (NG == 2)
-        if (!pa_merge<E>(o, m, l, (float4 *)kv, (float2 *)where)) return;
+        if (!pa_merge<E, NG>(o, m, l, (float4 *)kv, (float2 *)where)) return;
     if (c < wn) pa_store<T, HD>(p, u, o, m, l, 32 * wave + c, t, hh);
 }
 
@@ -1167,7 +1173,7 @@ template <typename T, int HD>
 static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
     const int rt = pa_rows(&p.c, p.a.n, p.a.n_seqs, p.a.h);
     if (rt == PM_RT) {
-        if constexpr (sizeof(T) == 2) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD>, 512, ws, st);
+        if constexpr (sizeof(T) == 2) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD>, 256 * pm_groups(HD), ws, st);
         else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD>, 256 * pm_halves32(HD), ws, st);
     }
     if (rt == 16) return pa_launch_rt<T, HD, 16, PD_KT>(p, k_pa_few<T, HD, 1>, 256, ws, st);
