@@ -658,8 +658,8 @@ __device__ const uint4 pa_zero[32] = {}; /* a row of zeros */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pa_s16x4 *pa_tptr;
 
-/* keys of a tile, and groups of four waves that take tiles in turn */
-constexpr int pm_groups(int hd) { return 2; }
+#define PM_NG 2 /* groups of waves that take tiles in turn */
+/* keys of a tile */
 constexpr int pm_kt(int hd, bool f32 = false) { return hd <= 128 && !f32 ? 64 : 32; }
 
 /* the rows' results of the other groups of four waves into the first one's,
@@ -701,16 +701,17 @@ __device__ __forceinline__ bool pa_merge(qm_f32x16 (&o)[E], float &m, float &l, 
 }
 
 template <int HD>
-__global__ __launch_bounds__(256 * pm_groups(HD), 1) void k_pa_many(PaArgs p) {
+__global__ __launch_bounds__(256 * PM_NG, 1) void k_pa_many(PaArgs p) {
     typedef uint16_t T;
-    constexpr int KT = pm_kt(HD), CR = HD / 8, NB = KT * CR / 256, NS = KT / 32, E = HD / 32, KS = HD / 16, NG = pm_groups(HD);
+    constexpr int KT = pm_kt(HD), CR = HD / 8, NB = KT * CR / 256, NS = KT / 32, E = HD / 32, KS = HD / 16;
+    constexpr int NG = PM_NG;
     constexpr int CH = PM_CHUNK / KT / NG; /* steps per look-up */
     __shared__ __attribute__((aligned(16))) uint4 kv[2][NG][2][KT * CR]; /* buffer, group's tile, k / v */
     __shared__ __attribute__((aligned(16))) ulonglong2 where[PM_CHUNK]; /* addresses of a key's k and v */
     PaUnit u;
     if (!pa_find<PM_RT, KT, false>(p, blockIdx.x, u)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), c = lane & 31, h = lane >> 5;
-    const int group = __builtin_amdgcn_readfirstlane(tid >> 8);
+    const int group = __builtin_amdgcn_readfirstlane(tid / 256);
     const int row0 = u.rtile * PM_RT, rows = u.s.count * p.G, nrow = min(PM_RT, rows - row0);
     const int first = u.s.len - u.s.count;
     const int p0 = first + row0 / p.G, p1 = first + (row0 + nrow - 1) / p.G;
@@ -725,9 +726,11 @@ __global__ __launch_bounds__(256 * pm_groups(HD), 1) void k_pa_many(PaArgs p) {
     const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
 
     const uint64_t zero = (uint64_t)pa_zero;
-    auto look = [&](int i0) { /* rows of the tiles i0.. of the part */
-        for (int k = tid; k < min(CH * NG, nt - i0) * KT; k += 256 * NG) {
-            const int j = pg_tile(tl, kt0 + i0 + k / KT) * KT + k % KT;
+    /* Addresses of the tiles i0.. of the part, zeros past its last: the steps
+     * copy the next step's tiles without asking whether there is one. */
+    auto look = [&](int i0) {
+        for (int k = tid; k < PM_CHUNK; k += 256 * NG) {
+            const int i = i0 + k / KT, j = i < nt ? pg_tile(tl, kt0 + i) * KT + k % KT : -1;
             const int64_t at = j <= p1 ? pg_row_at(&p.c, row, j) : -1;
             ulonglong2 w;
             w.x = at < 0 ? zero : (uint64_t)(kp + at);
@@ -739,23 +742,24 @@ __global__ __launch_bounds__(256 * pm_groups(HD), 1) void k_pa_many(PaArgs p) {
     /* this wave's place in its tile's K; V and the other buffer lie behind */
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(qm_lptr)&kv[0][group][0][0] + 1024 * wave);
     uint64_t vnext = 0;
-    auto copy = [&](int i) { /* step i: this group's tile, NG i + group */
-        vnext = 0;
-        if (NG * i + group >= nt) return;
-        const ulonglong2 *wh = where + (NG * (i % CH) + group) * KT;
-        const uint32_t dst = lds0 + (i & 1) * (NG * 2 * KT * CR * 16);
-#pragma unroll
-        for (int x = 0; x < NB; x++) {
-            const int L = x * 256 + wave * 64 + lane, rr = L / CR, pc = L - rr * CR;
-            const ulonglong2 w = wh[rr];
-            qm_copy<0>((const uint4 *)(w.x + 16 * (pc ^ pa_kswz<CR>(rr))), dst + 4096 * x);
-            qm_copy<0>((const uint4 *)(w.y + 16 * (pc ^ pa_vswz<CR>(rr))), dst + KT * CR * 16 + 4096 * x);
-        }
-        vnext = __ballot(wh[lane & (KT - 1)].x != zero);
+    auto rows_of = [&](int i) { return where + (NG * (i % CH) + group) * KT; };
+    /* this thread's piece x of the group's tile NG i + group, from the row's addresses w */
+    auto piece = [&](int i, int x, ulonglong2 w) {
+        const int L = x * 256 + wave * 64 + lane, rr = L / CR, pc = L - rr * CR;
+        const uint32_t dst = lds0 + (i & 1) * (NG * 2 * KT * CR * 16) + 4096 * x;
+        qm_copy<0>((const uint4 *)(w.x + 16 * (pc ^ pa_kswz<CR>(rr))), dst);
+        qm_copy<0>((const uint4 *)(w.y + 16 * (pc ^ pa_vswz<CR>(rr))), dst + KT * CR * 16);
     };
+    auto row_of = [&](int i, int x) { return rows_of(i)[(x * 256 + wave * 64 + lane) / CR]; };
+    auto copy = [&](int i) {
+#pragma unroll
+        for (int x = 0; x < NB; x++) piece(i, x, row_of(i, x));
+    };
+    auto pages = [&](int i) { return __ballot(rows_of(i)[lane & (KT - 1)].x != zero); };
     if (nt > 0) {
         look(0);
         copy(0);
+        vnext = pages(0);
     }
     const float scale = fabsf(p.a.scale);
     uint4 q[KS];
@@ -781,25 +785,38 @@ __global__ __launch_bounds__(256 * pm_groups(HD), 1) void k_pa_many(PaArgs p) {
     for (int i = 0; i < (nt + NG - 1) / NG; i++) {
         qm_sync<0>(); /* the step's tiles are in LDS; every wave is done with the last step's */
         const uint64_t valid = vnext;
-        if (NG * (i + 1) < nt) {
-            if ((i + 1) % CH == 0) look(NG * (i + 1));
-            copy(i + 1);
-        }
+        if (NG * (i + 1) < nt && (i + 1) % CH == 0) look(NG * (i + 1));
+        vnext = pages(i + 1);
         const int base = pg_tile(tl, kt0 + NG * i + group) * KT;
-        /* nothing of the tile is seen by this wave */
-        if (wn <= 0 || NG * i + group >= nt || base > pw1 || (p.a.window > 0 && base + KT <= pg_lo(pw0, p.a.window) && base >= p.a.sinks)) continue;
         const uint4 *kb = kv[i & 1][group][0], *vb = kv[i & 1][group][1];
         qm_f32x16 st[NS];
+        /* The next step's copies go out between the products: all at the start,
+         * they filled the address unit and held every wave for a fifth of the
+         * step (prompt of 8192: 324 us, so 319).  Past head dim 128 the
+         * registers that this takes cost more than it gives (183 and 207 us
+         * for a prompt of 8000 at 256). */
+        constexpr bool SPREAD = KS <= 8;
+        constexpr int PG = NB / (NS * KS / 4); /* pieces per four products */
+        if constexpr (!SPREAD) copy(i + 1);
 #pragma unroll
         for (int n = 0; n < NS; n++) {
 #pragma unroll
             for (int x = 0; x < 16; x++) st[n][x] = 0.0f;
 #pragma unroll
-            for (int s = 0; s < KS; s++)
-                st[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                    __builtin_bit_cast(qm_bf16x8, kb[(32 * n + c) * CR + ((2 * s + h) ^ pa_kswz<CR>(c))]),
-                    __builtin_bit_cast(qm_bf16x8, q[s]), st[n], 0, 0, 0);
+            for (int s0 = 0; s0 < KS; s0 += 4) {
+                if constexpr (SPREAD) {
+#pragma unroll
+                    for (int x = (n * KS + s0) / 4 * PG; x < ((n * KS + s0) / 4 + 1) * PG; x++) piece(i + 1, x, row_of(i + 1, x));
+                }
+#pragma unroll
+                for (int s = s0; s < s0 + 4; s++)
+                    st[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        __builtin_bit_cast(qm_bf16x8, kb[(32 * n + c) * CR + ((2 * s + h) ^ pa_kswz<CR>(c))]),
+                        __builtin_bit_cast(qm_bf16x8, q[s]), st[n], 0, 0, 0);
+            }
         }
+        /* a wave that sees nothing of the tile has formed scores in vain */
+        if (wn <= 0 || NG * i + group >= nt || base > pw1 || (p.a.window > 0 && base + KT <= pg_lo(pw0, p.a.window) && base >= p.a.sinks)) continue;
 #pragma unroll
         for (int n = 0; n < NS; n++) {
             const uint32_t v32 = (uint32_t)(valid >> (32 * n));
@@ -830,6 +847,7 @@ __global__ __launch_bounds__(256 * pm_groups(HD), 1) void k_pa_many(PaArgs p) {
                 }
             }
     }
+    qm_sync<0>(); /* the last step's copies, of a step that there is not, are done */
     if (__syncthreads_or(wn > 0 && pa_again<E, 16>(o, m, l, seen))) {
         pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 4 * NG);
         return;
@@ -1132,8 +1150,8 @@ static unsigned pa_join_rows(int64_t tasks, int rt) {
     return (unsigned)(r < 1 ? 1 : r > rt ? rt : r);
 }
 
-/* Row tile of the few-row kernel (16 or 32), or PM_RT for the many-row one,
- * by the rows that a sequence has on average. */
+/* Rows of a unit: 16 or 32 of the few-row kernel, or PM_RT of the many-row
+ * one, by the rows that a sequence has on average. */
 static int pa_rows(const pg_cache *c, int n, int n_seqs, int h) {
     const int64_t rows = (int64_t)n * (h / c->kvh);
     if (rows <= (int64_t)16 * n_seqs) return 16;
@@ -1141,8 +1159,8 @@ static int pa_rows(const pg_cache *c, int n, int n_seqs, int h) {
 }
 static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h) {
     const int rt = pa_rows(c, n, n_seqs, h);
-    const int kt = pm_kt(c->hd, c->dtype == QMOE_F32);
-    if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, kt, 256, c->dtype == QMOE_BF16 ? 12 : 2);
+    /* a join costs about 12 bf16 tiles in time, or 2 f32 ones */
+    if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, pm_kt(c->hd, c->dtype == QMOE_F32), 256, c->dtype == QMOE_BF16 ? 12 : 2);
     /* tables of up to 16 tiles (512 rows) are not cut: the join's launch costs
      * more than the shorter run of tiles gives */
     return pa_plan(c, n, n_seqs, h, rt, PD_KT, 1024, c->cap <= 16 * PD_KT ? 17 : 8);
@@ -1173,7 +1191,7 @@ template <typename T, int HD>
 static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
     const int rt = pa_rows(&p.c, p.a.n, p.a.n_seqs, p.a.h);
     if (rt == PM_RT) {
-        if constexpr (sizeof(T) == 2) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD>, 256 * pm_groups(HD), ws, st);
+        if constexpr (sizeof(T) == 2) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD>, 256 * PM_NG, ws, st);
         else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD>, 256 * pm_halves32(HD), ws, st);
     }
     if (rt == 16) return pa_launch_rt<T, HD, 16, PD_KT>(p, k_pa_few<T, HD, 1>, 256, ws, st);
