@@ -654,7 +654,7 @@ __device__ __forceinline__ void pa_store(const PaArgs &p, const PaUnit &u, const
  * Bound: matrix cores and, next to them, LDS (each wave reads the whole tile
  * for 32 rows) and the exponentials. */
 #define PM_CHUNK 1024
-__device__ const uint4 pa_zero[32] = {}; /* a row of zeros */
+__device__ const uint4 pa_zero[64] = {}; /* a row of zeros, up to 1 KB */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pa_s16x4 *pa_tptr;
 
@@ -885,6 +885,14 @@ __device__ __forceinline__ void pa_split8(const float x[8], uint4 w[3]) {
         w[i] = make_uint4(v[0], v[1], v[2], v[3]);
     }
 }
+/* four fp32 -> three bf16 parts */
+__device__ __forceinline__ void pa_split4(float4 x, uint2 w[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        w[i] = make_uint2(qk_cvt_pk_bf16(x.x, x.y), qk_cvt_pk_bf16(x.z, x.w));
+        x = make_float4(x.x - qk_bf16_lo(w[i].x), x.y - qk_bf16_hi(w[i].x), x.z - qk_bf16_lo(w[i].y), x.w - qk_bf16_hi(w[i].y));
+    }
+}
 /* sum of a * b over the parts, the smallest products first */
 __device__ __forceinline__ qm_f32x16 pa_mfma6(const uint4 a[3], const uint4 b[3], qm_f32x16 c) {
     constexpr int ia[6] = {2, 1, 0, 1, 0, 0}, ib[6] = {0, 1, 2, 0, 1, 0};
@@ -900,10 +908,10 @@ constexpr int pm_halves32(int hd) { return hd <= 128 ? 2 : 1; }
 template <int HD>
 __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p) {
     typedef float T;
-    constexpr int KT = 32, CR = HD / 8, NB = KT * CR / 256, E = HD / 32, KS = HD / 16, NG = pm_halves32(HD);
+    constexpr int KT = 32, CR = HD / 8, NB = KT * HD / 1024, E = HD / 32, KS = HD / 16, NG = pm_halves32(HD);
     constexpr int CH = PM_CHUNK / KT / NG; /* steps per look-up */
     __shared__ __attribute__((aligned(16))) uint4 kv[NG][2][3][KT * CR]; /* even / odd tile, k / v, part */
-    __shared__ __attribute__((aligned(16))) int64_t where[PM_CHUNK];
+    __shared__ __attribute__((aligned(16))) ulonglong2 where[PM_CHUNK]; /* addresses of a key's k and v */
     PaUnit u;
     if (!pa_find<PM_RT, KT, false>(p, blockIdx.x, u)) return;
     const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, h = lane >> 5;
@@ -920,48 +928,49 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
     const int hh = pa_head(p, u.kh, r - t * p.G);
     const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
     const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
-    auto look = [&](int i0) { /* rows of the tiles i0.. of the part */
-        for (int k = threadIdx.x; k < min(CH * NG, nt - i0) * KT; k += 256 * NG) {
-            const int j = pg_tile(tl, kt0 + i0 + k / KT) * KT + k % KT;
-            where[k] = j <= p1 ? pg_row_at(&p.c, row, j) : -1;
+    const uint64_t zero = (uint64_t)pa_zero;
+    auto look = [&](int i0) { /* as k_pa_many's */
+        for (int k = threadIdx.x; k < PM_CHUNK; k += 256 * NG) {
+            const int i = i0 + k / KT, j = i < nt ? pg_tile(tl, kt0 + i) * KT + k % KT : -1;
+            const int64_t at = j <= p1 ? pg_row_at(&p.c, row, j) : -1;
+            ulonglong2 w;
+            w.x = at < 0 ? zero : (uint64_t)(kp + at);
+            w.y = at < 0 ? zero : (uint64_t)(vp + at);
+            where[k] = w;
         }
         __syncthreads();
     };
-    float4 kx[NB][2], vx[NB][2];
+    float4 kx[NB], vx[NB]; /* this thread's pieces of four of the next step's tile */
+    auto rows_of = [&](int i) { return where + (NG * (i % CH) + odd) * KT; };
+    auto load_k = [&](int i, int x) {
+        const int L = x * 256 + tid, rr = L / (HD / 4);
+        kx[x] = qk_ld((const float4 *)rows_of(i)[rr].x + (L - rr * (HD / 4)));
+    };
+    auto load_v = [&](int i, int x) {
+        const int L = x * 256 + tid, rr = L / (HD / 4);
+        vx[x] = qk_ld((const float4 *)rows_of(i)[rr].y + (L - rr * (HD / 4)));
+    };
+    auto pages = [&](int i) { return (uint32_t)__ballot(rows_of(i)[lane & 31].x != zero); };
+    auto put = [&](int which, const float4 (&src)[NB]) {
+#pragma unroll
+        for (int x = 0; x < NB; x++) {
+            const int L = x * 256 + tid, rr = L / (HD / 4), q4 = L - rr * (HD / 4), pc = q4 >> 1;
+            const int at = 2 * (rr * CR + (pc ^ (which ? pa_vswz<CR>(rr) : pa_kswz<CR>(rr)))) + (q4 & 1);
+            uint2 w[3];
+            pa_split4(src[x], w);
+#pragma unroll
+            for (int y = 0; y < 3; y++) ((uint2 *)kv[odd][which][y])[at] = w[y];
+        }
+    };
     uint32_t vnext = 0;
-    auto load = [&](int i) { /* step i, this half's tile 2 i + odd, into registers; rows without a page as zeros */
-        vnext = 0;
-        if (NG * i + odd >= nt) return;
-        const int64_t *wh = where + (NG * (i % CH) + odd) * KT;
-#pragma unroll
-        for (int x = 0; x < NB; x++) {
-            const int L = x * 256 + tid, rr = L / CR, pc = L - rr * CR;
-            const int64_t at = wh[rr], safe = at < 0 ? 0 : at;
-            const float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int y = 0; y < 2; y++) {
-                const float4 a = qk_ld((const float4 *)(kp + safe + 8 * pc) + y), b = qk_ld((const float4 *)(vp + safe + 8 * pc) + y);
-                kx[x][y] = at < 0 ? z : a;
-                vx[x][y] = at < 0 ? z : b;
-            }
-        }
-        vnext = (uint32_t)__ballot(wh[lane & 31] >= 0);
-    };
-    auto put = [&](int which, const float4 (&src)[NB][2]) {
-#pragma unroll
-        for (int x = 0; x < NB; x++) {
-            const int L = x * 256 + tid, rr = L / CR, pc = L - rr * CR;
-            const int at = rr * CR + (pc ^ (which ? pa_vswz<CR>(rr) : pa_kswz<CR>(rr)));
-            const float v[8] = {src[x][0].x, src[x][0].y, src[x][0].z, src[x][0].w, src[x][1].x, src[x][1].y, src[x][1].z, src[x][1].w};
-            uint4 w[3];
-            pa_split8(v, w);
-#pragma unroll
-            for (int y = 0; y < 3; y++) kv[odd][which][y][at] = w[y];
-        }
-    };
     if (nt > 0) {
         look(0);
-        load(0);
+#pragma unroll
+        for (int x = 0; x < NB; x++) {
+            load_k(0, x);
+            load_v(0, x);
+        }
+        vnext = pages(0);
     }
     const float scale = fabsf(p.a.scale), sign = p.a.scale < 0.0f ? -1.0f : 1.0f;
     uint4 q[KS][3];
@@ -984,31 +993,34 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
     const int j = lane & 15, g16 = (lane >> 4) & 1, fv = pa_vswz<CR>(j >> 2);
-    if (odd < nt) put(0, kx);
+    if (nt > 0) put(0, kx);
     qk_lds_barrier();
     for (int i = 0; i < (nt + NG - 1) / NG; i++) {
         const uint32_t valid = vnext;
-        const bool mine = NG * i + odd < nt;
         /* K of the step is in LDS, and every wave is done with V of the last */
-        if (mine) put(1, vx);
-        if (NG * (i + 1) < nt) {
-            if ((i + 1) % CH == 0) look(NG * (i + 1));
-            load(i + 1);
-        }
+        put(1, vx);
+        if (NG * (i + 1) < nt && (i + 1) % CH == 0) look(NG * (i + 1));
+        vnext = pages(i + 1);
         const int base = pg_tile(tl, kt0 + NG * i + odd) * KT;
-        const bool act = mine && wn > 0 && base <= pw1 && !(p.a.window > 0 && base + KT <= pg_lo(pw0, p.a.window) && base >= p.a.sinks);
+        const bool act = NG * i + odd < nt && wn > 0 && base <= pw1 &&
+                         !(p.a.window > 0 && base + KT <= pg_lo(pw0, p.a.window) && base >= p.a.sinks);
         qm_f32x16 st[1];
+        const uint4 *kb = kv[odd][0][0];
+#pragma unroll
+        for (int x = 0; x < 16; x++) st[0][x] = 0.0f;
+        /* the next step's loads go out between the products (KS = 2 NB): all
+         * before them, they held every wave for a quarter of the step */
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            if (s & 1) load_v(i + 1, s >> 1);
+            else load_k(i + 1, s >> 1);
+            uint4 a[3];
+#pragma unroll
+            for (int y = 0; y < 3; y++) a[y] = kb[y * KT * CR + c * CR + ((2 * s + h) ^ pa_kswz<CR>(c))];
+            st[0] = pa_mfma6(a, q[s], st[0]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (act) {
-            const uint4 *kb = kv[odd][0][0];
-#pragma unroll
-            for (int x = 0; x < 16; x++) st[0][x] = 0.0f;
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                uint4 a[3];
-#pragma unroll
-                for (int y = 0; y < 3; y++) a[y] = kb[y * KT * CR + c * CR + ((2 * s + h) ^ pa_kswz<CR>(c))];
-                st[0] = pa_mfma6(a, q[s], st[0]);
-            }
             if (valid == 0xFFFFFFFFu && pa_full(p, pw0, pw1, base)) {
                 seen = true;
             } else {
@@ -1023,7 +1035,7 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
             for (int x = 0; x < 16; x++) l += st[0][x];
         }
         qk_lds_barrier(); /* V is in LDS, and every wave has its scores */
-        if (NG * (i + 1) + odd < nt) put(0, kx);
+        put(0, kx);
         if (act) {
             const uint4 *vb = kv[odd][1][0];
 #pragma unroll
