@@ -1008,12 +1008,12 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
         const uint4 *kb = kv[odd][0][0];
 #pragma unroll
         for (int x = 0; x < 16; x++) st[0][x] = 0.0f;
-        /* the next step's loads go out between the products (KS = 2 NB): all
-         * before them, they held every wave for a quarter of the step */
+        /* The next step's loads go out between the products, K's here and V's
+         * beside those of the weights (KS = 2 NB of each): all before them, they
+         * held every wave for a quarter of the step. */
 #pragma unroll
         for (int s = 0; s < KS; s++) {
-            if (s & 1) load_v(i + 1, s >> 1);
-            else load_k(i + 1, s >> 1);
+            if (!(s & 1)) load_k(i + 1, s >> 1);
             uint4 a[3];
 #pragma unroll
             for (int y = 0; y < 3; y++) a[y] = kb[y * KT * CR + c * CR + ((2 * s + h) ^ pa_kswz<CR>(c))];
@@ -1056,9 +1056,14 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
                         const uint2 aw = __builtin_bit_cast(uint2, lo), bw = __builtin_bit_cast(uint2, hi);
                         a[y] = make_uint4(aw.x, aw.y, bw.x, bw.y);
                     }
+                    if (!(d & 1)) load_v(i + 1, s * (E / 2) + (d >> 1));
                     o[d] = pa_mfma6(a, pw, o[d]);
+                    if (d & 1) __builtin_amdgcn_sched_barrier(0);
                 }
             }
+        } else {
+#pragma unroll
+            for (int x = 0; x < NB; x++) load_v(i + 1, x);
         }
         qk_lds_barrier();
     }
