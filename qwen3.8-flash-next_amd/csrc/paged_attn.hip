@@ -1079,7 +1079,7 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
 
 /* ------------------------------------------------------------ join
  * Rows of a task whose keys were cut into parts: lane = dims, up to PJ_FEW
- * parts a wave per row, more the four waves on one row, the parts in turn,
+ * parts a wave per row, more all W waves on one row, the parts in turn,
  * then a sum in wave order.  Bound: the parts read once, and for few rows the
  * latency of the loads. */
 #define PJ_FEW 16
@@ -1089,17 +1089,17 @@ __device__ __forceinline__ void pa_join_out(const PaArgs &p, const PaUnit &u, in
     pa_put4((T *)p.a.out + (int64_t)(u.s.start + t) * p.a.o_token + (int64_t)hh * p.a.o_head + d, y.x * f, y.y * f, y.z * f, y.w * f);
 }
 
-template <typename T, int HD, int RT, int KT>
-__global__ __launch_bounds__(256) void k_pa_join(PaArgs p) {
+template <typename T, int HD, int RT, int KT, int W>
+__global__ __launch_bounds__(64 * W) void k_pa_join(PaArgs p) {
     constexpr int Q = HD / 4; /* lanes of 4 dims */
-    __shared__ __attribute__((aligned(16))) float acc[4][HD];
-    __shared__ float lsum[4];
+    __shared__ __attribute__((aligned(16))) float acc[W][HD];
+    __shared__ float lsum[W];
     PaUnit u;
     if (!pa_find<RT, KT, true>(p, blockIdx.x, u)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const bool few = u.parts <= PJ_FEW;
-    const int step = few ? 1 : 4, i0 = few ? 0 : wave;
-    for (int rr = few ? blockIdx.y * 4 + wave : blockIdx.y; rr < min(RT, u.s.count * p.G - u.rtile * RT); rr += gridDim.y * (few ? 4 : 1)) {
+    const int step = few ? 1 : W, i0 = few ? 0 : wave;
+    for (int rr = few ? blockIdx.y * W + wave : blockIdx.y; rr < min(RT, u.s.count * p.G - u.rtile * RT); rr += gridDim.y * (few ? W : 1)) {
         auto at = [&](int i) { return (int64_t)(u.slot + i * p.c.kvh) * RT + rr; };
         float M = -INFINITY;
         for (int i = lane; i < u.parts; i += 64) M = fmaxf(M, qk_ld((const float *)(p.pml + at(i))));
@@ -1123,12 +1123,14 @@ __global__ __launch_bounds__(256) void k_pa_join(PaArgs p) {
         __syncthreads();
         if (tid < Q) {
             y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            L = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
+            for (int w = 0; w < W; w++) {
                 const float4 z = *(const float4 *)(acc[w] + 4 * tid);
                 y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+                L += lsum[w];
             }
-            pa_join_out<T, HD>(p, u, u.rtile * RT + rr, 4 * tid, y, pa_norm(M, lsum[0] + lsum[1] + lsum[2] + lsum[3]));
+            pa_join_out<T, HD>(p, u, u.rtile * RT + rr, 4 * tid, y, pa_norm(M, L));
         }
         __syncthreads();
     }
@@ -1180,7 +1182,9 @@ static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h) {
     if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, pm_kt(c->hd, c->dtype == QMOE_F32), 256, c->dtype == QMOE_BF16 ? 12 : 2);
     /* tables of up to 16 tiles (512 rows) are not cut: the join's launch costs
      * more than the shorter run of tiles gives */
-    return pa_plan(c, n, n_seqs, h, rt, PD_KT, 1024, c->cap <= 16 * PD_KT ? 17 : 8);
+    const int bytes = c->hd * (c->dtype == QMOE_BF16 ? 2 : 4) * (rt / 16); /* of a row's registers, as pd_occ */
+    const int wgs = bytes <= 128 ? 4 : bytes <= 256 ? 3 : bytes <= 512 ? 2 : 1; /* workgroups that a CU holds */
+    return pa_plan(c, n, n_seqs, h, rt, PD_KT, 256 * wgs, c->cap <= 16 * PD_KT ? 17 : 2);
 }
 
 static size_t pa_up(size_t v) { return (v + 255) / 256 * 256; }
@@ -1200,7 +1204,12 @@ static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), int threads, void *ws,
     hipLaunchKernelGGL(kernel, dim3((unsigned)q.grid), dim3(threads), 0, st, p);
     const int rc = QK_CHECK_LAUNCH();
     if (rc || q.join == 0) return rc;
-    hipLaunchKernelGGL((k_pa_join<T, HD, RT, KT>), dim3((unsigned)q.join, pa_join_rows(q.join, RT)), dim3(256), 0, st, p);
+    /* few tasks are long sequences on their own, a few rows of a hundred parts:
+     * 16 waves a row (one of 64000 rows: 36 us with 4, so 26); else 4 (64 of
+     * 1000: 26 us with 16, so 22) */
+    const dim3 grid((unsigned)q.join, pa_join_rows(q.join, RT));
+    if (q.join <= 16) hipLaunchKernelGGL((k_pa_join<T, HD, RT, KT, 16>), grid, dim3(1024), 0, st, p);
+    else hipLaunchKernelGGL((k_pa_join<T, HD, RT, KT, 4>), grid, dim3(256), 0, st, p);
     return QK_CHECK_LAUNCH();
 }
 
