@@ -658,7 +658,6 @@ __device__ const uint4 pa_zero[64] = {}; /* a row of zeros, up to 1 KB */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pa_s16x4 *pa_tptr;
 
-#define PM_NG 2 /* groups of waves that take tiles in turn */
 /* keys of a tile */
 constexpr int pm_kt(int hd, bool f32 = false) { return hd <= 128 && !f32 ? 64 : 32; }
 
@@ -700,14 +699,13 @@ __device__ __forceinline__ bool pa_merge(qm_f32x16 (&o)[E], float &m, float &l, 
     return group == 0;
 }
 
-template <int HD>
-__global__ __launch_bounds__(256 * PM_NG, 1) void k_pa_many(PaArgs p) {
+template <int HD, int NG>
+__global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
     typedef uint16_t T;
     constexpr int KT = pm_kt(HD), CR = HD / 8, NB = KT * CR / 256, NS = KT / 32, E = HD / 32, KS = HD / 16;
-    constexpr int NG = PM_NG;
-    constexpr int CH = PM_CHUNK / KT / NG; /* steps per look-up */
+    constexpr int KEYS = PM_CHUNK / 2 * NG, CH = KEYS / KT / NG; /* steps per look-up */
     __shared__ __attribute__((aligned(16))) uint4 kv[2][NG][2][KT * CR]; /* buffer, group's tile, k / v */
-    __shared__ __attribute__((aligned(16))) ulonglong2 where[PM_CHUNK]; /* addresses of a key's k and v */
+    __shared__ __attribute__((aligned(16))) ulonglong2 where[KEYS]; /* addresses of a key's k and v */
     PaUnit u;
     if (!pa_find<PM_RT, KT, false>(p, blockIdx.x, u)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), c = lane & 31, h = lane >> 5;
@@ -729,7 +727,7 @@ __global__ __launch_bounds__(256 * PM_NG, 1) void k_pa_many(PaArgs p) {
     /* Addresses of the tiles i0.. of the part, zeros past its last: the steps
      * copy the next step's tiles without asking whether there is one. */
     auto look = [&](int i0) {
-        for (int k = tid; k < PM_CHUNK; k += 256 * NG) {
+        for (int k = tid; k < KEYS; k += 256 * NG) {
             const int i = i0 + k / KT, j = i < nt ? pg_tile(tl, kt0 + i) * KT + k % KT : -1;
             const int64_t at = j <= p1 ? pg_row_at(&p.c, row, j) : -1;
             ulonglong2 w;
@@ -853,7 +851,8 @@ __global__ __launch_bounds__(256 * PM_NG, 1) void k_pa_many(PaArgs p) {
         return;
     }
     l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
-    if (!pa_merge<E, NG>(o, m, l, (float4 *)kv, (float2 *)where)) return;
+    if constexpr (NG > 1)
+        if (!pa_merge<E, NG>(o, m, l, (float4 *)kv, (float2 *)where)) return;
     if (c < wn) pa_store<T, HD>(p, u, o, m, l, 32 * wave + c, t, hh);
 }
 
@@ -1176,6 +1175,14 @@ static int pa_rows(const pg_cache *c, int n, int n_seqs, int h) {
     if (rows <= (int64_t)16 * n_seqs) return 16;
     return rows <= (int64_t)32 * n_seqs ? 32 : PM_RT;
 }
+/* Groups of four waves in a bf16 unit of the many-row kernel.  Two take the
+ * unit's tiles in turn and halve its time; where there are units enough for
+ * several rounds, two workgroups of one group per CU do better, since one
+ * starts and ends under the other's products (prompt of 1000: 27 and 30 us,
+ * of 8192: 320 and 308). */
+static int pa_groups(const pg_cache *c, int n, int h) {
+    return (int64_t)n * (h / c->kvh) / PM_RT * c->kvh >= 1000 && c->hd <= 128 ? 1 : 2;
+}
 static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h) {
     const int rt = pa_rows(c, n, n_seqs, h);
     /* a join costs about 12 bf16 tiles in time, or 2 f32 ones */
@@ -1217,8 +1224,11 @@ template <typename T, int HD>
 static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
     const int rt = pa_rows(&p.c, p.a.n, p.a.n_seqs, p.a.h);
     if (rt == PM_RT) {
-        if constexpr (sizeof(T) == 2) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD>, 256 * PM_NG, ws, st);
-        else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD>, 256 * pm_halves32(HD), ws, st);
+        if constexpr (sizeof(T) == 2) {
+            if constexpr (HD <= 128)
+                if (pa_groups(&p.c, p.a.n, p.a.h) == 1) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 1>, 256, ws, st);
+            return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 2>, 512, ws, st);
+        } else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD>, 256 * pm_halves32(HD), ws, st);
     }
     if (rt == 16) return pa_launch_rt<T, HD, 16, PD_KT>(p, k_pa_few<T, HD, 1>, 256, ws, st);
     return pa_launch_rt<T, HD, 32, PD_KT>(p, k_pa_few<T, HD, 2>, 256, ws, st);
