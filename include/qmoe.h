@@ -741,7 +741,7 @@ typedef struct {
     int sinks;              /* first rows that stay visible behind the window */
     int grouped;            /* 0: head h reads kv head h % n_kv_heads, as qmoe_attn_*;
                              * 1: kv head h / (n_heads / n_kv_heads) */
-    float scale;            /* 0: 1 / sqrt(head_dim) */
+    float scale;            /* 0: 1 / sqrt(head_dim); finite, also times log2(e) */
 } qmoe_paged_query;
 int qmoe_paged_attn(const qmoe_paged_cache *c, int layer, const qmoe_paged_batch *b, const qmoe_paged_query *q,
                     void *ws, size_t ws_bytes, void *stream, qmoe_err *err);

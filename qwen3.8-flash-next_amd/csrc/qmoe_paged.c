@@ -185,7 +185,9 @@ int qmoe_paged_attn(const qmoe_paged_cache *cache, int layer, const qmoe_paged_b
     if (pg_heads(&c, b->n, q->n_heads, err)) return -1;
     if (q->window < 0 || q->sinks < 0) return pg_fail(err, "window %d and sinks %d must be >= 0", q->window, q->sinks);
     if (q->grouped != 0 && q->grouped != 1) return pg_fail(err, "grouped %d is not 0 or 1", q->grouped);
-    if (!isfinite(q->scale)) return pg_fail(err, "scale is not finite");
+    /* the scores are kept in log2 units */
+    const float scale = (float)((q->scale != 0.0f ? (double)q->scale : 1.0 / sqrt((double)c.hd)) * 1.4426950408889634);
+    if (!isfinite(scale)) return pg_fail(err, "scale %g or its product with log2(e) is not finite", (double)q->scale);
     const int es = c.dtype == QMOE_BF16 ? 2 : 4;
     if (pg_stride(q->q_token_stride, b->n, es, "q_token_stride", err) || pg_stride(q->q_head_stride, q->n_heads, es, "q_head_stride", err) ||
         pg_stride(q->out_token_stride, b->n, es, "out_token_stride", err) ||
@@ -212,7 +214,7 @@ int qmoe_paged_attn(const qmoe_paged_cache *cache, int layer, const qmoe_paged_b
     a.window = q->window;
     a.sinks = q->window > 0 ? q->sinks : 0;
     a.grouped = q->grouped;
-    a.scale = (float)((q->scale != 0.0f ? (double)q->scale : 1.0 / sqrt((double)c.hd)) * 1.4426950408889634);
+    a.scale = scale;
     return pg_hip(err, qk_launch_pg_attn(&c, &a, ws, stream), "paged attention");
 }
 

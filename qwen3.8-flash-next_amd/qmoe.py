@@ -1147,8 +1147,11 @@ class PagedCache:
         own, with a window only the last `window` and the first `sinks`.
         Head h reads kv head h % n_kv_heads as the attention mixer's, with
         `grouped` h // (n_heads / n_kv_heads); scale None is
-        1 / sqrt(head_dim).  Rows of no sequence are left as out has them."""
+        1 / sqrt(head_dim).  Rows of no sequence are left as out has them
+        (undefined without out); out must not overlap q or the cache."""
         heads = q.shape[1] if q.dim() == 3 else 0
+        if scale == 0:
+            raise QmoeError("scale must not be 0 (None: 1 / sqrt(head_dim))")
         self._rows(q, heads, self._own, "q")
         n = q.shape[0]
         b, err = self._batch(n, starts, slots), QmoeErr()

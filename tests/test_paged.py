@@ -124,7 +124,8 @@ BAD_ATTN = [
     (dict(), dict(), dict(n_heads=7), 0, "n_heads"), (dict(), dict(n=1 << 29), dict(), 0, "heads are more"),
     (dict(), dict(), dict(window=-1), 0, "window"), (dict(), dict(), dict(sinks=-1), 0, "sinks"),
     (dict(), dict(), dict(grouped=2), 0, "grouped"), (dict(), dict(), dict(scale=float("nan")), 0, "scale"),
-    (dict(), dict(), dict(scale=float("inf")), 0, "scale"), (dict(), dict(), dict(q=None), 0, "q is NULL"),
+    (dict(), dict(), dict(scale=float("inf")), 0, "scale"), (dict(), dict(), dict(scale=-3e38), 0, "scale"),
+    (dict(), dict(), dict(q=None), 0, "q is NULL"),
     (dict(), dict(), dict(out=None), 0, "out is NULL"), (dict(), dict(), dict(q=A + 4), 0, "aligned"),
     (dict(), dict(), dict(out=A + 8), 0, "aligned"), (dict(), dict(), dict(q_token_stride=1025), 0, "q_token_stride"),
     (dict(), dict(), dict(q_head_stride=-128), 0, "q_head_stride"), (dict(), dict(), dict(out_token_stride=512), 0, "overlap"),
