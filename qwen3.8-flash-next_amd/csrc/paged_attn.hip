@@ -31,6 +31,8 @@ struct PaArgs {
     int extra;    /* key tiles that a join is worth (pg_share) */
     float *po;    /* partial O [slot, RT, HD], unscaled */
     float2 *pml;  /* [slot, RT]: maximum (log2 units), sum */
+    int4 *index;  /* [n_seqs], calls of more than PA_INDEX sequences: units, joined tasks
+                   * and split units before the sequence's, its parts */
 };
 
 /* query head of member g of kv head kh's group: heads kh, kh + kvh, ... (the
@@ -97,91 +99,140 @@ __device__ __forceinline__ int pa_scan(int v) {
     return v;
 }
 
-/* Unit `want` of the call (JOIN: the want-th (sequence, row tile, kv head)
- * that has parts to join); false past the last.  Every wave finds it by
- * itself, a lane per run of sequences, without LDS or barriers: this stands
- * before the first load of a page, and a decode call is a few microseconds
- * long.  The total is summed in fp32, in a fixed order. */
-template <int RT, int KT, bool JOIN>
-__device__ __forceinline__ bool pa_find(const PaArgs &p, int want, PaUnit &u) {
-    const int lane = threadIdx.x & 63, n = p.a.n_seqs, per = (n + 63) >> 6;
-    auto seq = [&](int i) { return pg_seq_at(&p.c, p.a.starts, p.a.slots, p.a.n, i); };
-    auto load = [&](const pg_seq &s) { return pg_load_of(s, p.G, RT, p.a.window, p.a.sinks, KT); };
-    pg_seq s0 = {-1, 0, 0, 0};
-    pg_load l0 = {0, 0, 0.0f};
+/* units, tasks that are joined and split units of a sequence */
+struct PaCount {
+    int parts, units, tasks, split;
+};
+__device__ __forceinline__ PaCount pa_count(const PaArgs &p, const pg_load &l, int share) {
+    PaCount c;
+    const int tasks = l.row_tiles * p.c.kvh;
+    c.parts = pg_parts(l.key_tiles, share);
+    c.units = tasks * c.parts;
+    c.tasks = c.parts > 1 ? tasks : 0;
+    c.split = c.parts > 1 ? c.units : 0;
+    return c;
+}
+__device__ __forceinline__ pg_seq pa_seq(const PaArgs &p, int i) { return pg_seq_at(&p.c, p.a.starts, p.a.slots, p.a.n, i); }
+
+/* Batches of more sequences than a wave has lanes: what precedes each one
+ * (units, joined tasks, split units) and its parts, by one workgroup in a
+ * launch of its own, which the units then search.  Units that each went over
+ * all sequences by themselves took 309 us for single tokens of 1024 sequences
+ * of 1000 rows, 198 with the index; of 100 sequences of 200 rows, 11.7 and
+ * 13.0 (the launch), of 1000, 38 and 35.  The total is summed in fp32, in a
+ * fixed order. */
+#define PA_INDEX 64
+__global__ __launch_bounds__(1024) void k_pa_index(PaArgs p, int rt, int kt) {
+    __shared__ float sum[16];
+    __shared__ int before[16][3];
+    const int tid = threadIdx.x, wave = tid >> 6, n = p.a.n_seqs, per = (n + 1023) >> 10;
+    const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    auto load = [&](int i) { return pg_load_of(pa_seq(p, i), p.G, rt, p.a.window, p.a.sinks, kt); };
+    pg_load last = {0, 0, 0.0f};
     float t = 0.0f;
-    for (int k = 0; k < per; k++) {
-        const int i = lane * per + k;
-        if (i < n) {
-            s0 = seq(i);
-            l0 = load(s0);
-            t += l0.work;
-        }
+    for (int i = i0; i < i1; i++) {
+        last = load(i);
+        t += last.work;
     }
     t = qk_group_sum<64>(t);
+    if ((tid & 63) == 0) sum[wave] = t;
+    __syncthreads();
+    t = 0.0f;
+    for (int w = 0; w < 16; w++) t += sum[w];
     const int share = pg_share(t, p.per_unit, p.extra);
-    auto count = [&](const pg_load &l, int &parts, int &units, int &split) {
-        parts = pg_parts(l.key_tiles, share);
-        const int tasks = l.row_tiles * p.c.kvh;
-        split = parts > 1 ? tasks * parts : 0;
-        units = JOIN ? (parts > 1 ? tasks : 0) : tasks * parts;
-    };
-    int parts = 1, units = 0, split = 0;
-    if (per == 1) {
-        count(l0, parts, units, split);
-    } else {
-        for (int k = 0; k < per; k++) {
-            const int i = lane * per + k;
-            if (i < n) {
-                int a, b, c;
-                count(load(seq(i)), a, b, c);
-                units += b;
-                split += c;
+    PaCount all = {0, 0, 0, 0};
+    for (int i = i0; i < i1; i++) {
+        const PaCount c = pa_count(p, per == 1 ? last : load(i), share);
+        all.units += c.units;
+        all.tasks += c.tasks;
+        all.split += c.split;
+    }
+    int x[3] = {pa_scan(all.units), pa_scan(all.tasks), pa_scan(all.split)};
+    if ((tid & 63) == 63)
+        for (int k = 0; k < 3; k++) before[wave][k] = x[k];
+    __syncthreads();
+    for (int k = 0; k < 3; k++)
+        for (int w = 0; w < wave; w++) x[k] += before[w][k];
+    x[0] -= all.units;
+    x[1] -= all.tasks;
+    x[2] -= all.split;
+    for (int i = i0; i < i1; i++) {
+        const PaCount c = pa_count(p, per == 1 ? last : load(i), share);
+        qk_st((float4 *)(p.index + i), __builtin_bit_cast(float4, make_int4(x[0], x[1], x[2], c.parts)));
+        x[0] += c.units;
+        x[1] += c.tasks;
+        x[2] += c.split;
+    }
+}
+
+/* Unit `want` of the call (JOIN: the want-th (sequence, row tile, kv head)
+ * that has parts to join); false past the last.  Every wave finds it by
+ * itself, a lane per sequence (of more: in the index), without LDS or
+ * barriers: this stands before the first load of a page, and a decode call is
+ * a few microseconds long. */
+template <int RT, int KT, bool JOIN>
+__device__ __forceinline__ bool pa_find(const PaArgs &p, int want, PaUnit &u) {
+    const int lane = threadIdx.x & 63, n = p.a.n_seqs;
+    int ubase, sbase; /* units and split units before the sequence's */
+    if (n <= PA_INDEX) {
+        pg_seq s = {-1, 0, 0, 0};
+        pg_load l = {0, 0, 0.0f};
+        if (lane < n) {
+            s = pa_seq(p, lane);
+            l = pg_load_of(s, p.G, RT, p.a.window, p.a.sinks, KT);
+        }
+        const PaCount c = pa_count(p, l, pg_share(qk_group_sum<64>(l.work), p.per_unit, p.extra));
+        const int units = JOIN ? c.tasks : c.units;
+        int ue, se;
+        if (RT == PM_RT) {
+            /* the sequences with the longest parts come first, so that the last
+             * units to start are short ones */
+            const int len = units ? (l.key_tiles + c.parts - 1) / c.parts : 0;
+            ue = se = 0;
+            for (int k = 0; k < n; k++) {
+                const int lk = __builtin_amdgcn_readlane(len, k);
+                const bool before = lk > len || (lk == len && k < lane);
+                ue += before ? __builtin_amdgcn_readlane(units, k) : 0;
+                se += before ? __builtin_amdgcn_readlane(c.split, k) : 0;
             }
+        } else {
+            ue = pa_scan(units) - units;
+            se = pa_scan(c.split) - c.split;
         }
-    }
-    int ue, se; /* units and split units before this lane's */
-    if (RT == PM_RT && per == 1) {
-        /* the sequences with the longest parts come first, so that the last
-         * units to start are short ones */
-        const int len = units ? (l0.key_tiles + parts - 1) / parts : 0;
-        ue = se = 0;
-        for (int k = 0; k < n; k++) {
-            const int lk = __builtin_amdgcn_readlane(len, k);
-            const bool before = lk > len || (lk == len && k < lane);
-            ue += before ? __builtin_amdgcn_readlane(units, k) : 0;
-            se += before ? __builtin_amdgcn_readlane(split, k) : 0;
-        }
+        const uint64_t here = __ballot(want >= ue && want < ue + units);
+        if (!here) return false;
+        const int at = __builtin_ctzll(here);
+        ubase = __builtin_amdgcn_readlane(ue, at);
+        sbase = __builtin_amdgcn_readlane(se, at);
+        u.parts = __builtin_amdgcn_readlane(c.parts, at);
+        u.s.slot = __builtin_amdgcn_readlane(s.slot, at);
+        u.s.start = __builtin_amdgcn_readlane(s.start, at);
+        u.s.count = __builtin_amdgcn_readlane(s.count, at);
+        u.s.len = __builtin_amdgcn_readlane(s.len, at);
     } else {
-        ue = pa_scan(units) - units;
-        se = pa_scan(split) - split;
-    }
-    const uint64_t here = __ballot(want >= ue && want < ue + units);
-    if (!here) return false;
-    const int at = __builtin_ctzll(here);
-    int ubase = __builtin_amdgcn_readlane(ue, at), sbase = __builtin_amdgcn_readlane(se, at);
-    if (per == 1) {
-        u.parts = __builtin_amdgcn_readlane(parts, at);
-        u.s.slot = __builtin_amdgcn_readlane(s0.slot, at);
-        u.s.start = __builtin_amdgcn_readlane(s0.start, at);
-        u.s.count = __builtin_amdgcn_readlane(s0.count, at);
-        u.s.len = __builtin_amdgcn_readlane(s0.len, at);
-    } else {
-        for (int k = 0; k < per; k++) {
-            const pg_seq s = seq(min(at * per + k, n - 1));
-            count(load(s), parts, units, split);
-            u.parts = __builtin_amdgcn_readfirstlane(parts);
-            u.s.slot = __builtin_amdgcn_readfirstlane(s.slot);
-            u.s.start = __builtin_amdgcn_readfirstlane(s.start);
-            u.s.count = __builtin_amdgcn_readfirstlane(s.count);
-            u.s.len = __builtin_amdgcn_readfirstlane(s.len);
-            const int nu = __builtin_amdgcn_readfirstlane(units);
-            if (want < ubase + nu) break;
-            ubase += nu;
-            sbase += __builtin_amdgcn_readfirstlane(split);
+        /* the last sequence with ubase <= want, 64 of the index at a time */
+        int lo = 0, span = n;
+        while (span > 1) {
+            const int step = (span + 63) >> 6;
+            const bool ok = lane * step < span && qk_ld((const int *)(p.index + lo + min(lane * step, span - 1)) + JOIN) <= want;
+            const int c = max(__popcll(__ballot(ok)), 1) - 1;
+            lo += c * step;
+            span = min(step, span - c * step);
         }
+        const int4 x = __builtin_bit_cast(int4, qk_ld((const float4 *)(p.index + lo)));
+        const pg_seq s = pa_seq(p, lo);
+        ubase = __builtin_amdgcn_readfirstlane(JOIN ? x.y : x.x);
+        sbase = __builtin_amdgcn_readfirstlane(x.z);
+        u.parts = __builtin_amdgcn_readfirstlane(x.w);
+        u.s.slot = __builtin_amdgcn_readfirstlane(s.slot);
+        u.s.start = __builtin_amdgcn_readfirstlane(s.start);
+        u.s.count = __builtin_amdgcn_readfirstlane(s.count);
+        u.s.len = __builtin_amdgcn_readfirstlane(s.len);
     }
-    const int rtiles = (u.s.count * p.G + RT - 1) / RT, q = (want - ubase) / p.c.kvh;
+    const int rtiles = (u.s.count * p.G + RT - 1) / RT, tasks = rtiles * p.c.kvh;
+    const int mine = JOIN ? (u.parts > 1 ? tasks : 0) : tasks * u.parts;
+    if ((uint32_t)want - (uint32_t)ubase >= (uint32_t)mine) return false; /* past the last */
+    const int q = (want - ubase) / p.c.kvh;
     u.kh = want - ubase - q * p.c.kvh;
     const int back = JOIN ? q : q / u.parts;
     u.part = JOIN ? 0 : q - back * u.parts;
@@ -1198,7 +1249,8 @@ static size_t pa_up(size_t v) { return (v + 255) / 256 * 256; }
 extern "C" size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h) {
     const PaPlan q = pa_plan_of(c, n, n_seqs, h);
     const int rt = pa_rows(c, n, n_seqs, h);
-    return 256 + pa_up((size_t)q.slots * rt * 8) + pa_up((size_t)q.slots * rt * c->hd * 4);
+    const size_t index = n_seqs > PA_INDEX ? pa_up((size_t)n_seqs * 16) : 0;
+    return 256 + index + pa_up((size_t)q.slots * rt * 8) + pa_up((size_t)q.slots * rt * c->hd * 4);
 }
 
 template <typename T, int HD, int RT, int KT>
@@ -1208,6 +1260,12 @@ static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), int threads, void *ws,
     p.extra = q.extra;
     p.pml = (float2 *)ws;
     p.po = (float *)((char *)ws + pa_up((size_t)q.slots * RT * 8));
+    p.index = (int4 *)((char *)p.po + pa_up((size_t)q.slots * RT * HD * 4));
+    if (p.a.n_seqs > PA_INDEX) {
+        hipLaunchKernelGGL(k_pa_index, dim3(1), dim3(1024), 0, st, p, RT, KT);
+        const int rc = QK_CHECK_LAUNCH();
+        if (rc) return rc;
+    }
     hipLaunchKernelGGL(kernel, dim3((unsigned)q.grid), dim3(threads), 0, st, p);
     const int rc = QK_CHECK_LAUNCH();
     if (rc || q.join == 0) return rc;
@@ -1252,6 +1310,7 @@ extern "C" int qk_launch_pg_attn(const pg_cache *c, const pg_attn *a, void *ws, 
     p.G = a->h / c->kvh;
     p.po = NULL;
     p.pml = NULL;
+    p.index = NULL;
     return c->dtype == QMOE_BF16 ? pa_launch_hd<uint16_t>(p, ws, (hipStream_t)stream)
                                  : pa_launch_hd<float>(p, ws, (hipStream_t)stream);
 }

@@ -121,8 +121,8 @@ QK_HD static inline pg_load pg_load_of(pg_seq s, int G, int rt, int window, int 
  * pg_per_unit(kv heads, units).  total is at least half of the sum of
  * row_tiles * key_tiles, so there are at most 2 units + tasks parts; a task of
  * parts > 1 has 1.5 shares at least, so at most 3 units of them belong to
- * such.  fp32 sums of 1024 terms and a tree are off by less than 2^-13.9, which the
- * factor in per_unit covers. */
+ * such.  fp32 sums of 64 terms and a tree are off by less than 2^-17, which the factor
+ * in per_unit covers. */
 QK_HD static inline float pg_per_unit(int kvh, int units) { return 1.0001f * (float)kvh / (float)units; }
 QK_HD static inline int pg_share(float total, float per_unit, int extra) {
     const float s = total * per_unit;

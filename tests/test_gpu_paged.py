@@ -9,8 +9,11 @@ row's largest scale * sum_i |q_i k_i|:
     and exp2 by a few 2^-24 of it, so p / sum p is off by a factor of at most
     1 + 2 (hd + 24) 2^-24 (B + 1): slack S on A;
   * sums over T keys and the rescalings: 2 (T + 64) 2^-24 of A;
-  * bf16 only: p rounded to bf16 (2^-8 of A: half a step), the output
-    rounded (2^-8 of it).
+  * bf16 only: each weight p_j becomes p_j (1 + e_j), |e_j| <= 2^-8 (half a
+    step), in the product with v and in the sum alike.  With w_j = p_j / sum p
+    and D = sum_j w_j e_j, |D| <= 2^-8, the result is off by
+    sum_j w_j e_j (v_j - out) / (1 + D), at most 2^-8 (A + |out|) / (1 - 2^-8).
+    The output is rounded: 2^-8 of it.
   f32 output rounding: 2^-24 of it.
 """
 import numpy as np
@@ -117,7 +120,7 @@ def reference(q, k, v, n_new, window, sinks, grouped, scale=None, hidden=()):
 def bound(out, A, B, hd, T, dtype):
     tol = A * (2 * (hd + 24) * U * (B + 1) + 2 * (T + 64) * U)
     if dtype == torch.bfloat16:
-        return tol + A * 2.0 ** -8 + out.abs() * 2.0 ** -8 + 1e-38
+        return tol + (A + out.abs()) / 255 + out.abs() * 2.0 ** -8 + 1e-38
     return tol + out.abs() * U + 1e-38
 
 
@@ -177,6 +180,92 @@ def test_longer_batches(dev, lens, counts, dtype):
     s = Setup(dev, HEADS[0 if len(lens) < 100 else 2], dtype, 32, lens, seed=len(lens))
     run_batch(s, counts)
     run_batch(s, counts, window=300, sinks=2)
+
+
+@pytest.mark.parametrize("shape,n", [((40, 1, 128), 16), ((48, 2, 64), 8)], ids=["128", "64"])
+def test_many_units(dev, shape, n):
+    """bf16 calls of more units than fill the card several times over, runs of more than 512 keys among them"""
+    lens = [300 + 37 * i % 500 for i in range(2 * n)]
+    counts = [min(m, 260) if i % 3 else min(m, 300) for i, m in enumerate(lens)]
+    s = Setup(dev, shape, torch.bfloat16, 24, lens, seed=21)
+    assert sum(counts) * shape[0] // 128 >= 1000
+    run_batch(s, counts)
+    run_batch(s, counts, window=130, sinks=70, grouped=True)
+    s.rows[3][5] = -1
+    s.table.copy_(i32(s.rows, dev))
+    s.v[0, s.rows[4][2], 7] = float("nan")  # rows computed one at a time beside the others
+    s.hv[4][55] = float("nan")
+    q, starts = s.queries(counts)
+    out = s.cache.attend(0, q.to(dev), i32(starts, dev))
+    for i in (3, 4, 5):
+        c, a = counts[i], starts[i]
+        want, A, B = reference(q[a:a + c], s.hk[i], s.hv[i], c, 0, 0, False, hidden=[(120, 144)] if i == 3 else ())
+        sees = torch.arange(lens[i] - c, lens[i]) >= 55 if i == 4 else torch.zeros(c, dtype=torch.bool)
+        assert torch.isnan(out[a:a + c].cpu()[sees]).all()
+        check(out[a:a + c].cpu()[~sees], want[~sees], A[~sees], B[~sees], s.hd, lens[i], s.dtype, i)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("shape", [(16, 2, 128), (4, 1, 256), (6, 2, 192), (8, 2, 64)], ids=str)
+def test_many_short_prompts(dev, shape, dtype):
+    """more sequences than a wave has lanes, of more rows than single tokens; parts that are joined"""
+    lens = [40 + (29 * i) % 90 for i in range(100)] + [2000, 0, 1]
+    counts = [20 + i % 21 for i in range(100)] + [70, 0, 1]
+    s = Setup(dev, shape, dtype, 16, lens, seed=22)
+    run_batch(s, counts)
+
+
+@pytest.mark.parametrize("n", [64, 65, 1024, 1025, 5000])
+def test_numbers_of_sequences(dev, n):
+    """single tokens of n sequences of a few rows, a long one among them, some without new rows"""
+    lens = [i % 7 for i in range(n)]
+    lens[n // 3] = 1500
+    s = Setup(dev, (4, 2, 64), torch.bfloat16, 4, lens, seed=n)
+    run_batch(s, [1 if m and i % 11 else 0 for i, m in enumerate(lens)])
+    run_batch(s, [min(m, 70) for m in lens], grouped=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("shape", [(16, 2, 128), (4, 1, 256), (6, 2, 192), (8, 2, 64), (40, 1, 128)], ids=str)
+@pytest.mark.parametrize("lens,counts", [([15000], [1]), ([15000, 3], [2, 0]), ([5000, 300, 2, 4100] * 4, [1, 1, 1, 1] * 4),
+                                         ([6000, 2500, 40, 0], [4, 1, 3, 1])], ids=["one", "one_of_two", "sixteen", "ragged"])
+def test_single_tokens_of_long_sequences(dev, shape, lens, counts, dtype):
+    s = Setup(dev, shape, dtype, 32, lens, seed=23)
+    run_batch(s, counts)
+    run_batch(s, counts, window=2100, sinks=3)
+
+
+def test_forks_of_large_tables(dev):
+    """tables of 60 x 250 entries: sources shared, swapped and cut, refusals, against the tables before"""
+    pkg = load_pkg()
+    slots, width, page = 60, 250, 4
+    c = pkg.PagedCache.allocate(1, 6000, page, 1, 64, slots, width, torch.bfloat16, dev)
+    rng = np.random.RandomState(24)
+    lens = rng.randint(0, 300, slots).tolist()
+    assert int(c.reserve(i32(lens, dev))) == 0
+    t, n = c.table.cpu(), c.lens.cpu()
+    dst = rng.permutation(slots).tolist()
+    src = rng.randint(0, slots, slots).tolist()
+    rows = rng.randint(-1, 400, slots).tolist()
+    for bad in ([dst[1]] + dst[1:], [-1] + dst[1:], [slots] + dst[1:]):
+        assert int(c.fork(i32(src, dev), i32(bad, dev))) == -1
+    assert int(c.fork(i32([slots] + src[1:], dev), i32(dst, dev))) == -1
+    assert torch.equal(c.table.cpu(), t) and torch.equal(c.lens.cpu(), n)
+    assert int(c.fork(i32(src, dev), i32(dst, dev), i32(rows, dev))) == 0
+    for a, b, r in zip(src, dst, rows):
+        m = min(max(r, 0), int(n[a]))
+        e = -(-m // page)
+        assert int(c.lens[b]) == m
+        assert torch.equal(c.table[b].cpu(), torch.cat([t[a, :e], torch.full((width - e,), -1, dtype=torch.int32)]))
+    held = c.table.cpu()[c.table.cpu() >= 0].long()
+    assert torch.equal(c.refs.cpu().long(), torch.bincount(held, minlength=6000))
+
+
+def test_a_scale_of_zero_is_refused(dev):
+    s = Setup(dev, HEADS[2], torch.float32, 8, [20])
+    q, starts = s.queries([2])
+    with pytest.raises(load_pkg().QmoeError, match="scale"):
+        s.cache.attend(0, q.to(dev), i32(starts, dev), scale=0.0)
 
 
 def test_slots_in_any_order_twice_and_out_of_range(dev):
