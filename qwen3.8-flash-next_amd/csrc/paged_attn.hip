@@ -29,6 +29,7 @@ struct PaArgs {
     int G;        /* query heads per kv head */
     float per_unit; /* kv heads / units that the call is cut into, rounded up */
     int extra;    /* key tiles that a join is worth (pg_share) */
+    int one, units; /* the same where no more than `units` units come of it */
     float *po;    /* partial O [slot, RT, HD], unscaled */
     float2 *pml;  /* [slot, RT]: maximum (log2 units), sum */
     int4 *index;  /* [n_seqs], calls of more than PA_INDEX sequences: units, joined tasks
@@ -106,7 +107,7 @@ struct PaCount {
 __device__ __forceinline__ PaCount pa_count(const PaArgs &p, const pg_load &l, int share) {
     PaCount c;
     const int tasks = l.row_tiles * p.c.kvh;
-    c.parts = pg_parts(l.key_tiles, share);
+    c.parts = pg_cuts(l.key_tiles, p.extra) ? pg_parts(l.key_tiles, share) : 1;
     c.units = tasks * c.parts;
     c.tasks = c.parts > 1 ? tasks : 0;
     c.split = c.parts > 1 ? c.units : 0;
@@ -139,18 +140,30 @@ __global__ __launch_bounds__(1024) void k_pa_index(PaArgs p, int rt, int kt) {
     __syncthreads();
     t = 0.0f;
     for (int w = 0; w < 16; w++) t += sum[w];
-    const int share = pg_share(t, p.per_unit, p.extra);
-    PaCount all = {0, 0, 0, 0};
-    for (int i = i0; i < i1; i++) {
-        const PaCount c = pa_count(p, per == 1 ? last : load(i), share);
-        all.units += c.units;
-        all.tasks += c.tasks;
-        all.split += c.split;
+    int share = pg_share(t, p.per_unit, p.one);
+    PaCount all;
+    int x[3];
+    for (;;) { /* twice at most */
+        all = {0, 0, 0, 0};
+        for (int i = i0; i < i1; i++) {
+            const PaCount c = pa_count(p, per == 1 ? last : load(i), share);
+            all.units += c.units;
+            all.tasks += c.tasks;
+            all.split += c.split;
+        }
+        x[0] = pa_scan(all.units);
+        x[1] = pa_scan(all.tasks);
+        x[2] = pa_scan(all.split);
+        if ((tid & 63) == 63)
+            for (int k = 0; k < 3; k++) before[wave][k] = x[k];
+        __syncthreads();
+        int units = 0;
+        for (int w = 0; w < 16; w++) units += before[w][0];
+        const int full = pg_share(t, p.per_unit, p.extra);
+        if (units <= p.units || share == full) break;
+        share = full;
+        __syncthreads();
     }
-    int x[3] = {pa_scan(all.units), pa_scan(all.tasks), pa_scan(all.split)};
-    if ((tid & 63) == 63)
-        for (int k = 0; k < 3; k++) before[wave][k] = x[k];
-    __syncthreads();
     for (int k = 0; k < 3; k++)
         for (int w = 0; w < wave; w++) x[k] += before[w][k];
     x[0] -= all.units;
@@ -181,7 +194,10 @@ __device__ __forceinline__ bool pa_find(const PaArgs &p, int want, PaUnit &u) {
             s = pa_seq(p, lane);
             l = pg_load_of(s, p.G, RT, p.a.window, p.a.sinks, KT);
         }
-        const PaCount c = pa_count(p, l, pg_share(qk_group_sum<64>(l.work), p.per_unit, p.extra));
+        const float total = qk_group_sum<64>(l.work);
+        PaCount c = pa_count(p, l, pg_share(total, p.per_unit, p.one));
+        if (p.one < p.extra && __builtin_amdgcn_readlane(pa_scan(c.units), 63) > p.units)
+            c = pa_count(p, l, pg_share(total, p.per_unit, p.extra));
         const int units = JOIN ? c.tasks : c.units;
         int ue, se;
         if (RT == PM_RT) {
@@ -1191,21 +1207,23 @@ __global__ __launch_bounds__(64 * W) void k_pa_join(PaArgs p) {
 /* how a call is cut: units asked for, the grid that holds them whatever the
  * lengths, tasks that can need a join, and the slots of partial results */
 struct PaPlan {
-    int units, extra;
+    int units, extra, one;
     int64_t grid, join, slots;
 };
 
-static PaPlan pa_plan(const pg_cache *c, int n, int n_seqs, int h, int rt, int kt, int units, int extra) {
+static PaPlan pa_plan(const pg_cache *c, int n, int n_seqs, int h, int rt, int kt, int units, int extra, int one) {
     PaPlan q;
     const int G = h / c->kvh;
     q.units = units;
     q.extra = extra;
+    q.one = one;
     /* sum of ceil(rows / rt) over the sequences that have rows */
     const int64_t rows = (int64_t)n * G, seqs = n_seqs < n ? n_seqs : n;
     const int64_t per_head = rows / rt + seqs < rows ? rows / rt + seqs : rows;
     const int64_t tasks = per_head * c->kvh;
     /* parts of the longest task, then the bounds that pg_share gives */
-    const int64_t parts = pg_parts(c->cap / kt + 2, extra + 1), most = tasks * parts;
+    const int longest = c->cap / kt + 2;
+    const int64_t parts = pg_cuts(longest, extra) ? pg_parts(longest, one + 1) : 1, most = tasks * parts;
     q.grid = most < 2 * (int64_t)units + tasks ? most : 2 * (int64_t)units + tasks;
     q.slots = parts == 1 ? 0 : most < 3 * (int64_t)units ? most : 3 * (int64_t)units;
     q.join = parts == 1 ? 0 : tasks < 3 * (int64_t)units / 2 ? tasks : 3 * (int64_t)units / 2; /* two parts at least */
@@ -1236,13 +1254,17 @@ static int pa_groups(const pg_cache *c, int n, int h) {
 }
 static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h) {
     const int rt = pa_rows(c, n, n_seqs, h);
-    /* a join costs about 12 bf16 tiles in time, or 2 f32 ones */
-    if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, pm_kt(c->hd, c->dtype == QMOE_F32), 256, c->dtype == QMOE_BF16 ? 12 : 2);
+    /* A join costs about 12 bf16 tiles in time, or 2 f32 ones.  Where all units
+     * run at once it costs 3, since the others fill CUs that had nothing to do:
+     * 64 tokens on 3000 rows 40 us with 12, so 33, on 4000 rows in 16 sequences
+     * 81 and 70; but a prompt of 2000 (256 tasks) 46 with 12 and 59 with 3. */
+    if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, pm_kt(c->hd, c->dtype == QMOE_F32), 256, c->dtype == QMOE_BF16 ? 12 : 2, c->dtype == QMOE_BF16 ? 3 : 2);
     /* tables of up to 16 tiles (512 rows) are not cut: the join's launch costs
      * more than the shorter run of tiles gives */
     const int bytes = c->hd * (c->dtype == QMOE_BF16 ? 2 : 4) * (rt / 16); /* of a row's registers, as pd_occ */
     const int wgs = bytes <= 128 ? 4 : bytes <= 256 ? 3 : bytes <= 512 ? 2 : 1; /* workgroups that a CU holds */
-    return pa_plan(c, n, n_seqs, h, rt, PD_KT, 256 * wgs, c->cap <= 16 * PD_KT ? 17 : 2);
+    const int extra = c->cap <= 16 * PD_KT ? 17 : 2;
+    return pa_plan(c, n, n_seqs, h, rt, PD_KT, 256 * wgs, extra, extra);
 }
 
 static size_t pa_up(size_t v) { return (v + 255) / 256 * 256; }
@@ -1258,6 +1280,8 @@ static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), int threads, void *ws,
     const PaPlan q = pa_plan_of(&p.c, p.a.n, p.a.n_seqs, p.a.h);
     p.per_unit = pg_per_unit(p.c.kvh, q.units);
     p.extra = q.extra;
+    p.one = q.one;
+    p.units = q.units;
     p.pml = (float2 *)ws;
     p.po = (float *)((char *)ws + pa_up((size_t)q.slots * RT * 8));
     p.index = (int4 *)((char *)p.po + pa_up((size_t)q.slots * RT * HD * 4));

@@ -121,19 +121,25 @@ QK_HD static inline pg_load pg_load_of(pg_seq s, int G, int rt, int window, int 
  * pg_per_unit(kv heads, units).  total is at least half of the sum of
  * row_tiles * key_tiles, so there are at most 2 units + tasks parts; a task of
  * parts > 1 has 1.5 shares at least, so at most 3 units of them belong to
- * such.  fp32 sums of 64 terms and a tree are off by less than 2^-17, which the factor
- * in per_unit covers. */
+ * such.  fp32 sums of 64 terms and a tree are off by less than 2^-17, which the
+ * factor in per_unit covers. */
 QK_HD static inline float pg_per_unit(int kvh, int units) { return 1.0001f * (float)kvh / (float)units; }
 QK_HD static inline int pg_share(float total, float per_unit, int extra) {
     const float s = total * per_unit;
     return (s < 1e9f ? (int)s : 1000000000) + 1 + extra;
 }
-/* to the nearest: a task of 1.4 shares is not worth a join */
+/* a task that is cut at all: into two parts by the smallest share there is */
+QK_HD static inline int pg_cuts(int key_tiles, int extra) { return key_tiles + (extra + 1) / 2 >= 2 * (extra + 1); }
+/* to the nearest: a task of 1.4 shares is not worth a join.  Key tiles and
+ * shares are below 2^30 each. */
 QK_HD static inline int pg_parts(int key_tiles, int share) {
-    const int n = (int)(((int64_t)key_tiles + share / 2) / share);
+    const int n = (int)(((uint32_t)key_tiles + (uint32_t)share / 2) / (uint32_t)share);
     return n < 1 ? 1 : n;
 }
-/* first of nt key tiles of part i */
-QK_HD static inline int pg_part(int nt, int i, int parts) { return (int)((int64_t)nt * i / parts); }
+/* first of nt key tiles of part i: the first nt % parts parts have one more */
+QK_HD static inline int pg_part(int nt, int i, int parts) {
+    const uint32_t q = (uint32_t)nt / (uint32_t)parts, r = (uint32_t)nt - q * (uint32_t)parts;
+    return (int)(q * (uint32_t)i) + pg_min(i, (int)r);
+}
 
 #endif
