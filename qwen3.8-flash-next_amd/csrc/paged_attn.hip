@@ -1238,11 +1238,31 @@ static unsigned pa_join_rows(int64_t tasks, int rt) {
 }
 
 /* Rows of a unit: 16 or 32 of the few-row kernel, or PM_RT of the many-row
- * one, by the rows that a sequence has on average. */
-static int pa_rows(const pg_cache *c, int n, int n_seqs, int h) {
-    const int64_t rows = (int64_t)n * (h / c->kvh);
+ * one.  Units of 16 rows read a page once per 16 rows, but start at once and
+ * have a short step: they are better as long as the call is short, measured by
+ * their number times the rows of a table (or the window): 32 tokens on 1000
+ * rows 27 us with 128 rows and 14.5 with 16, on 4000 rows of 4 sequences 30
+ * and 39; f32 31 and 20, 52 and 73.  The limits are where the two meet, over 1
+ * to 16 sequences, 1000 to 16000 rows and all head dims; f32 kernels past head
+ * dim 128 lack registers for more rows (8 tokens of 16 sequences on 4000 rows
+ * at 256: 151 and 71), and units of 32 rows take over at half the limit (4
+ * tokens of 16 sequences on 4000 rows 29 and 34).  Up to 8 units are 16 rows
+ * each whatever the table holds, which may be much more than the sequences
+ * have (8 tokens on 1000 rows 23 and 15, on 16000 22 and 23).  Past the limit,
+ * by the rows that a sequence has on average; 32 where the registers hold
+ * them. */
+static bool pa_two(const pg_cache *c) { return c->dtype == QMOE_BF16 ? c->hd <= 192 : c->hd <= 128; }
+static int pa_rows_long(const pg_cache *c, int64_t rows, int n_seqs) {
     if (rows <= (int64_t)16 * n_seqs) return 16;
-    return rows <= (int64_t)32 * n_seqs ? 32 : PM_RT;
+    return rows > (int64_t)32 * n_seqs ? PM_RT : pa_two(c) ? 32 : 16;
+}
+static int pa_rows(const pg_cache *c, const pg_attn *a) {
+    const int64_t rows = (int64_t)a->n * (a->h / c->kvh), units = rows * c->kvh / 16;
+    const int later = pa_rows_long(c, rows, a->n_seqs);
+    int64_t keys = c->cap, most = c->dtype == QMOE_BF16 || c->hd == 64 ? 1 << 18 : c->hd < 256 ? 1 << 17 : 1 << 19;
+    if (a->window > 0 && (int64_t)a->window + a->sinks < keys) keys = (int64_t)a->window + a->sinks;
+    if (later == 32) most /= 2;
+    return units <= 8 || units * keys <= most ? 16 : later;
 }
 /* Groups of four waves in a bf16 unit of the many-row kernel.  Two take the
  * unit's tiles in turn and halve its time; where there are units enough for
@@ -1252,8 +1272,7 @@ static int pa_rows(const pg_cache *c, int n, int n_seqs, int h) {
 static int pa_groups(const pg_cache *c, int n, int h) {
     return (int64_t)n * (h / c->kvh) / PM_RT * c->kvh >= 1000 && c->hd <= 128 ? 1 : 2;
 }
-static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h) {
-    const int rt = pa_rows(c, n, n_seqs, h);
+static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h, int rt) {
     /* A join costs about 12 bf16 tiles in time, or 2 f32 ones.  Where all units
      * run at once it costs 3, since the others fill CUs that had nothing to do:
      * 64 tokens on 3000 rows 40 us with 12, so 33, on 4000 rows in 16 sequences
@@ -1268,16 +1287,20 @@ static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h) {
 }
 
 static size_t pa_up(size_t v) { return (v + 255) / 256 * 256; }
-extern "C" size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h) {
-    const PaPlan q = pa_plan_of(c, n, n_seqs, h);
-    const int rt = pa_rows(c, n, n_seqs, h);
+static size_t pa_ws(const pg_cache *c, int n, int n_seqs, int h, int rt) {
+    const PaPlan q = pa_plan_of(c, n, n_seqs, h, rt);
     const size_t index = n_seqs > PA_INDEX ? pa_up((size_t)n_seqs * 16) : 0;
     return 256 + index + pa_up((size_t)q.slots * rt * 8) + pa_up((size_t)q.slots * rt * c->hd * 4);
+}
+/* of either choice of rows: the window is not known here */
+extern "C" size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h) {
+    const size_t a = pa_ws(c, n, n_seqs, h, 16), b = pa_ws(c, n, n_seqs, h, pa_rows_long(c, (int64_t)n * (h / c->kvh), n_seqs));
+    return a > b ? a : b;
 }
 
 template <typename T, int HD, int RT, int KT>
 static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), int threads, void *ws, hipStream_t st) {
-    const PaPlan q = pa_plan_of(&p.c, p.a.n, p.a.n_seqs, p.a.h);
+    const PaPlan q = pa_plan_of(&p.c, p.a.n, p.a.n_seqs, p.a.h, RT);
     p.per_unit = pg_per_unit(p.c.kvh, q.units);
     p.extra = q.extra;
     p.one = q.one;
@@ -1304,7 +1327,7 @@ static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), int threads, void *ws,
 
 template <typename T, int HD>
 static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
-    const int rt = pa_rows(&p.c, p.a.n, p.a.n_seqs, p.a.h);
+    const int rt = pa_rows(&p.c, &p.a);
     if (rt == PM_RT) {
         if constexpr (sizeof(T) == 2) {
             if constexpr (HD <= 128)
@@ -1312,8 +1335,9 @@ static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
             return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 2>, 512, ws, st);
         } else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD>, 256 * pm_halves32(HD), ws, st);
     }
-    if (rt == 16) return pa_launch_rt<T, HD, 16, PD_KT>(p, k_pa_few<T, HD, 1>, 256, ws, st);
-    return pa_launch_rt<T, HD, 32, PD_KT>(p, k_pa_few<T, HD, 2>, 256, ws, st);
+    if constexpr (HD <= (sizeof(T) == 2 ? 192 : 128)) /* pa_two */
+        if (rt == 32) return pa_launch_rt<T, HD, 32, PD_KT>(p, k_pa_few<T, HD, 2>, 256, ws, st);
+    return pa_launch_rt<T, HD, 16, PD_KT>(p, k_pa_few<T, HD, 1>, 256, ws, st);
 }
 
 template <typename T>
