@@ -39,7 +39,10 @@ def i32(x, dev):
 
 class Setup:
     """a cache with random pages for sequences of given lengths; the pages'
-    unused rows and the free pages hold `junk`"""
+    unused rows and the free pages hold `junk`.  The table has room for
+    `table_rows` rows at the least: short calls on short tables run on units
+    of few rows, whatever the calls' own."""
+    table_rows = 0
 
     def __init__(self, dev, shape, dtype, page, lens, seed=0, layers=1, spare=4, junk=0.0, order="rows", slots=None):
         self.h, self.kvh, self.hd = shape
@@ -71,15 +74,22 @@ class Setup:
                 m = min(page, n - j0)
                 self.k[layers - 1, self.rows[s][j0 // page], :m] = kk[j0:j0 + m].to(dev)
                 self.v[layers - 1, self.rows[s][j0 // page], :m] = vv[j0:j0 + m].to(dev)
-        self.table, self.refs = i32(self.rows, dev), i32(refs, dev)
+        self.full = torch.full((n_slots, max(width, -(-self.table_rows // page))), -1, dtype=torch.int32, device=dev)
+        self.table, self.refs = self.full[:, :width], i32(refs, dev)
+        self.table.copy_(i32(self.rows, dev))
         self.len_t = i32(list(lens) + [0] * (n_slots - len(lens)), dev)
-        self.cache = load_pkg().PagedCache(self.k, self.v, self.table, self.len_t, self.refs)
+        self.cache = load_pkg().PagedCache(self.k, self.v, self.full, self.len_t, self.refs)
         self.g = g
 
     def queries(self, counts):
         starts = np.concatenate([[0], np.cumsum(counts)]).tolist()
         q = torch.randn(starts[-1], self.h, self.hd, generator=self.g).to(self.dtype)
         return q, starts
+
+
+@pytest.fixture(params=[0, 1 << 20], ids=["short", "long"])
+def tables(request, monkeypatch):
+    monkeypatch.setattr(Setup, "table_rows", request.param)
 
 
 def reference(q, k, v, n_new, window, sinks, grouped, scale=None, hidden=()):
@@ -151,6 +161,7 @@ def run_batch(s, counts, window=0, sinks=0, grouped=False, scale=None, slots=Non
     return q, starts, out
 
 
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("page", [1, 5, 16, 24, 64, 100])
 @pytest.mark.parametrize("shape", range(len(HEADS)))
@@ -172,6 +183,7 @@ def test_windows_and_sinks(dev, window, sinks, dtype):
         run_batch(s, counts, window=window, sinks=sinks, grouped=shape == 1)
 
 
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("lens,counts", [([2500], [2500]), ([4000, 10], [1, 10]), ([3000] * 3, [2, 130, 600]),
                                          ([9000], [64]), ([70] * 200, [1] * 200), ([50] * 700, [1, 0] * 350)],
@@ -182,29 +194,58 @@ def test_longer_batches(dev, lens, counts, dtype):
     run_batch(s, counts, window=300, sinks=2)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("shape,n", [((40, 1, 128), 16), ((48, 2, 64), 8)], ids=["128", "64"])
-def test_many_units(dev, shape, n):
-    """bf16 calls of more units than fill the card several times over, runs of more than 512 keys among them"""
+def test_many_units(dev, shape, n, dtype):
+    """calls of more units than fill the card several times over, runs of more than 512 keys among them"""
     lens = [300 + 37 * i % 500 for i in range(2 * n)]
     counts = [min(m, 260) if i % 3 else min(m, 300) for i, m in enumerate(lens)]
-    s = Setup(dev, shape, torch.bfloat16, 24, lens, seed=21)
+    s = Setup(dev, shape, dtype, 24, lens, seed=21)
     assert sum(counts) * shape[0] // 128 >= 1000
     run_batch(s, counts)
     run_batch(s, counts, window=130, sinks=70, grouped=True)
     s.rows[3][5] = -1
     s.table.copy_(i32(s.rows, dev))
-    s.v[0, s.rows[4][2], 7] = float("nan")  # rows computed one at a time beside the others
-    s.hv[4][55] = float("nan")
+    s.v[0, s.rows[4][4], 4] = float("nan")  # key 100: its unit is computed one row at a time beside the others
+    s.hv[4][100] = float("nan")
     q, starts = s.queries(counts)
-    out = s.cache.attend(0, q.to(dev), i32(starts, dev))
-    for i in (3, 4, 5):
-        c, a = counts[i], starts[i]
-        want, A, B = reference(q[a:a + c], s.hk[i], s.hv[i], c, 0, 0, False, hidden=[(120, 144)] if i == 3 else ())
-        sees = torch.arange(lens[i] - c, lens[i]) >= 55 if i == 4 else torch.zeros(c, dtype=torch.bool)
-        assert torch.isnan(out[a:a + c].cpu()[sees]).all()
-        check(out[a:a + c].cpu()[~sees], want[~sees], A[~sees], B[~sees], s.hd, lens[i], s.dtype, i)
+    for window, sinks in ((0, 0), (130, 70)):
+        out = s.cache.attend(0, q.to(dev), i32(starts, dev), window=window, sinks=sinks)
+        for i in (3, 4, 5):
+            c, a = counts[i], starts[i]
+            want, A, B = reference(q[a:a + c], s.hk[i], s.hv[i], c, window, sinks, False, hidden=[(120, 144)] if i == 3 else ())
+            pos = torch.arange(lens[i] - c, lens[i])
+            sees = (pos >= 100) & ((pos < 230) | (window == 0)) & (i == 4)
+            assert torch.isnan(out[a:a + c].cpu()[sees]).all()
+            check(out[a:a + c].cpu()[~sees], want[~sees], A[~sees], B[~sees], s.hd, lens[i], dtype, (i, window))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("shape,window,sinks", [((64, 1, 64), 32, 0), ((64, 1, 64), 33, 40), ((32, 1, 128), 64, 4),
+                                                ((32, 1, 192), 100, 0), ((32, 1, 256), 130, 9)], ids=str)
+def test_windows_of_long_prompts(dev, shape, window, sinks, dtype):
+    """small windows on units of many rows"""
+    lens, counts = [713, 513, 900, 20, 0], [700, 513, 900, 1, 0]
+    s = Setup(dev, shape, dtype, 20, lens, seed=25)
+    run_batch(s, counts, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("hd", [64, 128, 192, 256])
+def test_a_few_tokens_per_sequence(dev, hd, dtype, monkeypatch):
+    """17 to 32 rows a sequence on long tables"""
+    monkeypatch.setattr(Setup, "table_rows", 1 << 18)
+    lens = [7000, 300, 3, 33, 64, 65, 700, 1, 90, 128, 513, 2, 40, 800, 77, 1000]
+    counts = [min(m, 2 + i % 4) for i, m in enumerate(lens)]
+    s = Setup(dev, (8, 1, hd), dtype, 16, lens, seed=26)
+    run_batch(s, counts)
+    run_batch(s, counts, window=6500, sinks=5)
+    s.rows[6][3] = s.rows[0][100] = -1
+    s.table.copy_(i32(s.rows, dev))
+    run_batch(s, counts, hidden={6: [(48, 64)], 0: [(1600, 1616)]})
+
+
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("shape", [(16, 2, 128), (4, 1, 256), (6, 2, 192), (8, 2, 64)], ids=str)
 def test_many_short_prompts(dev, shape, dtype):
@@ -268,6 +309,7 @@ def test_a_scale_of_zero_is_refused(dev):
         s.cache.attend(0, q.to(dev), i32(starts, dev), scale=0.0)
 
 
+@pytest.mark.usefixtures("tables")
 def test_slots_in_any_order_twice_and_out_of_range(dev):
     s = Setup(dev, HEADS[0], torch.bfloat16, 16, [100, 40, 77, 260], seed=3)
     run_batch(s, [1, 6, 1, 30, 2], slots=[2, 0, 2, 3, 0])
@@ -284,6 +326,7 @@ def test_scale_and_layer(dev):
     run_batch(s, [5, 2], scale=-0.25, layer=2)
 
 
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("counts", [[1, 1, 1], [40, 33, 90]], ids=["tokens", "chunks"])
 def test_released_and_bad_pages_are_not_seen(dev, counts, dtype):
@@ -317,6 +360,7 @@ def test_lengths_and_starts_out_of_range_are_clamped(dev):
     assert (guard[0] == 7).all() and (guard[7] == 7).all()
 
 
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 def test_rows_of_no_sequence_are_left_alone(dev, dtype):
     s = Setup(dev, HEADS[0], dtype, 16, [100, 30], seed=7)
@@ -330,6 +374,7 @@ def test_rows_of_no_sequence_are_left_alone(dev, dtype):
             check(out[starts[i + 1]:starts[i + 2]], want, A, B, s.hd, 100, dtype, i)
 
 
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("junk", [float("nan"), float("inf"), -3e38])
 @pytest.mark.parametrize("counts", [[1, 4, 1], [33, 80, 64]], ids=["tokens", "chunks"])
@@ -377,6 +422,7 @@ def test_what_unseen_rows_hold_does_not_matter(dev, counts, junk, dtype):
         check(y, want[blind], A[blind], B[blind], 128, 100, dtype, (i, "junk"))
 
 
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("counts", [[1, 1], [40, 50]], ids=["tokens", "chunks"])
 def test_infinite_scores_follow_the_formula(dev, counts, dtype):
@@ -399,6 +445,7 @@ def test_infinite_scores_follow_the_formula(dev, counts, dtype):
     check(out[:counts[0]][pos < 20], want[pos < 20], A[pos < 20], B[pos < 20], 128, 60, dtype, "before +inf")
 
 
+@pytest.mark.usefixtures("tables")
 def test_large_scores(dev):
     """scores of hundreds: the running maximum is subtracted before exp"""
     for dtype in (torch.bfloat16, torch.float32):
@@ -411,6 +458,7 @@ def test_large_scores(dev):
         run_batch(s, [90, 130])
 
 
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 def test_strides(dev, dtype):
     """heads before rows in the pages, heads before tokens in q and out, k and v interleaved"""
@@ -426,7 +474,7 @@ def test_strides(dev, dtype):
     assert torch.equal(out, same)
     assert (big[:, :4] == 9).all() and (big[:, 35:] == 9).all() and (big[:, :, 0] == 9).all() and (big[:, :, 2] == 9).all()
     pool = torch.stack([s.k, s.v], 2)  # [1, pages, 2, rows, heads, dim]
-    both = load_pkg().PagedCache(pool[:, :, 0], pool[:, :, 1], s.table, s.len_t, s.refs)
+    both = load_pkg().PagedCache(pool[:, :, 0], pool[:, :, 1], s.full, s.len_t, s.refs)
     assert torch.equal(both.attend(0, q.to(dev), i32(starts, dev)), same)
     # a broadcast query
     one = torch.randn(1, 16, 128, generator=s.g).to(dtype).to(dev)
@@ -447,13 +495,17 @@ def test_offsets_past_32_bits(dev, dtype):
     pkg = load_pkg()
     cache = pkg.PagedCache(k, v, i32([ids], dev), i32([T], dev), torch.zeros(n_pages, dtype=torch.int32, device=dev))
     cache.append(0, hk.to(dev), hv.to(dev), i32([0, T], dev))
-    for c in (1, 100):
+    wide = torch.full((1, 1 << 14), -1, dtype=torch.int32, device=dev)
+    wide[0, :4] = i32(ids, dev)
+    for c, table in ((1, cache.table), (100, cache.table), (100, wide)):
+        cache = pkg.PagedCache(k, v, table, cache.lens, cache.refs)
         q = torch.randn(c, 16, hd, generator=g).to(dtype)
         out = cache.attend(0, q.to(dev), i32([0, c], dev))
         want, A, B = reference(q, hk, hv, c, 0, 0, False)
         check(out, want, A, B, hd, T, dtype, c)
 
 
+@pytest.mark.usefixtures("tables")
 def test_results_repeat_to_the_bit(dev):
     for dtype in (torch.bfloat16, torch.float32):
         s = Setup(dev, HEADS[0], dtype, 16, [3000, 100, 777], seed=13)
