@@ -437,7 +437,11 @@ __device__ __forceinline__ bool pa_again(const V (&o)[N], float m, float l, bool
  * (two keys' words, one byte permute), and O^T's row x of tile e is dim
  * (HD / 16) x + e.  f32 runs on the fp32 matrix instructions, whose operands
  * are single elements.
- * Bound: HBM, the visible pages read once. */
+ * Bound: HBM, the visible pages read once: single tokens of 64 sequences of 64
+ * to 65536 rows (841 MB of bf16) 171 to 178 us, 4.8 TB/s, of 1024 of 1000
+ * rows 198 us, 5.3 TB/s; f32 under a window of 1024, 32 sequences (68 MB) 25 us,
+ * where starting, the join of the waves and the one run of eight tiles a wave
+ * count; a token on 333 rows 10 us, latency. */
 #define PD_KT 32
 typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
 
@@ -710,17 +714,25 @@ __device__ __forceinline__ void pa_store(const PaArgs &p, const PaUnit &u, const
 }
 
 /* ------------------------------------------------------------ many rows
- * Prompts, bf16: a unit is 128 rows, 32 per wave, and a part of the keys.
- * Tiles of KT keys of K and V are copied straight from the pages to LDS, two
- * buffers, one barrier per tile.  The copies' lanes pick the 16-byte pieces,
- * so a tile lies in rows with its pieces exchanged by the row's number (an
- * xor): K's operand reads (a lane per row) and V's transposing reads (a lane
- * per dim, four keys) then meet no bank twice.  Where a tile's rows lie is
- * looked up for 1024 keys at a time; a row without a page or after the last
- * query is copied from a piece of zeros.
- * Bound: matrix cores and, next to them, LDS (each wave reads the whole tile
- * for 32 rows) and the exponentials. */
-#define PM_CHUNK 1024
+ * Prompts, bf16: a unit is 128 rows, 32 per wave, and a part of the keys; NG
+ * groups of four waves take its tiles in turn and are added at the end
+ * (pa_merge).  Tiles of KT keys of K and V are copied straight from the pages
+ * to LDS, two buffers, one barrier per step.  The copies' lanes pick the
+ * 16-byte pieces, so a tile lies in rows with its pieces exchanged by the
+ * row's number (an xor): K's operand reads (a lane per row) and V's transposing
+ * reads (a lane per dim, four keys) then meet no bank twice (with the xor made
+ * for 32 banks, conflicts were a fifth of the cycles).  Where a tile's rows lie
+ * is looked up for 512 keys a group at a time; a row without a page or after
+ * the last query is copied from a row of zeros.
+ * Bound: a wave's own chain of a step.  A prompt of 8192 (16 heads on 2 of 128)
+ * takes 297 to 309 us, 890 to 925 TFLOP/s of 1180 of a large library product.  A
+ * step of 5400 clocks was scores 1200, maximum and exponentials 1200, sums of
+ * v 1250, issuing the copies 1100 (now between the products) and waiting at
+ * the barrier 100 to 970; the matrix cores work 40 % of it.  Without gain: a
+ * raised wave priority in either half, two groups half a step apart (360 us),
+ * scores of the next tile beside the softmax (337 to 348), three groups (326),
+ * units of 64 rows (short prompts 10 % better, long contexts 40 % worse). */
+#define PM_CHUNK 1024 /* keys of a look-up of two groups */
 __device__ const uint4 pa_zero[64] = {}; /* a row of zeros, up to 1 KB */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pa_s16x4 *pa_tptr;
@@ -926,13 +938,17 @@ __global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
 /* ------------------------------------------------------------ many rows, f32
  * The same unit at fp32 precision: K, V, Q and the weights as three bf16
  * parts each (hi + mid + lo, 24 bits) and six of the nine partial products
- * (the others are below 2^-24 of them), which run at 417 TFLOP/s against 157
+ * (the others are below 2^-24 of them), whose peak is 417 TFLOP/s against 157
  * of the fp32 instructions.  A tile is 32 keys; its rows come through
- * registers, where the workgroup splits them once for its four waves, into
- * one LDS buffer for K and one for V: V is written while the scores are
- * formed, the next tile's K while V is multiplied, one barrier after each.  Infinities, NaN and values that round to a bf16 infinity have no
- * parts: their differences are NaN, and the unit is computed again (pa_again).
- * Bound: matrix cores, six products per tile. */
+ * registers, where a group of four waves splits them once, into one LDS buffer
+ * for K and one for V: V is written while the scores are formed, the next
+ * tile's K while V is multiplied, one barrier after each.  Infinities, NaN and
+ * values that round to a bf16 infinity have no parts: their differences are
+ * NaN, and the unit is computed again (pa_again).
+ * Bound: matrix cores, six products per tile, and the splitting beside them:
+ * three prompt chunks and 29 single tokens on up to 6000 rows (25 GFLOP) 203
+ * us with the join, 125 TFLOP/s against 154 of a large library product in fp32;
+ * fp32 instructions took 631 us. */
 
 /* eight fp32 -> three bf16 parts */
 __device__ __forceinline__ void pa_split8(const float x[8], uint4 w[3]) {
@@ -1147,7 +1163,9 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
  * Rows of a task whose keys were cut into parts: lane = dims, up to PJ_FEW
  * parts a wave per row, more all W waves on one row, the parts in turn,
  * then a sum in wave order.  Bound: the parts read once, and for few rows the
- * latency of the loads. */
+ * latency of the loads: 5 us where little is cut, 10 us after 64 sequences of up
+ * to 65536 rows.  The launch is made wherever the tables are long enough for
+ * parts, since only the device knows the lengths. */
 #define PJ_FEW 16
 template <typename T, int HD>
 __device__ __forceinline__ void pa_join_out(const PaArgs &p, const PaUnit &u, int r, int d, float4 y, float f) {

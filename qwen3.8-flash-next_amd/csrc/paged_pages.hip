@@ -40,7 +40,8 @@ __device__ __forceinline__ int pg_scan(int v, int *lds, int &total) {
 
 /* ------------------------------------------------------------ append
  * One thread per 16 destination bytes of k or v.  Bound: HBM, each new row
- * read and written once. */
+ * read and written once: f32 rows of nine prompts (74 MB) 17.0 us, 4.4 TB/s;
+ * 64 single rows 4.1 us, a launch and four dependent loads. */
 struct PgAppend {
     pg_cache c;
     const void *src[2];
@@ -116,7 +117,8 @@ extern "C" int qk_launch_pg_append(const pg_cache *c, const void *k, const void 
 /* ------------------------------------------------------------ page copies
  * Pages (src, dst) of every layer's k and v.  A page is rows x heads x
  * 16-byte chunks with strides; dimensions that lie one after the other are
- * merged on the host, so a dense page is one run. */
+ * merged on the host, so a dense page is one run.  Bound: HBM: 136 pages of
+ * 12 layers (107 MB read and written) 18 us, 5.8 TB/s. */
 struct PgCopy {
     pg_cache c;
     const int2 *pairs;        /* (-1, -1): none */
@@ -177,7 +179,9 @@ static unsigned pg_copy_grid(const pg_cache *c, int64_t pairs) {
 
 /* ------------------------------------------------------------ reserve
  * One workgroup: the sequences' needs, their prefix sums, and as many free
- * pages, lowest first.  Bound: the latency of its reads of refs. */
+ * pages, lowest first.  One workgroup, since every page's rank depends on all
+ * sequences.  Bound: latency, of its reads of refs and of the scan over the
+ * batch: 5.3 us for 4 sequences, 13.4 for 256. */
 struct PgReserve {
     pg_cache c;
     const int32_t *slots, *n_new;
@@ -341,7 +345,8 @@ extern "C" int qk_launch_pg_reserve(const pg_cache *c, const int32_t *slots, con
 
 /* ------------------------------------------------------------ fork
  * Two launches, so that every source is read before any table is written
- * (beams that take each other's places).  One workgroup per pair. */
+ * (beams that take each other's places).  One workgroup per pair.  Bound:
+ * latency: 256 pairs of tables of 250 entries 3.9 + 5.3 us. */
 struct PgFork {
     pg_cache c;
     const int32_t *src, *dst, *rows;
@@ -392,7 +397,7 @@ __global__ __launch_bounds__(256) void k_pg_fork_write(PgFork a) {
 }
 
 /* The same in one launch, one workgroup, for batches whose entries fit LDS:
- * four branches of a short prompt. */
+ * four branches of a short prompt 3.1 us. */
 #define PG_FORK_SMALL 12288
 __global__ __launch_bounds__(1024) void k_pg_fork_small(PgFork a) {
     __shared__ int32_t entries[PG_FORK_SMALL];
@@ -460,7 +465,8 @@ extern "C" int qk_launch_pg_fork(const pg_cache *c, const int32_t *src, const in
 
 /* ------------------------------------------------------------ evict
  * Pages whose rows no later query of the slot can see.  An entry is taken
- * out with an exchange, so a slot that is named twice releases it once. */
+ * out with an exchange, so a slot that is named twice releases it once.
+ * Bound: latency, 4.2 us for 256 slots. */
 struct PgEvict {
     pg_cache c;
     const int32_t *slots;
@@ -494,7 +500,9 @@ extern "C" int qk_launch_pg_evict(const pg_cache *c, const int32_t *slots, int n
  * U used pages: the used pages from U on, in order, move to the free pages
  * below U, in order (as many of the one as of the other), so no move's
  * destination is another's source.  One workgroup finds the moves, then one
- * launch copies them and rewrites the tables. */
+ * launch copies them and rewrites the tables.  Bound: HBM, the moved pages: of
+ * 4096 half used pages of 12 layers (405 MB) 7 us for the plan and 81 for the
+ * move, 5.0 TB/s; of 256 in one layer 4 + 4.5. */
 struct PgCompact {
     PgCopy p;
     int32_t *used, *n_moves, *to; /* to [n_pages]: where a page is afterwards */
