@@ -425,8 +425,8 @@ __device__ __forceinline__ bool pa_again(const V (&o)[N], float m, float l, bool
 }
 
 /* ------------------------------------------------------------ few rows
- * Decode: a unit is 16 NC rows (a group's heads of one to a few tokens) and a
- * part of the keys; its four waves take the part's tiles of 32 keys in turn
+ * Decode and short calls: a unit is 16 NC rows (a group's heads of one to a
+ * few tokens) and a part of the keys; its four waves take the part's tiles of 32 keys in turn
  * and join through LDS at the end.  K and V go straight from the pages to
  * registers in operand order, so the main loop has no barrier and the loads
  * of eight or more waves per CU are in flight.  16-wide instructions: lane =
@@ -438,10 +438,9 @@ __device__ __forceinline__ bool pa_again(const V (&o)[N], float m, float l, bool
  * (HD / 16) x + e.  f32 runs on the fp32 matrix instructions, whose operands
  * are single elements.
  * Bound: HBM, the visible pages read once: single tokens of 64 sequences of 64
- * to 65536 rows (841 MB of bf16) 171 to 178 us, 4.8 TB/s, of 1024 of 1000
- * rows 198 us, 5.3 TB/s; f32 under a window of 1024, 32 sequences (68 MB) 25 us,
- * where starting, the join of the waves and the one run of eight tiles a wave
- * count; a token on 333 rows 10 us, latency. */
+ * to 65536 rows (841 MB of bf16) 171 to 178 us, 4.8 TB/s, of 1024 sequences
+ * of 1000 rows 198 us, 5.3 TB/s.  Short calls: latency, f32 under a window of
+ * 1024 of 32 sequences (68 MB) 25 us, a token on 333 rows 10, a prompt of 64 8. */
 #define PD_KT 32
 typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
 
