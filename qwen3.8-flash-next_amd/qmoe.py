@@ -1122,6 +1122,12 @@ class PagedCache:
         need = lib().qmoe_paged_ws_bytes(self._cp, call, n, n_seqs, heads)
         return self._torch.empty(max(need, 16), dtype=self._u8, device=self.device)
 
+    @staticmethod
+    def _span(window, sinks):
+        """ctypes would cut larger numbers off without a word"""
+        if not (0 <= window < 2 ** 31 and 0 <= sinks < 2 ** 31):
+            raise QmoeError(f"window {window} and sinks {sinks} must be in [0, 2^31)")
+
     def _status(self):
         return self._torch.empty(1, dtype=self._i32, device=self.device)
 
@@ -1152,6 +1158,7 @@ class PagedCache:
         heads = q.shape[1] if q.dim() == 3 else 0
         if scale == 0:
             raise QmoeError("scale must not be 0 (None: 1 / sqrt(head_dim))")
+        self._span(window, sinks)
         self._rows(q, heads, self._own, "q")
         n = q.shape[0]
         b, err = self._batch(n, starts, slots), QmoeErr()
@@ -1210,6 +1217,7 @@ class PagedCache:
 
     def evict(self, window, sinks=0, slots=None, stream=None):
         """releases the pages that no later query sees under this window and sinks"""
+        self._span(window, sinks)
         sl, err = self._ints(slots, None, "slots"), QmoeErr()
         m = self.table.shape[0] if slots is None else slots.shape[0]
 

@@ -302,11 +302,40 @@ def test_forks_of_large_tables(dev):
     assert torch.equal(c.refs.cpu().long(), torch.bincount(held, minlength=6000))
 
 
-def test_a_scale_of_zero_is_refused(dev):
+def test_numbers_that_c_would_read_differently_are_refused(dev):
     s = Setup(dev, HEADS[2], torch.float32, 8, [20])
     q, starts = s.queries([2])
-    with pytest.raises(load_pkg().QmoeError, match="scale"):
-        s.cache.attend(0, q.to(dev), i32(starts, dev), scale=0.0)
+    q, starts, error = q.to(dev), i32(starts, dev), load_pkg().QmoeError
+    with pytest.raises(error, match="scale"):
+        s.cache.attend(0, q, starts, scale=0.0)
+    for kw in (dict(window=2 ** 32 + 5), dict(window=-1), dict(window=4, sinks=2 ** 32)):
+        with pytest.raises(error, match="window"):
+            s.cache.attend(0, q, starts, **kw)
+    with pytest.raises(error, match="window"):
+        s.cache.evict(2 ** 32 + 5)
+    assert s.table.tolist() == s.rows
+
+
+@pytest.mark.usefixtures("tables")
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("n", [90, 400])
+def test_starts_in_no_order_stay_inside(dev, n, dtype):
+    """100 sequences whose starts descend, overlap and leave [0, n), slots out of range, lengths past the table:
+    only rows that some sequence claims are written"""
+    s = Setup(dev, HEADS[0], dtype, 16, [int(x) for x in np.random.RandomState(n).randint(0, 700, 20)], seed=n)
+    rng = np.random.RandomState(n + 1)
+    for _ in range(3):
+        starts = rng.randint(-50, n + 50, 101)
+        slots = rng.randint(-2, 23, 100).tolist()
+        s.len_t.copy_(i32(rng.randint(-100, 3000, 20).tolist(), dev))
+        claimed = np.zeros(n, dtype=bool)
+        for a, b in zip(starts[:-1], starts[1:]):
+            claimed[max(a, 0):max(min(b, n), 0)] = True
+        guard = torch.full((n + 64, s.h, s.hd), 7.0, dtype=dtype, device=dev)
+        q = torch.randn(n, s.h, s.hd, generator=s.g).to(dtype).to(dev)
+        s.cache.attend(0, q, i32(starts.tolist(), dev), i32(slots, dev), out=guard[32:32 + n])
+        assert (guard[:32] == 7).all() and (guard[32 + n:] == 7).all()
+        assert (guard[32:32 + n].cpu()[~torch.from_numpy(claimed)] == 7).all()
 
 
 @pytest.mark.usefixtures("tables")
