@@ -181,7 +181,9 @@ static unsigned pg_copy_grid(const pg_cache *c, int64_t pairs) {
  * One workgroup: the sequences' needs, their prefix sums, and as many free
  * pages, lowest first.  One workgroup, since every page's rank depends on all
  * sequences.  Bound: latency, of its reads of refs and of the scan over the
- * batch: 5.3 us for 4 sequences, 13.4 for 256. */
+ * batch: 5.3 us for 4 sequences, 13.4 for 256.  Without gain: several threads
+ * per sequence in the scan (12.9, but 7.3 for 4), the free pages counted under
+ * the loads of the batch (13.6). */
 struct PgReserve {
     pg_cache c;
     const int32_t *slots, *n_new;
