@@ -1284,8 +1284,9 @@ static int pa_rows(const pg_cache *c, const pg_attn *a) {
 /* Groups of four waves in a bf16 unit of the many-row kernel.  Two take the
  * unit's tiles in turn and halve its time; where there are units enough for
  * several rounds, two workgroups of one group per CU do better, since one
- * starts and ends under the other's products (prompt of 1000: 27 and 30 us,
- * of 8192: 320 and 308). */
+ * starts and ends under the other's products (two and one: a prompt of 1000 27
+ * and 30 us, of 8192 320 and 308, of 16000 1249 and 1151, three of 4000 300 and
+ * 264). */
 static int pa_groups(const pg_cache *c, int n, int h) {
     return (int64_t)n * (h / c->kvh) / PM_RT * c->kvh >= 1000 && c->hd <= 128 ? 1 : 2;
 }
@@ -1294,7 +1295,8 @@ static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h, int rt) {
      * run at once it costs 3, since the others fill CUs that had nothing to do:
      * 64 tokens on 3000 rows 40 us with 12, so 33, on 4000 rows in 16 sequences
      * 81 and 70; but a prompt of 2000 (256 tasks) 46 with 12 and 59 with 3. */
-    if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, pm_kt(c->hd, c->dtype == QMOE_F32), 256, c->dtype == QMOE_BF16 ? 12 : 2, c->dtype == QMOE_BF16 ? 3 : 2);
+    if (rt == PM_RT && c->dtype == QMOE_BF16) return pa_plan(c, n, n_seqs, h, PM_RT, pm_kt(c->hd), 256, 12, 3);
+    if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, pm_kt(c->hd, true), 256, 2, 2);
     /* tables of up to 16 tiles (512 rows) are not cut: the join's launch costs
      * more than the shorter run of tiles gives */
     const int bytes = c->hd * (c->dtype == QMOE_BF16 ? 2 : 4) * (rt / 16); /* of a row's registers, as pd_occ */
