@@ -1065,6 +1065,7 @@ class PagedCache:
                                  table.data_ptr(), max(table.stride(0), table.shape[1]) if table.shape[0] == 1 else table.stride(0),
                                  lens.data_ptr(), refs.data_ptr(), table.shape[0], table.shape[1])
         self._cp = ctypes.byref(self._c)
+        self._need = {}  # workspace bytes by a call's sizes
         if self.device.type != "cuda":
             raise QmoeError(f"a paged cache lives on the GPU, not on {self.device}")
 
@@ -1119,8 +1120,12 @@ class PagedCache:
 
     def _work(self, call, n=0, n_seqs=0, heads=0):
         """the call's workspace; a call that the library refuses gets 16 bytes"""
-        need = lib().qmoe_paged_ws_bytes(self._cp, call, n, n_seqs, heads)
-        return self._torch.empty(max(need, 16), dtype=self._u8, device=self.device)
+        need = self._need.get((call, n, n_seqs, heads))
+        if need is None:
+            if len(self._need) > 4096:
+                self._need.clear()
+            need = self._need[call, n, n_seqs, heads] = max(lib().qmoe_paged_ws_bytes(self._cp, call, n, n_seqs, heads), 16)
+        return self._torch.empty(need, dtype=self._u8, device=self.device)
 
     @staticmethod
     def _span(window, sinks):
