@@ -750,10 +750,10 @@ int qmoe_paged_attn(const qmoe_paged_cache *c, int layer, const qmoe_paged_batch
  * them to lens.  Free pages go to the batch in order, lowest first.  Where a
  * slot's last page is partly filled and held by others too, the slot gets a
  * copy of it in every layer; of several slots of the batch that alone hold
- * it, the last keeps it.  *status (device): 0; or the pages lacking; or -1
- * for a slot out of range or named twice, a negative n_new, a length or a
- * sum past the table, or a partly filled last page that was released.
- * Unless 0, nothing is changed.  n_seqs <= 1024. */
+ * it, the last keeps it.  *status (device): 0; or the pages lacking (2^31 - 1
+ * where they are more); or -1 for a slot out of range or named twice, a
+ * negative n_new, a length or a sum past the table, or a partly filled last
+ * page that was released.  Unless 0, nothing is changed.  n_seqs <= 1024. */
 int qmoe_paged_reserve(const qmoe_paged_cache *c, const int32_t *slots, const int32_t *n_new, int n_seqs,
                        int32_t *status, void *ws, size_t ws_bytes, void *stream, qmoe_err *err);
 

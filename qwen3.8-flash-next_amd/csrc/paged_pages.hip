@@ -203,6 +203,7 @@ __global__ __launch_bounds__(1024) void k_pg_reserve(PgReserve a) {
     __shared__ __attribute__((aligned(16))) int slot_of[PG_MAX_BATCH], part_of[PG_MAX_BATCH];
     __shared__ int base_of[PG_MAX_BATCH], first_of[PG_MAX_BATCH];
     __shared__ int tmp[16];
+    __shared__ unsigned long long wanted;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int R = (int)a.c.page_rows.d;
     const bool live = tid < a.n;
@@ -227,6 +228,7 @@ __global__ __launch_bounds__(1024) void k_pg_reserve(PgReserve a) {
     }
     slot_of[tid] = slot;
     part_of[tid] = part;
+    if (tid == 0) wanted = 0;
     __syncthreads();
     /* the same slot twice; how many of the batch write to this page, and
      * whether a later one does.  Four of the batch per LDS read, counts in
@@ -259,8 +261,9 @@ __global__ __launch_bounds__(1024) void k_pg_reserve(PgReserve a) {
     }
     const int e1 = len - e0 * R > 0 ? e0 + 1 : e0; /* first entry without a page */
     const int fresh = live ? (int)pg_div_of(a.c.page_rows, (uint32_t)(len + add + R - 1)) - e1 : 0;
-    /* a need past the pool is refused whatever its size, so the sum fits */
-    const int need = min(max(fresh, 0), a.c.n_pages) + copy;
+    /* one page more than the pool has is past it whatever the others need, and
+     * 1024 such needs sum in 32 bits; a refused call sums them whole */
+    const int need = min(max(fresh, 0), a.c.n_pages + 1) + copy;
     int total;
     const int base = pg_scan(need, tmp, total);
     base_of[tid] = base;
@@ -280,7 +283,9 @@ __global__ __launch_bounds__(1024) void k_pg_reserve(PgReserve a) {
         int have, before = pg_scan(lane == 0 ? cnt : 0, tmp, have);
         before = __builtin_amdgcn_readfirstlane(before);
         if (have < total) {
-            pg_refuse(a, total - have);
+            if (live) atomicAdd(&wanted, (unsigned long long)(max(fresh, 0) + copy));
+            __syncthreads();
+            pg_refuse(a, (int)min(wanted - (unsigned long long)have, 0x7FFFFFFFull));
             return;
         }
         for (int p = p0; p < p1 && before < total; p += 256)

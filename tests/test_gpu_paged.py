@@ -773,6 +773,28 @@ def test_reserve_refusals_change_nothing(dev):
     assert int(c.reserve(i32([1], dev), i32([0], dev))) == -1
 
 
+def test_needs_past_the_pool_are_refused_whatever_their_size(dev):
+    """tables longer than the pool, every page free: the pages lacking are exact, and nothing changes"""
+    pkg = load_pkg()
+    c = pkg.PagedCache.allocate(1, 10, 1, 1, 64, 4, 1000, torch.float32, dev)
+    state = [t.clone() for t in (c.table, c.lens, c.refs)]
+    for n_new, slots, want in (([500], [0], 490), ([0, 500], [1, 0], 490), ([500, 0], [1, 0], 490), ([11], [3], 1),
+                               ([1000] * 4, [3, 1, 0, 2], 3990), ([5, 5, 1], [0, 1, 2], 1), ([10, 1], [0, 1], 1)):
+        assert int(c.reserve(i32(n_new, dev), i32(slots, dev))) == want, (n_new, slots)
+        assert all(torch.equal(a, b) for a, b in zip(state, (c.table, c.lens, c.refs)))
+    assert int(c.reserve(i32([0, 4, 0, 6], dev))) == 0
+    assert c.lens.tolist() == [0, 4, 0, 6] and c.table[1, :5].tolist() == [0, 1, 2, 3, -1] and int(c.refs.sum()) == 10
+    assert int(c.reserve(i32([500, 20], dev), i32([0, 1], dev))) == 520
+    # a shared partly filled page whose copy is one page more; then lacks of more than 31 bits
+    c = pkg.PagedCache.allocate(1, 3, 4, 1, 64, 3, 1000, torch.float32, dev)
+    assert int(c.reserve(i32([6], dev), i32([0], dev))) == 0 and int(c.fork(i32([0], dev), i32([1], dev))) == 0
+    assert int(c.reserve(i32([4000 - 6], dev), i32([1], dev))) == 998  # 998 pages and the copy, one page free
+    big = pkg.PagedCache.allocate(1, 10, 1, 1, 64, 3, 1 << 30, torch.bfloat16, dev)
+    assert int(big.reserve(i32([1 << 30], dev), i32([2], dev))) == (1 << 30) - 10
+    assert int(big.reserve(i32([1 << 30, 1 << 30, 1 << 30], dev))) == 2 ** 31 - 1
+    assert big.lens.tolist() == [0, 0, 0] and int(big.refs.sum()) == 0 and int(big.table[:, :20].max()) == -1
+
+
 def test_the_last_writer_keeps_a_shared_page(dev):
     pkg = load_pkg()
     c = pkg.PagedCache.allocate(1, 12, 8, 1, 64, 5, 4, torch.float32, dev)
