@@ -276,8 +276,8 @@ __device__ __forceinline__ bool pa_full(const PaArgs &p, int p0, int p1, int bas
 }
 
 /* ------------------------------------------------- one row at a time
- * fp32 on the vector ALU, keys of the unit's part only, for units with
- * results that are not finite (pa_again): a masked key is never multiplied
+ * fp32 on the vector ALU, keys of the unit's part only, for units whose
+ * results are not finite or whose weights vanish (pa_again): a masked key is never multiplied
  * here.  Waves take the unit's rows in turn. */
 template <typename T, int HD, int RT, int KT>
 __device__ __forceinline__ void pa_slow(const PaArgs &p, const PaUnit &u, int kt0, int kt1, pg_tiles tl, int waves) {
@@ -412,16 +412,22 @@ __device__ __forceinline__ int pa_vswz(int rr) { return CR % 16 == 0 ? (rr & 3) 
 /* A row that some query of the unit does not see may hold an infinity or NaN,
  * and weight 0 times that is NaN: such a unit is computed again one row at a
  * time.  It shows in the sums themselves, so the loops need no test: O or the
- * sum of weights is not finite (also where that is the right result), or
- * every score seen was -inf. */
+ * sum of weights is not finite (also where that is the right result), or the
+ * sum of a row that sees something is next to nothing.  That is 0 where every
+ * score seen was -inf.  Else the largest weight is 2^d, since the weights are
+ * exp2 of a product that is not rounded before m is subtracted while m is one
+ * that was: |d| is half a step of m, below 1 up to m = 2^24, but -128 at 2^31,
+ * where all weights vanish.  From 2^-64 on, what is lost below fp32's range is
+ * less than 2^-60 of the sum. */
+#define PA_LEAST 0x1p-64f
 template <int N, int W, typename V>
-__device__ __forceinline__ bool pa_again(const V (&o)[N], float m, float l, bool seen) {
+__device__ __forceinline__ bool pa_again(const V (&o)[N], float l, bool seen) {
     float x = l == l ? fabsf(l) : INFINITY;
 #pragma unroll
     for (int d = 0; d < N; d++)
 #pragma unroll
         for (int i = 0; i < W; i++) x = fmaxf(x, o[d][i] == o[d][i] ? fabsf(o[d][i]) : INFINITY);
-    return !(x < INFINITY) || (m == -INFINITY && seen);
+    return !(x < INFINITY) || (seen && l < PA_LEAST);
 }
 
 /* ------------------------------------------------------------ few rows
@@ -630,9 +636,9 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
     bool again = false;
 #pragma unroll
     for (int x = 0; x < NC; x++) {
-        again |= pa_again<E, 4>(o[x], m[x], l[x], seen[x]);
         l[x] += __uint_as_float(qk_xor16_u(__float_as_uint(l[x])));
         l[x] += __uint_as_float(qk_xor32_u(__float_as_uint(l[x])));
+        again |= pa_again<E, 4>(o[x], l[x], seen[x]);
         l[x] = pa_sum(m[x], l[x], seen[x]);
         if (g == 0) ml[wave][16 * x + c] = make_float2(m[x], l[x]);
     }
@@ -924,11 +930,11 @@ __global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
             }
     }
     qm_sync<0>(); /* the last step's copies, of a step that there is not, are done */
-    if (__syncthreads_or(wn > 0 && pa_again<E, 16>(o, m, l, seen))) {
+    l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
+    if (__syncthreads_or(wn > 0 && pa_again<E, 16>(o, l, seen))) {
         pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 4 * NG);
         return;
     }
-    l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
     if constexpr (NG > 1)
         if (!pa_merge<E, NG>(o, m, l, (float4 *)kv, (float2 *)where)) return;
     if (c < wn) pa_store<T, HD>(p, u, o, m, l, 32 * wave + c, t, hh);
@@ -1148,11 +1154,11 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
         }
         qk_lds_barrier();
     }
-    if (__syncthreads_or(wn > 0 && pa_again<E, 16>(o, m, l, seen))) {
+    l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
+    if (__syncthreads_or(wn > 0 && pa_again<E, 16>(o, l, seen))) {
         pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 4 * NG);
         return;
     }
-    l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
     if constexpr (NG == 2)
         if (!pa_merge<E, NG>(o, m, l, (float4 *)kv, (float2 *)where)) return;
     if (c < wn) pa_store<T, HD>(p, u, o, m, l, 32 * wave + c, t, hh);

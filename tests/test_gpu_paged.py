@@ -488,6 +488,44 @@ def test_large_scores(dev):
 
 
 @pytest.mark.usefixtures("tables")
+@pytest.mark.parametrize("sign", [1, -1], ids=["positive", "negative"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("shape,lens,counts", [((4, 2, 64), [40, 33, 200], [1, 3, 5]), ((16, 2, 128), [300, 170], [250, 130]),
+                                               ((4, 1, 256), [90, 300], [60, 200]), ((4, 2, 64), [9000], [2]),
+                                               ((16, 2, 128), [4000, 100], [300, 1]), ((6, 2, 192), [60] * 70, [1] * 70)],
+                         ids=["few", "many", "many_256", "few_joined", "many_joined", "indexed"])
+def test_scores_past_what_fp32_resolves(dev, shape, lens, counts, dtype, sign):
+    """scores of 2^34 and more, of both signs, whose steps in fp32 are far wider than exp's range.  One key's score is
+    at least twice as large (or half as negative) as any other's, so in 64 bits its weight is 1 and all others are 0:
+    the output is its v, with the sums' and the output's roundings."""
+    s = Setup(dev, shape, dtype, 16, lens, seed=27)
+    h, kvh, hd = shape
+    g = torch.Generator().manual_seed(28)
+    starts = s.queries(counts)[1]
+    u = (torch.randint(0, 2, (kvh, hd), generator=g) * 2 - 1).float()
+    wins = [(n - c) // 2 for n, c in zip(lens, counts)]
+    for i, n in enumerate(lens):
+        rest = torch.rand(n, kvh, 1, generator=g) * 0.4
+        a = (0.1 + rest) if sign > 0 else (2.1 + 4 * rest)
+        a[wins[i]] = 1.0
+        a = a * (2.0 ** 16 * (1 + torch.rand(1, kvh, 1, generator=g)))
+        k = (a * u).to(dtype).to(dev)
+        for j0 in range(0, n, 16):
+            m = min(16, n - j0)
+            s.k[0, s.rows[i][j0 // 16], :m] = k[j0:j0 + m]
+    # one factor for all rows of a call, so that the fp32 rounding of the largest score, up or down, is the same in
+    # all rows of a unit
+    for draw in range(8):
+        q = (2.0 ** 16 * (1 + torch.rand(1, generator=g)) * u[torch.arange(h) % kvh]).to(dtype).expand(starts[-1], h, hd)
+        out = s.cache.attend(0, q.to(dev), i32(starts, dev), scale=sign * hd ** -0.5).double().cpu()
+        for i, n in enumerate(lens):
+            want = s.hv[i][wins[i]].double()[torch.arange(h) % kvh][None]
+            err = (out[starts[i]:starts[i + 1]] - want).abs()
+            tol = want.abs() * (2 * (n + 64) * U + torch.finfo(dtype).eps / 2)
+            assert (err <= tol).all(), (draw, i, int((~(err <= tol)).sum()))
+
+
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 def test_strides(dev, dtype):
     """heads before rows in the pages, heads before tokens in q and out, k and v interleaved"""
