@@ -701,12 +701,19 @@ typedef struct {
  * that slot's lens: row t has position lens - (starts[i+1] - t).  Values out
  * of range are clamped on the device (starts into [0, n], lens into [0, table
  * rows]); a slot out of range has no rows.  Rows of the call outside every
- * sequence are left alone. */
+ * sequence are left alone.
+ *
+ * The last rows of lens are the batch's own only if the qmoe_paged_reserve
+ * that was to make room for them did: where it refused, they are rows that
+ * are cached already, which qmoe_paged_append would overwrite.  Give its
+ * status here wherever it may refuse (a pool can be full): unless it is 0 when
+ * the call runs, the call writes nothing. */
 typedef struct {
     const int32_t *starts;  /* [n_seqs + 1] device, ascending */
     const int32_t *slots;   /* [n_seqs] device, or NULL (n_seqs <= n_slots) */
     int n;                  /* rows of the call */
     int n_seqs;             /* <= 65536 */
+    const int32_t *status;  /* device, 4-byte aligned; or NULL: as 0 */
 } qmoe_paged_batch;
 
 /* workspace bytes of a call; 0 for arguments that the call refuses.  n and
@@ -753,7 +760,8 @@ int qmoe_paged_attn(const qmoe_paged_cache *c, int layer, const qmoe_paged_batch
  * it, the last keeps it.  *status (device): 0; or the pages lacking (2^31 - 1
  * where they are more); or -1 for a slot out of range or named twice, a
  * negative n_new, a length or a sum past the table, or a partly filled last
- * page that was released.  Unless 0, nothing is changed.  n_seqs <= 1024. */
+ * page that was released.  Unless 0, nothing is changed, and the batch that
+ * follows must not be appended (qmoe_paged_batch's status).  n_seqs <= 1024. */
 int qmoe_paged_reserve(const qmoe_paged_cache *c, const int32_t *slots, const int32_t *n_new, int n_seqs,
                        int32_t *status, void *ws, size_t ws_bytes, void *stream, qmoe_err *err);
 

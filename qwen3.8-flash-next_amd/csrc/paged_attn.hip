@@ -23,6 +23,8 @@ typedef float qm_f32x16 __attribute__((ext_vector_type(16)));
 
 #define PM_RT 128 /* rows of a unit of the many-row kernels */
 
+__device__ const uint4 pa_zero[64] = {}; /* a row of zeros, up to 1 KB */
+
 struct PaArgs {
     pg_cache c;   /* k and v of the call's layer */
     pg_attn a;
@@ -179,13 +181,15 @@ __global__ __launch_bounds__(1024) void k_pa_index(PaArgs p, int rt, int kt) {
 }
 
 /* Unit `want` of the call (JOIN: the want-th (sequence, row tile, kv head)
- * that has parts to join); false past the last.  Every wave finds it by
+ * that has parts to join); false past the last, and for a refused batch.  Every wave finds it by
  * itself, a lane per sequence (of more: in the index), without LDS or
  * barriers: this stands before the first load of a page, and a decode call is
  * a few microseconds long. */
 template <int RT, int KT, bool JOIN>
 __device__ __forceinline__ bool pa_find(const PaArgs &p, int want, PaUnit &u) {
     const int lane = threadIdx.x & 63, n = p.a.n_seqs;
+    /* in flight beside the lengths; with a branch before them a token took 10.4 us, so 10.1 */
+    const int refused = qk_ld(p.a.status ? p.a.status : (const int32_t *)pa_zero);
     int ubase, sbase; /* units and split units before the sequence's */
     if (n <= PA_INDEX) {
         pg_seq s = {-1, 0, 0, 0};
@@ -247,7 +251,7 @@ __device__ __forceinline__ bool pa_find(const PaArgs &p, int want, PaUnit &u) {
     }
     const int rtiles = (u.s.count * p.G + RT - 1) / RT, tasks = rtiles * p.c.kvh;
     const int mine = JOIN ? (u.parts > 1 ? tasks : 0) : tasks * u.parts;
-    if ((uint32_t)want - (uint32_t)ubase >= (uint32_t)mine) return false; /* past the last */
+    if ((uint32_t)want - (uint32_t)ubase >= (uint32_t)mine || refused) return false; /* past the last */
     const int q = (want - ubase) / p.c.kvh;
     u.kh = want - ubase - q * p.c.kvh;
     const int back = JOIN ? q : q / u.parts;
@@ -738,7 +742,6 @@ __device__ __forceinline__ void pa_store(const PaArgs &p, const PaUnit &u, const
  * scores of the next tile beside the softmax (337 to 348), three groups (326),
  * units of 64 rows (short prompts 10 % better, long contexts 40 % worse). */
 #define PM_CHUNK 1024 /* keys of a look-up of two groups */
-__device__ const uint4 pa_zero[64] = {}; /* a row of zeros, up to 1 KB */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pa_s16x4 *pa_tptr;
 

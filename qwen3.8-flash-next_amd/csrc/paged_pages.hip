@@ -46,7 +46,7 @@ struct PgAppend {
     pg_cache c;
     const void *src[2];
     int64_t token[2], head[2];
-    const int32_t *starts, *slots;
+    const int32_t *starts, *slots, *status;
     int n, n_seqs;
     pg_div per_row, per_head; /* 16-byte chunks */
 };
@@ -69,6 +69,7 @@ __device__ __forceinline__ int pg_find(const int32_t *starts, int n_seqs, int t)
 template <typename S, typename D>
 __global__ __launch_bounds__(256) void k_pg_append(PgAppend a) {
     constexpr int E = 16 / sizeof(D); /* elements per chunk */
+    const int refused = a.status ? qk_ld(a.status) : 0;
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
     const uint32_t t = pg_div_of(a.per_row, i), r = i - t * a.per_row.d;
     if (t >= (uint32_t)a.n) return;
@@ -79,7 +80,7 @@ __global__ __launch_bounds__(256) void k_pg_append(PgAppend a) {
     const int pos = q.len - q.count + (int)t - q.start;
     if (q.slot < 0 || (int)t < q.start || (int)t >= q.start + q.count) return;
     const int64_t at = pg_row_at(&a.c, a.c.table + q.slot * a.c.table_stride, pos);
-    if (at < 0) return;
+    if (at < 0 || refused) return;
     const int which = blockIdx.y;
     const S *src = (const S *)a.src[which] + t * a.token[which] + hd * a.head[which] + ch * E;
     D *dst = (D *)(which ? a.c.v : a.c.k) + at + hd * a.c.head_stride + ch * E;
@@ -95,7 +96,7 @@ __global__ __launch_bounds__(256) void k_pg_append(PgAppend a) {
 
 extern "C" int qk_launch_pg_append(const pg_cache *c, const void *k, const void *v, int src_dtype, int64_t k_token,
                                    int64_t k_head, int64_t v_token, int64_t v_head, const int32_t *starts,
-                                   const int32_t *slots, int n, int n_seqs, void *stream) {
+                                   const int32_t *slots, const int32_t *status, int n, int n_seqs, void *stream) {
     hipStream_t st = (hipStream_t)stream;
     PgAppend a;
     const int E = c->dtype == QMOE_BF16 ? 8 : 4;
@@ -103,7 +104,7 @@ extern "C" int qk_launch_pg_append(const pg_cache *c, const void *k, const void 
     a.src[0] = k; a.src[1] = v;
     a.token[0] = k_token; a.token[1] = v_token;
     a.head[0] = k_head; a.head[1] = v_head;
-    a.starts = starts; a.slots = slots;
+    a.starts = starts; a.slots = slots; a.status = status;
     a.n = n; a.n_seqs = n_seqs;
     a.per_head = pg_div_make((uint32_t)(c->hd / E));
     a.per_row = pg_div_make((uint32_t)(c->kvh * (c->hd / E)));

@@ -474,7 +474,7 @@ typedef struct {
     const void *q;
     void *out;
     int64_t q_token, q_head, o_token, o_head; /* strides, elements */
-    const int32_t *starts, *slots;
+    const int32_t *starts, *slots, *status; /* status: NULL, or nothing is written unless it holds 0 */
     int n, n_seqs, h, window, sinks, grouped;
     float scale;           /* score * this, log2 units: softmax scale * log2(e) */
 } pg_attn;
@@ -483,8 +483,8 @@ typedef struct {
 size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h);
 int qk_launch_pg_attn(const pg_cache *c, const pg_attn *a, void *ws, void *stream);
 int qk_launch_pg_append(const pg_cache *c, const void *k, const void *v, int src_dtype, int64_t k_token, int64_t k_head,
-                        int64_t v_token, int64_t v_head, const int32_t *starts, const int32_t *slots, int n, int n_seqs,
-                        void *stream);
+                        int64_t v_token, int64_t v_head, const int32_t *starts, const int32_t *slots,
+                        const int32_t *status, int n, int n_seqs, void *stream);
 size_t qk_pg_reserve_ws(const pg_cache *c, int n_seqs);
 int qk_launch_pg_reserve(const pg_cache *c, const int32_t *slots, const int32_t *n_new, int n_seqs, int32_t *status,
                          void *ws, void *stream);

@@ -119,6 +119,7 @@ static int pg_batch(const pg_cache *c, const qmoe_paged_batch *b, qmoe_err *err)
     if (b->n < 0) return pg_fail(err, "n = %d is negative", b->n);
     if (pg_seqs(c, b->slots, b->n_seqs, PG_MAX_SEQS, err)) return -1;
     if (b->n_seqs > 0 && b->n > 0 && !b->starts) return pg_fail(err, "starts is NULL");
+    if ((uintptr_t)b->status & 3) return pg_fail(err, "status must be 4-byte aligned");
     return 0;
 }
 
@@ -172,8 +173,8 @@ int qmoe_paged_append(const qmoe_paged_cache *q, int layer, const qmoe_paged_bat
     if (!k || !v) return pg_fail(err, "%s is NULL", k ? "v" : "k");
     if (pg_misaligned(k) || pg_misaligned(v)) return pg_fail(err, "k and v must be 16-byte aligned");
     return pg_hip(err,
-                  qk_launch_pg_append(&c, k, v, src_dtype, k_token, k_head, v_token, v_head, b->starts, b->slots, b->n,
-                                      b->n_seqs, stream),
+                  qk_launch_pg_append(&c, k, v, src_dtype, k_token, k_head, v_token, v_head, b->starts, b->slots, b->status,
+                                      b->n, b->n_seqs, stream),
                   "paged append");
 }
 
@@ -208,6 +209,7 @@ int qmoe_paged_attn(const qmoe_paged_cache *cache, int layer, const qmoe_paged_b
     a.o_head = q->out_head_stride;
     a.starts = b->starts;
     a.slots = b->slots;
+    a.status = b->status;
     a.n = b->n;
     a.n_seqs = b->n_seqs;
     a.h = q->n_heads;

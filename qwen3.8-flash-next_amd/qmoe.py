@@ -116,7 +116,8 @@ class QmoePagedCache(ctypes.Structure):
 
 
 class QmoePagedBatch(ctypes.Structure):
-    _fields_ = [("starts", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("n", ctypes.c_int), ("n_seqs", ctypes.c_int)]
+    _fields_ = [("starts", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("n", ctypes.c_int), ("n_seqs", ctypes.c_int),
+                ("status", ctypes.c_void_p)]
 
 
 class QmoePagedQuery(ctypes.Structure):
@@ -1037,8 +1038,11 @@ class PagedCache:
     Batches are ragged: starts [n_seqs + 1] int32 cuts the rows of a call
     into sequences, slots [n_seqs] int32 names their slots (None: sequence i
     is slot i), and a sequence's rows are the last ones of its lens.  One
-    serving step is reserve (room for the new rows), then per layer append
-    and attend.  Calls return without waiting and may be captured in a HIP
+    serving step is status = reserve(...) (room for the new rows), then per
+    layer append(..., status=status) and attend(..., status=status): where
+    reserve was refused, the last rows of lens are cached already, and with
+    its status the two write nothing (without it append would overwrite
+    them).  Calls return without waiting and may be captured in a HIP
     graph; a call's workspace comes from torch's allocator on the call's
     stream."""
 
@@ -1111,12 +1115,13 @@ class PagedCache:
             raise QmoeError(f"{what} must be [n, {heads}, {self.hd}] {' or '.join(str(d) for d in dtypes)} with the head "
                             f"dim contiguous on {self.device}")
 
-    def _batch(self, n, starts, slots):
+    def _batch(self, n, starts, slots, status):
         p = self._ints(starts, None, "starts")
         if p is None or starts.shape[0] < 1:
             raise QmoeError("starts must hold one number more than there are sequences")
         m = starts.shape[0] - 1
-        return QmoePagedBatch(p, None if slots is None else self._ints(slots, m, "slots"), n, m)
+        return QmoePagedBatch(p, None if slots is None else self._ints(slots, m, "slots"), n, m,
+                              None if status is None else self._ints(status, 1, "status"))
 
     def _work(self, call, n=0, n_seqs=0, heads=0):
         """the call's workspace; a call that the library refuses gets 16 bytes"""
@@ -1137,14 +1142,15 @@ class PagedCache:
         return self._torch.empty(1, dtype=self._i32, device=self.device)
 
     # -- rows
-    def append(self, layer, k, v, starts, slots=None, stream=None):
+    def append(self, layer, k, v, starts, slots=None, stream=None, status=None):
         """new rows k, v [n, n_kv_heads, head_dim] into the pages of `layer`
-        (the pages' type, or f32 rounded into bf16 pages)"""
+        (the pages' type, or f32 rounded into bf16 pages); nothing is written
+        unless `status` (of the reserve that made room for them) is 0"""
         self._rows(k, self.kvh, self._src, "k")
         self._rows(v, self.kvh, self._src, "v")
         if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
             raise QmoeError("k and v must have the same rows and type")
-        b, err = self._batch(k.shape[0], starts, slots), QmoeErr()
+        b, err = self._batch(k.shape[0], starts, slots, status), QmoeErr()
 
         def call(st):
             _check(lib().qmoe_paged_append(self._cp, layer, ctypes.byref(b), k.data_ptr(), v.data_ptr(), _dtype_code(k),
@@ -1152,21 +1158,23 @@ class PagedCache:
                    "qmoe_paged_append")
         self._on(stream, call)
 
-    def attend(self, layer, q, starts, slots=None, window=0, sinks=0, scale=None, grouped=False, out=None, stream=None):
+    def attend(self, layer, q, starts, slots=None, window=0, sinks=0, scale=None, grouped=False, out=None, stream=None,
+               status=None):
         """q [n, n_heads, head_dim] of the pages' type -> softmax(scale q.k) v
         over the rows each query sees, [n, n_heads, head_dim]: those up to its
         own, with a window only the last `window` and the first `sinks`.
         Head h reads kv head h % n_kv_heads as the attention mixer's, with
         `grouped` h // (n_heads / n_kv_heads); scale None is
-        1 / sqrt(head_dim).  Rows of no sequence are left as out has them
-        (undefined without out); out must not overlap q or the cache."""
+        1 / sqrt(head_dim).  Rows of no sequence, and all rows unless `status`
+        (of the reserve that made room for them) is 0, are left as out has
+        them (undefined without out); out must not overlap q or the cache."""
         heads = q.shape[1] if q.dim() == 3 else 0
         if scale == 0:
             raise QmoeError("scale must not be 0 (None: 1 / sqrt(head_dim))")
         self._span(window, sinks)
         self._rows(q, heads, self._own, "q")
         n = q.shape[0]
-        b, err = self._batch(n, starts, slots), QmoeErr()
+        b, err = self._batch(n, starts, slots, status), QmoeErr()
         if out is not None:
             self._rows(out, heads, self._own, "out")
             if out.shape[0] != n:

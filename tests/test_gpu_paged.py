@@ -976,6 +976,72 @@ def test_a_captured_step_follows_the_cache(dev):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("rows,more", [([20, 20], [9, 1]), ([300, 100], [200, 90]), ([3000, 40], [1, 30]), ([7] * 80, [9] * 80)],
+                         ids=["tokens", "chunks", "joined", "indexed"])
+def test_a_refused_step_writes_nothing(dev, rows, more, dtype):
+    """reserve, append and attend of a pool that is full, eager and captured, with the reserve's status: the cache and
+    the output stay as they are, shared pages among them; after pages were released the same calls and the same graph
+    do what they do without a status"""
+    pkg = load_pkg()
+    h, kvh, hd, page, n = 8, 2, 64, 8, len(rows)
+    g = torch.Generator(device=dev).manual_seed(29)
+    held = sum(-(-r // page) for r in rows)
+    lacks = sum(-(-(r + m) // page) - r // page for r, m in zip(rows, more))  # new pages, copies of shared last ones
+    c = pkg.PagedCache.allocate(2, held + lacks, page, kvh, hd, 2 * n, 1000, dtype, dev)
+    c.k.zero_()
+    c.v.zero_()
+    starts0 = i32(np.concatenate([[0], np.cumsum(rows)]).tolist(), dev)
+    k0, v0 = (torch.randn(sum(rows), kvh, hd, generator=g, device=dev).to(dtype) for _ in range(2))
+    status = c.reserve(i32(rows, dev))
+    for layer in range(2):
+        c.append(layer, k0, v0, starts0, status=status)
+    src, dst = i32(list(range(n)), dev), i32(list(range(n, 2 * n)), dev)
+    assert int(status) == 0 and int(c.fork(src, dst)) == 0
+    free = c.refs == 0
+    c.refs[free] = 1  # pages of other sequences
+    starts, add = i32(np.concatenate([[0], np.cumsum(more)]).tolist(), dev), i32(more, dev)
+    q, k, v = (torch.randn(sum(more), m, hd, generator=g, device=dev).to(dtype) for m in (h, kvh, kvh))
+    outs = [torch.full((sum(more), h, hd), 5.0, dtype=dtype, device=dev) for _ in range(2)]
+    before = [t.clone() for t in (c.k, c.v, c.table, c.lens, c.refs)]
+
+    def step():
+        status = c.reserve(add, dst)
+        for layer in range(2):
+            c.append(layer, k, v, starts, dst, status=status)
+            c.attend(layer, q, starts, dst, out=outs[layer], status=status)
+        return status
+
+    def untouched():
+        return all(torch.equal(a, b) for a, b in zip(before, (c.k, c.v, c.table, c.lens, c.refs))) and \
+            all((o == 5).all() for o in outs)
+
+    assert int(step()) == lacks and untouched()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        status = step()
+    for _ in range(2):
+        graph.replay()
+        assert int(status) == lacks and untouched()
+    twice = c.reserve(add, torch.zeros_like(dst))
+    c.append(0, k, v, starts, dst, status=twice)
+    assert int(twice) == -1 and untouched()
+    c.refs[free] = 0  # the others are done
+    graph.replay()
+    assert int(status) == 0 and int((c.refs == 0).sum()) == 0
+    for i, (r, m) in enumerate(zip(rows, more)):
+        a, b = int(starts[i]), int(starts[i + 1])
+        kk, vv = (torch.cat([x[int(starts0[i]):int(starts0[i + 1])], y[a:b]]).cpu() for x, y in ((k0, k), (v0, v)))
+        for layer in range(2):
+            want, A, B = reference(q[a:b].cpu(), kk, vv, m, 0, 0, False)
+            check(outs[layer][a:b], want, A, B, hd, r + m, dtype, (i, layer))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 def test_a_serving_run(dev, dtype):
     """prompts in chunks, branches forked, single tokens, a window, pages released and compacted: every output
     against 64 bits over that sequence's own history"""

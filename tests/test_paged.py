@@ -203,3 +203,12 @@ def test_the_class_refuses_other_tensors():
                      ((k, k, table, lens, refs), "GPU")):
         with pytest.raises(pkg.QmoeError, match=msg):
             pkg.PagedCache(*bad)
+
+
+def test_a_misaligned_status_is_refused():
+    pkg = load_pkg()
+    L, e = pkg.lib(), pkg.QmoeErr()
+    c, b, q = cache(pkg), batch(pkg, status=A + 2), query(pkg)
+    cp, bp, ep = (ctypes.byref(x) for x in (c, b, e))
+    assert L.qmoe_paged_append(cp, 0, bp, A, A, pkg.BF16, 256, 128, 256, 128, None, ep) == -1 and b"status" in e.msg
+    assert L.qmoe_paged_attn(cp, 0, bp, ctypes.byref(q), A, 1 << 40, None, ep) == -1 and b"status" in e.msg
