@@ -774,10 +774,14 @@ int qmoe_paged_reserve(const qmoe_paged_cache *c, const int32_t *slots, const in
 int qmoe_paged_fork(const qmoe_paged_cache *c, const int32_t *src, const int32_t *dst, const int32_t *rows, int n_seqs,
                     int32_t *status, void *ws, size_t ws_bytes, void *stream, qmoe_err *err);
 
-/* Releases the pages of the slots (NULL: slots 0 .. n_seqs - 1) that no later
- * query sees under this window (>= 1) and sinks: all rows behind the window
- * of a query at position lens, none of them a sink.  Slots out of range are
- * passed over. */
+/* Releases the pages of the slots (NULL: slots 0 .. n_seqs - 1) that no query
+ * at position lens or after it sees under this window (>= 1) and sinks: all
+ * rows behind the window of a query at lens, none of them a sink.  Slots out
+ * of range are passed over.  Its place is after a step's last attention and
+ * before the next reserve, when the next query is at lens.  While r rows at
+ * the end of lens are still to be attended (after a reserve), or may yet be
+ * cut off (qmoe_paged_fork), earlier queries will come: give window + r, the
+ * largest r of the slots.  A released row cannot be had back. */
 int qmoe_paged_evict(const qmoe_paged_cache *c, const int32_t *slots, int n_seqs, int window, int sinks, void *stream,
                      qmoe_err *err);
 

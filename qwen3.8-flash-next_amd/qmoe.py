@@ -1228,9 +1228,17 @@ class PagedCache:
         """cuts slots to their first rows[i] rows (0 frees a slot)"""
         return self.fork(slots, slots, rows, stream)
 
-    def evict(self, window, sinks=0, slots=None, stream=None):
-        """releases the pages that no later query sees under this window and sinks"""
+    def evict(self, window, sinks=0, slots=None, stream=None, ahead=0):
+        """releases the pages that no query at position lens - ahead or after
+        it sees under this window and sinks.  ahead is 0 between a step's last
+        attend and the next reserve; else the most rows at the end of a slot's
+        lens that are still to be attended (rows reserved) or that trim may
+        yet cut off.  A released row cannot be had back."""
         self._span(window, sinks)
+        if not 0 <= ahead < 2 ** 31:
+            raise QmoeError(f"ahead {ahead} must be in [0, 2^31)")
+        if window:  # 0 is refused below; past any table nothing lies behind the window
+            window = min(window + ahead, 2 ** 31 - 1)
         sl, err = self._ints(slots, None, "slots"), QmoeErr()
         m = self.table.shape[0] if slots is None else slots.shape[0]
 

@@ -861,6 +861,59 @@ def test_beams_trade_places(dev):
     assert torch.equal(c.refs.cpu(), want)
 
 
+@pytest.mark.parametrize("page,window,sinks,ahead", [(4, 9, 0, 5), (8, 1, 3, 1), (1, 30, 7, 40), (16, 64, 4, 33)], ids=str)
+def test_evict_spares_what_reserved_and_cut_off_rows_need(dev, page, window, sinks, ahead):
+    """pages released between a reserve and its attend, and before rows are cut off and written anew: every query
+    sees its whole window, and every page behind the first of them is free"""
+    pkg = load_pkg()
+    h, kvh, hd, lens = 4, 2, 64, [50, 120, 7]
+    c = pkg.PagedCache.allocate(1, 400, page, kvh, hd, 3, 400, torch.float32, dev)
+    g = torch.Generator().manual_seed(30)
+    hist = [[torch.zeros(0, kvh, hd)] * 2 for _ in lens]
+
+    def attend(counts, status):
+        starts = np.concatenate([[0], np.cumsum(counts)]).tolist()
+        q, k, v = (torch.randn(sum(counts), n, hd, generator=g) for n in (h, kvh, kvh))
+        c.append(0, k.to(dev), v.to(dev), i32(starts, dev), status=status)
+        out = c.attend(0, q.to(dev), i32(starts, dev), window=window, sinks=sinks, status=status)
+        assert int(status) == 0
+        for i, m in enumerate(counts):
+            a, b = starts[i], starts[i + 1]
+            hist[i] = [torch.cat([hist[i][0], k[a:b]]), torch.cat([hist[i][1], v[a:b]])]
+            want, A, B = reference(q[a:b], *hist[i], m, window, sinks, False)
+            check(out[a:b], want, A, B, hd, hist[i][0].shape[0], torch.float32, (i, m))
+
+    def released(back):
+        """pages of the slots that no query from lens - back on sees"""
+        return sum((c.table[i].cpu()[e] < 0) == ((e + 1) * page <= n - back - window + 1 and e * page >= sinks)
+                   for i, n in enumerate(c.lens.tolist()) for e in range(-(-n // page))) == sum(-(-n // page) for n in c.lens.tolist())
+
+    attend(lens, c.reserve(i32(lens, dev)))
+    counts = [ahead, 1, max(1, ahead // 2)]
+    status = c.reserve(i32(counts, dev))
+    c.evict(window, sinks, ahead=ahead)  # the batch's rows are yet to be attended
+    assert released(ahead)
+    attend(counts, status)
+    c.evict(window, sinks, ahead=min(ahead, 7))  # up to 7 rows may be taken back
+    assert released(min(ahead, 7))
+    back = [min(ahead, 7), 1, 0]
+    assert int(c.trim(i32([0, 1, 2], dev), i32([x.shape[0] - b for (x, _), b in zip(hist, back)], dev))) == 0
+    hist[:] = [[x[:x.shape[0] - b] for x in hh] for hh, b in zip(hist, back)]
+    attend([3, 1, 2], c.reserve(i32([3, 1, 2], dev)))
+    c.evict(window, sinks)
+    assert released(0)
+    attend([1, 1, 1], c.reserve(i32([1, 1, 1], dev)))
+    held = c.table.cpu()[c.table.cpu() >= 0].long()
+    assert torch.equal(c.refs.cpu().long(), torch.bincount(held, minlength=400))
+    with pytest.raises(pkg.QmoeError, match="ahead"):
+        c.evict(window, sinks, ahead=-1)
+    with pytest.raises(pkg.QmoeError, match="window"):
+        c.evict(0, sinks, ahead=3)
+    before = c.table.clone()
+    c.evict(2 ** 31 - 1, 0, ahead=2 ** 31 - 1)
+    assert torch.equal(c.table, before)
+
+
 @pytest.mark.parametrize("order", ["rows", "heads"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 def test_compact_moves_contents(dev, dtype, order):
