@@ -1138,6 +1138,12 @@ class PagedCache:
         if not (0 <= window < 2 ** 31 and 0 <= sinks < 2 ** 31):
             raise QmoeError(f"window {window} and sinks {sinks} must be in [0, 2^31)")
 
+    @staticmethod
+    def _scale(scale):
+        """0 in f32, what the library reads as the default, is no scale that a caller means"""
+        if scale is not None and ctypes.c_float(scale).value == 0.0:
+            raise QmoeError(f"scale {scale} must not be 0 or round to it in f32 (None: 1 / sqrt(head_dim))")
+
     def _status(self):
         return self._torch.empty(1, dtype=self._i32, device=self.device)
 
@@ -1165,12 +1171,11 @@ class PagedCache:
         own, with a window only the last `window` and the first `sinks`.
         Head h reads kv head h % n_kv_heads as the attention mixer's, with
         `grouped` h // (n_heads / n_kv_heads); scale None is
-        1 / sqrt(head_dim).  Rows of no sequence, and all rows unless `status`
+        1 / sqrt(head_dim), others are taken in f32.  Rows of no sequence, and all rows unless `status`
         (of the reserve that made room for them) is 0, are left as out has
         them (undefined without out); out must not overlap q or the cache."""
         heads = q.shape[1] if q.dim() == 3 else 0
-        if scale == 0:
-            raise QmoeError("scale must not be 0 (None: 1 / sqrt(head_dim))")
+        self._scale(scale)
         self._span(window, sinks)
         self._rows(q, heads, self._own, "q")
         n = q.shape[0]

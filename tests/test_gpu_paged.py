@@ -339,6 +339,20 @@ def test_starts_in_no_order_stay_inside(dev, n, dtype):
 
 
 @pytest.mark.usefixtures("tables")
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_tiny_scales(dev, dtype):
+    """the smallest that f32 holds weigh all visible rows alike; smaller ones are refused, not taken for the default"""
+    s = Setup(dev, HEADS[0], dtype, 16, [300, 77], seed=31)
+    for counts in ([1, 2], [200, 70]):
+        run_batch(s, counts, scale=2.0 ** -149)
+        run_batch(s, counts, scale=-2.0 ** -148, window=33, sinks=2)
+        q, starts = s.queries(counts)
+        for bad in (1e-46, -1e-46, 1e-300):
+            with pytest.raises(load_pkg().QmoeError, match="scale"):
+                s.cache.attend(0, q.to(dev), i32(starts, dev), scale=bad)
+
+
+@pytest.mark.usefixtures("tables")
 def test_slots_in_any_order_twice_and_out_of_range(dev):
     s = Setup(dev, HEADS[0], torch.bfloat16, 16, [100, 40, 77, 260], seed=3)
     run_batch(s, [1, 6, 1, 30, 2], slots=[2, 0, 2, 3, 0])

@@ -189,6 +189,15 @@ def test_calls_with_nothing_to_do_touch_nothing():
     assert L.qmoe_paged_evict(cp, A, 0, 4, 0, None, ep) == 0
 
 
+def test_scales_that_round_to_the_default_are_refused():
+    pkg = load_pkg()
+    for bad in (0, 0.0, -0.0, 1e-46, -1e-46, 1e-300):
+        with pytest.raises(pkg.QmoeError, match="scale"):
+            pkg.PagedCache._scale(bad)
+    for good in (None, 1e-45, -1e-38, 1.0, float("nan"), float("inf")):  # the last two are refused by the library
+        pkg.PagedCache._scale(good)
+
+
 def test_the_class_refuses_other_tensors():
     import torch
     pkg = load_pkg()
