@@ -127,6 +127,7 @@ class QmoePagedQuery(ctypes.Structure):
 
 
 PAGED_ATTN, PAGED_RESERVE, PAGED_FORK, PAGED_COMPACT = 0, 1, 2, 3
+_INT_END = 2 ** 31
 
 
 class QmoeStTensor(ctypes.Structure):
@@ -1052,6 +1053,8 @@ class PagedCache:
             raise QmoeError("k and v must be [layers, pages, rows, kv heads, head dim] with one shape, type and strides")
         if k.stride(4) != 1:
             raise QmoeError("the head dim of k and v must be contiguous")
+        for nm, t in (("k", k), ("table", table)):
+            self._fits(nm, *t.shape)
         self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
         self.device, self.dtype = k.device, k.dtype
         self._torch, self._i32, self._u8 = torch, torch.int32, torch.uint8
@@ -1064,7 +1067,7 @@ class PagedCache:
             if nm != "v" and (t.dtype != torch.int32 or t.stride(-1) != 1 and t.shape[-1] > 1):
                 raise QmoeError(f"{nm} must be int32 with contiguous rows")
         L, P, R, kvh, hd = k.shape
-        self.kvh, self.hd = kvh, hd
+        self.n_layers, self.kvh, self.hd = L, kvh, hd
         self._c = QmoePagedCache(k.data_ptr(), v.data_ptr(), *k.stride()[:4], _dtype_code(k), L, P, R, kvh, hd,
                                  table.data_ptr(), max(table.stride(0), table.shape[1]) if table.shape[0] == 1 else table.stride(0),
                                  lens.data_ptr(), refs.data_ptr(), table.shape[0], table.shape[1])
@@ -1107,6 +1110,8 @@ class PagedCache:
                 not t.is_contiguous():
             raise QmoeError(f"{what} must be a contiguous int32 vector" + (f" of {n}" if n is not None else "") +
                             f" on {self.device}")
+        if n is None and t.shape[0] >= _INT_END:
+            self._fits(what, t.shape[0])
         return t.data_ptr()
 
     def _rows(self, t, heads, dtypes, what):
@@ -1133,15 +1138,20 @@ class PagedCache:
         return self._torch.empty(need, dtype=self._u8, device=self.device)
 
     @staticmethod
-    def _span(window, sinks):
+    def _fits(what, *sizes):
         """ctypes would cut larger numbers off without a word"""
+        if max(sizes) >= _INT_END:
+            raise QmoeError(f"{what} has a size of {max(sizes)}; sizes must be below 2^31")
+
+    @staticmethod
+    def _span(window, sinks):
         if not (0 <= window < 2 ** 31 and 0 <= sinks < 2 ** 31):
             raise QmoeError(f"window {window} and sinks {sinks} must be in [0, 2^31)")
 
     @staticmethod
     def _scale(scale):
         """0 in f32, what the library reads as the default, is no scale that a caller means"""
-        if scale is not None and ctypes.c_float(scale).value == 0.0:
+        if ctypes.c_float(scale).value == 0.0:
             raise QmoeError(f"scale {scale} must not be 0 or round to it in f32 (None: 1 / sqrt(head_dim))")
 
     def _status(self):
@@ -1152,11 +1162,16 @@ class PagedCache:
         """new rows k, v [n, n_kv_heads, head_dim] into the pages of `layer`
         (the pages' type, or f32 rounded into bf16 pages); nothing is written
         unless `status` (of the reserve that made room for them) is 0"""
+        if not 0 <= layer < self.n_layers:
+            raise QmoeError(f"layer {layer} out of range [0, {self.n_layers})")
         self._rows(k, self.kvh, self._src, "k")
         self._rows(v, self.kvh, self._src, "v")
-        if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
+        n = k.shape[0]
+        if n != v.shape[0] or k.dtype != v.dtype:
             raise QmoeError("k and v must have the same rows and type")
-        b, err = self._batch(k.shape[0], starts, slots, status), QmoeErr()
+        if n >= _INT_END:
+            self._fits("k", n)
+        b, err = self._batch(n, starts, slots, status), QmoeErr()
 
         def call(st):
             _check(lib().qmoe_paged_append(self._cp, layer, ctypes.byref(b), k.data_ptr(), v.data_ptr(), _dtype_code(k),
@@ -1175,10 +1190,16 @@ class PagedCache:
         (of the reserve that made room for them) is 0, are left as out has
         them (undefined without out); out must not overlap q or the cache."""
         heads = q.shape[1] if q.dim() == 3 else 0
-        self._scale(scale)
-        self._span(window, sinks)
+        if not 0 <= layer < self.n_layers:
+            raise QmoeError(f"layer {layer} out of range [0, {self.n_layers})")
+        if scale is not None:
+            self._scale(scale)
+        if window or sinks:
+            self._span(window, sinks)
         self._rows(q, heads, self._own, "q")
         n = q.shape[0]
+        if n >= _INT_END or heads >= _INT_END:
+            self._fits("q", n, heads)
         b, err = self._batch(n, starts, slots, status), QmoeErr()
         if out is not None:
             self._rows(out, heads, self._own, "out")

@@ -316,6 +316,25 @@ def test_numbers_that_c_would_read_differently_are_refused(dev):
     assert s.table.tolist() == s.rows
 
 
+def test_layers_and_rows_that_c_would_cut_off_are_refused(dev):
+    s = Setup(dev, HEADS[2], torch.float32, 8, [20], layers=2)
+    q, starts = s.queries([2])
+    q, starts, error = q.to(dev), i32(starts, dev), load_pkg().QmoeError
+    new = torch.zeros(2, 2, 64, device=dev)
+    before = s.k.clone()
+    for layer in (2 ** 32, 2 ** 32 + 1, -2 ** 32, -1, 2):
+        with pytest.raises(error, match="layer"):
+            s.cache.attend(layer, q, starts)
+        with pytest.raises(error, match="layer"):
+            s.cache.append(layer, new, new, starts)
+    # broadcast rows, which take no memory: 2^32 + 2 of them would be read as 2
+    with pytest.raises(error, match="below 2\\^31"):
+        s.cache.append(0, new[:1].expand(2 ** 32 + 2, 2, 64), new[:1].expand(2 ** 32 + 2, 2, 64), starts)
+    with pytest.raises(error, match="below 2\\^31"):
+        s.cache.attend(0, q[:1].expand(2 ** 32 + 2, 4, 64), starts, out=q)
+    assert torch.equal(s.k, before)
+
+
 @pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("n", [90, 400])

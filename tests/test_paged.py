@@ -194,8 +194,21 @@ def test_scales_that_round_to_the_default_are_refused():
     for bad in (0, 0.0, -0.0, 1e-46, -1e-46, 1e-300):
         with pytest.raises(pkg.QmoeError, match="scale"):
             pkg.PagedCache._scale(bad)
-    for good in (None, 1e-45, -1e-38, 1.0, float("nan"), float("inf")):  # the last two are refused by the library
+    for good in (1e-45, -1e-38, 1.0, float("nan"), float("inf")):  # the last two are refused by the library
         pkg.PagedCache._scale(good)
+
+
+def test_sizes_that_c_would_cut_off_are_refused():
+    import torch
+    pkg = load_pkg()
+    i32 = torch.int32
+    k, lens, refs = torch.zeros(1, 4, 8, 2, 64), torch.zeros(3, dtype=i32), torch.zeros(4, dtype=i32)
+    table = torch.zeros(3, 5, dtype=i32)
+    many = k[:, :1].expand(1, 2 ** 32 + 4, 8, 2, 64)
+    wide = table[:, :1].expand(3, 2 ** 32 + 5)
+    for bad in ((many, many, table, lens, refs), (k, k, wide, lens, refs)):
+        with pytest.raises(pkg.QmoeError, match="below 2\\^31"):
+            pkg.PagedCache(*bad)
 
 
 def test_the_class_refuses_other_tensors():
