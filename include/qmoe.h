@@ -777,11 +777,12 @@ int qmoe_paged_fork(const qmoe_paged_cache *c, const int32_t *src, const int32_t
 /* Releases the pages of the slots (NULL: slots 0 .. n_seqs - 1) that no query
  * at position lens or after it sees under this window (>= 1) and sinks: all
  * rows behind the window of a query at lens, none of them a sink.  Slots out
- * of range are passed over.  Its place is after a step's last attention and
- * before the next reserve, when the next query is at lens.  While r rows at
- * the end of lens are still to be attended (after a reserve), or may yet be
- * cut off (qmoe_paged_fork), earlier queries will come: give window + r, the
- * largest r of the slots.  A released row cannot be had back. */
+ * of range are passed over; n_seqs has no limit but n_slots where slots is
+ * NULL.  Its place is after a step's last attention and before the next
+ * reserve, when the next query is at lens.  While r rows at the end of lens
+ * are still to be attended (after a reserve), or may yet be cut off
+ * (qmoe_paged_fork), earlier queries will come: give window + r, the largest r
+ * of the slots.  A released row cannot be had back. */
 int qmoe_paged_evict(const qmoe_paged_cache *c, const int32_t *slots, int n_seqs, int window, int sinks, void *stream,
                      qmoe_err *err);
 

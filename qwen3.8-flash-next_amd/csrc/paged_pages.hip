@@ -478,20 +478,22 @@ extern "C" int qk_launch_pg_fork(const pg_cache *c, const int32_t *src, const in
 struct PgEvict {
     pg_cache c;
     const int32_t *slots;
-    int window, sinks;
+    int n, window, sinks;
 };
 
 __global__ __launch_bounds__(256) void k_pg_evict(PgEvict a) {
-    const int slot = a.slots ? qk_ld(a.slots + blockIdx.x) : (int)blockIdx.x;
-    if (slot < 0 || slot >= a.c.n_slots) return;
     const int R = (int)a.c.page_rows.d;
-    /* the next query is at position len at the least */
-    const int len = min(max(qk_ld(a.c.lens + slot), 0), a.c.cap), lo = pg_lo(len, a.window);
-    int32_t *row = a.c.table + slot * a.c.table_stride;
-    for (int e = threadIdx.x; (e + 1) * R <= lo; e += 256) {
-        if (e * R < a.sinks) continue;
-        const int was = atomicExch(row + e, -1);
-        if (was >= 0 && was < a.c.n_pages) atomicSub(a.c.refs + was, 1);
+    for (int64_t i = blockIdx.x; i < a.n; i += gridDim.x) {
+        const int slot = a.slots ? qk_ld(a.slots + i) : (int)i;
+        if (slot < 0 || slot >= a.c.n_slots) continue;
+        /* the next query is at position len at the least */
+        const int len = min(max(qk_ld(a.c.lens + slot), 0), a.c.cap), lo = pg_lo(len, a.window);
+        int32_t *row = a.c.table + slot * a.c.table_stride;
+        for (int e = threadIdx.x; (e + 1) * R <= lo; e += 256) {
+            if (e * R < a.sinks) continue;
+            const int was = atomicExch(row + e, -1);
+            if (was >= 0 && was < a.c.n_pages) atomicSub(a.c.refs + was, 1);
+        }
     }
 }
 
@@ -499,8 +501,8 @@ extern "C" int qk_launch_pg_evict(const pg_cache *c, const int32_t *slots, int n
                                   void *stream) {
     PgEvict a;
     a.c = *c;
-    a.slots = slots; a.window = window; a.sinks = sinks;
-    hipLaunchKernelGGL(k_pg_evict, dim3(n_seqs), dim3(256), 0, (hipStream_t)stream, a);
+    a.slots = slots; a.n = n_seqs; a.window = window; a.sinks = sinks;
+    hipLaunchKernelGGL(k_pg_evict, dim3(n_seqs < 65536 ? n_seqs : 65536), dim3(256), 0, (hipStream_t)stream, a);
     return QK_CHECK_LAUNCH();
 }
 

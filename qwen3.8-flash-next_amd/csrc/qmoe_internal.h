@@ -468,7 +468,7 @@ typedef struct {
 #define PG_MAX_ROWS (1 << 30)  /* rows of a table, rows of a call times heads */
 #define PG_MAX_BATCH 1024      /* sequences of a reserve or fork call */
 #define PG_MAX_PAGES (1 << 20) /* pages of a pool: a batch's needs sum in 32 bits */
-#define PG_MAX_SEQS (1 << 16)  /* sequences of an append, attention or evict call */
+#define PG_MAX_SEQS (1 << 16)  /* sequences of an append or attention call */
 
 typedef struct {
     const void *q;

@@ -3,6 +3,7 @@
  * launches of paged_pages.hip and paged_attn.hip.  Holds no state: the cache
  * and the workspaces are the caller's.
  */
+#include <limits.h>
 #include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
@@ -244,7 +245,7 @@ int qmoe_paged_fork(const qmoe_paged_cache *q, const int32_t *src, const int32_t
 int qmoe_paged_evict(const qmoe_paged_cache *q, const int32_t *slots, int n_seqs, int window, int sinks, void *stream,
                      qmoe_err *err) {
     pg_cache c;
-    if (pg_cache_of(q, &c, err) || pg_seqs(&c, slots, n_seqs, PG_MAX_SEQS, err)) return -1;
+    if (pg_cache_of(q, &c, err) || pg_seqs(&c, slots, n_seqs, INT_MAX, err)) return -1;
     if (window < 1 || sinks < 0) return pg_fail(err, "window %d must be >= 1 and sinks %d >= 0", window, sinks);
     if (n_seqs == 0) return 0;
     return pg_hip(err, qk_launch_pg_evict(&c, slots, n_seqs, window, sinks, stream), "paged evict");

@@ -947,6 +947,21 @@ def test_evict_spares_what_reserved_and_cut_off_rows_need(dev, page, window, sin
     assert torch.equal(c.table, before)
 
 
+@pytest.mark.parametrize("slots", [65536, 65537, 200001])
+def test_evict_on_many_slots(dev, slots):
+    """more slots than a launch has workgroups: a page of each, behind the window or not"""
+    pkg = load_pkg()
+    c = pkg.PagedCache.allocate(1, slots, 2, 1, 64, slots, 2, torch.bfloat16, dev)
+    for named in (None, torch.randperm(slots, generator=torch.Generator().manual_seed(32)).to(torch.int32).to(dev)):
+        c.table[:, 0] = torch.arange(slots, device=dev).int()
+        c.refs.fill_(1)
+        c.lens.copy_(torch.arange(slots, device=dev) % 5)  # rows 0 and 1 are behind a window of 1 from length 2 on
+        c.evict(1, 0, named)
+        gone = c.lens >= 2
+        assert torch.equal(c.table[:, 0] < 0, gone) and torch.equal(c.refs == 0, gone)
+        assert torch.equal(c.table[:, 0][~gone], torch.arange(slots, device=dev).int()[~gone])
+
+
 @pytest.mark.parametrize("order", ["rows", "heads"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 def test_compact_moves_contents(dev, dtype, order):
