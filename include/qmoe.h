@@ -743,7 +743,9 @@ typedef struct {
     const void *q;
     void *out;              /* not overlapping q or the cache */
     int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride; /* elements, multiples of 16 bytes */
-    int n_heads;            /* a multiple of n_kv_heads; n * n_heads <= 2^30 */
+    int n_heads;            /* a multiple of n_kv_heads; n * n_heads <= 2^30, and the call's workgroups
+                             * (about one per sequence, kv head and 16 to 128 rows of a kv head's
+                             * group) times their 256 or 512 threads below 2^32 */
     int window;             /* 0: none */
     int sinks;              /* first rows that stay visible behind the window */
     int grouped;            /* 0: head h reads kv head h % n_kv_heads, as qmoe_attn_*;

@@ -1320,14 +1320,23 @@ static size_t pa_ws(const pg_cache *c, int n, int n_seqs, int h, int rt) {
     const size_t index = n_seqs > PA_INDEX ? pa_up((size_t)n_seqs * 16) : 0;
     return 256 + index + pa_up((size_t)q.slots * rt * 8) + pa_up((size_t)q.slots * rt * c->hd * 4);
 }
-/* of either choice of rows: the window is not known here */
+static int pa_threads(const pg_cache *c, int n, int h, int rt) {
+    if (rt != PM_RT) return 256;
+    return 256 * (c->dtype == QMOE_BF16 ? pa_groups(c, n, h) : pm_halves32(c->hd));
+}
+/* of either choice of rows: the window is not known here.  0 where a launch
+ * would have 2^32 threads or more, which HIP does not take; units of 16 rows
+ * that are chosen because the call is short (pa_rows) are below 2^24, and more
+ * than the longer ones would be. */
 extern "C" size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h) {
-    const size_t a = pa_ws(c, n, n_seqs, h, 16), b = pa_ws(c, n, n_seqs, h, pa_rows_long(c, (int64_t)n * (h / c->kvh), n_seqs));
+    const int rt = pa_rows_long(c, (int64_t)n * (h / c->kvh), n_seqs);
+    if (pa_plan_of(c, n, n_seqs, h, rt).grid * pa_threads(c, n, h, rt) > 0xFFFFFFFFll) return 0;
+    const size_t a = pa_ws(c, n, n_seqs, h, 16), b = pa_ws(c, n, n_seqs, h, rt);
     return a > b ? a : b;
 }
 
 template <typename T, int HD, int RT, int KT>
-static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), int threads, void *ws, hipStream_t st) {
+static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), void *ws, hipStream_t st) {
     const PaPlan q = pa_plan_of(&p.c, p.a.n, p.a.n_seqs, p.a.h, RT);
     p.per_unit = pg_per_unit(p.c.kvh, q.units);
     p.extra = q.extra;
@@ -1341,7 +1350,7 @@ static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), int threads, void *ws,
         const int rc = QK_CHECK_LAUNCH();
         if (rc) return rc;
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)q.grid), dim3(threads), 0, st, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)q.grid), dim3(pa_threads(&p.c, p.a.n, p.a.h, RT)), 0, st, p);
     const int rc = QK_CHECK_LAUNCH();
     if (rc || q.join == 0) return rc;
     /* few tasks are long sequences on their own, a few rows of a hundred parts:
@@ -1359,13 +1368,13 @@ static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
     if (rt == PM_RT) {
         if constexpr (sizeof(T) == 2) {
             if constexpr (HD <= 128)
-                if (pa_groups(&p.c, p.a.n, p.a.h) == 1) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 1>, 256, ws, st);
-            return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 2>, 512, ws, st);
-        } else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD>, 256 * pm_halves32(HD), ws, st);
+                if (pa_groups(&p.c, p.a.n, p.a.h) == 1) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 1>, ws, st);
+            return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 2>, ws, st);
+        } else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD>, ws, st);
     }
     if constexpr (HD <= (sizeof(T) == 2 ? 192 : 128)) /* pa_two */
-        if (rt == 32) return pa_launch_rt<T, HD, 32, PD_KT>(p, k_pa_few<T, HD, 2>, 256, ws, st);
-    return pa_launch_rt<T, HD, 16, PD_KT>(p, k_pa_few<T, HD, 1>, 256, ws, st);
+        if (rt == 32) return pa_launch_rt<T, HD, 32, PD_KT>(p, k_pa_few<T, HD, 2>, ws, st);
+    return pa_launch_rt<T, HD, 16, PD_KT>(p, k_pa_few<T, HD, 1>, ws, st);
 }
 
 template <typename T>

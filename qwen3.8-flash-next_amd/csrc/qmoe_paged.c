@@ -198,9 +198,11 @@ int qmoe_paged_attn(const qmoe_paged_cache *cache, int layer, const qmoe_paged_b
     const int64_t stride[2] = {q->out_token_stride, q->out_head_stride}, size[2] = {b->n, q->n_heads};
     if (pg_apart(stride, size, 2, c.hd)) return pg_fail(err, "the strides let elements of out overlap");
     if (b->n == 0 || b->n_seqs == 0) return 0;
+    const size_t need = qk_pg_attn_ws(&c, b->n, b->n_seqs, q->n_heads);
+    if (!need) return pg_fail(err, "%d rows of %d sequences and %d heads are more work than one launch holds", b->n, b->n_seqs, q->n_heads);
     if (!q->q || !q->out) return pg_fail(err, "%s is NULL", q->q ? "out" : "q");
     if (pg_misaligned(q->q) || pg_misaligned(q->out)) return pg_fail(err, "q and out must be 16-byte aligned");
-    if (pg_work(ws, ws_bytes, qk_pg_attn_ws(&c, b->n, b->n_seqs, q->n_heads), err)) return -1;
+    if (pg_work(ws, ws_bytes, need, err)) return -1;
     pg_attn a;
     a.q = q->q;
     a.out = q->out;

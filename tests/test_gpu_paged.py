@@ -276,6 +276,21 @@ def test_single_tokens_of_long_sequences(dev, shape, lens, counts, dtype):
     run_batch(s, counts, window=2100, sinks=3)
 
 
+def test_the_largest_number_of_units(dev):
+    """16 776 960 workgroups: single tokens of 65535 sequences with one row, on 256 kv heads; one more is refused"""
+    pkg = load_pkg()
+    n, kvh, hd = 65536, 256, 64
+    k, v = (torch.randn(1, 2, 1, kvh, hd, device=dev).bfloat16() for _ in range(2))
+    cache = pkg.PagedCache(k, v, (torch.arange(n, device=dev).int() % 2)[:, None].contiguous(), torch.ones(n, dtype=torch.int32, device=dev),
+                           i32([n // 2] * 2, dev))
+    q = torch.ones(1, kvh, hd, dtype=torch.bfloat16, device=dev).expand(n, kvh, hd)
+    starts = torch.arange(n + 1, device=dev).int()
+    with pytest.raises(pkg.QmoeError, match="more work"):
+        cache.attend(0, q, starts)
+    out = cache.attend(0, q[:-1], starts[:-1])
+    assert torch.equal(out[0::2], v[0, 0].expand(n // 2, kvh, hd)) and torch.equal(out[1::2], v[0, 1].expand(n // 2 - 1, kvh, hd))
+
+
 def test_forks_of_large_tables(dev):
     """tables of 60 x 250 entries: sources shared, swapped and cut, refusals, against the tables before"""
     pkg = load_pkg()

@@ -178,6 +178,30 @@ def test_other_bad_calls_are_refused():
         refused(run(A + 8, need), "workspace")
 
 
+# a workgroup of 256 threads per sequence and kv head; 128 rows of 512 threads
+@pytest.mark.parametrize("ckw,n,n_seqs,heads,fits", [
+    (dict(n_kv_heads=256, head_dim=64, max_pages=1), 65536, 65536, 256, False),
+    (dict(n_kv_heads=256, head_dim=64, max_pages=1), 65535, 65535, 256, True),
+    (dict(n_kv_heads=256, head_dim=64, max_pages=4096), 65535, 65535, 256, False),  # and parts of the keys
+    (dict(n_kv_heads=256, head_dim=64, max_pages=4096), 65527, 65527, 256, True),
+    (dict(n_kv_heads=1024, head_dim=256, max_pages=1, dtype=0), 1 << 20, 1 << 15, 1024, False),
+    (dict(n_kv_heads=1024, head_dim=64, max_pages=1), 1 << 20, 65536, 1024, False),
+    (dict(n_kv_heads=8, head_dim=64, max_pages=1), 1 << 20, 1, 1024, True),
+])
+def test_more_work_than_a_launch_holds_is_refused(ckw, n, n_seqs, heads, fits):
+    pkg = load_pkg()
+    L, e = pkg.lib(), pkg.QmoeErr()
+    hd = ckw["head_dim"]
+    c = cache(pkg, **dict(dict(head_stride=hd, row_stride=hd * ckw["n_kv_heads"], page_stride=16 * hd * ckw["n_kv_heads"],
+                               layer_stride=1 << 40, n_slots=65536, table_stride=ckw["max_pages"]), **ckw))
+    assert (L.qmoe_paged_ws_bytes(ctypes.byref(c), 0, n, n_seqs, heads) > 0) == fits
+    if not fits:
+        q = query(pkg, n_heads=heads, q_token_stride=heads * hd, q_head_stride=hd, out_token_stride=heads * hd, out_head_stride=hd)
+        b = batch(pkg, n=n, n_seqs=n_seqs)
+        rc = L.qmoe_paged_attn(ctypes.byref(c), 0, ctypes.byref(b), ctypes.byref(q), A, 1 << 40, None, ctypes.byref(e))
+        assert rc == -1 and b"more work" in e.msg, e.msg
+
+
 def test_calls_with_nothing_to_do_touch_nothing():
     pkg = load_pkg()
     L, e = pkg.lib(), pkg.QmoeErr()
