@@ -116,6 +116,31 @@ def test_null_arguments_are_refused():
     assert L.qmoe_paged_evict(None, A, 3, 64, 0, None, None) == -1
 
 
+def test_every_null_argument_is_named():
+    """each call on its own, its message read before the next"""
+    pkg = load_pkg()
+    L, e, big = pkg.lib(), pkg.QmoeErr(), 1 << 40
+    structs = cache(pkg), batch(pkg), query(pkg), query(pkg, q=None), query(pkg, out=None), batch(pkg, starts=None), e
+    cp, bp, qp, no_q, no_out, no_starts, ep = (ctypes.byref(x) for x in structs)
+    append = lambda b, k, v: L.qmoe_paged_append(cp, 0, b, k, v, pkg.BF16, 256, 128, 256, 128, None, ep)
+    attn = lambda b, q, ws=A: L.qmoe_paged_attn(cp, 0, b, q, ws, big, None, ep)
+    reserve = lambda add, status=A, ws=A: L.qmoe_paged_reserve(cp, A, add, 3, status, ws, big, None, ep)
+    fork = lambda src, dst, status=A, ws=A: L.qmoe_paged_fork(cp, src, dst, None, 3, status, ws, big, None, ep)
+    compact = lambda used, ws=A: L.qmoe_paged_compact(cp, used, ws, big, None, ep)
+    for call, args, msg in ((append, (None, A, A), "batch is NULL"), (append, (bp, None, A), "k is NULL"),
+                            (append, (bp, A, None), "v is NULL"), (append, (no_starts, A, A), "starts is NULL"),
+                            (attn, (None, qp), "batch is NULL"), (attn, (bp, None), "query is NULL"),
+                            (attn, (bp, no_q), "q is NULL"), (attn, (bp, no_out), "out is NULL"),
+                            (attn, (no_starts, qp), "starts is NULL"), (attn, (bp, qp, None), "workspace is NULL"),
+                            (reserve, (None,), "n_new is NULL"), (reserve, (A, None), "status is NULL"),
+                            (reserve, (A, A, None), "workspace is NULL"), (fork, (None, A), "src is NULL"),
+                            (fork, (A, None), "dst is NULL"), (fork, (A, A, None), "status is NULL"),
+                            (fork, (A, A, A, None), "workspace is NULL"), (compact, (None,), "used is NULL"),
+                            (compact, (A, None), "workspace is NULL")):
+        e.msg = b"nothing"
+        assert call(*args) == -1 and msg in e.msg.decode(), (msg, e.msg)
+
+
 BAD_ATTN = [
     (dict(), dict(n=-1), dict(), 0, "n = -1"), (dict(), dict(n_seqs=-1), dict(), 0, "n_seqs"),
     (dict(), dict(n_seqs=70000), dict(), 0, "n_seqs"), (dict(), dict(slots=None, n_seqs=5), dict(), 0, "slots"),
