@@ -390,7 +390,6 @@ __global__ __launch_bounds__(256) void k_pg_fork_write(PgFork a) {
         return;
     }
     if (i == 0 && tid == 0) *a.status = 0;
-    if (i >= a.n) return; /* an empty batch still reports */
     const int d = qk_ld(a.dst + i), len = qk_ld(a.head + i).x;
     const int keep = (int)pg_div_of(a.c.page_rows, (uint32_t)(len + (int)a.c.page_rows.d - 1));
     int32_t *row = a.c.table + d * a.c.table_stride;
@@ -404,8 +403,9 @@ __global__ __launch_bounds__(256) void k_pg_fork_write(PgFork a) {
     if (tid == 0) a.c.lens[d] = len;
 }
 
-/* The same in one launch, one workgroup, for batches whose entries fit LDS:
- * four branches of a short prompt 3.1 us. */
+/* The same in one launch, one workgroup, for batches whose entries fit LDS
+ * (empty ones, which report too, among them): four branches of a short prompt
+ * 3.1 us. */
 #define PG_FORK_SMALL 12288
 __global__ __launch_bounds__(1024) void k_pg_fork_small(PgFork a) {
     __shared__ int32_t entries[PG_FORK_SMALL];
@@ -462,12 +462,10 @@ extern "C" int qk_launch_pg_fork(const pg_cache *c, const int32_t *src, const in
         hipLaunchKernelGGL(k_pg_fork_small, dim3(1), dim3(1024), 0, st, a);
         return QK_CHECK_LAUNCH();
     }
-    if (n_seqs > 0) {
-        hipLaunchKernelGGL(k_pg_fork_read, dim3(n_seqs), dim3(256), 0, st, a);
-        const int rc = QK_CHECK_LAUNCH();
-        if (rc) return rc;
-    }
-    hipLaunchKernelGGL(k_pg_fork_write, dim3(n_seqs > 0 ? n_seqs : 1), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(k_pg_fork_read, dim3(n_seqs), dim3(256), 0, st, a);
+    const int rc = QK_CHECK_LAUNCH();
+    if (rc) return rc;
+    hipLaunchKernelGGL(k_pg_fork_write, dim3(n_seqs), dim3(256), 0, st, a);
     return QK_CHECK_LAUNCH();
 }
 
