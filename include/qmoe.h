@@ -736,9 +736,10 @@ int qmoe_paged_append(const qmoe_paged_cache *c, int layer, const qmoe_paged_bat
  *   j <= p, with a page, and (window == 0 or p - j < window or j < sinks).
  * A query that sees no row gives zeros; rows outside its sight never reach
  * its output, whatever they hold.  q and out [n, n_heads, head_dim] have the
- * pages' type; scores, softmax statistics and sums are fp32, and with bf16
- * the softmax weights are rounded to bf16 for the product with v.  Results
- * are the same from call to call. */
+ * pages' type; scores, softmax statistics and sums are fp32.  For the product
+ * with v the softmax weights of bf16 calls have 16 bits in calls of few rows
+ * (single tokens among them), and are rounded to bf16 in longer ones.
+ * Results are the same from call to call. */
 typedef struct {
     const void *q;
     void *out;              /* not overlapping q or the cache */

@@ -392,8 +392,12 @@ __device__ __forceinline__ void pa_softmax(qm_f32x16 (&st)[NS], float scale, flo
         for (int i = 0; i < 16; i++) st[t][i] = __builtin_amdgcn_exp2f(fmaf(st[t][i], scale, -ms));
 }
 
-/* eight weights of a row as a B operand; l takes the sum of the rounded
- * weights, so that they add up to one again */
+/* Eight weights of a row as a B operand, rounded to bf16: half a step, 2^-8 of
+ * each, 0.0015 of the result beside the 0.0017 of its own rounding (relative
+ * L2 on normal inputs, 0.0022 together).  A second part, as k_pa_few's, takes
+ * that away, but doubles the products with v, which bound a prompt: of 8192
+ * 305 and 408 us, of 1000 26 and 30.  l takes the sum of the rounded weights,
+ * so that they add up to one again. */
 __device__ __forceinline__ qm_bf16x8 pa_pack(const qm_f32x16 &st, int s, float &l) {
     uint32_t w[4];
 #pragma unroll
@@ -445,7 +449,9 @@ __device__ __forceinline__ bool pa_again(const V (&o)[N], float l, bool seen) {
  * quarter has every fourth piece of 16 bytes.  V: a lane takes HD / 16 dims of
  * the eight keys its quarter of P^T has; bf16 pairs are turned in registers
  * (two keys' words, one byte permute), and O^T's row x of tile e is dim
- * (HD / 16) x + e.  f32 runs on the fp32 matrix instructions, whose operands
+ * (HD / 16) x + e.  The weights of bf16 calls are taken in two bf16 parts (16
+ * bits), which leaves the output's rounding alone; the pages' loads hide the
+ * second product (64 tokens 172 us with one part, 173 with two).  f32 runs on the fp32 matrix instructions, whose operands
  * are single elements.
  * Bound: HBM, the visible pages read once: single tokens of 64 sequences of 64
  * to 65536 rows (841 MB of bf16) 171 to 178 us, 4.8 TB/s, of 1024 sequences
@@ -602,20 +608,22 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
             for (int k = 0; k < 8; k++) {
                 const float w = __builtin_amdgcn_exp2f(fmaf(st[x][k >> 2][k & 3], scale, -ms));
                 st[x][k >> 2][k & 3] = w;
-                if constexpr (!B16) l[x] += w;
+                l[x] += w;
             }
         }
         if constexpr (B16) {
-            qm_bf16x8 pw[NC];
+            qm_bf16x8 pw[NC][2]; /* a weight in two bf16 parts */
 #pragma unroll
-            for (int x = 0; x < NC; x++) { /* l: the sum of the rounded weights, as pa_pack */
-                uint32_t w[4];
+            for (int x = 0; x < NC; x++) {
+                uint32_t w[4], y[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    w[k] = qk_cvt_pk_bf16(st[x][k >> 1][2 * (k & 1)], st[x][k >> 1][2 * (k & 1) + 1]);
-                    l[x] = qk_dot2(w[k], QK_BF16_ONES, l[x]);
+                    const float a = st[x][k >> 1][2 * (k & 1)], b = st[x][k >> 1][2 * (k & 1) + 1];
+                    w[k] = qk_cvt_pk_bf16(a, b);
+                    y[k] = qk_cvt_pk_bf16(a - qk_bf16_lo(w[k]), b - qk_bf16_hi(w[k]));
                 }
-                pw[x] = __builtin_bit_cast(qm_bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+                pw[x][0] = __builtin_bit_cast(qm_bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+                pw[x][1] = __builtin_bit_cast(qm_bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
             }
 #pragma unroll
             for (int e = 0; e < E; e++) {
@@ -625,7 +633,9 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
                     w[x] = __builtin_amdgcn_perm(vx[2 * x + 1][e >> 1], vx[2 * x][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
                 const qm_bf16x8 a = __builtin_bit_cast(qm_bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
 #pragma unroll
-                for (int x = 0; x < NC; x++) o[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pw[x], o[x][e], 0, 0, 0);
+                for (int x = 0; x < NC; x++)
+#pragma unroll
+                    for (int y = 1; y >= 0; y--) o[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pw[x][y], o[x][e], 0, 0, 0);
             }
         } else {
 #pragma unroll

@@ -386,6 +386,26 @@ def test_tiny_scales(dev, dtype):
                 s.cache.attend(0, q.to(dev), i32(starts, dev), scale=bad)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 192, 256])
+def test_weights_of_few_rows_have_16_bits(dev, hd, monkeypatch):
+    """bf16 calls of 16 and 32 rows a unit.  A weight is taken as bf16(w) + bf16(w - bf16(w)): the first is off by
+    2^-8 w at the most, the second by 2^-8 of that, so the sum of w v is off by 2^-16 A beside the fp32 terms of the
+    bar above.  A small scale keeps those small (B is below 1), and sums that nearly cancel show the weights' error,
+    which rounding the weights to bf16 makes 2^-9 A / sqrt(keys) and more."""
+    for table_rows, counts in ((0, [1, 1, 1]), (1 << 18, [3, 4, 3])):
+        monkeypatch.setattr(Setup, "table_rows", table_rows)
+        s = Setup(dev, (8, 1, hd), torch.bfloat16, 16, [20, 33, 60], seed=33)
+        q, starts = s.queries(counts)
+        out = s.cache.attend(0, q.to(dev), i32(starts, dev), scale=0.02 * hd ** -0.5).double().cpu()
+        for i, c in enumerate(counts):
+            T = s.lens[i]
+            want, A, B = reference(q[starts[i]:starts[i + 1]], s.hk[i], s.hv[i], c, 0, 0, False, 0.02 * hd ** -0.5)
+            assert float(B.max()) < 1
+            tol = A * (2 * (hd + 24) * U * (B + 1) + 2 * (T + 64) * U + 2.0 ** -16) + want.abs() * 2.0 ** -8
+            err = (out[starts[i]:starts[i + 1]] - want).abs()
+            assert (err <= tol).all(), (i, T, float((err / tol).max()))
+
+
 @pytest.mark.usefixtures("tables")
 def test_slots_in_any_order_twice_and_out_of_range(dev):
     s = Setup(dev, HEADS[0], torch.bfloat16, 16, [100, 40, 77, 260], seed=3)
