@@ -726,7 +726,8 @@ size_t qmoe_paged_ws_bytes(const qmoe_paged_cache *c, int call, int n, int n_seq
  * to nearest even).  Strides in elements, multiples of 16 bytes, dims
  * contiguous, k and v 16-byte aligned.  A row with no page, or at a negative
  * position (more new rows than cached ones), is not written.  A batch names
- * a slot once. */
+ * a slot once, and its rows have room from qmoe_paged_reserve: refs are not
+ * looked at here, a page that others hold is written for them too. */
 int qmoe_paged_append(const qmoe_paged_cache *c, int layer, const qmoe_paged_batch *b, const void *k, const void *v,
                       int src_dtype, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
                       int64_t v_head_stride, void *stream, qmoe_err *err);

@@ -121,9 +121,11 @@ __device__ __forceinline__ pg_seq pa_seq(const PaArgs &p, int i) { return pg_seq
  * (units, joined tasks, split units) and its parts, by one workgroup in a
  * launch of its own, which the units then search.  Units that each went over
  * all sequences by themselves took 309 us for single tokens of 1024 sequences
- * of 1000 rows, 198 with the index; of 100 sequences of 200 rows, 11.7 and
- * 13.0 (the launch), of 1000, 38 and 35.  The total is summed in fp32, in a
- * fixed order. */
+ * of 1000 rows, 198 with the index; of 100 sequences of 200 rows 11.7 and
+ * 13.0 (the launch), of 1000 rows 38 and 35.  So the two meet between 64 and some
+ * hundred sequences, by their lengths, which the host does not know: the limit
+ * is where a lane per sequence ends and the other way would need a loop.  The
+ * total is summed in fp32, in a fixed order. */
 #define PA_INDEX 64
 __global__ __launch_bounds__(1024) void k_pa_index(PaArgs p, int rt, int kt) {
     __shared__ float sum[16];
@@ -440,12 +442,13 @@ __device__ __forceinline__ bool pa_again(const V (&o)[N], float l, bool seen) {
 
 /* ------------------------------------------------------------ few rows
  * Decode and short calls: a unit is 16 NC rows (a group's heads of one to a
- * few tokens) and a part of the keys; its four waves take the part's tiles of 32 keys in turn
- * and join through LDS at the end.  K and V go straight from the pages to
- * registers in operand order, so the main loop has no barrier and the loads
- * of eight or more waves per CU are in flight.  16-wide instructions: lane =
- * (row or key c = lane % 16, quarter g = lane / 16); the scores of a tile
- * leave lane (c, g) the keys 16 n + 4 g + b of row c.  K: lane c = key, a
+ * few tokens) and a part of the keys; its four waves take the part's tiles of
+ * 32 keys in turn and join through LDS at the end.  K and V go straight from
+ * the pages to registers in operand order, so the main loop has no barrier and
+ * the loads of 8 to 20 waves per CU are in flight; of four where the registers
+ * hold one workgroup only (pd_occ 1: f32 past head dim 128, 32 rows of f32 at
+ * 128 and of bf16 at 192).  16-wide instructions: lane = (row or key
+ * c = lane % 16, quarter g = lane / 16); the scores of a tile leave lane (c, g) the keys 16 n + 4 g + b of row c.  K: lane c = key, a
  * quarter has every fourth piece of 16 bytes.  V: a lane takes HD / 16 dims of
  * the eight keys its quarter of P^T has; bf16 pairs are turned in registers
  * (two keys' words, one byte permute), and O^T's row x of tile e is dim
@@ -454,9 +457,10 @@ __device__ __forceinline__ bool pa_again(const V (&o)[N], float l, bool seen) {
  * second product (64 tokens 172 us with one part, 173 with two).  f32 runs on the fp32 matrix instructions, whose operands
  * are single elements.
  * Bound: HBM, the visible pages read once: single tokens of 64 sequences of 64
- * to 65536 rows (841 MB of bf16) 171 to 178 us, 4.8 TB/s, of 1024 sequences
- * of 1000 rows 198 us, 5.3 TB/s.  Short calls: latency, f32 under a window of
- * 1024 of 32 sequences (68 MB) 25 us, a token on 333 rows 10, a prompt of 64 8. */
+ * to 65536 rows (841 MB of bf16) 177 us with the join's 10, 4.75 TB/s; of 1024
+ * sequences of 1000 rows 204 us, 5.2 TB/s, in f32 405; a kernel that only reads
+ * reaches 5.9.  Short calls: latency, f32 under a window of 1024 of 32
+ * sequences (68 MB) 25 us, a token on 333 rows 10, a prompt of 64 8. */
 #define PD_KT 32
 typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
 
@@ -744,10 +748,10 @@ __device__ __forceinline__ void pa_store(const PaArgs &p, const PaUnit &u, const
  * is looked up for 512 keys a group at a time; a row without a page or after
  * the last query is copied from a row of zeros.
  * Bound: a wave's own chain of a step.  A prompt of 8192 (16 heads on 2 of 128)
- * takes 297 to 309 us, 890 to 925 TFLOP/s of 1180 of a large library product.  A
- * step of 5400 clocks was scores 1200, maximum and exponentials 1200, sums of
- * v 1250, issuing the copies 1100 (now between the products) and waiting at
- * the barrier 100 to 970; the matrix cores work 40 % of it.  Without gain: a
+ * takes 294 to 312 us by the card, 880 to 936 TFLOP/s of 1180 of a large library
+ * product.  A step of 5400 clocks was scores 1200, maximum and exponentials
+ * 1200, sums of v 1250, issuing the copies 1100 (now between the products) and
+ * waiting at the barrier 100 to 970; the matrix cores work 40 % of it.  Without gain: a
  * raised wave priority in either half, two groups half a step apart (360 us),
  * scores of the next tile beside the softmax (337 to 348), three groups (326),
  * units of 64 rows (short prompts 10 % better, long contexts 40 % worse). */

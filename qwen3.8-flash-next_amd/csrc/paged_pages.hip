@@ -118,8 +118,10 @@ extern "C" int qk_launch_pg_append(const pg_cache *c, const void *k, const void 
 /* ------------------------------------------------------------ page copies
  * Pages (src, dst) of every layer's k and v.  A page is rows x heads x
  * 16-byte chunks with strides; dimensions that lie one after the other are
- * merged on the host, so a dense page is one run.  Bound: HBM: 136 pages of
- * 12 layers (107 MB read and written) 18 us, 5.8 TB/s. */
+ * merged on the host, so a dense page is one run.  Bound: memory: 256 copies of
+ * 16 pages of 12 layers (101 MB written; the 6 MB of the sources are read from
+ * HBM once and 15 times from caches) 18 us, 5.6 TB/s of writes, which stay in
+ * the memory-side cache. */
 struct PgCopy {
     pg_cache c;
     const int2 *pairs;        /* (-1, -1): none */
@@ -181,8 +183,9 @@ static unsigned pg_copy_grid(const pg_cache *c, int64_t pairs) {
 /* ------------------------------------------------------------ reserve
  * One workgroup: the sequences' needs, their prefix sums, and as many free
  * pages, lowest first.  One workgroup, since every page's rank depends on all
- * sequences.  Bound: latency, of its reads of refs and of the scan over the
- * batch: 5.3 us for 4 sequences, 13.4 for 256.  Without gain: several threads
+ * sequences.  Bound: latency, of its reads of refs (5.3 us for 4 sequences) and
+ * of the comparison of every sequence with every other, about 8 of the 13.5 us
+ * for 256.  Without gain: several threads
  * per sequence in the scan (12.9, but 7.3 for 4), the free pages counted under
  * the loads of the batch (13.6). */
 struct PgReserve {
