@@ -447,15 +447,16 @@ __device__ __forceinline__ bool pa_again(const V (&o)[N], float l, bool seen) {
  * the pages to registers in operand order, so the main loop has no barrier and
  * the loads of 8 to 20 waves per CU are in flight; of four where the registers
  * hold one workgroup only (pd_occ 1: f32 past head dim 128, 32 rows of f32 at
- * 128 and of bf16 at 192).  16-wide instructions: lane = (row or key
- * c = lane % 16, quarter g = lane / 16); the scores of a tile leave lane (c, g) the keys 16 n + 4 g + b of row c.  K: lane c = key, a
- * quarter has every fourth piece of 16 bytes.  V: a lane takes HD / 16 dims of
- * the eight keys its quarter of P^T has; bf16 pairs are turned in registers
- * (two keys' words, one byte permute), and O^T's row x of tile e is dim
- * (HD / 16) x + e.  The weights of bf16 calls are taken in two bf16 parts (16
- * bits), which leaves the output's rounding alone; the pages' loads hide the
- * second product (64 tokens 172 us with one part, 173 with two).  f32 runs on the fp32 matrix instructions, whose operands
- * are single elements.
+ * 128 and of bf16 at 192).  16-wide instructions: lane = (row or key c = lane %
+ * 16, quarter g = lane / 16); the scores of a tile leave lane (c, g) the keys 16
+ * n + 4 g + b of row c.  K: lane c = key, a quarter has every fourth piece of 16
+ * bytes.  V: a lane takes HD / 16 dims of the eight keys its quarter of P^T has;
+ * bf16 pairs are turned in registers (two keys' words, one byte permute), and
+ * O^T's row x of tile e is dim (HD / 16) x + e.  The weights of bf16 calls are
+ * taken in two bf16 parts (16 bits), which leaves the output's rounding alone;
+ * the pages' loads hide the second product (64 tokens 172 us with one part, 173
+ * with two).  f32 runs on the fp32 matrix instructions, whose operands are single
+ * elements.
  * Bound: HBM, the visible pages read once: single tokens of 64 sequences of 64
  * to 65536 rows (841 MB of bf16) 177 us with the join's 10, 4.75 TB/s; of 1024
  * sequences of 1000 rows 204 us, 5.2 TB/s, in f32 405; a kernel that only reads
