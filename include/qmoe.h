@@ -716,9 +716,11 @@ typedef struct {
     const int32_t *status;  /* device, 4-byte aligned; or NULL: as 0 */
 } qmoe_paged_batch;
 
-/* workspace bytes of a call; 0 for arguments that the call refuses.  n and
- * n_heads count for QMOE_PAGED_ATTN only, n_seqs not for QMOE_PAGED_COMPACT. */
-enum { QMOE_PAGED_ATTN = 0, QMOE_PAGED_RESERVE = 1, QMOE_PAGED_FORK = 2, QMOE_PAGED_COMPACT = 3 };
+/* workspace bytes of a call; 0 for arguments that the call refuses.  n counts
+ * for QMOE_PAGED_ATTN (qmoe_paged_attn and qmoe_paged_attn_tree) and
+ * QMOE_PAGED_KEEP only, n_heads for the first, n_seqs not for
+ * QMOE_PAGED_COMPACT. */
+enum { QMOE_PAGED_ATTN = 0, QMOE_PAGED_RESERVE = 1, QMOE_PAGED_FORK = 2, QMOE_PAGED_COMPACT = 3, QMOE_PAGED_KEEP = 4 };
 size_t qmoe_paged_ws_bytes(const qmoe_paged_cache *c, int call, int n, int n_seqs, int n_heads);
 
 /* Writes the batch's new rows k, v [n, n_kv_heads, head_dim] into the pages
@@ -795,6 +797,97 @@ int qmoe_paged_evict(const qmoe_paged_cache *c, const int32_t *slots, int n_seqs
  * contents (every layer), all tables and refs follow.  *used (device) = U. */
 int qmoe_paged_compact(const qmoe_paged_cache *c, int32_t *used, void *ws, size_t ws_bytes, void *stream,
                        qmoe_err *err);
+
+/* Drafted tokens.  A server that guesses several tokens ahead checks them all
+ * in one call: the drafts of a sequence are its new rows of a batch, arranged
+ * as trees.  qmoe_paged_reserve makes room for them; qmoe_paged_tree_build
+ * finds, once per step, what qmoe_paged_append_rotary and qmoe_paged_attn_tree
+ * of every layer need; qmoe_paged_follow finds the path that the target's own
+ * choices take, and qmoe_paged_keep keeps its rows and gives the others' room
+ * back.
+ *
+ * Row t of a sequence is the child of its row parents[t] (-1: of the cached
+ * rows before the call, a root).  Parents come before their children: a row
+ * whose parent is not in [-1, t), or is no node itself, is no node.  Rows are
+ * numbered within their sequence, of which the first 32 * words are looked
+ * at; rows past them are no nodes. */
+typedef struct {
+    int32_t *depths;        /* [n] device: 0 for a root, a child's is its parent's + 1; -1: no node */
+    uint32_t *seen;         /* [n, words] device: bit r % 32 of word r / 32 of row t: r is t or an ancestor of t */
+    int words;              /* 1 .. 32: as many as the largest sequence's rows / 32, rounded up */
+} qmoe_paged_tree;
+
+/* Writes the depths and bits of the rows of every sequence (starts as in
+ * qmoe_paged_batch); rows of no sequence are left alone. */
+int qmoe_paged_tree_build(const int32_t *parents, const int32_t *starts, int n, int n_seqs, const qmoe_paged_tree *t,
+                          void *stream, qmoe_err *err);
+
+/* qmoe_paged_attn of trees.  With first = lens - (the sequence's new rows),
+ * row t stands at position first + depths[t] and sees the cached rows j <
+ * first as a query at that position would, and of the new rows those in its
+ * bits (up to its own), whose positions are first + their depths: the window
+ * and the sinks count in positions.  A row that is no node gives zeros.  The
+ * bits may be the caller's own, of any rows r <= t (bits past t do not count,
+ * depths are brought into [-1, t], a seen row's into [0, r]).  Workspace as
+ * QMOE_PAGED_ATTN. */
+int qmoe_paged_attn_tree(const qmoe_paged_cache *c, int layer, const qmoe_paged_batch *b, const qmoe_paged_query *q,
+                         const qmoe_paged_tree *t, void *ws, size_t ws_bytes, void *stream, qmoe_err *err);
+
+/* qmoe_paged_append with the position rotation on the way, and of q beside
+ * it.  Row t of a sequence is rotated at position first + t, with a tree at
+ * first + depths[t].  Every head of q and k is first normed where a weight is
+ * given, x / sqrt(mean x^2 + eps) * w (the attention mixer's q_norm and
+ * k_norm), then of its first rot elements the pairs (a, b) at position p
+ * become (a cos - b sin, a sin + b cos), angle p * freqs[i] for pair i: (i, i
+ * + rot / 2), the mixer's order, or (2i, 2i + 1) where interleaved.  Angles
+ * are exact to fp32 up to position 2^29, whatever their size; norms and
+ * rotation are fp32, and each result is rounded once.  v is copied.  Rows of
+ * q go to out, k and v to the pages.
+ *
+ * Not written: rows of no sequence, rows that are no node, rows at a negative
+ * position, and all where the batch's status is not 0; k and v of a row with
+ * no page. */
+typedef struct {
+    const void *q;          /* [n, n_heads, head_dim], or NULL with n_heads 0 */
+    const void *k, *v;      /* [n, n_kv_heads, head_dim] */
+    void *out;              /* like q, in the pages' type; may be q itself (same type and strides), else not overlapping it */
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride; /* elements, multiples of 16 bytes */
+    int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+    int src_dtype;          /* of q, k and v: the pages', or QMOE_F32 for bf16 pages */
+    int n_heads;
+    const float *freqs;     /* [rot / 2] device: radians per position */
+    int rot;                /* even, 2 .. head_dim */
+    int interleaved;        /* 0 or 1 */
+    const float *q_norm, *k_norm; /* [head_dim] device, or NULL: not normed */
+    float eps;              /* >= 0, finite */
+} qmoe_paged_rotary;
+int qmoe_paged_append_rotary(const qmoe_paged_cache *c, int layer, const qmoe_paged_batch *b, const qmoe_paged_rotary *r,
+                             const qmoe_paged_tree *t, void *stream, qmoe_err *err);
+
+/* The path that the target takes through each tree.  tokens [n] are the rows'
+ * own tokens, chosen [n] what the target chose after them.  The path starts at
+ * row 0 and goes on to the lowest child whose token is the one chosen after
+ * its parent.  rows [n]: the path's rows at the first places of their
+ * sequence, -1 after them; counts [n_seqs]: their number (0 for a sequence
+ * without rows); next [n_seqs]: what was chosen after the last one, -1 for
+ * none.  parents and t as qmoe_paged_tree_build's. */
+int qmoe_paged_follow(const qmoe_paged_tree *t, const int32_t *parents, const int32_t *tokens, const int32_t *chosen,
+                      const int32_t *starts, int n, int n_seqs, int32_t *rows, int32_t *counts, int32_t *next,
+                      void *stream, qmoe_err *err);
+
+/* Keeps counts[i] of the batch's rows of every sequence, numbered as
+ * qmoe_paged_follow's: the k-th, rows[starts[i] + k], becomes row first + k in
+ * every layer, lens becomes first + counts[i], and pages after it are
+ * released (qmoe_paged_fork with rows cuts without moving).  A path's row k
+ * has depth k: it was rotated for the place that it goes to.
+ * *status (device): 0; the batch's own status where that is not 0; or -1 for
+ * starts out of order or range, a slot out of range or named twice, a length
+ * below the sequence's new rows or past the table, counts out of [0, new
+ * rows], rows that do not ascend within them, or a row that would move from
+ * no page, or to none, or to one that other slots hold too.  Unless 0, nothing
+ * is changed.  n_seqs <= 1024. */
+int qmoe_paged_keep(const qmoe_paged_cache *c, const qmoe_paged_batch *b, const int32_t *rows, const int32_t *counts,
+                    int32_t *status, void *ws, size_t ws_bytes, void *stream, qmoe_err *err);
 
 #ifdef __cplusplus
 }

@@ -281,18 +281,82 @@ __device__ __forceinline__ bool pa_full(const PaArgs &p, int p0, int p1, int bas
     return base + 31 <= p0 && (p.a.window == 0 || base >= pg_lo(p1, p.a.window) || base + 31 < p.a.sinks);
 }
 
+/* Trees of drafted tokens (TREE): row t of a sequence lies at cached row
+ * first + t as ever, but its position is first + its depth, and of the
+ * sequence's own rows it sees those in its bits (its ancestors and itself),
+ * whose depths stand for their positions.  A row that is no node (depth -1)
+ * sees nothing.  Depths are at most the row's own number, so the tiles of
+ * positions first .. first + t hold all that rows up to t see. */
+struct PaSee {
+    int pos, t;
+    bool node;
+};
+template <bool TREE>
+__device__ __forceinline__ PaSee pa_see(const PaArgs &p, const pg_seq &s, int t) {
+    PaSee r;
+    r.t = t;
+    int d = t;
+    if constexpr (TREE) d = min(max(qk_ld(p.a.depths + s.start + t), -1), t);
+    r.node = d >= 0;
+    r.pos = s.len - s.count + d;
+    return r;
+}
+/* the sequence's rows i0 .. i0 + 31 that row r sees */
+__device__ __forceinline__ uint32_t pa_kin(const PaArgs &p, const pg_seq &s, const PaSee &r, int i0) {
+    const uint32_t *bits = p.a.seen + (int64_t)(s.start + r.t) * p.a.words;
+    const int k = i0 >> 5;
+    const uint32_t lo = (uint32_t)k < (uint32_t)p.a.words ? qk_ld(bits + k) : 0u;
+    const uint32_t hi = (uint32_t)(k + 1) < (uint32_t)p.a.words ? qk_ld(bits + k + 1) : 0u;
+    uint32_t w = __builtin_amdgcn_alignbit(hi, lo, i0 & 31) & pa_upto(r.t, i0);
+    const int first = s.len - s.count, depth = r.pos - first;
+    if (p.a.window > 0 && depth >= p.a.window) /* a window shorter than the tree is deep */
+        for (uint32_t todo = w; todo; todo &= todo - 1) {
+            const int b = __builtin_ctz(todo), d = min(max(qk_ld(p.a.depths + s.start + i0 + b), 0), i0 + b);
+            if (depth - d >= p.a.window && first + d >= p.a.sinks) w &= ~(1u << b);
+        }
+    return w;
+}
+/* the keys base..base+31 that a row sees */
+template <bool TREE>
+__device__ __forceinline__ uint32_t pa_row_mask(const PaArgs &p, const pg_seq &s, const PaSee &r, int base) {
+    if constexpr (!TREE) return pa_mask(p, r.pos, base);
+    if (!r.node) return 0u;
+    const int first = s.len - s.count;
+    uint32_t w = pa_upto(first - 1, base);
+    if (p.a.window > 0) w &= ~pa_upto(pg_lo(r.pos, p.a.window) - 1, base) | pa_upto(p.a.sinks - 1, base);
+    return base + 31 < first ? w : w | pa_kin(p, s, r, base - first);
+}
+/* key j alone */
+template <bool TREE>
+__device__ __forceinline__ bool pa_row_sees(const PaArgs &p, const pg_seq &s, const PaSee &r, int j) {
+    if constexpr (!TREE) return pg_sees(r.pos, j, p.a.window, p.a.sinks);
+    const int first = s.len - s.count;
+    if (!r.node) return false;
+    if (j < first) return pg_sees(r.pos, j, p.a.window, p.a.sinks);
+    return j - first <= r.t && (pa_kin(p, s, r, j - first) & 1u);
+}
+/* the first position of rows from t on: of a tree any row's may be the root's */
+template <bool TREE>
+__device__ __forceinline__ int pa_from(const pg_seq &s, int t) { return s.len - s.count + (TREE ? 0 : t); }
+/* pa_full of rows at positions p0..p1; of a tree only what lies before it, where every row is a node */
+template <bool TREE>
+__device__ __forceinline__ bool pa_all(const PaArgs &p, const pg_seq &s, bool nodes, int p0, int p1, int base) {
+    return TREE ? nodes && pa_full(p, s.len - s.count - 1, p1, base) : pa_full(p, p0, p1, base);
+}
+
 /* ------------------------------------------------- one row at a time
  * fp32 on the vector ALU, keys of the unit's part only, for units whose
  * results are not finite or whose weights vanish (pa_again): a masked key is never multiplied
  * here.  Waves take the unit's rows in turn. */
-template <typename T, int HD, int RT, int KT>
+template <typename T, int HD, int RT, int KT, bool TREE>
 __device__ __forceinline__ void pa_slow(const PaArgs &p, const PaUnit &u, int kt0, int kt1, pg_tiles tl, int waves) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
     const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
     const int rows = u.s.count * p.G;
     for (int r = u.rtile * RT + wave; r < min(u.rtile * RT + RT, rows); r += waves) {
-        const int t = r / p.G, hh = pa_head(p, u.kh, r - t * p.G), pos = u.s.len - u.s.count + t;
+        const int t = r / p.G, hh = pa_head(p, u.kh, r - t * p.G);
+        const PaSee see = pa_see<TREE>(p, u.s, t);
         const T *q = (const T *)p.a.q + (int64_t)(u.s.start + t) * p.a.q_token + (int64_t)hh * p.a.q_head;
         float m = -INFINITY, l = 0.0f, acc[HD / 16];
         bool seen = false;
@@ -301,7 +365,7 @@ __device__ __forceinline__ void pa_slow(const PaArgs &p, const PaUnit &u, int kt
         for (int b = kt0 * KT; b < kt1 * KT; b += 64) { /* the part's tiles in runs of 64 keys */
             const int i = (b + lane) / KT;
             const int j = i < kt1 ? pg_tile(tl, i) * KT + (b + lane) % KT : 0x7FFFFFFF;
-            const int64_t at = pg_sees(pos, j, p.a.window, p.a.sinks) ? pg_row_at(&p.c, row, j) : -1;
+            const int64_t at = pa_row_sees<TREE>(p, u.s, see, j) ? pg_row_at(&p.c, row, j) : -1;
             float sc = -INFINITY;
             if (at >= 0) {
                 float d = 0.0f;
@@ -468,7 +532,7 @@ typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
 template <typename T, int HD, int NC>
 constexpr int pd_occ() { return NC * HD * (int)sizeof(T) <= 512 ? 2 : 1; }
 
-template <typename T, int HD, int NC>
+template <typename T, int HD, int NC, bool TREE>
 __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p) {
     constexpr int RT = 16 * NC;
     constexpr int E = HD / 16;  /* dims per lane of V = tiles of O */
@@ -485,7 +549,7 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
     const int row0 = u.rtile * RT, nrow = min(RT, u.s.count * p.G - row0);
     const int first = u.s.len - u.s.count;
-    const int p0 = first + row0 / p.G, p1 = first + (row0 + nrow - 1) / p.G;
+    const int p0 = pa_from<TREE>(u.s, row0 / p.G), p1 = first + (row0 + nrow - 1) / p.G;
     const pg_tiles tl = pg_tiles_of(p0, p1, p.a.window, p.a.sinks, PD_KT);
     const int kt0 = pg_part(tl.nt, u.part, u.parts), kt1 = pg_part(tl.nt, u.part + 1, u.parts);
     const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
@@ -500,14 +564,16 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
     const float scale = fabsf(p.a.scale);
     const uint32_t flip = p.a.scale < 0.0f ? (B16 ? 0x80008000u : 0x80000000u) : 0u;
     uint4 q[NC][QN];
-    int pos[NC];
+    PaSee see[NC];
+    bool nodes = true;
     float m[NC], l[NC];
     bool seen[NC];
     pa_f32x4 o[NC][E];
 #pragma unroll
     for (int x = 0; x < NC; x++) {
         const int r = row0 + min(16 * x + c, nrow - 1), t = r / p.G;
-        pos[x] = first + t;
+        see[x] = pa_see<TREE>(p, u.s, t);
+        nodes = nodes && see[x].node;
         const T *src = (const T *)p.a.q + (int64_t)(u.s.start + t) * p.a.q_token + (int64_t)pa_head(p, u.kh, r - t * p.G) * p.a.q_head + g * PE;
 #pragma unroll
         for (int s = 0; s < QN; s++) {
@@ -521,6 +587,7 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
         for (int e = 0; e < E; e++) o[x][e] = pa_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
+    if constexpr (TREE) nodes = __all(nodes);
     for (int i = kt0 + wave; i < kt1; i += 4) {
         const int base = pg_tile(tl, i) * PD_KT;
         const uint32_t valid = (uint32_t)__ballot(next >= 0);
@@ -574,10 +641,10 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
                 }
                 st[x][n] = a;
             }
-        if (valid != 0xFFFFFFFFu || !pa_full(p, p0, p1, base)) {
+        if (valid != 0xFFFFFFFFu || !pa_all<TREE>(p, u.s, nodes, p0, p1, base)) {
 #pragma unroll
             for (int x = 0; x < NC; x++) {
-                uint32_t mw = pa_mask(p, pos[x], base) & valid;
+                uint32_t mw = pa_row_mask<TREE>(p, u.s, see[x], base) & valid;
                 seen[x] |= mw != 0;
                 mw >>= 4 * g;
 #pragma unroll
@@ -662,7 +729,7 @@ __global__ __launch_bounds__(256, (pd_occ<T, HD, NC>())) void k_pa_few(PaArgs p)
         if (g == 0) ml[wave][16 * x + c] = make_float2(m[x], l[x]);
     }
     if (__syncthreads_or(again)) {
-        pa_slow<T, HD, RT, PD_KT>(p, u, kt0, kt1, tl, 4);
+        pa_slow<T, HD, RT, PD_KT, TREE>(p, u, kt0, kt1, tl, 4);
         return;
     }
     float M[NC], L[NC], f[NC];
@@ -801,7 +868,7 @@ __device__ __forceinline__ bool pa_merge(qm_f32x16 (&o)[E], float &m, float &l, 
     return group == 0;
 }
 
-template <int HD, int NG>
+template <int HD, int NG, bool TREE>
 __global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
     typedef uint16_t T;
     constexpr int KT = pm_kt(HD), CR = HD / 8, NB = KT * CR / 256, NS = KT / 32, E = HD / 32, KS = HD / 16;
@@ -814,13 +881,15 @@ __global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
     const int group = __builtin_amdgcn_readfirstlane(tid / 256);
     const int row0 = u.rtile * PM_RT, rows = u.s.count * p.G, nrow = min(PM_RT, rows - row0);
     const int first = u.s.len - u.s.count;
-    const int p0 = first + row0 / p.G, p1 = first + (row0 + nrow - 1) / p.G;
+    const int p0 = pa_from<TREE>(u.s, row0 / p.G), p1 = first + (row0 + nrow - 1) / p.G;
     const pg_tiles tl = pg_tiles_of(p0, p1, p.a.window, p.a.sinks, KT);
     const int kt0 = pg_part(tl.nt, u.part, u.parts), kt1 = pg_part(tl.nt, u.part + 1, u.parts), nt = kt1 - kt0;
     /* this wave's rows; a wave past the last row copies and waits only */
     const int w0 = row0 + 32 * wave, wn = min(32, rows - w0);
-    const int pw0 = first + w0 / p.G, pw1 = first + (w0 + wn - 1) / p.G;
-    const int r = min(w0 + c, rows - 1), t = r / p.G, pos = first + t;
+    const int pw0 = pa_from<TREE>(u.s, w0 / p.G), pw1 = first + (w0 + wn - 1) / p.G;
+    const int r = min(w0 + c, rows - 1), t = r / p.G;
+    const PaSee see = pa_see<TREE>(p, u.s, t);
+    const bool nodes = !TREE || __all(see.node);
     const int hh = pa_head(p, u.kh, r - t * p.G);
     const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
     const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
@@ -920,11 +989,11 @@ __global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
 #pragma unroll
         for (int n = 0; n < NS; n++) {
             const uint32_t v32 = (uint32_t)(valid >> (32 * n));
-            if (v32 == 0xFFFFFFFFu && pa_full(p, pw0, pw1, base + 32 * n)) {
+            if (v32 == 0xFFFFFFFFu && pa_all<TREE>(p, u.s, nodes, pw0, pw1, base + 32 * n)) {
                 seen = true;
                 continue;
             }
-            uint32_t mw = pa_mask(p, pos, base + 32 * n) & v32;
+            uint32_t mw = pa_row_mask<TREE>(p, u.s, see, base + 32 * n) & v32;
             seen |= mw != 0;
             mw >>= 4 * h;
 #pragma unroll
@@ -950,7 +1019,7 @@ __global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
     qm_sync<0>(); /* the last step's copies, of a step that there is not, are done */
     l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
     if (__syncthreads_or(wn > 0 && pa_again<E, 16>(o, l, seen))) {
-        pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 4 * NG);
+        pa_slow<T, HD, PM_RT, KT, TREE>(p, u, kt0, kt1, tl, 4 * NG);
         return;
     }
     if constexpr (NG > 1)
@@ -1010,7 +1079,7 @@ __device__ __forceinline__ qm_f32x16 pa_mfma6(const uint4 a[3], const uint4 b[3]
 /* head dims past 128: four waves, whose registers and LDS are full */
 constexpr int pm_halves32(int hd) { return hd <= 128 ? 2 : 1; }
 
-template <int HD>
+template <int HD, bool TREE>
 __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p) {
     typedef float T;
     constexpr int KT = 32, CR = HD / 8, NB = KT * HD / 1024, E = HD / 32, KS = HD / 16, NG = pm_halves32(HD);
@@ -1023,13 +1092,15 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
     const int odd = NG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int row0 = u.rtile * PM_RT, rows = u.s.count * p.G, nrow = min(PM_RT, rows - row0);
     const int first = u.s.len - u.s.count;
-    const int p0 = first + row0 / p.G, p1 = first + (row0 + nrow - 1) / p.G;
+    const int p0 = pa_from<TREE>(u.s, row0 / p.G), p1 = first + (row0 + nrow - 1) / p.G;
     const pg_tiles tl = pg_tiles_of(p0, p1, p.a.window, p.a.sinks, KT);
     const int kt0 = pg_part(tl.nt, u.part, u.parts), kt1 = pg_part(tl.nt, u.part + 1, u.parts), nt = kt1 - kt0;
     /* this wave's rows; a wave past the last row loads and waits only */
     const int w0 = row0 + 32 * wave, wn = min(32, rows - w0);
-    const int pw0 = first + w0 / p.G, pw1 = first + (w0 + wn - 1) / p.G;
-    const int r = min(w0 + c, rows - 1), t = r / p.G, pos = first + t;
+    const int pw0 = pa_from<TREE>(u.s, w0 / p.G), pw1 = first + (w0 + wn - 1) / p.G;
+    const int r = min(w0 + c, rows - 1), t = r / p.G;
+    const PaSee see = pa_see<TREE>(p, u.s, t);
+    const bool nodes = !TREE || __all(see.node);
     const int hh = pa_head(p, u.kh, r - t * p.G);
     const T *kp = (const T *)p.c.k + (int64_t)u.kh * p.c.head_stride, *vp = (const T *)p.c.v + (int64_t)u.kh * p.c.head_stride;
     const int32_t *row = p.c.table + (int64_t)u.s.slot * p.c.table_stride;
@@ -1126,10 +1197,10 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
             __builtin_amdgcn_sched_barrier(0);
         }
         if (act) {
-            if (valid == 0xFFFFFFFFu && pa_full(p, pw0, pw1, base)) {
+            if (valid == 0xFFFFFFFFu && pa_all<TREE>(p, u.s, nodes, pw0, pw1, base)) {
                 seen = true;
             } else {
-                uint32_t mw = pa_mask(p, pos, base) & valid;
+                uint32_t mw = pa_row_mask<TREE>(p, u.s, see, base) & valid;
                 seen |= mw != 0;
                 mw >>= 4 * h;
 #pragma unroll
@@ -1174,7 +1245,7 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
     }
     l += __uint_as_float(qk_xor32_u(__float_as_uint(l)));
     if (__syncthreads_or(wn > 0 && pa_again<E, 16>(o, l, seen))) {
-        pa_slow<T, HD, PM_RT, KT>(p, u, kt0, kt1, tl, 4 * NG);
+        pa_slow<T, HD, PM_RT, KT, TREE>(p, u, kt0, kt1, tl, 4 * NG);
         return;
     }
     if constexpr (NG == 2)
@@ -1377,28 +1448,28 @@ static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), void *ws, hipStream_t 
     return QK_CHECK_LAUNCH();
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool TREE>
 static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
     const int rt = pa_rows(&p.c, &p.a);
     if (rt == PM_RT) {
         if constexpr (sizeof(T) == 2) {
             if constexpr (HD <= 128)
-                if (pa_groups(&p.c, p.a.n, p.a.h) == 1) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 1>, ws, st);
-            return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 2>, ws, st);
-        } else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD>, ws, st);
+                if (pa_groups(&p.c, p.a.n, p.a.h) == 1) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 1, TREE>, ws, st);
+            return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 2, TREE>, ws, st);
+        } else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD, TREE>, ws, st);
     }
     if constexpr (HD <= (sizeof(T) == 2 ? 192 : 128)) /* pa_two */
-        if (rt == 32) return pa_launch_rt<T, HD, 32, PD_KT>(p, k_pa_few<T, HD, 2>, ws, st);
-    return pa_launch_rt<T, HD, 16, PD_KT>(p, k_pa_few<T, HD, 1>, ws, st);
+        if (rt == 32) return pa_launch_rt<T, HD, 32, PD_KT>(p, k_pa_few<T, HD, 2, TREE>, ws, st);
+    return pa_launch_rt<T, HD, 16, PD_KT>(p, k_pa_few<T, HD, 1, TREE>, ws, st);
 }
 
-template <typename T>
+template <typename T, bool TREE>
 static int pa_launch_hd(const PaArgs &p, void *ws, hipStream_t st) {
     switch (p.c.hd) {
-    case 64: return pa_launch<T, 64>(p, ws, st);
-    case 128: return pa_launch<T, 128>(p, ws, st);
-    case 192: return pa_launch<T, 192>(p, ws, st);
-    case 256: return pa_launch<T, 256>(p, ws, st);
+    case 64: return pa_launch<T, 64, TREE>(p, ws, st);
+    case 128: return pa_launch<T, 128, TREE>(p, ws, st);
+    case 192: return pa_launch<T, 192, TREE>(p, ws, st);
+    case 256: return pa_launch<T, 256, TREE>(p, ws, st);
     default: return (int)hipErrorInvalidValue;
     }
 }
@@ -1411,6 +1482,7 @@ extern "C" int qk_launch_pg_attn(const pg_cache *c, const pg_attn *a, void *ws, 
     p.po = NULL;
     p.pml = NULL;
     p.index = NULL;
-    return c->dtype == QMOE_BF16 ? pa_launch_hd<uint16_t>(p, ws, (hipStream_t)stream)
-                                 : pa_launch_hd<float>(p, ws, (hipStream_t)stream);
+    hipStream_t st = (hipStream_t)stream;
+    if (a->depths) return c->dtype == QMOE_BF16 ? pa_launch_hd<uint16_t, true>(p, ws, st) : pa_launch_hd<float, true>(p, ws, st);
+    return c->dtype == QMOE_BF16 ? pa_launch_hd<uint16_t, false>(p, ws, st) : pa_launch_hd<float, false>(p, ws, st);
 }

@@ -1,0 +1,444 @@
+/*
+ * paged_tree.hip -- decoding with drafted tokens on a paged cache: appending
+ * rows with the position rotation applied on the way, what the rows of a tree
+ * of drafted tokens see (their attention is paged_attn.hip's), the path that
+ * the target's choices take through it, and keeping that path's rows.
+ *
+ * As in paged_pages.hip, lengths and tables stay on the device, and every
+ * result is the same from call to call.
+ */
+#include "qk_device.h"
+#include "gemv_parts.h"
+#include "paged_parts.h"
+
+/* ------------------------------------------------------------ rotation
+ * A workgroup per new row: cos and sin of its rot / 2 angles once, then its
+ * heads of q, k and v, 8 elements a lane.  A head of q or k is normed first
+ * where a weight is given: y = x / sqrt(mean x^2 + eps) * w, the sum in fp32
+ * over the head's lanes.  Pairs (a, b) become (a cos - b sin, a sin + b cos);
+ * in halves (i, i + rot / 2) a lane's partners lie with others and come
+ * through LDS. */
+struct PgRotary {
+    pg_cache c;
+    const void *q, *k, *v;
+    void *out;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head; /* elements */
+    const float *freqs, *q_norm, *k_norm;
+    const int32_t *starts, *slots, *status, *depths;
+    float eps;
+    int n, n_seqs, h, half, inter; /* half = rot / 2 */
+};
+
+/* cos and sin of position * freq, whose fp32 value is off by a radian at far
+ * positions: x = position * freq in 64 bits (exact up to position 2^29: 29 and
+ * 24 bits), x / 2 pi in two parts, so that no bit of it is lost with the whole
+ * turns, and the nearest quarter turn taken off.  What is left, at most 1/8, is
+ * rounded to fp32, and sin and cos of 2 pi r are their Taylor series (the first
+ * term left out is below 2e-9, the sums are off by about one step of fp32). */
+__device__ __forceinline__ float2 pg_turn(int pos, float freq) {
+    const double x = (double)pos * (double)freq;
+    const double t = x * 0x1.45f306dc9c883p-3, e = fma(x, 0x1.45f306dc9c883p-3, -t) + x * -0x1.6b01ec5417056p-57;
+    const double whole = rint(t), f = (t - whole) + e, quarter = rint(4.0 * f);
+    const float r = (float)(f - 0.25 * quarter), r2 = r * r;
+    float s = fmaf(r2, 4.205869394e+01f, -7.670585975e+01f);
+    s = fmaf(r2, s, 8.160524928e+01f);
+    s = fmaf(r2, s, -4.134170224e+01f);
+    s = fmaf(r2, s, 6.283185307e+00f) * r;
+    float c = fmaf(r2, -2.642625678e+01f, 6.024464137e+01f);
+    c = fmaf(r2, c, -8.545681721e+01f);
+    c = fmaf(r2, c, 6.493939402e+01f);
+    c = fmaf(r2, c, -1.973920880e+01f);
+    c = fmaf(r2, c, 1.0f);
+    const int n = (int)quarter & 3;
+    const float a = n & 1 ? s : c, b = n & 1 ? c : s;
+    /* (c, s) turned by n quarters: (c, s), (-s, c), (-c, -s), (s, -c) */
+    return make_float2(n == 1 || n == 2 ? -a : a, n & 2 ? -b : b);
+}
+
+template <typename T>
+__device__ __forceinline__ void pg_get8(const T *p, float x[8]) {
+    if constexpr (sizeof(T) == 2) {
+        const uint4 w = qk_ld((const uint4 *)p);
+        x[0] = qk_bf16_lo(w.x); x[1] = qk_bf16_hi(w.x); x[2] = qk_bf16_lo(w.y); x[3] = qk_bf16_hi(w.y);
+        x[4] = qk_bf16_lo(w.z); x[5] = qk_bf16_hi(w.z); x[6] = qk_bf16_lo(w.w); x[7] = qk_bf16_hi(w.w);
+    } else {
+        const float4 a = qk_ld((const float4 *)p), b = qk_ld((const float4 *)p + 1);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    }
+}
+/* f32 -> bf16 rounds to nearest even: the page type's own rounding */
+template <typename T>
+__device__ __forceinline__ void pg_put8(T *p, const float x[8]) {
+    if constexpr (sizeof(T) == 2) {
+        const uint4 w = make_uint4(qk_cvt_pk_bf16(x[0], x[1]), qk_cvt_pk_bf16(x[2], x[3]), qk_cvt_pk_bf16(x[4], x[5]),
+                                   qk_cvt_pk_bf16(x[6], x[7]));
+        qk_st((float4 *)p, __builtin_bit_cast(float4, w));
+    } else {
+        qk_st((float4 *)p, make_float4(x[0], x[1], x[2], x[3]));
+        qk_st((float4 *)p + 1, make_float4(x[4], x[5], x[6], x[7]));
+    }
+}
+
+template <typename S, typename D, int HD>
+__global__ __launch_bounds__(256) void k_pg_rotary(PgRotary a) {
+    constexpr int LP = HD <= 64 ? 8 : HD <= 128 ? 16 : 32; /* lanes of a head; of 192, 24 of them hold elements */
+    constexpr int RP = 256 / LP;
+    __shared__ float2 turn[HD / 2];
+    __shared__ __attribute__((aligned(16))) float buf[RP][HD + 4];
+    const int tid = threadIdx.x, slot = tid / LP, e0 = 8 * (tid % LP), rot = 2 * a.half;
+    const int refused = a.status ? qk_ld(a.status) : 0;
+    for (int t = blockIdx.x; t < a.n; t += gridDim.x) {
+        const int s = pg_find(a.starts, a.n_seqs, t);
+        if (s >= a.n_seqs || refused) continue; /* all of the workgroup alike, as every test up to the heads */
+        const pg_seq q = pg_seq_at(&a.c, a.starts, a.slots, a.n, s);
+        const int first = q.len - q.count, row = t - q.start;
+        int pos = first + row;
+        if (q.slot < 0 || row < 0 || row >= q.count || pos < 0) continue;
+        const int64_t at = pg_row_at(&a.c, a.c.table + q.slot * a.c.table_stride, pos);
+        if (a.depths) {
+            const int d = min(qk_ld(a.depths + t), row);
+            if (d < 0 || first + d < 0) continue;
+            pos = first + d;
+        }
+        __syncthreads(); /* the last row's angles are read */
+        if (tid < a.half) turn[tid] = pg_turn(pos, qk_ld(a.freqs + tid));
+        __syncthreads();
+        for (int r = slot; r < a.h + 2 * a.c.kvh; r += RP) {
+            const int which = r < a.h ? 0 : r < a.h + a.c.kvh ? 1 : 2, hd = r - (which == 0 ? 0 : which == 1 ? a.h : a.h + a.c.kvh);
+            if (which && at < 0) continue; /* no page */
+            const bool on = HD != 192 || e0 < HD;
+            const int e1 = on ? e0 : 0;
+            const S *src = which == 0 ? (const S *)a.q + t * a.q_token + hd * a.q_head
+                                      : which == 1 ? (const S *)a.k + t * a.k_token + hd * a.k_head
+                                                   : (const S *)a.v + t * a.v_token + hd * a.v_head;
+            D *dst = which == 0 ? (D *)a.out + t * a.o_token + hd * a.o_head
+                                : (D *)(which == 1 ? a.c.k : a.c.v) + at + hd * a.c.head_stride;
+            float x[8], y[8];
+            pg_get8(src + e1, x);
+            const float *w = which == 0 ? a.q_norm : a.k_norm;
+            if (which < 2 && w) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+                ss = qk_group_sum<LP>(on ? ss : 0.0f);
+                const float f = 1.0f / sqrtf(ss / (float)HD + a.eps);
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = (x[i] * f) * qk_ld(w + e1 + i);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = x[i];
+            if (which < 2) {
+                if (a.inter) {
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2)
+                        if (e0 + i < rot) {
+                            const float2 c = turn[(e0 + i) / 2];
+                            y[i] = x[i] * c.x - x[i + 1] * c.y;
+                            y[i + 1] = x[i] * c.y + x[i + 1] * c.x;
+                        }
+                } else {
+                    float *b = buf[slot];
+                    qk_wave_lds_sync();
+                    if (on) {
+                        *(float4 *)(b + e0) = make_float4(x[0], x[1], x[2], x[3]);
+                        *(float4 *)(b + e0 + 4) = make_float4(x[4], x[5], x[6], x[7]);
+                    }
+                    qk_wave_lds_sync();
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int e = e0 + i;
+                        if (e < a.half) y[i] = x[i] * turn[e].x - b[e + a.half] * turn[e].y;
+                        else if (e < rot) y[i] = b[e - a.half] * turn[e - a.half].y + x[i] * turn[e - a.half].x;
+                    }
+                }
+            }
+            if (on) pg_put8(dst + e0, y);
+        }
+    }
+}
+
+template <typename S, typename D>
+static int pg_rotary_hd(const PgRotary &a, hipStream_t st) {
+    const dim3 grid(a.n < (1 << 20) ? a.n : 1 << 20), wg(256);
+    switch (a.c.hd) {
+    case 64: hipLaunchKernelGGL((k_pg_rotary<S, D, 64>), grid, wg, 0, st, a); break;
+    case 128: hipLaunchKernelGGL((k_pg_rotary<S, D, 128>), grid, wg, 0, st, a); break;
+    case 192: hipLaunchKernelGGL((k_pg_rotary<S, D, 192>), grid, wg, 0, st, a); break;
+    case 256: hipLaunchKernelGGL((k_pg_rotary<S, D, 256>), grid, wg, 0, st, a); break;
+    default: return (int)hipErrorInvalidValue;
+    }
+    return QK_CHECK_LAUNCH();
+}
+
+extern "C" int qk_launch_pg_rotary(const pg_cache *c, const qmoe_paged_rotary *r, const int32_t *starts, const int32_t *slots,
+                                   const int32_t *status, const int32_t *depths, int n, int n_seqs, void *stream) {
+    hipStream_t st = (hipStream_t)stream;
+    PgRotary a;
+    a.c = *c;
+    a.q = r->q; a.k = r->k; a.v = r->v; a.out = r->out;
+    a.q_token = r->q_token_stride; a.q_head = r->q_head_stride;
+    a.k_token = r->k_token_stride; a.k_head = r->k_head_stride;
+    a.v_token = r->v_token_stride; a.v_head = r->v_head_stride;
+    a.o_token = r->out_token_stride; a.o_head = r->out_head_stride;
+    a.freqs = r->freqs; a.q_norm = r->q_norm; a.k_norm = r->k_norm;
+    a.starts = starts; a.slots = slots; a.status = status; a.depths = depths;
+    a.eps = r->eps;
+    a.n = n; a.n_seqs = n_seqs;
+    a.h = r->n_heads; a.half = r->rot / 2; a.inter = r->interleaved;
+    if (c->dtype == QMOE_F32) return pg_rotary_hd<float, float>(a, st);
+    return r->src_dtype == QMOE_F32 ? pg_rotary_hd<float, uint16_t>(a, st) : pg_rotary_hd<uint16_t, uint16_t>(a, st);
+}
+
+/* ------------------------------------------------------------ trees
+ * Depth and ancestors of every drafted row, a workgroup per sequence, a thread
+ * per (row, word of 32 of its bits).  A thread walks from its row to the root;
+ * a run of rows whose parents are the rows before them is one step, so a
+ * chain, however long, is one. */
+#define PG_TREE_ROWS 1024
+
+struct PgTree {
+    const int32_t *parents, *starts;
+    int n, words;
+    int32_t *depths;
+    uint32_t *seen;
+};
+
+/* rows [start, start + count) of sequence i of the call, brought into [0, n) */
+__device__ __forceinline__ int2 pg_rows_of(const int32_t *starts, int n, int i) {
+    const int a = min(max(qk_ld(starts + i), 0), n), b = min(qk_ld(starts + i + 1), n);
+    return make_int2(a, max(b - a, 0));
+}
+
+__global__ __launch_bounds__(256) void k_pg_tree(PgTree a) {
+    __shared__ int up[PG_TREE_ROWS];
+    __shared__ uint32_t head[PG_TREE_ROWS / 32]; /* bit t: row t is not the child of row t - 1 */
+    const int tid = threadIdx.x;
+    const int2 s = pg_rows_of(a.starts, a.n, blockIdx.x);
+    const int c = min(s.y, 32 * a.words);
+    if (tid < PG_TREE_ROWS / 32) head[tid] = 0;
+    __syncthreads();
+    for (int t = tid; t < c; t += 256) {
+        const int p = qk_ld(a.parents + s.x + t);
+        up[t] = p >= -1 && p < t ? p : -2;
+        if (t == 0 || p != t - 1) atomicOr(&head[t >> 5], 1u << (t & 31));
+    }
+    __syncthreads();
+    for (int x = tid; x < c * a.words; x += 256) {
+        const int t = x / a.words, w = x - t * a.words;
+        int rows = 0, at = t;
+        uint32_t bits = 0;
+        while (at >= 0) {
+            int k = at >> 5;
+            uint32_t m = head[k] & ((2u << (at & 31)) - 1u);
+            while (!m) m = head[--k]; /* row 0's bit is set */
+            const int b = 32 * k + 31 - __builtin_clz(m); /* the run's first row */
+            const int lo = max(b - 32 * w, 0), hi = min(at - 32 * w, 31);
+            if (lo <= hi) bits |= (0xFFFFFFFFu << lo) & (0xFFFFFFFFu >> (31 - hi));
+            rows += at - b + 1;
+            at = up[b];
+        }
+        a.seen[(int64_t)(s.x + t) * a.words + w] = at == -1 ? bits : 0u;
+        if (w == 0) a.depths[s.x + t] = at == -1 ? rows - 1 : -1;
+    }
+    for (int t = c + tid; t < s.y; t += 256) { /* past what the words hold: no nodes */
+        for (int w = 0; w < a.words; w++) a.seen[(int64_t)(s.x + t) * a.words + w] = 0u;
+        a.depths[s.x + t] = -1;
+    }
+}
+
+extern "C" int qk_launch_pg_tree(const int32_t *parents, const int32_t *starts, int n, int n_seqs, int32_t *depths,
+                                 uint32_t *seen, int words, void *stream) {
+    const PgTree a = {parents, starts, n, words, depths, seen};
+    hipLaunchKernelGGL(k_pg_tree, dim3(n_seqs), dim3(256), 0, (hipStream_t)stream, a);
+    return QK_CHECK_LAUNCH();
+}
+
+/* ------------------------------------------------------------ follow
+ * The path that the target's choices take, a workgroup per sequence.  A row
+ * is taken where its token is the one chosen after its parent and no lower
+ * child of that parent has it too; a row is on the path where it and all its
+ * ancestors are taken (row 0 always), so its place is its depth and no walk is
+ * needed. */
+struct PgFollow {
+    const int32_t *parents, *tokens, *chosen, *starts, *depths;
+    const uint32_t *seen;
+    int n, words;
+    int32_t *rows, *counts, *next;
+};
+
+__global__ __launch_bounds__(256) void k_pg_follow(PgFollow a) {
+    __shared__ int kid[PG_TREE_ROWS], path[PG_TREE_ROWS];
+    __shared__ uint32_t taken[PG_TREE_ROWS / 32];
+    __shared__ int deepest;
+    const int tid = threadIdx.x;
+    const int2 s = pg_rows_of(a.starts, a.n, blockIdx.x);
+    const int c = min(s.y, 32 * a.words);
+    for (int t = tid; t < c; t += 256) {
+        kid[t] = PG_TREE_ROWS;
+        path[t] = -1;
+    }
+    if (tid < PG_TREE_ROWS / 32) taken[tid] = 0;
+    if (tid == 0) deepest = -1;
+    __syncthreads();
+    for (int t = tid; t < c; t += 256) {
+        const int p = qk_ld(a.parents + s.x + t);
+        if (p >= 0 && p < t && qk_ld(a.tokens + s.x + t) == qk_ld(a.chosen + s.x + p)) atomicMin(&kid[p], t);
+    }
+    __syncthreads();
+    for (int t = tid; t < c; t += 256) {
+        const int p = qk_ld(a.parents + s.x + t);
+        if (t == 0 || (p >= 0 && p < t && kid[p] == t)) atomicOr(&taken[t >> 5], 1u << (t & 31));
+    }
+    __syncthreads();
+    for (int t = tid; t < c; t += 256) {
+        const int d = min(qk_ld(a.depths + s.x + t), t);
+        bool on = d >= 0 && (taken[t >> 5] >> (t & 31) & 1u);
+        for (int w = 0; on && w <= t >> 5; w++) on = !(qk_ld(a.seen + (int64_t)(s.x + t) * a.words + w) & ~taken[w]);
+        /* other roots than row 0 are never taken, so a path has one row of each depth */
+        if (on) {
+            path[d] = t;
+            atomicMax(&deepest, d);
+        }
+    }
+    __syncthreads();
+    for (int t = tid; t < s.y; t += 256) a.rows[s.x + t] = t < c ? path[t] : -1;
+    if (tid == 0) {
+        a.counts[blockIdx.x] = deepest + 1;
+        a.next[blockIdx.x] = deepest < 0 || path[deepest] < 0 ? -1 : qk_ld(a.chosen + s.x + path[deepest]);
+    }
+}
+
+extern "C" int qk_launch_pg_follow(const int32_t *parents, const int32_t *tokens, const int32_t *chosen, const int32_t *starts,
+                                   const int32_t *depths, const uint32_t *seen, int words, int n, int n_seqs, int32_t *rows,
+                                   int32_t *counts, int32_t *next, void *stream) {
+    const PgFollow a = {parents, tokens, chosen, starts, depths, seen, n, words, rows, counts, next};
+    hipLaunchKernelGGL(k_pg_follow, dim3(n_seqs), dim3(256), 0, (hipStream_t)stream, a);
+    return QK_CHECK_LAUNCH();
+}
+
+/* ------------------------------------------------------------ keep
+ * Two launches, so that a batch with a sequence that is refused is left as it
+ * was: the first finds where every kept row lies and goes to, a workgroup per
+ * sequence, the second moves them and cuts the tables.  Kept rows ascend, so
+ * row k goes to a place at or before its own and behind those of the rows
+ * before it: a thread that moves its 16 bytes of every row of a sequence, in
+ * order, 8 loads before their stores, never reads what it has written. */
+struct PgKeep {
+    pg_cache c;
+    const int32_t *starts, *slots, *status, *rows, *counts;
+    int n, n_seqs;
+    int32_t *result;
+    int4 *head;          /* [n_seqs]: refused (1, or the batch's status), slot (-1: none), rows kept, lens now */
+    longlong2 *moves;    /* [n]: element offsets from, to */
+    pg_div cols, heads;  /* 16-byte pieces of a row, of a head */
+};
+
+__global__ __launch_bounds__(256) void k_pg_keep_find(PgKeep a) {
+    const int i = blockIdx.x, tid = threadIdx.x;
+    const int from = qk_ld(a.starts + i), to = qk_ld(a.starts + i + 1), count = to - from;
+    const int slot = a.slots ? qk_ld(a.slots + i) : i, keep = qk_ld(a.counts + i);
+    bool bad = from < 0 || to < from || to > a.n || slot < 0 || slot >= a.c.n_slots || keep < 0 || keep > count;
+    if (a.slots)
+        for (int j = tid; j < a.n_seqs; j += 256) bad |= j != i && qk_ld(a.slots + j) == slot;
+    bad = __syncthreads_or(bad);
+    int len = 0;
+    if (!bad) {
+        len = qk_ld(a.c.lens + slot);
+        bad = len < count || len > a.c.cap;
+        const int first = len - count;
+        const int32_t *row = a.c.table + slot * a.c.table_stride;
+        for (int k = tid; !bad && k < keep; k += 256) {
+            const int r = qk_ld(a.rows + from + k), before = k ? qk_ld(a.rows + from + k - 1) : -1;
+            bad = r <= before || r >= count;
+            longlong2 m = {0, 0};
+            if (!bad && r != k) {
+                m.x = pg_row_at(&a.c, row, first + r);
+                m.y = pg_row_at(&a.c, row, first + k);
+                bad = m.x < 0 || m.y < 0 ||
+                      qk_ld(a.c.refs + qk_ld(row + pg_div_of(a.c.page_rows, (uint32_t)(first + k)))) > 1;
+            }
+            a.moves[from + k] = m;
+        }
+        bad = __syncthreads_or(bad);
+        len -= count;
+    }
+    const int refused = a.status ? qk_ld(a.status) : 0;
+    if (tid == 0) a.head[i] = make_int4(refused ? refused : bad ? -1 : 0, slot, keep, len + keep);
+}
+
+__global__ __launch_bounds__(256) void k_pg_keep_move(PgKeep a) {
+    const int i = blockIdx.y, tid = threadIdx.x;
+    int bad = 0;
+    for (int j = tid; j < a.n_seqs; j += 256) bad |= qk_ld((const int *)(a.head + j)) != 0;
+    if (__syncthreads_or(bad)) {
+        if (i == 0 && blockIdx.x == 0 && tid == 0) {
+            const int refused = a.status ? qk_ld(a.status) : 0;
+            *a.result = refused ? refused : -1;
+        }
+        return;
+    }
+    const int4 h = qk_ld(a.head + i);
+    const int es = a.c.dtype == QMOE_BF16 ? 2 : 4;
+    if (blockIdx.x == 0) { /* the slot's length, and the pages behind it */
+        const int R = (int)a.c.page_rows.d;
+        int32_t *row = a.c.table + h.y * a.c.table_stride;
+        const int count = qk_ld(a.starts + i + 1) - qk_ld(a.starts + i), was = h.w - h.z + count;
+        for (int e = (h.w + R - 1) / R + tid; e < (was + R - 1) / R; e += 256) {
+            const int p = qk_ld(row + e);
+            if (p >= 0 && p < a.c.n_pages) atomicSub(a.c.refs + p, 1);
+            row[e] = -1;
+        }
+        if (tid == 0) a.c.lens[h.y] = h.w;
+        if (i == 0 && tid == 0) *a.result = 0;
+    }
+    const longlong2 *mv = a.moves + qk_ld(a.starts + i);
+    const int64_t pieces = (int64_t)2 * a.c.n_layers * a.cols.d;
+    for (int64_t x = (int64_t)blockIdx.x * 256 + tid; x < pieces; x += (int64_t)gridDim.x * 256) {
+        const int lv = (int)(x / a.cols.d);
+        const uint32_t col = (uint32_t)(x - (int64_t)lv * a.cols.d), hd = pg_div_of(a.heads, col), ch = col - hd * a.heads.d;
+        char *base = (char *)(lv & 1 ? a.c.v : a.c.k) + ((lv >> 1) * a.c.layer_stride + hd * a.c.head_stride) * es + 16 * ch;
+        for (int k0 = 0; k0 < h.z; k0 += 8) {
+            float4 y[8];
+            longlong2 m[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                m[k] = __builtin_bit_cast(longlong2, qk_ld((const float4 *)(mv + min(k0 + k, h.z - 1))));
+                y[k] = qk_ld((const float4 *)(base + m[k].x * es));
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (k0 + k < h.z && m[k].x != m[k].y) qk_st((float4 *)(base + m[k].y * es), y[k]);
+        }
+    }
+}
+
+static size_t pg_up(size_t v) { return (v + 255) / 256 * 256; }
+extern "C" size_t qk_pg_keep_ws(int n, int n_seqs) { return pg_up((size_t)n_seqs * 16) + pg_up((size_t)n * 16); }
+
+/* an empty batch reports too */
+__global__ void k_pg_keep_none(const int32_t *status, int32_t *result) { *result = status ? qk_ld(status) : 0; }
+
+extern "C" int qk_launch_pg_keep(const pg_cache *c, const int32_t *starts, const int32_t *slots, const int32_t *status, int n,
+                                 int n_seqs, const int32_t *rows, const int32_t *counts, int32_t *result, void *ws, void *stream) {
+    hipStream_t st = (hipStream_t)stream;
+    PgKeep a;
+    const int per_head = c->hd * (c->dtype == QMOE_BF16 ? 2 : 4) / 16;
+    a.c = *c;
+    a.starts = starts; a.slots = slots; a.status = status; a.rows = rows; a.counts = counts;
+    a.n = n; a.n_seqs = n_seqs; a.result = result;
+    a.head = (int4 *)ws;
+    a.moves = (longlong2 *)((char *)ws + pg_up((size_t)n_seqs * 16));
+    a.cols = pg_div_make((uint32_t)(c->kvh * per_head));
+    a.heads = pg_div_make((uint32_t)per_head);
+    if (n_seqs == 0) {
+        hipLaunchKernelGGL(k_pg_keep_none, dim3(1), dim3(1), 0, st, status, result);
+        return QK_CHECK_LAUNCH();
+    }
+    hipLaunchKernelGGL(k_pg_keep_find, dim3(n_seqs), dim3(256), 0, st, a);
+    const int rc = QK_CHECK_LAUNCH();
+    if (rc) return rc;
+    const int64_t blocks = ((int64_t)2 * c->n_layers * a.cols.d + 255) / 256;
+    hipLaunchKernelGGL(k_pg_keep_move, dim3((unsigned)(blocks < 1024 ? blocks : 1024), n_seqs), dim3(256), 0, st, a);
+    return QK_CHECK_LAUNCH();
+}

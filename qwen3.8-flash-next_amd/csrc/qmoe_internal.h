@@ -477,6 +477,9 @@ typedef struct {
     const int32_t *starts, *slots, *status; /* status: NULL, or nothing is written unless it holds 0 */
     int n, n_seqs, h, window, sinks, grouped;
     float scale;           /* score * this, log2 units: softmax scale * log2(e) */
+    const int32_t *depths; /* [n], trees of drafted tokens (qmoe_paged_tree); NULL: the rows are in causal order */
+    const uint32_t *seen;  /* [n, words] */
+    int words;
 } pg_attn;
 
 /* workspace bytes (attention: 0 for a call that no launch holds) and launches; 0 or a hipError_t */
@@ -492,6 +495,17 @@ size_t qk_pg_fork_ws(const pg_cache *c, int n_seqs);
 int qk_launch_pg_fork(const pg_cache *c, const int32_t *src, const int32_t *dst, const int32_t *rows, int n_seqs,
                       int32_t *status, void *ws, void *stream);
 int qk_launch_pg_evict(const pg_cache *c, const int32_t *slots, int n_seqs, int window, int sinks, void *stream);
+/* paged_tree.hip; depths NULL: rows in causal order */
+int qk_launch_pg_rotary(const pg_cache *c, const qmoe_paged_rotary *r, const int32_t *starts, const int32_t *slots,
+                        const int32_t *status, const int32_t *depths, int n, int n_seqs, void *stream);
+int qk_launch_pg_tree(const int32_t *parents, const int32_t *starts, int n, int n_seqs, int32_t *depths, uint32_t *seen,
+                      int words, void *stream);
+int qk_launch_pg_follow(const int32_t *parents, const int32_t *tokens, const int32_t *chosen, const int32_t *starts,
+                        const int32_t *depths, const uint32_t *seen, int words, int n, int n_seqs, int32_t *rows,
+                        int32_t *counts, int32_t *next, void *stream);
+size_t qk_pg_keep_ws(int n, int n_seqs);
+int qk_launch_pg_keep(const pg_cache *c, const int32_t *starts, const int32_t *slots, const int32_t *status, int n, int n_seqs,
+                      const int32_t *rows, const int32_t *counts, int32_t *result, void *ws, void *stream);
 size_t qk_pg_compact_ws(const pg_cache *c);
 int qk_launch_pg_compact(const pg_cache *c, int32_t *used, void *ws, void *stream);
 

@@ -154,6 +154,7 @@ size_t qmoe_paged_ws_bytes(const qmoe_paged_cache *q, int call, int n, int n_seq
     case QMOE_PAGED_RESERVE: return n_seqs > PG_MAX_BATCH ? 0 : qk_pg_reserve_ws(&c, n_seqs);
     case QMOE_PAGED_FORK: return n_seqs > PG_MAX_BATCH ? 0 : qk_pg_fork_ws(&c, n_seqs);
     case QMOE_PAGED_COMPACT: return qk_pg_compact_ws(&c);
+    case QMOE_PAGED_KEEP: return n < 0 || n_seqs > PG_MAX_BATCH ? 0 : qk_pg_keep_ws(n, n_seqs);
     default: return 0;
     }
 }
@@ -179,8 +180,25 @@ int qmoe_paged_append(const qmoe_paged_cache *q, int layer, const qmoe_paged_bat
                   "paged append");
 }
 
-int qmoe_paged_attn(const qmoe_paged_cache *cache, int layer, const qmoe_paged_batch *b, const qmoe_paged_query *q,
-                    void *ws, size_t ws_bytes, void *stream, qmoe_err *err) {
+/* the tree of a call of n rows */
+static int pg_tree_of(const qmoe_paged_tree *t, int n, qmoe_err *err) {
+    if (!t) return pg_fail(err, "tree is NULL");
+    if (t->words < 1 || t->words > 32) return pg_fail(err, "words %d out of range [1, 32]", t->words);
+    if (n > 0 && (!t->depths || !t->seen)) return pg_fail(err, "%s is NULL", t->depths ? "seen" : "depths");
+    if (((uintptr_t)t->depths | (uintptr_t)t->seen) & 3) return pg_fail(err, "depths and seen must be 4-byte aligned");
+    return 0;
+}
+
+/* rows of a call without a cache */
+static int pg_call(const int32_t *starts, int n, int n_seqs, qmoe_err *err) {
+    if (n < 0 || n > PG_MAX_ROWS) return pg_fail(err, "n = %d out of range [0, %d]", n, PG_MAX_ROWS);
+    if (n_seqs < 0 || n_seqs > PG_MAX_SEQS) return pg_fail(err, "n_seqs = %d out of range [0, %d]", n_seqs, PG_MAX_SEQS);
+    if (n_seqs > 0 && !starts) return pg_fail(err, "starts is NULL");
+    return 0;
+}
+
+static int pg_attention(const qmoe_paged_cache *cache, int layer, const qmoe_paged_batch *b, const qmoe_paged_query *q,
+                        const qmoe_paged_tree *t, void *ws, size_t ws_bytes, void *stream, qmoe_err *err) {
     pg_cache c;
     if (pg_cache_of(cache, &c, err) || pg_layer(&c, layer, err) || pg_batch(&c, b, err)) return -1;
     if (!q) return pg_fail(err, "query is NULL");
@@ -220,7 +238,97 @@ int qmoe_paged_attn(const qmoe_paged_cache *cache, int layer, const qmoe_paged_b
     a.sinks = q->window > 0 ? q->sinks : 0;
     a.grouped = q->grouped;
     a.scale = scale;
+    a.depths = t ? t->depths : NULL;
+    a.seen = t ? t->seen : NULL;
+    a.words = t ? t->words : 0;
     return pg_hip(err, qk_launch_pg_attn(&c, &a, ws, stream), "paged attention");
+}
+
+int qmoe_paged_attn(const qmoe_paged_cache *c, int layer, const qmoe_paged_batch *b, const qmoe_paged_query *q, void *ws,
+                    size_t ws_bytes, void *stream, qmoe_err *err) {
+    return pg_attention(c, layer, b, q, NULL, ws, ws_bytes, stream, err);
+}
+
+int qmoe_paged_attn_tree(const qmoe_paged_cache *c, int layer, const qmoe_paged_batch *b, const qmoe_paged_query *q,
+                         const qmoe_paged_tree *t, void *ws, size_t ws_bytes, void *stream, qmoe_err *err) {
+    if (err) err->msg[0] = 0;
+    if (pg_tree_of(t, b ? b->n : 0, err)) return -1;
+    return pg_attention(c, layer, b, q, t, ws, ws_bytes, stream, err);
+}
+
+int qmoe_paged_tree_build(const int32_t *parents, const int32_t *starts, int n, int n_seqs, const qmoe_paged_tree *t,
+                          void *stream, qmoe_err *err) {
+    if (err) err->msg[0] = 0;
+    if (pg_tree_of(t, n, err) || pg_call(starts, n, n_seqs, err)) return -1;
+    if (n == 0 || n_seqs == 0) return 0;
+    if (!parents) return pg_fail(err, "parents is NULL");
+    return pg_hip(err, qk_launch_pg_tree(parents, starts, n, n_seqs, t->depths, t->seen, t->words, stream), "paged tree");
+}
+
+int qmoe_paged_append_rotary(const qmoe_paged_cache *q, int layer, const qmoe_paged_batch *b, const qmoe_paged_rotary *r,
+                             const qmoe_paged_tree *t, void *stream, qmoe_err *err) {
+    pg_cache c;
+    if (pg_cache_of(q, &c, err) || pg_layer(&c, layer, err) || pg_batch(&c, b, err)) return -1;
+    if (!r) return pg_fail(err, "rotary is NULL");
+    if (t && pg_tree_of(t, b->n, err)) return -1;
+    if (r->src_dtype != c.dtype && r->src_dtype != QMOE_F32)
+        return pg_fail(err, "rows of dtype %d for pages of dtype %d (the pages' type, or f32)", r->src_dtype, c.dtype);
+    if (r->n_heads < 0 || (int64_t)b->n * r->n_heads > PG_MAX_ROWS)
+        return pg_fail(err, "%d rows of %d heads out of range [0, %d]", b->n, r->n_heads, PG_MAX_ROWS);
+    if (r->rot < 2 || r->rot > c.hd || r->rot % 2) return pg_fail(err, "rot %d is not even in [2, head_dim = %d]", r->rot, c.hd);
+    if (r->interleaved != 0 && r->interleaved != 1) return pg_fail(err, "interleaved %d is not 0 or 1", r->interleaved);
+    if (!(r->eps >= 0.0f) || !isfinite(r->eps)) return pg_fail(err, "eps %g is not finite and >= 0", (double)r->eps);
+    const int es = r->src_dtype == QMOE_BF16 ? 2 : 4, os = c.dtype == QMOE_BF16 ? 2 : 4;
+    if (pg_stride(r->q_token_stride, b->n, es, "q_token_stride", err) || pg_stride(r->q_head_stride, r->n_heads, es, "q_head_stride", err) ||
+        pg_stride(r->k_token_stride, b->n, es, "k_token_stride", err) || pg_stride(r->k_head_stride, c.kvh, es, "k_head_stride", err) ||
+        pg_stride(r->v_token_stride, b->n, es, "v_token_stride", err) || pg_stride(r->v_head_stride, c.kvh, es, "v_head_stride", err) ||
+        pg_stride(r->out_token_stride, b->n, os, "out_token_stride", err) ||
+        pg_stride(r->out_head_stride, r->n_heads, os, "out_head_stride", err))
+        return -1;
+    const int64_t stride[2] = {r->out_token_stride, r->out_head_stride}, size[2] = {b->n, r->n_heads};
+    if (r->n_heads > 0 && pg_apart(stride, size, 2, c.hd)) return pg_fail(err, "the strides let elements of out overlap");
+    if (b->n == 0 || b->n_seqs == 0) return 0;
+    if (!r->k || !r->v || !r->freqs) return pg_fail(err, "%s is NULL", !r->k ? "k" : !r->v ? "v" : "freqs");
+    if (r->n_heads > 0 && (!r->q || !r->out)) return pg_fail(err, "%s is NULL", r->q ? "out" : "q");
+    if (pg_misaligned(r->k) || pg_misaligned(r->v) || (r->n_heads > 0 && (pg_misaligned(r->q) || pg_misaligned(r->out))))
+        return pg_fail(err, "q, k, v and out must be 16-byte aligned");
+    if (((uintptr_t)r->freqs | (uintptr_t)r->q_norm | (uintptr_t)r->k_norm) & 3)
+        return pg_fail(err, "freqs, q_norm and k_norm must be 4-byte aligned");
+    if (r->n_heads > 0 && r->q == r->out &&
+        (es != os || (b->n > 1 && r->q_token_stride != r->out_token_stride) ||
+         (r->n_heads > 1 && r->q_head_stride != r->out_head_stride)))
+        return pg_fail(err, "out is q, but not with the same type and strides");
+    return pg_hip(err,
+                  qk_launch_pg_rotary(&c, r, b->starts, b->slots, b->status, t ? t->depths : NULL, b->n, b->n_seqs, stream),
+                  "paged rotary append");
+}
+
+int qmoe_paged_follow(const qmoe_paged_tree *t, const int32_t *parents, const int32_t *tokens, const int32_t *chosen,
+                      const int32_t *starts, int n, int n_seqs, int32_t *rows, int32_t *counts, int32_t *next, void *stream,
+                      qmoe_err *err) {
+    if (err) err->msg[0] = 0;
+    if (pg_tree_of(t, n, err) || pg_call(starts, n, n_seqs, err)) return -1;
+    if (n_seqs == 0) return 0;
+    if (!counts || !next) return pg_fail(err, "%s is NULL", counts ? "next" : "counts");
+    if (n > 0 && (!parents || !tokens || !chosen || !rows))
+        return pg_fail(err, "%s is NULL", !parents ? "parents" : !tokens ? "tokens" : !chosen ? "chosen" : "rows");
+    return pg_hip(err,
+                  qk_launch_pg_follow(parents, tokens, chosen, starts, t->depths, t->seen, t->words, n, n_seqs, rows, counts,
+                                      next, stream),
+                  "paged follow");
+}
+
+int qmoe_paged_keep(const qmoe_paged_cache *q, const qmoe_paged_batch *b, const int32_t *rows, const int32_t *counts,
+                    int32_t *status, void *ws, size_t ws_bytes, void *stream, qmoe_err *err) {
+    pg_cache c;
+    if (pg_cache_of(q, &c, err) || pg_batch(&c, b, err) || pg_seqs(&c, b->slots, b->n_seqs, PG_MAX_BATCH, err)) return -1;
+    if (!status) return pg_fail(err, "status is NULL");
+    if ((uintptr_t)status & 3) return pg_fail(err, "status must be 4-byte aligned");
+    if (b->n_seqs > 0 && (!b->starts || !counts)) return pg_fail(err, "%s is NULL", b->starts ? "counts" : "starts");
+    if (b->n_seqs > 0 && b->n > 0 && !rows) return pg_fail(err, "rows is NULL");
+    if (pg_work(ws, ws_bytes, qk_pg_keep_ws(b->n, b->n_seqs), err)) return -1;
+    return pg_hip(err, qk_launch_pg_keep(&c, b->starts, b->slots, b->status, b->n, b->n_seqs, rows, counts, status, ws, stream),
+                  "paged keep");
 }
 
 int qmoe_paged_reserve(const qmoe_paged_cache *q, const int32_t *slots, const int32_t *n_new, int n_seqs,

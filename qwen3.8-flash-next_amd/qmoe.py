@@ -126,7 +126,19 @@ class QmoePagedQuery(ctypes.Structure):
                [(f, ctypes.c_int) for f in ("n_heads", "window", "sinks", "grouped")] + [("scale", ctypes.c_float)]
 
 
-PAGED_ATTN, PAGED_RESERVE, PAGED_FORK, PAGED_COMPACT = 0, 1, 2, 3
+class QmoePagedTree(ctypes.Structure):
+    _fields_ = [("depths", ctypes.c_void_p), ("seen", ctypes.c_void_p), ("words", ctypes.c_int)]
+
+
+class QmoePagedRotary(ctypes.Structure):
+    _fields_ = [(f, ctypes.c_void_p) for f in ("q", "k", "v", "out")] + \
+               [(f, ctypes.c_int64) for f in ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+                                              "v_token_stride", "v_head_stride", "out_token_stride", "out_head_stride")] + \
+               [("src_dtype", ctypes.c_int), ("n_heads", ctypes.c_int), ("freqs", ctypes.c_void_p), ("rot", ctypes.c_int),
+                ("interleaved", ctypes.c_int), ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float)]
+
+
+PAGED_ATTN, PAGED_RESERVE, PAGED_FORK, PAGED_COMPACT, PAGED_KEEP = 0, 1, 2, 3, 4
 _INT_END = 2 ** 31
 
 
@@ -190,6 +202,17 @@ SIGNATURES = {
                              ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_evict": (_I, [ctypes.POINTER(QmoePagedCache), _P, _I, _I, _I, _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_compact": (_I, [ctypes.POINTER(QmoePagedCache), _P, _P, ctypes.c_size_t, _P, ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_tree_build": (_I, [_P, _P, _I, _I, ctypes.POINTER(QmoePagedTree), _P, ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_attn_tree": (_I, [ctypes.POINTER(QmoePagedCache), _I, ctypes.POINTER(QmoePagedBatch),
+                                  ctypes.POINTER(QmoePagedQuery), ctypes.POINTER(QmoePagedTree), _P, ctypes.c_size_t, _P,
+                                  ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_append_rotary": (_I, [ctypes.POINTER(QmoePagedCache), _I, ctypes.POINTER(QmoePagedBatch),
+                                      ctypes.POINTER(QmoePagedRotary), ctypes.POINTER(QmoePagedTree), _P,
+                                      ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_follow": (_I, [ctypes.POINTER(QmoePagedTree), _P, _P, _P, _P, _I, _I, _P, _P, _P, _P,
+                               ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_keep": (_I, [ctypes.POINTER(QmoePagedCache), ctypes.POINTER(QmoePagedBatch), _P, _P, _P, _P, ctypes.c_size_t,
+                             _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_dn_create": (_I, [ctypes.POINTER(_P), ctypes.POINTER(QmoeDnConfig), ctypes.POINTER(QmoeErr)]),
     "qmoe_dn_destroy": (None, [_P]),
     "qmoe_dn_upload_layer": (_I, [_P, _I, ctypes.POINTER(QmoeDnWeights), ctypes.POINTER(QmoeErr)]),
@@ -1026,6 +1049,19 @@ class GatedResidualContext:
         return hyper
 
 
+class DraftTree:
+    """drafted rows of a batch as PagedCache.tree has found them: parents and
+    starts as given, depths [n] int32 (-1: no node) and seen [n, words] int32
+    (bit r of row t: r is t or an ancestor of t), on the device.  It depends on
+    nothing else, so one tree serves every layer, and every step whose drafts
+    have this form."""
+
+    def __init__(self, parents, starts, depths, seen):
+        self.parents, self.starts, self.depths, self.seen = parents, starts, depths, seen
+        self._c = QmoePagedTree(depths.data_ptr(), seen.data_ptr(), seen.shape[1])
+        self._p = ctypes.byref(self._c)
+
+
 class PagedCache:
     """k and v of many sequences in pages of a pool (qmoe_paged_*), on the
     caller's tensors:
@@ -1045,7 +1081,11 @@ class PagedCache:
     its status the two write nothing (without it append would overwrite
     them).  Calls return without waiting and may be captured in a HIP
     graph; a call's workspace comes from torch's allocator on the call's
-    stream."""
+    stream.
+
+    A step of drafted tokens: status = reserve(...) for all drafts, t =
+    tree(parents, starts), per layer append_rotary(..., tree=t) and
+    attend_tree(..., t), then follow(t, ...) and keep(...)."""
 
     def __init__(self, k, v, table, lens, refs):
         import torch
@@ -1114,6 +1154,16 @@ class PagedCache:
             self._fits(what, t.shape[0])
         return t.data_ptr()
 
+    def _floats(self, t, n, what):
+        """device address of a f32 vector of n (or None)"""
+        if t is None:
+            return None
+        if t.dtype != self._torch.float32 or t.device != self.device or t.dim() != 1 or (n is not None and t.shape[0] != n) or \
+                not t.is_contiguous():
+            raise QmoeError(f"{what} must be a contiguous float32 vector" + (f" of {n}" if n is not None else "") +
+                            f" on {self.device}")
+        return t.data_ptr()
+
     def _rows(self, t, heads, dtypes, what):
         if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.hd or t.dtype not in dtypes or t.stride(2) != 1 or \
                 t.device != self.device:
@@ -1179,6 +1229,58 @@ class PagedCache:
                    "qmoe_paged_append")
         self._on(stream, call)
 
+    def append_rotary(self, layer, k, v, starts, freqs, q=None, slots=None, tree=None, q_norm=None, k_norm=None, eps=1e-6,
+                      interleaved=False, out=None, stream=None, status=None):
+        """append() of k rotated at its rows' positions, and of q [n, n_heads,
+        head_dim] (the type of k and v) rotated beside it, which is returned in
+        the pages' type (out, if given: also q itself where the types agree).
+        freqs [rot / 2] f32 are radians per position: pair i of a head's first
+        rot elements, (i, i + rot / 2) as the attention mixer's or (2i, 2i + 1)
+        with `interleaved`, is turned by position * freqs[i], exact for far
+        positions.  q_norm, k_norm [head_dim] f32: x / sqrt(mean x^2 + eps) * w
+        per head before.  A row's position is its place in the sequence, with
+        `tree` (DraftTree of the same starts) the rows before the drafts plus
+        its depth.  Rows of q that are of no sequence or no node, and all
+        unless `status` is 0, are left as out has them."""
+        if not 0 <= layer < self.n_layers:
+            raise QmoeError(f"layer {layer} out of range [0, {self.n_layers})")
+        self._rows(k, self.kvh, self._src, "k")
+        self._rows(v, self.kvh, self._src, "v")
+        n, heads = k.shape[0], 0
+        if n != v.shape[0] or k.dtype != v.dtype:
+            raise QmoeError("k and v must have the same rows and type")
+        if q is not None:
+            heads = q.shape[1] if q.dim() == 3 else 0
+            self._rows(q, heads, (k.dtype,), "q")
+            if q.shape[0] != n:
+                raise QmoeError(f"q has {q.shape[0]} rows, k {n}")
+            if out is not None:
+                self._rows(out, heads, self._own, "out")
+                if out.shape[0] != n:
+                    raise QmoeError(f"out has {out.shape[0]} rows, q {n}")
+        elif out is not None or q_norm is not None:
+            raise QmoeError("out and q_norm are given without q")
+        if n >= _INT_END or heads >= _INT_END:
+            self._fits("k", n, heads)
+        f = self._floats(freqs, None, "freqs")
+        if f is None or not 1 <= freqs.shape[0] <= self.hd // 2:
+            raise QmoeError(f"freqs must hold 1 to {self.hd // 2} numbers")
+        qn, kn = self._floats(q_norm, self.hd, "q_norm"), self._floats(k_norm, self.hd, "k_norm")
+        b, t, err = self._batch(n, starts, slots, status), self._tree(tree, n), QmoeErr()
+
+        def call(st):
+            o = out
+            if q is not None and out is None:
+                o = self._torch.empty((n, heads, self.hd), dtype=self.dtype, device=self.device)
+            a = QmoePagedRotary(None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), None if o is None else o.data_ptr(),
+                                *((0, 0) if q is None else q.stride()[:2]), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                                *((0, 0) if o is None else o.stride()[:2]), _dtype_code(k), heads, f, 2 * freqs.shape[0],
+                                1 if interleaved else 0, qn, kn, eps)
+            _check(lib().qmoe_paged_append_rotary(self._cp, layer, ctypes.byref(b), ctypes.byref(a), t, st, ctypes.byref(err)),
+                   err, "qmoe_paged_append_rotary")
+            return o
+        return self._on(stream, call)
+
     def attend(self, layer, q, starts, slots=None, window=0, sinks=0, scale=None, grouped=False, out=None, stream=None,
                status=None):
         """q [n, n_heads, head_dim] of the pages' type -> softmax(scale q.k) v
@@ -1189,6 +1291,9 @@ class PagedCache:
         1 / sqrt(head_dim), others are taken in f32.  Rows of no sequence, and all rows unless `status`
         (of the reserve that made room for them) is 0, are left as out has
         them (undefined without out); out must not overlap q or the cache."""
+        return self._attend(layer, q, starts, None, slots, window, sinks, scale, grouped, out, stream, status)
+
+    def _attend(self, layer, q, starts, tree, slots, window, sinks, scale, grouped, out, stream, status):
         heads = q.shape[1] if q.dim() == 3 else 0
         if not 0 <= layer < self.n_layers:
             raise QmoeError(f"layer {layer} out of range [0, {self.n_layers})")
@@ -1201,6 +1306,7 @@ class PagedCache:
         if n >= _INT_END or heads >= _INT_END:
             self._fits("q", n, heads)
         b, err = self._batch(n, starts, slots, status), QmoeErr()
+        t = self._tree(tree, n)
         if out is not None:
             self._rows(out, heads, self._own, "out")
             if out.shape[0] != n:
@@ -1211,9 +1317,96 @@ class PagedCache:
             a = QmoePagedQuery(q.data_ptr(), o.data_ptr(), q.stride(0), q.stride(1), o.stride(0), o.stride(1), heads, window,
                                sinks, 1 if grouped else 0, 0.0 if scale is None else scale)
             ws = self._work(PAGED_ATTN, n, b.n_seqs, heads)
-            _check(lib().qmoe_paged_attn(self._cp, layer, ctypes.byref(b), ctypes.byref(a), ws.data_ptr(), ws.numel(), st,
-                                         ctypes.byref(err)), err, "qmoe_paged_attn")
+            if t is None:
+                _check(lib().qmoe_paged_attn(self._cp, layer, ctypes.byref(b), ctypes.byref(a), ws.data_ptr(), ws.numel(), st,
+                                             ctypes.byref(err)), err, "qmoe_paged_attn")
+            else:
+                _check(lib().qmoe_paged_attn_tree(self._cp, layer, ctypes.byref(b), ctypes.byref(a), t, ws.data_ptr(),
+                                                  ws.numel(), st, ctypes.byref(err)), err, "qmoe_paged_attn_tree")
             return o
+        return self._on(stream, call)
+
+    # -- drafted tokens
+    def tree(self, parents, starts, most=None, stream=None):
+        """the trees of a batch of drafted rows, made once per step (or kept
+        while the drafts have the same form): parents [n] int32 names every
+        row's parent among its sequence's rows, -1 for a root, which follows
+        the rows before the drafts.  A parent lies before its children; a row
+        for which it does not is no node, nor are its descendants, nor the
+        rows past the first `most` of a sequence (None: all) or past 1024.
+        Returns a DraftTree for append_rotary, attend_tree, follow and keep."""
+        p = self._ints(parents, None, "parents")
+        s = self._ints(starts, None, "starts")
+        if p is None or s is None or starts.shape[0] < 1:
+            raise QmoeError("parents must be given, and starts hold one number more than there are sequences")
+        n, m, err = parents.shape[0], starts.shape[0] - 1, QmoeErr()
+        if most is not None and not 0 <= most < 2 ** 31:
+            raise QmoeError(f"most {most} must be in [0, 2^31)")
+        words = max(1, min(32, -(-min(n, n if most is None else most) // 32)))
+
+        def call(st):
+            depths = self._torch.empty(n, dtype=self._i32, device=self.device)
+            seen = self._torch.empty((n, words), dtype=self._i32, device=self.device)
+            t = DraftTree(parents, starts, depths, seen)
+            _check(lib().qmoe_paged_tree_build(p, s, n, m, t._p, st, ctypes.byref(err)), err, "qmoe_paged_tree_build")
+            return t
+        return self._on(stream, call)
+
+    def _tree(self, tree, n):
+        if tree is None:
+            return None
+        if tree.depths.device != self.device or tree.depths.shape[0] != n:
+            raise QmoeError(f"the tree has {tree.depths.shape[0]} rows on {tree.depths.device}, the call {n} on {self.device}")
+        return tree._p
+
+    def attend_tree(self, layer, q, tree, slots=None, window=0, sinks=0, scale=None, grouped=False, out=None, stream=None,
+                    status=None):
+        """attend() of drafted rows: a row stands at the position of its depth
+        after the rows before the drafts, and sees those as attend() has it
+        there, and of the drafts its ancestors and itself.  Window and sinks
+        count in positions.  Rows that are no node give zeros."""
+        if tree is None:
+            raise QmoeError("tree must be given")
+        return self._attend(layer, q, tree.starts, tree, slots, window, sinks, scale, grouped, out, stream, status)
+
+    def follow(self, tree, tokens, chosen, stream=None):
+        """the path that the target takes: tokens [n] int32 of the drafted
+        rows, chosen [n] int32 what the target chose after each of them.  From
+        row 0 of a sequence on, the lowest child whose token is the chosen one.
+        Returns (rows [n]: the path's rows at the first places of their
+        sequence, -1 after them; counts [n_seqs]; next [n_seqs]: what was chosen
+        after the last one, -1 for none)."""
+        n = tree.depths.shape[0]
+        t, m, err = self._tree(tree, n), tree.starts.shape[0] - 1, QmoeErr()
+        if tokens is None or chosen is None or tree.parents is None:
+            raise QmoeError("tokens, chosen and the tree's parents must be given")
+        a, b = self._ints(tokens, n, "tokens"), self._ints(chosen, n, "chosen")
+
+        def call(st):
+            rows = self._torch.empty(n, dtype=self._i32, device=self.device)
+            counts, last = (self._torch.empty(m, dtype=self._i32, device=self.device) for _ in range(2))
+            _check(lib().qmoe_paged_follow(t, tree.parents.data_ptr(), a, b, tree.starts.data_ptr(), n, m, rows.data_ptr(),
+                                           counts.data_ptr(), last.data_ptr(), st, ctypes.byref(err)), err, "qmoe_paged_follow")
+            return rows, counts, last
+        return self._on(stream, call)
+
+    def keep(self, rows, counts, starts, slots=None, stream=None, status=None):
+        """keeps counts[i] of the batch's rows of every sequence, those that
+        rows names (as follow returns them, ascending), moved together in every
+        layer; the other rows are cut off and their pages released.  Returns an
+        int32 [1] on the device: 0, the batch's `status` where that is not 0, or
+        -1 (refused; nothing is changed unless 0)."""
+        if rows is None or counts is None:
+            raise QmoeError("rows and counts must be given")
+        r, n = self._ints(rows, None, "rows"), rows.shape[0]
+        b, err = self._batch(n, starts, slots, status), QmoeErr()
+        c = self._ints(counts, b.n_seqs, "counts")
+
+        def call(st):
+            result, ws = self._status(), self._work(PAGED_KEEP, n, b.n_seqs)
+            _check(lib().qmoe_paged_keep(self._cp, ctypes.byref(b), r, c, result.data_ptr(), ws.data_ptr(), ws.numel(), st,
+                                         ctypes.byref(err)), err, "qmoe_paged_keep")
+            return result
         return self._on(stream, call)
 
     # -- pages
