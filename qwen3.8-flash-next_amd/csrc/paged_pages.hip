@@ -51,6 +51,21 @@ struct PgAppend {
     pg_div per_row, per_head; /* 16-byte chunks */
 };
 
+/* the sequence that has row t of the call: the last i with starts[i] <= t
+ * among those that lie in order; rows of no sequence give n_seqs */
+__device__ __forceinline__ int pg_find(const int32_t *starts, int n_seqs, int t) {
+    int lo = 0, hi = n_seqs; /* starts[lo] <= t < starts[hi] */
+    if (t < qk_ld(starts) || t >= qk_ld(starts + n_seqs)) return n_seqs;
+    /* one new row per sequence, the decode step: row t is sequence t's */
+    if (t < n_seqs && qk_ld(starts + t) == t && qk_ld(starts + t + 1) == t + 1) return t;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (qk_ld(starts + mid) <= t) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
 template <typename S, typename D>
 __global__ __launch_bounds__(256) void k_pg_append(PgAppend a) {
     constexpr int E = 16 / sizeof(D); /* elements per chunk */

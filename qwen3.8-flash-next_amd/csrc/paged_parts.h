@@ -66,21 +66,6 @@ PG_FN pg_seq pg_seq_at(const pg_cache *c, const int32_t *starts, const int32_t *
     return s;
 }
 
-/* the sequence that has row t of the call: the last i with starts[i] <= t
- * among those that lie in order; rows of no sequence give n_seqs */
-PG_FN int pg_find(const int32_t *starts, int n_seqs, int t) {
-    int lo = 0, hi = n_seqs; /* starts[lo] <= t < starts[hi] */
-    if (t < PG_GET(starts) || t >= PG_GET(starts + n_seqs)) return n_seqs;
-    /* one new row per sequence, the decode step: row t is sequence t's */
-    if (t < n_seqs && PG_GET(starts + t) == t && PG_GET(starts + t + 1) == t + 1) return t;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (PG_GET(starts + mid) <= t) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-
 /* keys that the query at position p sees: [lo, p] and [0, sinks) below lo */
 QK_HD static inline int pg_lo(int p, int window) { return window > 0 && p >= window ? p - window + 1 : 0; }
 QK_HD static inline int pg_sees(int p, int j, int window, int sinks) {

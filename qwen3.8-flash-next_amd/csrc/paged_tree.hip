@@ -27,7 +27,9 @@ struct PgRotary {
     const int32_t *starts, *slots, *status, *depths;
     float eps;
     int n, n_seqs, h, half, inter; /* half = rot / 2 */
+    pg_div per_row;      /* heads of q, k and v of a token */
 };
+#define PG_ROTARY_MANY 2048
 
 /* cos and sin of position * freq, whose fp32 value is off by a radian at far
  * positions: x = position * freq in 64 bits (exact up to position 2^29: 29 and
@@ -80,95 +82,166 @@ __device__ __forceinline__ void pg_put8(T *p, const float x[8]) {
     }
 }
 
-template <typename S, typename D, int HD>
-__global__ __launch_bounds__(256) void k_pg_rotary(PgRotary a) {
-    constexpr int LP = HD <= 64 ? 8 : HD <= 128 ? 16 : 32; /* lanes of a head; of 192, 24 of them hold elements */
-    constexpr int RP = 256 / LP;
-    __shared__ float2 turn[HD / 2];
-    __shared__ __attribute__((aligned(16))) float buf[RP][HD + 4];
-    const int tid = threadIdx.x, slot = tid / LP, e0 = 8 * (tid % LP), rot = 2 * a.half;
-    const int refused = a.status ? qk_ld(a.status) : 0;
-    for (int t = blockIdx.x; t < a.n; t += gridDim.x) {
-        const int s = pg_find(a.starts, a.n_seqs, t);
-        if (s >= a.n_seqs || refused) continue; /* all of the workgroup alike, as every test up to the heads */
-        const pg_seq q = pg_seq_at(&a.c, a.starts, a.slots, a.n, s);
-        const int first = q.len - q.count, row = t - q.start;
-        int pos = first + row;
-        if (q.slot < 0 || row < 0 || row >= q.count || pos < 0) continue;
-        const int64_t at = pg_row_at(&a.c, a.c.table + q.slot * a.c.table_stride, pos);
-        if (a.depths) {
-            const int d = min(qk_ld(a.depths + t), row);
-            if (d < 0 || first + d < 0) continue;
-            pos = first + d;
-        }
-        __syncthreads(); /* the last row's angles are read */
-        if (tid < a.half) turn[tid] = pg_turn(pos, qk_ld(a.freqs + tid));
-        __syncthreads();
-        for (int r = slot; r < a.h + 2 * a.c.kvh; r += RP) {
-            const int which = r < a.h ? 0 : r < a.h + a.c.kvh ? 1 : 2, hd = r - (which == 0 ? 0 : which == 1 ? a.h : a.h + a.c.kvh);
-            if (which && at < 0) continue; /* no page */
-            const bool on = HD != 192 || e0 < HD;
-            const int e1 = on ? e0 : 0;
-            const S *src = which == 0 ? (const S *)a.q + t * a.q_token + hd * a.q_head
-                                      : which == 1 ? (const S *)a.k + t * a.k_token + hd * a.k_head
-                                                   : (const S *)a.v + t * a.v_token + hd * a.v_head;
-            D *dst = which == 0 ? (D *)a.out + t * a.o_token + hd * a.o_head
-                                : (D *)(which == 1 ? a.c.k : a.c.v) + at + hd * a.c.head_stride;
-            float x[8], y[8];
-            pg_get8(src + e1, x);
-            const float *w = which == 0 ? a.q_norm : a.k_norm;
-            if (which < 2 && w) {
-                float ss = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
-                ss = qk_group_sum<LP>(on ? ss : 0.0f);
-                const float f = 1.0f / sqrtf(ss / (float)HD + a.eps);
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = (x[i] * f) * qk_ld(w + e1 + i);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) y[i] = x[i];
-            if (which < 2) {
-                if (a.inter) {
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2)
-                        if (e0 + i < rot) {
-                            const float2 c = turn[(e0 + i) / 2];
-                            y[i] = x[i] * c.x - x[i + 1] * c.y;
-                            y[i + 1] = x[i] * c.y + x[i + 1] * c.x;
-                        }
-                } else {
-                    float *b = buf[slot];
-                    qk_wave_lds_sync();
-                    if (on) {
-                        *(float4 *)(b + e0) = make_float4(x[0], x[1], x[2], x[3]);
-                        *(float4 *)(b + e0 + 4) = make_float4(x[4], x[5], x[6], x[7]);
-                    }
-                    qk_wave_lds_sync();
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int e = e0 + i;
-                        if (e < a.half) y[i] = x[i] * turn[e].x - b[e + a.half] * turn[e].y;
-                        else if (e < rot) y[i] = b[e - a.half] * turn[e - a.half].y + x[i] * turn[e - a.half].x;
-                    }
-                }
-            }
-            if (on) pg_put8(dst + e0, y);
-        }
+/* the sequence that has row t, as pg_find, by a whole wave: 64 starts at a time */
+__device__ __forceinline__ int pg_find_wave(const int32_t *starts, int n_seqs, int t) {
+    const int lane = threadIdx.x & 63;
+    const int end = qk_ld(starts + n_seqs); /* in flight beside the first round */
+    int lo = 0, span = n_seqs;
+    while (true) {
+        const int step = (span + 63) >> 6, i = lo + lane * step;
+        const int c = __popcll(__ballot(lane * step < span && qk_ld(starts + min(i, n_seqs - 1)) <= t));
+        if (c == 0) return n_seqs;
+        lo += (c - 1) * step;
+        if (step == 1) return t < end ? lo : n_seqs;
+        span = min(step, span - (c - 1) * step);
     }
 }
 
-template <typename S, typename D>
+template <typename S, typename D, int HD, int TOK>
+__global__ __launch_bounds__(256) void k_pg_rotary(PgRotary a) {
+    constexpr int LP = HD <= 64 ? 8 : HD <= 128 ? 16 : 32; /* lanes of a head; of 192, 24 of them hold elements */
+    constexpr int RP = 256 / LP;
+    struct Row {
+        int64_t at;   /* of its place in the pages, or -1 */
+        int pos;      /* -1: nothing of it is written */
+    };
+    __shared__ __attribute__((aligned(16))) float cs[TOK][HD / 2], sn[TOK][HD / 2], buf[RP][HD + 4];
+    __shared__ Row rows[TOK];
+    const int tid = threadIdx.x, wave = tid >> 6, slot = tid / LP, e0 = 8 * (tid % LP), rot = 2 * a.half;
+    const bool on = HD != 192 || e0 < HD;
+    const int e1 = on ? e0 : 0, t0 = blockIdx.x * TOK, R = (int)a.per_row.d, end = min(TOK, a.n - t0) * R;
+    /* a head of the workgroup's tokens: which of q, k and v, and where it lies; their loads need
+     * no position and go out first */
+    struct Head {
+        int t, which, hd;
+    };
+    auto head = [&](int r) {
+        Head h;
+        h.t = TOK == 1 ? 0 : (int)pg_div_of(a.per_row, (uint32_t)r);
+        const int x = r - h.t * R;
+        h.which = x < a.h ? 0 : x < a.h + a.c.kvh ? 1 : 2;
+        h.hd = x - (h.which == 0 ? 0 : h.which == 1 ? a.h : a.h + a.c.kvh);
+        return h;
+    };
+    auto load = [&](int r, float x[8]) {
+        const Head h = head(min(r, end - 1));
+        const int64_t t = t0 + h.t;
+        pg_get8((h.which == 0 ? (const S *)a.q + t * a.q_token + h.hd * a.q_head
+                              : h.which == 1 ? (const S *)a.k + t * a.k_token + h.hd * a.k_head
+                                             : (const S *)a.v + t * a.v_token + h.hd * a.v_head) + e1, x);
+    };
+    float next[8];
+    load(slot, next);
+    const float freq = qk_ld(a.freqs + (tid < TOK * a.half ? tid % a.half : 0));
+    const int refused = a.status ? qk_ld(a.status) : 0;
+    for (int k = wave; k < TOK; k += 4) {
+        const int t = t0 + k, s = t < a.n ? pg_find_wave(a.starts, a.n_seqs, t) : a.n_seqs;
+        Row w = {-1, -1};
+        if (s < a.n_seqs && !refused) {
+            const int depth = a.depths ? qk_ld(a.depths + t) : 0;
+            const pg_seq q = pg_seq_at(&a.c, a.starts, a.slots, a.n, s);
+            const int first = q.len - q.count, row = t - q.start, place = first + row;
+            if (q.slot >= 0 && row >= 0 && row < q.count && place >= 0 && depth >= 0) {
+                w.at = pg_row_at(&a.c, a.c.table + q.slot * a.c.table_stride, place);
+                w.pos = a.depths ? first + min(depth, row) : place; /* below 0: a node before the first row */
+            }
+        }
+        if ((tid & 63) == 0) rows[k] = w;
+    }
+    __syncthreads();
+    for (int i = tid; i < TOK * a.half; i += 256) {
+        const int k = i / a.half, f = i - k * a.half;
+        const float2 c = pg_turn(max(rows[k].pos, 0), i == tid ? freq : qk_ld(a.freqs + f));
+        cs[k][f] = c.x;
+        sn[k][f] = c.y;
+    }
+    __syncthreads();
+    for (int r = slot; r < end; r += RP) {
+        const Head h = head(r);
+        const Row w = rows[h.t];
+        float x[8], y[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = next[i];
+        load(r + RP, next);
+        if (w.pos < 0 || (h.which && w.at < 0)) continue;
+        const int64_t t = t0 + h.t;
+        D *dst = h.which == 0 ? (D *)a.out + t * a.o_token + h.hd * a.o_head
+                              : (D *)(h.which == 1 ? a.c.k : a.c.v) + w.at + h.hd * a.c.head_stride;
+        const float *nw = h.which == 0 ? a.q_norm : a.k_norm;
+        if (h.which < 2 && nw) {
+            float wt[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) wt[i] = qk_ld(nw + e1 + i);
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+            ss = qk_group_sum<LP>(on ? ss : 0.0f);
+            const float f = 1.0f / sqrtf(ss / (float)HD + a.eps);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = (x[i] * f) * wt[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = x[i];
+        if (h.which < 2) {
+            const float *c = cs[h.t], *s = sn[h.t];
+            if (a.inter) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2)
+                    if (e0 + i < rot) {
+                        const int f = (e0 + i) / 2;
+                        y[i] = x[i] * c[f] - x[i + 1] * s[f];
+                        y[i + 1] = x[i] * s[f] + x[i + 1] * c[f];
+                    }
+            } else {
+                float *b = buf[slot];
+                qk_wave_lds_sync();
+                if (on) {
+                    *(float4 *)(b + e0) = make_float4(x[0], x[1], x[2], x[3]);
+                    *(float4 *)(b + e0 + 4) = make_float4(x[4], x[5], x[6], x[7]);
+                }
+                qk_wave_lds_sync();
+                if (a.half % 8 == 0) { /* the lane's partners are another lane's eight */
+                    if (e0 < rot) {
+                        const bool up = e0 >= a.half;
+                        const int f = up ? e0 - a.half : e0;
+                        const float4 *p = (const float4 *)(b + (up ? f : f + a.half));
+                        const float4 p0 = p[0], p1 = p[1], c0 = *(const float4 *)(c + f), c1 = *(const float4 *)(c + f + 4),
+                                     s0 = *(const float4 *)(s + f), s1 = *(const float4 *)(s + f + 4);
+                        const float pp[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+                        const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+                        const float ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+                        for (int i = 0; i < 8; i++) y[i] = up ? pp[i] * ss[i] + x[i] * cc[i] : x[i] * cc[i] - pp[i] * ss[i];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int e = e0 + i;
+                        if (e < a.half) y[i] = x[i] * c[e] - b[e + a.half] * s[e];
+                        else if (e < rot) y[i] = b[e - a.half] * s[e - a.half] + x[i] * c[e - a.half];
+                    }
+                }
+            }
+        }
+        if (on) pg_put8(dst + e0, y);
+    }
+}
+
+template <typename S, typename D, int TOK>
 static int pg_rotary_hd(const PgRotary &a, hipStream_t st) {
-    const dim3 grid(a.n < (1 << 20) ? a.n : 1 << 20), wg(256);
+    const dim3 grid((unsigned)(((int64_t)a.n + TOK - 1) / TOK)), wg(256);
     switch (a.c.hd) {
-    case 64: hipLaunchKernelGGL((k_pg_rotary<S, D, 64>), grid, wg, 0, st, a); break;
-    case 128: hipLaunchKernelGGL((k_pg_rotary<S, D, 128>), grid, wg, 0, st, a); break;
-    case 192: hipLaunchKernelGGL((k_pg_rotary<S, D, 192>), grid, wg, 0, st, a); break;
-    case 256: hipLaunchKernelGGL((k_pg_rotary<S, D, 256>), grid, wg, 0, st, a); break;
+    case 64: hipLaunchKernelGGL((k_pg_rotary<S, D, 64, TOK>), grid, wg, 0, st, a); break;
+    case 128: hipLaunchKernelGGL((k_pg_rotary<S, D, 128, TOK>), grid, wg, 0, st, a); break;
+    case 192: hipLaunchKernelGGL((k_pg_rotary<S, D, 192, TOK>), grid, wg, 0, st, a); break;
+    case 256: hipLaunchKernelGGL((k_pg_rotary<S, D, 256, TOK>), grid, wg, 0, st, a); break;
     default: return (int)hipErrorInvalidValue;
     }
     return QK_CHECK_LAUNCH();
+}
+template <typename S, typename D>
+static int pg_rotary_tok(const PgRotary &a, hipStream_t st) {
+    return a.n >= PG_ROTARY_MANY ? pg_rotary_hd<S, D, 4>(a, st) : pg_rotary_hd<S, D, 1>(a, st);
 }
 
 extern "C" int qk_launch_pg_rotary(const pg_cache *c, const qmoe_paged_rotary *r, const int32_t *starts, const int32_t *slots,
@@ -186,8 +259,9 @@ extern "C" int qk_launch_pg_rotary(const pg_cache *c, const qmoe_paged_rotary *r
     a.eps = r->eps;
     a.n = n; a.n_seqs = n_seqs;
     a.h = r->n_heads; a.half = r->rot / 2; a.inter = r->interleaved;
-    if (c->dtype == QMOE_F32) return pg_rotary_hd<float, float>(a, st);
-    return r->src_dtype == QMOE_F32 ? pg_rotary_hd<float, uint16_t>(a, st) : pg_rotary_hd<uint16_t, uint16_t>(a, st);
+    a.per_row = pg_div_make((uint32_t)(r->n_heads + 2 * c->kvh));
+    if (c->dtype == QMOE_F32) return pg_rotary_tok<float, float>(a, st);
+    return r->src_dtype == QMOE_F32 ? pg_rotary_tok<float, uint16_t>(a, st) : pg_rotary_tok<uint16_t, uint16_t>(a, st);
 }
 
 /* ------------------------------------------------------------ trees

@@ -469,6 +469,7 @@ typedef struct {
 #define PG_MAX_BATCH 1024      /* sequences of a reserve or fork call */
 #define PG_MAX_PAGES (1 << 20) /* pages of a pool: a batch's needs sum in 32 bits */
 #define PG_MAX_SEQS (1 << 16)  /* sequences of an append or attention call */
+#define PG_MAX_ROTARY 67000000 /* rows of a rotary append: 64 threads each, below 2^32 */
 
 typedef struct {
     const void *q;

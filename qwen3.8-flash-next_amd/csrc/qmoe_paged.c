@@ -275,6 +275,7 @@ int qmoe_paged_append_rotary(const qmoe_paged_cache *q, int layer, const qmoe_pa
         return pg_fail(err, "rows of dtype %d for pages of dtype %d (the pages' type, or f32)", r->src_dtype, c.dtype);
     if (r->n_heads < 0 || (int64_t)b->n * r->n_heads > PG_MAX_ROWS)
         return pg_fail(err, "%d rows of %d heads out of range [0, %d]", b->n, r->n_heads, PG_MAX_ROWS);
+    if (b->n > PG_MAX_ROTARY) return pg_fail(err, "n = %d rows are too many for one call", b->n);
     if (r->rot < 2 || r->rot > c.hd || r->rot % 2) return pg_fail(err, "rot %d is not even in [2, head_dim = %d]", r->rot, c.hd);
     if (r->interleaved != 0 && r->interleaved != 1) return pg_fail(err, "interleaved %d is not 0 or 1", r->interleaved);
     if (!(r->eps >= 0.0f) || !isfinite(r->eps)) return pg_fail(err, "eps %g is not finite and >= 0", (double)r->eps);

@@ -11,7 +11,9 @@ raises at import time instead of falling back to anything else.
 from __future__ import annotations
 
 import ctypes
+import operator
 import os
+import struct
 from dataclasses import dataclass
 from typing import Optional
 
@@ -138,6 +140,9 @@ class QmoePagedRotary(ctypes.Structure):
                 ("interleaved", ctypes.c_int), ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float)]
 
 
+# the same structs as bytes: a call fills one in 0.4 us, a ctypes one of 20 fields in 4
+_BATCH, _QUERY, _ROTARY = (struct.Struct(f) for f in ("@PPiiP", "@PP4q4if", "@4P8q2iP2iPPf"))
+
 PAGED_ATTN, PAGED_RESERVE, PAGED_FORK, PAGED_COMPACT, PAGED_KEEP = 0, 1, 2, 3, 4
 _INT_END = 2 ** 31
 
@@ -191,11 +196,11 @@ SIGNATURES = {
     "qmoe_gr_mix": (_I, [_P, _I, _P, _I, _P, _P, _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_gr_inject": (_I, [_P, _P, _P, _I, _P, _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_ws_bytes": (ctypes.c_size_t, [ctypes.POINTER(QmoePagedCache), _I, _I, _I, _I]),
-    "qmoe_paged_append": (_I, [ctypes.POINTER(QmoePagedCache), _I, ctypes.POINTER(QmoePagedBatch), _P, _P, _I,
+    "qmoe_paged_append": (_I, [ctypes.POINTER(QmoePagedCache), _I, _P, _P, _P, _I,
                                ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _P,
                                ctypes.POINTER(QmoeErr)]),
-    "qmoe_paged_attn": (_I, [ctypes.POINTER(QmoePagedCache), _I, ctypes.POINTER(QmoePagedBatch),
-                             ctypes.POINTER(QmoePagedQuery), _P, ctypes.c_size_t, _P, ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_attn": (_I, [ctypes.POINTER(QmoePagedCache), _I, _P,
+                             _P, _P, ctypes.c_size_t, _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_reserve": (_I, [ctypes.POINTER(QmoePagedCache), _P, _P, _I, _P, _P, ctypes.c_size_t, _P,
                                 ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_fork": (_I, [ctypes.POINTER(QmoePagedCache), _P, _P, _P, _I, _P, _P, ctypes.c_size_t, _P,
@@ -203,15 +208,15 @@ SIGNATURES = {
     "qmoe_paged_evict": (_I, [ctypes.POINTER(QmoePagedCache), _P, _I, _I, _I, _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_compact": (_I, [ctypes.POINTER(QmoePagedCache), _P, _P, ctypes.c_size_t, _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_tree_build": (_I, [_P, _P, _I, _I, ctypes.POINTER(QmoePagedTree), _P, ctypes.POINTER(QmoeErr)]),
-    "qmoe_paged_attn_tree": (_I, [ctypes.POINTER(QmoePagedCache), _I, ctypes.POINTER(QmoePagedBatch),
-                                  ctypes.POINTER(QmoePagedQuery), ctypes.POINTER(QmoePagedTree), _P, ctypes.c_size_t, _P,
+    "qmoe_paged_attn_tree": (_I, [ctypes.POINTER(QmoePagedCache), _I, _P,
+                                  _P, ctypes.POINTER(QmoePagedTree), _P, ctypes.c_size_t, _P,
                                   ctypes.POINTER(QmoeErr)]),
-    "qmoe_paged_append_rotary": (_I, [ctypes.POINTER(QmoePagedCache), _I, ctypes.POINTER(QmoePagedBatch),
-                                      ctypes.POINTER(QmoePagedRotary), ctypes.POINTER(QmoePagedTree), _P,
+    "qmoe_paged_append_rotary": (_I, [ctypes.POINTER(QmoePagedCache), _I, _P,
+                                      _P, ctypes.POINTER(QmoePagedTree), _P,
                                       ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_follow": (_I, [ctypes.POINTER(QmoePagedTree), _P, _P, _P, _P, _I, _I, _P, _P, _P, _P,
                                ctypes.POINTER(QmoeErr)]),
-    "qmoe_paged_keep": (_I, [ctypes.POINTER(QmoePagedCache), ctypes.POINTER(QmoePagedBatch), _P, _P, _P, _P, ctypes.c_size_t,
+    "qmoe_paged_keep": (_I, [ctypes.POINTER(QmoePagedCache), _P, _P, _P, _P, _P, ctypes.c_size_t,
                              _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_dn_create": (_I, [ctypes.POINTER(_P), ctypes.POINTER(QmoeDnConfig), ctypes.POINTER(QmoeErr)]),
     "qmoe_dn_destroy": (None, [_P]),
@@ -1056,10 +1061,27 @@ class DraftTree:
     nothing else, so one tree serves every layer, and every step whose drafts
     have this form."""
 
-    def __init__(self, parents, starts, depths, seen):
-        self.parents, self.starts, self.depths, self.seen = parents, starts, depths, seen
-        self._c = QmoePagedTree(depths.data_ptr(), seen.data_ptr(), seen.shape[1])
+    def __init__(self, parents, starts, depths, seen, n=None, words=None):
+        """depths None: both lie in `seen`, n depths before the words"""
+        self.parents, self.starts, self._depths, self._seen = parents, starts, depths, seen
+        self.n, self.words, self.index = n, words, seen.get_device()
+        at = seen.data_ptr()
+        if depths is not None:
+            if seen.dim() != 2 or depths.dim() != 1 or seen.shape[0] != depths.shape[0] or seen.element_size() != 4 or \
+                    depths.element_size() != 4 or not seen.is_contiguous() or not depths.is_contiguous() or \
+                    depths.get_device() != self.index:
+                raise QmoeError("depths [n] and seen [n, words] must be contiguous, of 32 bits and on one device")
+            self.n, self.words = seen.shape
+        self._c = QmoePagedTree(at if depths is None else depths.data_ptr(), at + 4 * self.n if depths is None else at, self.words)
         self._p = ctypes.byref(self._c)
+
+    @property
+    def depths(self):
+        return self._seen[:self.n] if self._depths is None else self._depths
+
+    @property
+    def seen(self):
+        return self._seen[self.n:].view(self.n, self.words) if self._depths is None else self._seen
 
 
 class PagedCache:
@@ -1097,7 +1119,7 @@ class PagedCache:
             self._fits(nm, *t.shape)
         self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
         self.device, self.dtype = k.device, k.dtype
-        self._torch, self._i32, self._u8 = torch, torch.int32, torch.uint8
+        self._torch, self._i32, self._f32 = torch, torch.int32, torch.float32
         self._own = (k.dtype,)  # types of q and out, and of appended rows
         self._src = (k.dtype,) if k.dtype == torch.float32 else (k.dtype, torch.float32)
         for nm, t, shape in (("v", v, v.shape), ("table", table, (lens.numel(), table.shape[-1])),
@@ -1113,6 +1135,8 @@ class PagedCache:
                                  lens.data_ptr(), refs.data_ptr(), table.shape[0], table.shape[1])
         self._cp = ctypes.byref(self._c)
         self._need = {}  # workspace bytes by a call's sizes
+        self._index, self._code = k.get_device(), _dtype_code(k)
+        self._no_bytes = torch.empty(0, dtype=torch.uint8, device=self.device)
         if self.device.type != "cuda":
             raise QmoeError(f"a paged cache lives on the GPU, not on {self.device}")
 
@@ -1132,8 +1156,8 @@ class PagedCache:
         the call's stream as torch's, so that what the call allocates belongs
         to that stream"""
         torch = self._torch
-        if stream is None and self.device.index == torch.cuda.current_device():
-            return call(torch._C._cuda_getCurrentRawStream(self.device.index))
+        if stream is None and self._index == torch._C._cuda_getDevice():
+            return call(torch._C._cuda_getCurrentRawStream(self._index))
         with torch.cuda.device(self.device):
             if stream is None:
                 return call(torch._C._cuda_getCurrentRawStream(self.device.index))
@@ -1146,8 +1170,8 @@ class PagedCache:
         """device address of an int32 vector of n (or None)"""
         if t is None:
             return None
-        if t.dtype != self._i32 or t.device != self.device or t.dim() != 1 or (n is not None and t.shape[0] != n) or \
-                not t.is_contiguous():
+        if t.dtype != self._i32 or t.get_device() != self._index or t.dim() != 1 or not t.is_contiguous() or \
+                (n is not None and t.numel() != n):
             raise QmoeError(f"{what} must be a contiguous int32 vector" + (f" of {n}" if n is not None else "") +
                             f" on {self.device}")
         if n is None and t.shape[0] >= _INT_END:
@@ -1158,25 +1182,34 @@ class PagedCache:
         """device address of a f32 vector of n (or None)"""
         if t is None:
             return None
-        if t.dtype != self._torch.float32 or t.device != self.device or t.dim() != 1 or (n is not None and t.shape[0] != n) or \
-                not t.is_contiguous():
+        if t.dtype != self._f32 or t.get_device() != self._index or t.dim() != 1 or not t.is_contiguous() or \
+                (n is not None and t.numel() != n):
             raise QmoeError(f"{what} must be a contiguous float32 vector" + (f" of {n}" if n is not None else "") +
                             f" on {self.device}")
         return t.data_ptr()
 
     def _rows(self, t, heads, dtypes, what):
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.hd or t.dtype not in dtypes or t.stride(2) != 1 or \
-                t.device != self.device:
-            raise QmoeError(f"{what} must be [n, {heads}, {self.hd}] {' or '.join(str(d) for d in dtypes)} with the head "
-                            f"dim contiguous on {self.device}")
+        """(rows, token stride, head stride, address) of rows [n, heads, head dim]"""
+        shape = t.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.hd or t.dtype not in dtypes or t.get_device() != self._index:
+            self._bad_rows(heads, dtypes, what)
+        a, b, c = t.stride()
+        if c != 1:
+            self._bad_rows(heads, dtypes, what)
+        return shape[0], a, b, t.data_ptr()
+
+    def _bad_rows(self, heads, dtypes, what):
+        raise QmoeError(f"{what} must be [n, {heads}, {self.hd}] {' or '.join(str(d) for d in dtypes)} with the head "
+                        f"dim contiguous on {self.device}")
 
     def _batch(self, n, starts, slots, status):
+        """(the batch as C has it, its sequences)"""
         p = self._ints(starts, None, "starts")
-        if p is None or starts.shape[0] < 1:
+        if p is None or starts.numel() < 1:
             raise QmoeError("starts must hold one number more than there are sequences")
-        m = starts.shape[0] - 1
-        return QmoePagedBatch(p, None if slots is None else self._ints(slots, m, "slots"), n, m,
-                              None if status is None else self._ints(status, 1, "status"))
+        m = starts.numel() - 1
+        return _BATCH.pack(p, 0 if slots is None else self._ints(slots, m, "slots"), n, m,
+                           0 if status is None else self._ints(status, 1, "status")), m
 
     def _work(self, call, n=0, n_seqs=0, heads=0):
         """the call's workspace; a call that the library refuses gets 16 bytes"""
@@ -1185,7 +1218,7 @@ class PagedCache:
             if len(self._need) > 4096:
                 self._need.clear()
             need = self._need[call, n, n_seqs, heads] = max(lib().qmoe_paged_ws_bytes(self._cp, call, n, n_seqs, heads), 16)
-        return self._torch.empty(need, dtype=self._u8, device=self.device)
+        return self._no_bytes.new_empty(need)
 
     @staticmethod
     def _fits(what, *sizes):
@@ -1205,7 +1238,7 @@ class PagedCache:
             raise QmoeError(f"scale {scale} must not be 0 or round to it in f32 (None: 1 / sqrt(head_dim))")
 
     def _status(self):
-        return self._torch.empty(1, dtype=self._i32, device=self.device)
+        return self.lens.new_empty(1)
 
     # -- rows
     def append(self, layer, k, v, starts, slots=None, stream=None, status=None):
@@ -1214,19 +1247,17 @@ class PagedCache:
         unless `status` (of the reserve that made room for them) is 0"""
         if not 0 <= layer < self.n_layers:
             raise QmoeError(f"layer {layer} out of range [0, {self.n_layers})")
-        self._rows(k, self.kvh, self._src, "k")
-        self._rows(v, self.kvh, self._src, "v")
-        n = k.shape[0]
-        if n != v.shape[0] or k.dtype != v.dtype:
+        n, kt, kh, kp = self._rows(k, self.kvh, self._src, "k")
+        m, vt, vh, vp = self._rows(v, self.kvh, self._src, "v")
+        if n != m or k.dtype != v.dtype:
             raise QmoeError("k and v must have the same rows and type")
         if n >= _INT_END:
             self._fits("k", n)
-        b, err = self._batch(n, starts, slots, status), QmoeErr()
+        (b, _), err = self._batch(n, starts, slots, status), QmoeErr()
 
         def call(st):
-            _check(lib().qmoe_paged_append(self._cp, layer, ctypes.byref(b), k.data_ptr(), v.data_ptr(), _dtype_code(k),
-                                           k.stride(0), k.stride(1), v.stride(0), v.stride(1), st, ctypes.byref(err)), err,
-                   "qmoe_paged_append")
+            _check(lib().qmoe_paged_append(self._cp, layer, b, kp, vp, _dtype_code(k), kt, kh, vt, vh, st, ctypes.byref(err)),
+                   err, "qmoe_paged_append")
         self._on(stream, call)
 
     def append_rotary(self, layer, k, v, starts, freqs, q=None, slots=None, tree=None, q_norm=None, k_norm=None, eps=1e-6,
@@ -1244,40 +1275,39 @@ class PagedCache:
         unless `status` is 0, are left as out has them."""
         if not 0 <= layer < self.n_layers:
             raise QmoeError(f"layer {layer} out of range [0, {self.n_layers})")
-        self._rows(k, self.kvh, self._src, "k")
-        self._rows(v, self.kvh, self._src, "v")
-        n, heads = k.shape[0], 0
-        if n != v.shape[0] or k.dtype != v.dtype:
+        n, kt, kh, kp = self._rows(k, self.kvh, self._src, "k")
+        m, vt, vh, vp = self._rows(v, self.kvh, self._src, "v")
+        if n != m or k.dtype != v.dtype:
             raise QmoeError("k and v must have the same rows and type")
+        heads = qt = qh = qp = ot = oh = op = 0
         if q is not None:
             heads = q.shape[1] if q.dim() == 3 else 0
-            self._rows(q, heads, (k.dtype,), "q")
-            if q.shape[0] != n:
-                raise QmoeError(f"q has {q.shape[0]} rows, k {n}")
+            m, qt, qh, qp = self._rows(q, heads, (k.dtype,), "q")
+            if m != n:
+                raise QmoeError(f"q has {m} rows, k {n}")
             if out is not None:
-                self._rows(out, heads, self._own, "out")
-                if out.shape[0] != n:
-                    raise QmoeError(f"out has {out.shape[0]} rows, q {n}")
+                m, ot, oh, op = self._rows(out, heads, self._own, "out")
+                if m != n:
+                    raise QmoeError(f"out has {m} rows, q {n}")
         elif out is not None or q_norm is not None:
             raise QmoeError("out and q_norm are given without q")
         if n >= _INT_END or heads >= _INT_END:
             self._fits("k", n, heads)
         f = self._floats(freqs, None, "freqs")
-        if f is None or not 1 <= freqs.shape[0] <= self.hd // 2:
+        if f is None or not 1 <= freqs.numel() <= self.hd // 2:
             raise QmoeError(f"freqs must hold 1 to {self.hd // 2} numbers")
         qn, kn = self._floats(q_norm, self.hd, "q_norm"), self._floats(k_norm, self.hd, "k_norm")
-        b, t, err = self._batch(n, starts, slots, status), self._tree(tree, n), QmoeErr()
+        (b, _), t, err = self._batch(n, starts, slots, status), self._tree(tree, n), QmoeErr()
+        rot, code, eps = 2 * freqs.numel(), _dtype_code(k), ctypes.c_float(eps).value
 
         def call(st):
-            o = out
+            o, place = out, (ot, oh, op)
             if q is not None and out is None:
-                o = self._torch.empty((n, heads, self.hd), dtype=self.dtype, device=self.device)
-            a = QmoePagedRotary(None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), None if o is None else o.data_ptr(),
-                                *((0, 0) if q is None else q.stride()[:2]), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                                *((0, 0) if o is None else o.stride()[:2]), _dtype_code(k), heads, f, 2 * freqs.shape[0],
-                                1 if interleaved else 0, qn, kn, eps)
-            _check(lib().qmoe_paged_append_rotary(self._cp, layer, ctypes.byref(b), ctypes.byref(a), t, st, ctypes.byref(err)),
-                   err, "qmoe_paged_append_rotary")
+                o = self.k.new_empty((n, heads, self.hd))
+                place = heads * self.hd, self.hd, o.data_ptr()
+            a = _ROTARY.pack(qp, kp, vp, place[2], qt, qh, kt, kh, vt, vh, place[0], place[1], code, heads, f, rot,
+                             1 if interleaved else 0, qn or 0, kn or 0, eps)
+            _check(lib().qmoe_paged_append_rotary(self._cp, layer, b, a, t, st, ctypes.byref(err)), err, "qmoe_paged_append_rotary")
             return o
         return self._on(stream, call)
 
@@ -1301,28 +1331,34 @@ class PagedCache:
             self._scale(scale)
         if window or sinks:
             self._span(window, sinks)
-        self._rows(q, heads, self._own, "q")
-        n = q.shape[0]
+            window, sinks = operator.index(window), operator.index(sinks)
+        else:
+            window = sinks = 0
+        n, qt, qh, qp = self._rows(q, heads, self._own, "q")
         if n >= _INT_END or heads >= _INT_END:
             self._fits("q", n, heads)
-        b, err = self._batch(n, starts, slots, status), QmoeErr()
+        (b, m), err = self._batch(n, starts, slots, status), QmoeErr()
         t = self._tree(tree, n)
         if out is not None:
-            self._rows(out, heads, self._own, "out")
-            if out.shape[0] != n:
-                raise QmoeError(f"out has {out.shape[0]} rows, q {n}")
+            rows, ot, oh, op = self._rows(out, heads, self._own, "out")
+            if rows != n:
+                raise QmoeError(f"out has {rows} rows, q {n}")
+        scale = 0.0 if scale is None else ctypes.c_float(scale).value
 
         def call(st):
-            o = self._torch.empty((n, heads, self.hd), dtype=self.dtype, device=self.device) if out is None else out
-            a = QmoePagedQuery(q.data_ptr(), o.data_ptr(), q.stride(0), q.stride(1), o.stride(0), o.stride(1), heads, window,
-                               sinks, 1 if grouped else 0, 0.0 if scale is None else scale)
-            ws = self._work(PAGED_ATTN, n, b.n_seqs, heads)
-            if t is None:
-                _check(lib().qmoe_paged_attn(self._cp, layer, ctypes.byref(b), ctypes.byref(a), ws.data_ptr(), ws.numel(), st,
-                                             ctypes.byref(err)), err, "qmoe_paged_attn")
+            if out is None:
+                o = self.k.new_empty((n, heads, self.hd))
+                place = o.data_ptr(), qt, qh, heads * self.hd, self.hd
             else:
-                _check(lib().qmoe_paged_attn_tree(self._cp, layer, ctypes.byref(b), ctypes.byref(a), t, ws.data_ptr(),
-                                                  ws.numel(), st, ctypes.byref(err)), err, "qmoe_paged_attn_tree")
+                o, place = out, (op, qt, qh, ot, oh)
+            a = _QUERY.pack(qp, *place, heads, window, sinks, 1 if grouped else 0, scale)
+            ws = self._work(PAGED_ATTN, n, m, heads)
+            if t is None:
+                _check(lib().qmoe_paged_attn(self._cp, layer, b, a, ws.data_ptr(), ws.numel(), st, ctypes.byref(err)), err,
+                       "qmoe_paged_attn")
+            else:
+                _check(lib().qmoe_paged_attn_tree(self._cp, layer, b, a, t, ws.data_ptr(), ws.numel(), st, ctypes.byref(err)), err,
+                       "qmoe_paged_attn_tree")
             return o
         return self._on(stream, call)
 
@@ -1337,17 +1373,15 @@ class PagedCache:
         Returns a DraftTree for append_rotary, attend_tree, follow and keep."""
         p = self._ints(parents, None, "parents")
         s = self._ints(starts, None, "starts")
-        if p is None or s is None or starts.shape[0] < 1:
+        if p is None or s is None or starts.numel() < 1:
             raise QmoeError("parents must be given, and starts hold one number more than there are sequences")
-        n, m, err = parents.shape[0], starts.shape[0] - 1, QmoeErr()
+        n, m, err = parents.numel(), starts.numel() - 1, QmoeErr()
         if most is not None and not 0 <= most < 2 ** 31:
             raise QmoeError(f"most {most} must be in [0, 2^31)")
         words = max(1, min(32, -(-min(n, n if most is None else most) // 32)))
 
         def call(st):
-            depths = self._torch.empty(n, dtype=self._i32, device=self.device)
-            seen = self._torch.empty((n, words), dtype=self._i32, device=self.device)
-            t = DraftTree(parents, starts, depths, seen)
+            t = DraftTree(parents, starts, None, self.lens.new_empty(n * (words + 1)), n, words)
             _check(lib().qmoe_paged_tree_build(p, s, n, m, t._p, st, ctypes.byref(err)), err, "qmoe_paged_tree_build")
             return t
         return self._on(stream, call)
@@ -1355,8 +1389,8 @@ class PagedCache:
     def _tree(self, tree, n):
         if tree is None:
             return None
-        if tree.depths.device != self.device or tree.depths.shape[0] != n:
-            raise QmoeError(f"the tree has {tree.depths.shape[0]} rows on {tree.depths.device}, the call {n} on {self.device}")
+        if tree.index != self._index or tree.n != n:
+            raise QmoeError(f"the tree has {tree.n} rows on device {tree.index}, the call {n} on {self.device}")
         return tree._p
 
     def attend_tree(self, layer, q, tree, slots=None, window=0, sinks=0, scale=None, grouped=False, out=None, stream=None,
@@ -1376,15 +1410,14 @@ class PagedCache:
         Returns (rows [n]: the path's rows at the first places of their
         sequence, -1 after them; counts [n_seqs]; next [n_seqs]: what was chosen
         after the last one, -1 for none)."""
-        n = tree.depths.shape[0]
-        t, m, err = self._tree(tree, n), tree.starts.shape[0] - 1, QmoeErr()
+        n = tree.n
+        t, m, err = self._tree(tree, n), tree.starts.numel() - 1, QmoeErr()
         if tokens is None or chosen is None or tree.parents is None:
             raise QmoeError("tokens, chosen and the tree's parents must be given")
         a, b = self._ints(tokens, n, "tokens"), self._ints(chosen, n, "chosen")
 
         def call(st):
-            rows = self._torch.empty(n, dtype=self._i32, device=self.device)
-            counts, last = (self._torch.empty(m, dtype=self._i32, device=self.device) for _ in range(2))
+            rows, counts, last = self.lens.new_empty(n), self.lens.new_empty(m), self.lens.new_empty(m)
             _check(lib().qmoe_paged_follow(t, tree.parents.data_ptr(), a, b, tree.starts.data_ptr(), n, m, rows.data_ptr(),
                                            counts.data_ptr(), last.data_ptr(), st, ctypes.byref(err)), err, "qmoe_paged_follow")
             return rows, counts, last
@@ -1398,13 +1431,13 @@ class PagedCache:
         -1 (refused; nothing is changed unless 0)."""
         if rows is None or counts is None:
             raise QmoeError("rows and counts must be given")
-        r, n = self._ints(rows, None, "rows"), rows.shape[0]
-        b, err = self._batch(n, starts, slots, status), QmoeErr()
-        c = self._ints(counts, b.n_seqs, "counts")
+        r, n = self._ints(rows, None, "rows"), rows.numel()
+        (b, m), err = self._batch(n, starts, slots, status), QmoeErr()
+        c = self._ints(counts, m, "counts")
 
         def call(st):
-            result, ws = self._status(), self._work(PAGED_KEEP, n, b.n_seqs)
-            _check(lib().qmoe_paged_keep(self._cp, ctypes.byref(b), r, c, result.data_ptr(), ws.data_ptr(), ws.numel(), st,
+            result, ws = self._status(), self._work(PAGED_KEEP, n, m)
+            _check(lib().qmoe_paged_keep(self._cp, b, r, c, result.data_ptr(), ws.data_ptr(), ws.numel(), st,
                                          ctypes.byref(err)), err, "qmoe_paged_keep")
             return result
         return self._on(stream, call)
