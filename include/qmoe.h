@@ -717,10 +717,10 @@ typedef struct {
 } qmoe_paged_batch;
 
 /* workspace bytes of a call; 0 for arguments that the call refuses.  n counts
- * for QMOE_PAGED_ATTN (qmoe_paged_attn and qmoe_paged_attn_tree) and
- * QMOE_PAGED_KEEP only, n_heads for the first, n_seqs not for
- * QMOE_PAGED_COMPACT. */
-enum { QMOE_PAGED_ATTN = 0, QMOE_PAGED_RESERVE = 1, QMOE_PAGED_FORK = 2, QMOE_PAGED_COMPACT = 3, QMOE_PAGED_KEEP = 4 };
+ * for QMOE_PAGED_ATTN, QMOE_PAGED_ATTN_TREE and QMOE_PAGED_KEEP only, n_heads
+ * for the first two, n_seqs not for QMOE_PAGED_COMPACT. */
+enum { QMOE_PAGED_ATTN = 0, QMOE_PAGED_RESERVE = 1, QMOE_PAGED_FORK = 2, QMOE_PAGED_COMPACT = 3, QMOE_PAGED_KEEP = 4,
+       QMOE_PAGED_ATTN_TREE = 5 };
 size_t qmoe_paged_ws_bytes(const qmoe_paged_cache *c, int call, int n, int n_seqs, int n_heads);
 
 /* Writes the batch's new rows k, v [n, n_kv_heads, head_dim] into the pages
@@ -828,8 +828,8 @@ int qmoe_paged_tree_build(const int32_t *parents, const int32_t *starts, int n, 
  * bits (up to its own), whose positions are first + their depths: the window
  * and the sinks count in positions.  A row that is no node gives zeros.  The
  * bits may be the caller's own, of any rows r <= t (bits past t do not count,
- * depths are brought into [-1, t], a seen row's into [0, r]).  Workspace as
- * QMOE_PAGED_ATTN. */
+ * depths are brought into [-1, t], a seen row's into [0, r]).  Workspace:
+ * QMOE_PAGED_ATTN_TREE. */
 int qmoe_paged_attn_tree(const qmoe_paged_cache *c, int layer, const qmoe_paged_batch *b, const qmoe_paged_query *q,
                          const qmoe_paged_tree *t, void *ws, size_t ws_bytes, void *stream, qmoe_err *err);
 

@@ -36,6 +36,9 @@ struct PaArgs {
     float2 *pml;  /* [slot, RT]: maximum (log2 units), sum */
     int4 *index;  /* [n_seqs], calls of more than PA_INDEX sequences: units, joined tasks
                    * and split units before the sequence's, its parts */
+    int4 *split;  /* [joins, 2], trees on units of PM_RT rows: of a task that is cut, rows (0: none), start, row tile,
+                   * kv head; first slot, parts */
+    int joins;
 };
 
 /* query head of member g of kv head kh's group: heads kh, kh + kvh, ... (the
@@ -205,21 +208,20 @@ __device__ __forceinline__ bool pa_find(const PaArgs &p, int want, PaUnit &u) {
         if (p.one < p.extra && __builtin_amdgcn_readlane(pa_scan(c.units), 63) > p.units)
             c = pa_count(p, l, pg_share(total, p.per_unit, p.extra));
         const int units = JOIN ? c.tasks : c.units;
-        int ue, se;
-        if (RT == PM_RT) {
+        int ue = 0, se = pa_scan(c.split) - c.split;
+        if (RT == PM_RT && !JOIN) {
             /* the sequences with the longest parts come first, so that the last
-             * units to start are short ones */
+             * units to start are short ones; joins, and where parts lie, keep
+             * the batch's order: this loop is most of what a wave without a task
+             * does, and a join's launch has many */
             const int len = units ? (l.key_tiles + c.parts - 1) / c.parts : 0;
-            ue = se = 0;
             for (int k = 0; k < n; k++) {
                 const int lk = __builtin_amdgcn_readlane(len, k);
                 const bool before = lk > len || (lk == len && k < lane);
                 ue += before ? __builtin_amdgcn_readlane(units, k) : 0;
-                se += before ? __builtin_amdgcn_readlane(c.split, k) : 0;
             }
         } else {
             ue = pa_scan(units) - units;
-            se = pa_scan(c.split) - c.split;
         }
         const uint64_t here = __ballot(want >= ue && want < ue + units);
         if (!here) return false;
@@ -804,6 +806,201 @@ __device__ __forceinline__ void pa_store(const PaArgs &p, const PaUnit &u, const
     if (u.parts > 1 && h == 0) p.pml[(int64_t)u.slot * PM_RT + rr] = make_float2(m, l);
 }
 
+/* ------------------------------------------------------------ units of trees
+ * Trees on units of PM_RT rows.  All row tiles of a sequence have about the
+ * same keys, those before the drafts, so what a call takes is its longest
+ * part: with tasks (sequence, row tile, kv head) for all units that run at
+ * once or fewer, the shortest length at which every task, cut into parts of
+ * that length or less, still gets a unit for each of them.  Parts of about the
+ * mean length, as in pa_find, are up to half longer and leave units without
+ * work: 16 nodes of 64 sequences of 4000 rows 93 us, so 75; up to 16 of 64 of
+ * 64 to 32768 105, so 85 (of each layer).  Parts are not made for less than
+ * PA_JOIN tiles that they save. */
+#define PA_JOIN 10
+
+struct PaNeed {
+    pg_seq s;
+    int rows, len; /* row tiles, key tiles of one of them */
+};
+template <int KT>
+__device__ __forceinline__ PaNeed pa_need(const PaArgs &p, int i) {
+    PaNeed q;
+    q.s = pa_seq(p, i);
+    q.rows = (q.s.count * p.G + PM_RT - 1) / PM_RT;
+    /* one tile at the least: a task of no keys has zeros to write */
+    q.len = max(pg_tiles_of(q.s.len - q.s.count, q.s.len - 1, p.a.window, p.a.sinks, KT).nt, 1);
+    return q;
+}
+__device__ __forceinline__ int pa_cuts(int len, int most) { return (int)(((uint32_t)len + (uint32_t)most - 1) / (uint32_t)most); }
+
+/* The length of a part from the tasks, the longest of them, and tiles in all
+ * (fp32, the same in every wave; its rounding is far below the factor's);
+ * units_at(length) sums over the sequences.  More tasks than units: parts of
+ * the units' mean, so that fewer tasks than units are cut, and at most twice
+ * as many units belong to such. */
+template <typename F>
+__device__ __forceinline__ int pa_length(int tasks, int longest, float total, int units, F units_at) {
+    int lo = (int)(1.0001f * total / (float)units) + 1;
+    if (tasks <= units && lo < longest) {
+        int hi = min(longest, (int)(total / (float)(units - tasks + 1)) + 2);
+        if (units_at(hi) > units) hi = longest; /* of a rounded total */
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (units_at(mid) <= units) hi = mid;
+            else lo = mid + 1;
+        }
+    }
+    return longest - lo < PA_JOIN ? max(longest, 1) : lo;
+}
+__device__ __forceinline__ int pa_sum(int v) { return __builtin_amdgcn_readlane(pa_scan(v), 63); }
+__device__ __forceinline__ int pa_most(int v) { return (int)qk_wave_max_u32((uint32_t)v); }
+
+/* Calls of more sequences than a wave has lanes: what precedes each one (units,
+ * units and tasks that are split), its parts, by one workgroup before; at
+ * [n_seqs] what they come to. */
+template <int KT>
+__global__ __launch_bounds__(1024) void k_pa_tree_index(PaArgs p) {
+    __shared__ int part[4][16];
+    __shared__ float sums[16];
+    const int tid = threadIdx.x, wave = tid >> 6, n = p.a.n_seqs, per = (n + 1023) >> 10;
+    const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    auto over = [&](int v, int k) { /* the workgroup's sum */
+        v = pa_sum(v);
+        __syncthreads();
+        if ((tid & 63) == 0) part[k][wave] = v;
+        __syncthreads();
+        int t = 0;
+        for (int w = 0; w < 16; w++) t += part[k][w];
+        return t;
+    };
+    int tasks = 0, longest = 0;
+    float total = 0.0f;
+    PaNeed last = {{-1, 0, 0, 0}, 0, 1};
+    for (int i = i0; i < i1; i++) {
+        last = pa_need<KT>(p, i);
+        tasks += last.rows * p.c.kvh;
+        longest = max(longest, last.rows ? last.len : 0);
+        total += (float)(last.rows * p.c.kvh) * (float)last.len;
+    }
+    total = qk_group_sum<64>(total);
+    longest = pa_most(longest);
+    if ((tid & 63) == 0) {
+        sums[wave] = total;
+        part[1][wave] = longest;
+    }
+    tasks = over(tasks, 0);
+    total = 0.0f;
+    for (int w = 0; w < 16; w++) {
+        total += sums[w];
+        longest = max(longest, part[1][w]);
+    }
+    const int most = pa_length(tasks, longest, total, p.units, [&](int length) {
+        int v = 0;
+        for (int i = i0; i < i1; i++) {
+            const PaNeed q = per == 1 ? last : pa_need<KT>(p, i);
+            v += q.rows * p.c.kvh * pa_cuts(q.len, length);
+        }
+        return over(v, 0);
+    });
+    int x[3] = {0, 0, 0};
+    for (int i = i0; i < i1; i++) {
+        const PaNeed q = per == 1 ? last : pa_need<KT>(p, i);
+        const int c = pa_cuts(q.len, most), t = q.rows * p.c.kvh;
+        x[0] += t * c;
+        x[1] += c > 1 ? t * c : 0;
+        x[2] += c > 1 ? t : 0;
+    }
+    int y[3];
+    for (int k = 0; k < 3; k++) y[k] = pa_scan(x[k]);
+    __syncthreads();
+    if ((tid & 63) == 63)
+        for (int k = 0; k < 3; k++) part[1 + k][wave] = y[k];
+    __syncthreads();
+    for (int k = 0; k < 3; k++)
+        for (int w = 0; w < wave; w++) y[k] += part[1 + k][w];
+    if (tid == 1023) qk_st((float4 *)(p.index + n), __builtin_bit_cast(float4, make_int4(y[0], y[1], y[2], 0)));
+    for (int k = 0; k < 3; k++) y[k] -= x[k];
+    for (int i = i0; i < i1; i++) {
+        const PaNeed q = per == 1 ? last : pa_need<KT>(p, i);
+        const int c = pa_cuts(q.len, most), t = q.rows * p.c.kvh;
+        qk_st((float4 *)(p.index + i), __builtin_bit_cast(float4, make_int4(y[0], y[1], y[2], c)));
+        y[0] += t * c;
+        y[1] += c > 1 ? t * c : 0;
+        y[2] += c > 1 ? t : 0;
+    }
+}
+
+/* Unit blockIdx.x of the call, as pa_find; in the order of the batch, since
+ * all run at once or are whole tasks.  The first unit of a split task leaves in
+ * `split` what the join needs, others that there is no such task, so that a
+ * join's workgroup reads one record. */
+template <int KT>
+__device__ __forceinline__ bool pa_tree_find(const PaArgs &p, PaUnit &u) {
+    const int lane = threadIdx.x & 63, n = p.a.n_seqs, want = blockIdx.x;
+    const int refused = qk_ld(p.a.status ? p.a.status : (const int32_t *)pa_zero);
+    int ubase, sbase, tbase, tasks; /* units, split units and split tasks before the sequence's, split tasks in all */
+    bool is;
+    if (n <= PA_INDEX) {
+        PaNeed q = {{-1, 0, 0, 0}, 0, 1};
+        if (lane < n) q = pa_need<KT>(p, lane);
+        const int mine = q.rows * p.c.kvh;
+        const float total = qk_group_sum<64>((float)mine * (float)q.len);
+        const int most = pa_length(pa_sum(mine), pa_most(q.rows ? q.len : 0), total, p.units,
+                                   [&](int length) { return pa_sum(mine * pa_cuts(q.len, length)); });
+        const int parts = pa_cuts(q.len, most), units = mine * parts, ue = pa_scan(units);
+        const int cut = parts > 1 ? mine : 0, se = pa_scan(cut * parts), te = pa_scan(cut);
+        tasks = __builtin_amdgcn_readlane(te, 63);
+        const uint64_t here = __ballot(want < ue);
+        is = here != 0;
+        const int at = is ? __builtin_ctzll(here) : 0;
+        u.parts = __builtin_amdgcn_readlane(parts, at);
+        ubase = __builtin_amdgcn_readlane(ue - units, at);
+        sbase = __builtin_amdgcn_readlane(se - cut * parts, at);
+        tbase = __builtin_amdgcn_readlane(te - cut, at);
+        u.s.slot = __builtin_amdgcn_readlane(q.s.slot, at);
+        u.s.start = __builtin_amdgcn_readlane(q.s.start, at);
+        u.s.count = __builtin_amdgcn_readlane(q.s.count, at);
+        u.s.len = __builtin_amdgcn_readlane(q.s.len, at);
+    } else {
+        const int4 all = __builtin_bit_cast(int4, qk_ld((const float4 *)(p.index + n)));
+        tasks = __builtin_amdgcn_readfirstlane(all.z);
+        is = want < __builtin_amdgcn_readfirstlane(all.x);
+        int lo = 0, span = n; /* the last sequence with ubase <= want, 64 of the index at a time */
+        while (span > 1) {
+            const int step = (span + 63) >> 6;
+            const bool ok = lane * step < span && qk_ld((const int *)(p.index + lo + min(lane * step, span - 1))) <= want;
+            const int c = max(__popcll(__ballot(ok)), 1) - 1;
+            lo += c * step;
+            span = min(step, span - c * step);
+        }
+        const int4 x = __builtin_bit_cast(int4, qk_ld((const float4 *)(p.index + lo)));
+        const pg_seq s = pa_seq(p, lo);
+        ubase = __builtin_amdgcn_readfirstlane(x.x);
+        sbase = __builtin_amdgcn_readfirstlane(x.y);
+        tbase = __builtin_amdgcn_readfirstlane(x.z);
+        u.parts = __builtin_amdgcn_readfirstlane(x.w);
+        u.s.slot = __builtin_amdgcn_readfirstlane(s.slot);
+        u.s.start = __builtin_amdgcn_readfirstlane(s.start);
+        u.s.count = __builtin_amdgcn_readfirstlane(s.count);
+        u.s.len = __builtin_amdgcn_readfirstlane(s.len);
+    }
+    if (threadIdx.x == 0 && want < p.joins && (refused || want >= tasks))
+        qk_st((float4 *)(p.split + 2 * want), make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+    if (!is || refused) return false;
+    /* row tile, part, kv head */
+    const int q = (want - ubase) / p.c.kvh;
+    u.kh = want - ubase - q * p.c.kvh;
+    u.rtile = q / u.parts;
+    u.part = q - u.rtile * u.parts;
+    u.slot = sbase + want - ubase;
+    if (threadIdx.x == 0 && u.parts > 1 && u.part == 0) {
+        float4 *rec = (float4 *)(p.split + 2 * (tbase + u.rtile * p.c.kvh + u.kh));
+        qk_st(rec, __builtin_bit_cast(float4, make_int4(min(PM_RT, u.s.count * p.G - u.rtile * PM_RT), u.s.start, u.rtile, u.kh)));
+        qk_st(rec + 1, __builtin_bit_cast(float4, make_int4(u.slot, u.parts, 0, 0)));
+    }
+    return true;
+}
+
 /* ------------------------------------------------------------ many rows
  * Prompts, bf16: a unit is 128 rows, 32 per wave, and a part of the keys; NG
  * groups of four waves take its tiles in turn and are added at the end
@@ -876,7 +1073,7 @@ __global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
     __shared__ __attribute__((aligned(16))) uint4 kv[2][NG][2][KT * CR]; /* buffer, group's tile, k / v */
     __shared__ __attribute__((aligned(16))) ulonglong2 where[KEYS]; /* addresses of a key's k and v */
     PaUnit u;
-    if (!pa_find<PM_RT, KT, false>(p, blockIdx.x, u)) return;
+    if (TREE ? !pa_tree_find<KT>(p, u) : !pa_find<PM_RT, KT, false>(p, blockIdx.x, u)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), c = lane & 31, h = lane >> 5;
     const int group = __builtin_amdgcn_readfirstlane(tid / 256);
     const int row0 = u.rtile * PM_RT, rows = u.s.count * p.G, nrow = min(PM_RT, rows - row0);
@@ -1087,7 +1284,7 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
     __shared__ __attribute__((aligned(16))) uint4 kv[NG][2][3][KT * CR]; /* even / odd tile, k / v, part */
     __shared__ __attribute__((aligned(16))) ulonglong2 where[PM_CHUNK]; /* addresses of a key's k and v */
     PaUnit u;
-    if (!pa_find<PM_RT, KT, false>(p, blockIdx.x, u)) return;
+    if (TREE ? !pa_tree_find<KT>(p, u) : !pa_find<PM_RT, KT, false>(p, blockIdx.x, u)) return;
     const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, h = lane >> 5;
     const int odd = NG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int row0 = u.rtile * PM_RT, rows = u.s.count * p.G, nrow = min(PM_RT, rows - row0);
@@ -1116,7 +1313,7 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
         }
         __syncthreads();
     };
-    float4 kx[NB], vx[NB]; /* this thread's pieces of four of the next step's tile */
+    float4 kx[NB], vx[NB]; /* this threadIdx.x's pieces of four of the next step's tile */
     auto rows_of = [&](int i) { return where + (NG * (i % CH) + odd) * KT; };
     auto load_k = [&](int i, int x) {
         const int L = x * 256 + tid, rr = L / (HD / 4);
@@ -1314,6 +1511,86 @@ __global__ __launch_bounds__(64 * W) void k_pa_join(PaArgs p) {
     }
 }
 
+/* The same of trees on units of PM_RT rows, whose units leave a record of every
+ * task that is cut.  A row has HD / 4 lanes, which load up to PT_FEW parts at
+ * once; of more parts the groups of the workgroup's lanes take runs of a row's,
+ * which are added in their order. */
+#define PT_FEW 8
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void k_pa_tree_join(PaArgs p) {
+    constexpr int Q = HD / 4, LP = Q <= 16 ? 16 : Q <= 32 ? 32 : 64, W = 256 / LP; /* lanes of a row, groups of them */
+    __shared__ __attribute__((aligned(16))) float4 acc[2][W][LP];
+    __shared__ float2 ml[2][W];
+    const int4 b = qk_ld(p.split + 2 * blockIdx.x), c = qk_ld(p.split + 2 * blockIdx.x + 1);
+    const int tid = threadIdx.x, g = tid / LP, d = tid % LP;
+    const bool on = d < Q;
+    const int slot = c.x, parts = __builtin_amdgcn_readfirstlane(c.y), rows = __builtin_amdgcn_readfirstlane(b.x);
+    PaUnit w;
+    w.s.start = b.y;
+    w.rtile = b.z;
+    w.kh = b.w;
+    auto add = [](float2 m, float4 x, float M, float &L, float4 &y) {
+        const float f = m.x == M ? 1.0f : __builtin_amdgcn_exp2f(m.x - M);
+        L = fmaf(m.y, f, L);
+        y = make_float4(fmaf(x.x, f, y.x), fmaf(x.y, f, y.y), fmaf(x.z, f, y.z), fmaf(x.w, f, y.w));
+    };
+    /* parts [k0, k1) of row r onto M, L, y */
+    auto sum = [&](int k0, int k1, int r, float &M, float &L, float4 &y) {
+        for (int k = k0; k < k1; k += PT_FEW) {
+            float2 m[PT_FEW];
+            float4 x[PT_FEW];
+            float top = M;
+#pragma unroll
+            for (int j = 0; j < PT_FEW; j++)
+                if (k + j < k1) {
+                    const int64_t at = (int64_t)(slot + (k + j) * p.c.kvh) * PM_RT + r;
+                    m[j].x = qk_ld((const float *)(p.pml + at));
+                    m[j].y = qk_ld((const float *)(p.pml + at) + 1);
+                    x[j] = qk_ld((const float4 *)(p.po + at * HD + 4 * (on ? d : 0)));
+                }
+#pragma unroll
+            for (int j = 0; j < PT_FEW; j++)
+                if (k + j < k1) top = fmaxf(top, m[j].x);
+            if (k > k0) {
+                const float f = M == top ? 1.0f : __builtin_amdgcn_exp2f(M - top);
+                L *= f;
+                y = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+            }
+            M = top;
+#pragma unroll
+            for (int j = 0; j < PT_FEW; j++)
+                if (k + j < k1) add(m[j], x[j], M, L, y);
+        }
+    };
+    if (parts <= PT_FEW) {
+        for (int r = blockIdx.y * W + g; r < rows; r += gridDim.y * W) {
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float M = -INFINITY, L = 0.0f;
+            sum(0, parts, r, M, L, y);
+            if (on) pa_join_out<T, HD>(p, w, w.rtile * PM_RT + r, 4 * d, y, pa_norm(M, L));
+        }
+        return;
+    }
+    const int run = (parts + W - 1) / W;
+    for (int r = blockIdx.y, i = 0; r < rows; r += gridDim.y, i ^= 1) { /* two buffers: one barrier a row */
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float M = -INFINITY, L = 0.0f;
+        sum(min(g * run, parts), min(g * run + run, parts), r, M, L, y);
+        acc[i][g][d] = y;
+        if (d == 0) ml[i][g] = make_float2(M, L);
+        __syncthreads();
+        if (g == 0) {
+            float A = -INFINITY, S = 0.0f;
+            y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < W; k++) A = fmaxf(A, ml[i][k].x);
+#pragma unroll
+            for (int k = 0; k < W; k++) add(ml[i][k], acc[i][k][d], A, S, y);
+            if (on) pa_join_out<T, HD>(p, w, w.rtile * PM_RT + r, 4 * d, y, pa_norm(A, S));
+        }
+    }
+}
+
 /* ------------------------------------------------------------ host side */
 
 /* how a call is cut: units asked for, the grid that holds them whatever the
@@ -1373,6 +1650,25 @@ static int pa_rows(const pg_cache *c, const pg_attn *a) {
     const int later = pa_rows_long(c, rows, a->n_seqs);
     int64_t keys = c->cap, most = c->dtype == QMOE_BF16 || c->hd == 64 ? 1 << 18 : c->hd < 256 ? 1 << 17 : 1 << 19;
     if (a->window > 0 && (int64_t)a->window + a->sinks < keys) keys = (int64_t)a->window + a->sinks;
+    if (later == 32) most /= 2;
+    return units <= 8 || units * keys <= most ? 16 : later;
+}
+/* The same for trees, whose units of PM_RT rows start sooner and are cut by
+ * their longest part: they take over at a quarter of the limits (64 nodes of a
+ * sequence of 4000 rows 33 us with 16 rows and 25, 32 of 8 sequences at head
+ * dim 256 58 and 43, f32 16 of one of 8000 41 and 35; 32 of 4 of 1000 rows 23
+ * and 25), and, where there is one for every fourth CU, from units of 32 rows
+ * of bf16 (4 nodes of 64 sequences of 4000 rows 72 and 64, of 32 47 and 41; of
+ * 16 33 and 38; f32 163 and 187). */
+static int pa_tree_rows_long(const pg_cache *c, int64_t rows, int n_seqs) {
+    const int rt = pa_rows_long(c, rows, n_seqs);
+    return rt == 16 && rows <= (int64_t)16 * n_seqs ? 16 : c->dtype == QMOE_BF16 && (int64_t)n_seqs * c->kvh >= 64 ? PM_RT : rt;
+}
+static int pa_tree_rows(const pg_cache *c, const pg_attn *a) {
+    const int64_t rows = (int64_t)a->n * (a->h / c->kvh), units = rows * c->kvh / 16;
+    int64_t keys = c->cap, most = c->dtype == QMOE_BF16 || c->hd == 64 ? 1 << 16 : c->hd < 256 ? 1 << 15 : 1 << 17;
+    if (a->window > 0 && (int64_t)a->window + a->sinks < keys) keys = (int64_t)a->window + a->sinks;
+    const int later = pa_tree_rows_long(c, rows, a->n_seqs);
     if (later == 32) most /= 2;
     return units <= 8 || units * keys <= most ? 16 : later;
 }
@@ -1448,15 +1744,81 @@ static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), void *ws, hipStream_t 
     return QK_CHECK_LAUNCH();
 }
 
+/* Trees on units of PM_RT rows: as many units as run at once, two to a CU
+ * where a unit is one group of four waves; the grid that holds the call's, the
+ * slots of partial results and the tasks that may be cut. */
+struct PaTreePlan {
+    int units, slots, joins;
+    int64_t grid;
+};
+static int pa_tree_groups(const pg_cache *c) { return c->dtype == QMOE_BF16 && c->hd <= 128 ? 1 : 2; }
+static PaTreePlan pa_tree_plan(const pg_cache *c, int n, int n_seqs, int h) {
+    PaTreePlan q;
+    q.units = pa_tree_groups(c) == 1 ? 512 : 256;
+    const int64_t rows = (int64_t)n * (h / c->kvh), seqs = n_seqs < n ? n_seqs : n;
+    const int64_t per_head = rows / PM_RT + seqs < rows ? rows / PM_RT + seqs : rows, tasks = per_head * c->kvh;
+    const bool cut = c->cap / pm_kt(c->hd, c->dtype == QMOE_F32) + 2 >= PA_JOIN + 1; /* the longest task may be cut at all */
+    q.grid = tasks <= q.units ? q.units : tasks + q.units;
+    q.slots = !cut ? 0 : (tasks <= q.units ? 1 : 2) * q.units;
+    q.joins = !cut ? 0 : (int)(tasks < q.units ? tasks : q.units);
+    return q;
+}
+static size_t pa_tree_ws(const pg_cache *c, int n, int n_seqs, int h) {
+    const PaTreePlan q = pa_tree_plan(c, n, n_seqs, h);
+    const size_t rows = (size_t)q.slots * PM_RT, index = n_seqs > PA_INDEX ? ((size_t)n_seqs + 1) * 16 : 0;
+    return rows * c->hd * 4 + rows * 8 + pa_up((size_t)q.joins * 32) + pa_up(index);
+}
+extern "C" size_t qk_pg_attn_tree_ws(const pg_cache *c, int n, int n_seqs, int h) {
+    const int rt = pa_tree_rows_long(c, (int64_t)n * (h / c->kvh), n_seqs);
+    const int64_t grid = rt == PM_RT ? 2 * pa_tree_plan(c, n, n_seqs, h).grid : pa_plan_of(c, n, n_seqs, h, rt).grid;
+    if (grid * 256 > 0xFFFFFFFFll) return 0;
+    const size_t a = pa_ws(c, n, n_seqs, h, 16), b = rt == PM_RT ? pa_tree_ws(c, n, n_seqs, h) : pa_ws(c, n, n_seqs, h, rt);
+    return a > b ? a : b;
+}
+
+/* workgroups of a task: of a few long ones, in a hundred parts, a row each */
+static unsigned pa_tree_join_rows(int joins) {
+    const int r = 8192 / joins;
+    return (unsigned)(r < 4 ? 4 : r > PM_RT ? PM_RT : r);
+}
+
+template <typename T, int HD, int KT>
+static int pa_launch_tree(PaArgs p, void (*kernel)(PaArgs), int threads, void *ws, hipStream_t st) {
+    const PaTreePlan q = pa_tree_plan(&p.c, p.a.n, p.a.n_seqs, p.a.h);
+    const size_t rows = (size_t)q.slots * PM_RT;
+    p.units = q.units;
+    p.joins = q.joins;
+    p.po = (float *)ws;
+    p.pml = (float2 *)(p.po + rows * HD);
+    p.split = (int4 *)(p.pml + rows);
+    p.index = (int4 *)((char *)p.split + pa_up((size_t)q.joins * 32));
+    if (p.a.n_seqs > PA_INDEX) {
+        hipLaunchKernelGGL((k_pa_tree_index<KT>), dim3(1), dim3(1024), 0, st, p);
+        const int rc = QK_CHECK_LAUNCH();
+        if (rc) return rc;
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)q.grid), dim3(threads), 0, st, p);
+    const int rc = QK_CHECK_LAUNCH();
+    if (rc || q.joins == 0) return rc;
+    hipLaunchKernelGGL((k_pa_tree_join<T, HD>), dim3(q.joins, pa_tree_join_rows(q.joins)), dim3(256), 0, st, p);
+    return QK_CHECK_LAUNCH();
+}
+
 template <typename T, int HD, bool TREE>
 static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
-    const int rt = pa_rows(&p.c, &p.a);
+    const int rt = TREE ? pa_tree_rows(&p.c, &p.a) : pa_rows(&p.c, &p.a);
+    if (TREE && rt == PM_RT) {
+        if constexpr (sizeof(T) == 2) {
+            constexpr int NG = HD <= 128 ? 1 : 2; /* pa_tree_groups */
+            return pa_launch_tree<T, HD, pm_kt(HD)>(p, k_pa_many<HD, NG, true>, 256 * NG, ws, st);
+        } else return pa_launch_tree<T, HD, pm_kt(HD, true)>(p, k_pa_many32<HD, true>, 256 * pm_halves32(HD), ws, st);
+    }
     if (rt == PM_RT) {
         if constexpr (sizeof(T) == 2) {
             if constexpr (HD <= 128)
-                if (pa_groups(&p.c, p.a.n, p.a.h) == 1) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 1, TREE>, ws, st);
-            return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 2, TREE>, ws, st);
-        } else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD, TREE>, ws, st);
+                if (pa_groups(&p.c, p.a.n, p.a.h) == 1) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 1, false>, ws, st);
+            return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 2, false>, ws, st);
+        } else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD, false>, ws, st);
     }
     if constexpr (HD <= (sizeof(T) == 2 ? 192 : 128)) /* pa_two */
         if (rt == 32) return pa_launch_rt<T, HD, 32, PD_KT>(p, k_pa_few<T, HD, 2, TREE>, ws, st);
@@ -1482,6 +1844,8 @@ extern "C" int qk_launch_pg_attn(const pg_cache *c, const pg_attn *a, void *ws, 
     p.po = NULL;
     p.pml = NULL;
     p.index = NULL;
+    p.split = NULL;
+    p.joins = 0;
     hipStream_t st = (hipStream_t)stream;
     if (a->depths) return c->dtype == QMOE_BF16 ? pa_launch_hd<uint16_t, true>(p, ws, st) : pa_launch_hd<float, true>(p, ws, st);
     return c->dtype == QMOE_BF16 ? pa_launch_hd<uint16_t, false>(p, ws, st) : pa_launch_hd<float, false>(p, ws, st);

@@ -284,7 +284,7 @@ __device__ __forceinline__ int2 pg_rows_of(const int32_t *starts, int n, int i) 
     return make_int2(a, max(b - a, 0));
 }
 
-__global__ __launch_bounds__(256) void k_pg_tree(PgTree a) {
+__global__ __launch_bounds__(1024) void k_pg_tree(PgTree a) {
     __shared__ int up[PG_TREE_ROWS];
     __shared__ uint32_t head[PG_TREE_ROWS / 32]; /* bit t: row t is not the child of row t - 1 */
     const int tid = threadIdx.x;
@@ -292,13 +292,13 @@ __global__ __launch_bounds__(256) void k_pg_tree(PgTree a) {
     const int c = min(s.y, 32 * a.words);
     if (tid < PG_TREE_ROWS / 32) head[tid] = 0;
     __syncthreads();
-    for (int t = tid; t < c; t += 256) {
+    for (int t = tid; t < c; t += blockDim.x) {
         const int p = qk_ld(a.parents + s.x + t);
         up[t] = p >= -1 && p < t ? p : -2;
         if (t == 0 || p != t - 1) atomicOr(&head[t >> 5], 1u << (t & 31));
     }
     __syncthreads();
-    for (int x = tid; x < c * a.words; x += 256) {
+    for (int x = tid; x < c * a.words; x += blockDim.x) {
         const int t = x / a.words, w = x - t * a.words;
         int rows = 0, at = t;
         uint32_t bits = 0;
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256) void k_pg_tree(PgTree a) {
         a.seen[(int64_t)(s.x + t) * a.words + w] = at == -1 ? bits : 0u;
         if (w == 0) a.depths[s.x + t] = at == -1 ? rows - 1 : -1;
     }
-    for (int t = c + tid; t < s.y; t += 256) { /* past what the words hold: no nodes */
+    for (int t = c + tid; t < s.y; t += blockDim.x) { /* past what the words hold: no nodes */
         for (int w = 0; w < a.words; w++) a.seen[(int64_t)(s.x + t) * a.words + w] = 0u;
         a.depths[s.x + t] = -1;
     }
@@ -324,7 +324,8 @@ __global__ __launch_bounds__(256) void k_pg_tree(PgTree a) {
 extern "C" int qk_launch_pg_tree(const int32_t *parents, const int32_t *starts, int n, int n_seqs, int32_t *depths,
                                  uint32_t *seen, int words, void *stream) {
     const PgTree a = {parents, starts, n, words, depths, seen};
-    hipLaunchKernelGGL(k_pg_tree, dim3(n_seqs), dim3(256), 0, (hipStream_t)stream, a);
+    /* 256 nodes of 8 sequences 10 us with 256 threads, 5 with 1024 */
+    hipLaunchKernelGGL(k_pg_tree, dim3(n_seqs), dim3(words > 2 ? 1024 : 256), 0, (hipStream_t)stream, a);
     return QK_CHECK_LAUNCH();
 }
 

@@ -485,6 +485,7 @@ typedef struct {
 
 /* workspace bytes (attention: 0 for a call that no launch holds) and launches; 0 or a hipError_t */
 size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h);
+size_t qk_pg_attn_tree_ws(const pg_cache *c, int n, int n_seqs, int h);
 int qk_launch_pg_attn(const pg_cache *c, const pg_attn *a, void *ws, void *stream);
 int qk_launch_pg_append(const pg_cache *c, const void *k, const void *v, int src_dtype, int64_t k_token, int64_t k_head,
                         int64_t v_token, int64_t v_head, const int32_t *starts, const int32_t *slots,

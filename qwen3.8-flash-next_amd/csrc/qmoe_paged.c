@@ -151,6 +151,9 @@ size_t qmoe_paged_ws_bytes(const qmoe_paged_cache *q, int call, int n, int n_seq
     case QMOE_PAGED_ATTN:
         if (n < 0 || n_seqs > PG_MAX_SEQS || pg_heads(&c, n, n_heads, NULL)) return 0;
         return qk_pg_attn_ws(&c, n, n_seqs, n_heads);
+    case QMOE_PAGED_ATTN_TREE:
+        if (n < 0 || n_seqs > PG_MAX_SEQS || pg_heads(&c, n, n_heads, NULL)) return 0;
+        return qk_pg_attn_tree_ws(&c, n, n_seqs, n_heads);
     case QMOE_PAGED_RESERVE: return n_seqs > PG_MAX_BATCH ? 0 : qk_pg_reserve_ws(&c, n_seqs);
     case QMOE_PAGED_FORK: return n_seqs > PG_MAX_BATCH ? 0 : qk_pg_fork_ws(&c, n_seqs);
     case QMOE_PAGED_COMPACT: return qk_pg_compact_ws(&c);
@@ -216,7 +219,7 @@ static int pg_attention(const qmoe_paged_cache *cache, int layer, const qmoe_pag
     const int64_t stride[2] = {q->out_token_stride, q->out_head_stride}, size[2] = {b->n, q->n_heads};
     if (pg_apart(stride, size, 2, c.hd)) return pg_fail(err, "the strides let elements of out overlap");
     if (b->n == 0 || b->n_seqs == 0) return 0;
-    const size_t need = qk_pg_attn_ws(&c, b->n, b->n_seqs, q->n_heads);
+    const size_t need = t ? qk_pg_attn_tree_ws(&c, b->n, b->n_seqs, q->n_heads) : qk_pg_attn_ws(&c, b->n, b->n_seqs, q->n_heads);
     if (!need) return pg_fail(err, "%d rows of %d sequences and %d heads are more work than one launch holds", b->n, b->n_seqs, q->n_heads);
     if (!q->q || !q->out) return pg_fail(err, "%s is NULL", q->q ? "out" : "q");
     if (pg_misaligned(q->q) || pg_misaligned(q->out)) return pg_fail(err, "q and out must be 16-byte aligned");

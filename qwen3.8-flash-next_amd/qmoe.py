@@ -143,7 +143,7 @@ class QmoePagedRotary(ctypes.Structure):
 # the same structs as bytes: a call fills one in 0.4 us, a ctypes one of 20 fields in 4
 _BATCH, _QUERY, _ROTARY = (struct.Struct(f) for f in ("@PPiiP", "@PP4q4if", "@4P8q2iP2iPPf"))
 
-PAGED_ATTN, PAGED_RESERVE, PAGED_FORK, PAGED_COMPACT, PAGED_KEEP = 0, 1, 2, 3, 4
+PAGED_ATTN, PAGED_RESERVE, PAGED_FORK, PAGED_COMPACT, PAGED_KEEP, PAGED_ATTN_TREE = 0, 1, 2, 3, 4, 5
 _INT_END = 2 ** 31
 
 
@@ -1352,7 +1352,7 @@ class PagedCache:
             else:
                 o, place = out, (op, qt, qh, ot, oh)
             a = _QUERY.pack(qp, *place, heads, window, sinks, 1 if grouped else 0, scale)
-            ws = self._work(PAGED_ATTN, n, m, heads)
+            ws = self._work(PAGED_ATTN if t is None else PAGED_ATTN_TREE, n, m, heads)
             if t is None:
                 _check(lib().qmoe_paged_attn(self._cp, layer, b, a, ws.data_ptr(), ws.numel(), st, ctypes.byref(err)), err,
                        "qmoe_paged_attn")

@@ -192,8 +192,10 @@ def test_windows_and_sinks(dev, window, sinks, dtype):
 @pytest.mark.usefixtures("tables")
 @DTYPES
 @pytest.mark.parametrize("lens,counts", [([4000, 10], [9, 10]), ([3000] * 3, [2, 130, 600]), ([9000], [256]),
-                                         ([1500, 1100], [1024, 1000]), ([70] * 200, [6] * 200), ([50] * 700, [3, 0] * 350)],
-                         ids=["long", "chunks", "wide", "largest", "many", "more_than_512"])
+                                         ([1500, 1100], [1024, 1000]), ([70] * 200, [6] * 200), ([50] * 700, [3, 0] * 350),
+                                         ([20 + 97 * i % 2500 for i in range(90)], [5 + i % 13 for i in range(90)]),
+                                         ([40, 33, 7] * 400, [20, 33, 0] * 400)],
+                         ids=["long", "chunks", "wide", "largest", "many", "more_than_512", "indexed", "more_than_1024"])
 def test_longer_trees(dev, lens, counts, dtype):
     r = random.Random(len(lens))
     s = Setup(dev, HEADS[0 if len(lens) < 100 else 2], dtype, 32, lens, seed=len(lens))

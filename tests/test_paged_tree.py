@@ -152,7 +152,11 @@ def test_other_bad_calls_are_refused():
     x.refused(x.keep(ws=A + 8, size=need), "workspace")
     assert x.L.qmoe_paged_ws_bytes(x.c, pkg.PAGED_KEEP, 5, 1025, 0) == 0
     assert x.L.qmoe_paged_ws_bytes(x.c, pkg.PAGED_KEEP, -1, 3, 0) == 0
-    assert x.L.qmoe_paged_ws_bytes(x.c, 5, 5, 3, 8) == 0
+    assert x.L.qmoe_paged_ws_bytes(x.c, 6, 5, 3, 8) == 0
+    need = x.L.qmoe_paged_ws_bytes(x.c, pkg.PAGED_ATTN_TREE, 5, 3, 8)
+    assert need > 0
+    x.refused(x.attn(size=need - 1), "workspace")
+    x.refused(x.attn(ws=A + 8, size=need), "workspace")
 
 
 def test_calls_with_nothing_to_do_touch_nothing():
