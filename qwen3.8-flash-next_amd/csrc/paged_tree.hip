@@ -395,55 +395,99 @@ extern "C" int qk_launch_pg_follow(const int32_t *parents, const int32_t *tokens
 /* ------------------------------------------------------------ keep
  * Two launches, so that a batch with a sequence that is refused is left as it
  * was: the first finds where every kept row lies and goes to, a workgroup per
- * sequence, the second moves them and cuts the tables.  Kept rows ascend, so
- * row k goes to a place at or before its own and behind those of the rows
- * before it: a thread that moves its 16 bytes of every row of a sequence, in
- * order, 8 loads before their stores, never reads what it has written. */
+ * sequence, the second moves them and cuts the tables.  Small batches take one,
+ * of one workgroup.  Kept rows ascend, so row k goes to a place at or before
+ * its own and behind those of the rows before it: a thread that moves its 16
+ * bytes of every row of a sequence, in order, 8 loads before their stores,
+ * never reads what it has written. */
 struct PgKeep {
     pg_cache c;
     const int32_t *starts, *slots, *status, *rows, *counts;
     int n, n_seqs;
     int32_t *result;
-    int4 *head;          /* [n_seqs]: refused (1, or the batch's status), slot (-1: none), rows kept, lens now */
+    int4 *head;          /* [n_seqs]: refused (1, or the batch's status), slot, rows kept, lens now */
     longlong2 *moves;    /* [n]: element offsets from, to */
     pg_div cols, heads;  /* 16-byte pieces of a row, of a head */
 };
 
+/* sequence i: its rows of the call, its slot and what is kept; true where it is refused as far as
+ * that shows (the slot named twice, and the rows, are for the caller's lanes) */
+struct PgKept {
+    int from, count, slot, keep, len;
+};
+__device__ __forceinline__ bool pg_kept(const PgKeep &a, int i, PgKept &q) {
+    const int to = qk_ld(a.starts + i + 1);
+    q.from = qk_ld(a.starts + i);
+    q.slot = a.slots ? qk_ld(a.slots + i) : i;
+    q.keep = qk_ld(a.counts + i);
+    q.count = to - q.from;
+    q.len = 0;
+    if (q.from < 0 || to < q.from || to > a.n || q.slot < 0 || q.slot >= a.c.n_slots || q.keep < 0 || q.keep > q.count) return true;
+    q.len = qk_ld(a.c.lens + q.slot);
+    return q.len < q.count || q.len > a.c.cap;
+}
+/* where kept row k moves from and to (equal: it stays); true where it is refused */
+__device__ __forceinline__ bool pg_move_of(const PgKeep &a, const PgKept &q, int k, longlong2 &m) {
+    const int r = qk_ld(a.rows + q.from + k), before = k ? qk_ld(a.rows + q.from + k - 1) : -1, first = q.len - q.count;
+    m.x = m.y = 0;
+    if (r <= before || r >= q.count) return true;
+    if (r == k) return false;
+    const int32_t *row = a.c.table + q.slot * a.c.table_stride;
+    m.x = pg_row_at(&a.c, row, first + r);
+    m.y = pg_row_at(&a.c, row, first + k);
+    return m.x < 0 || m.y < 0 || qk_ld(a.c.refs + qk_ld(row + pg_div_of(a.c.page_rows, (uint32_t)(first + k)))) > 1;
+}
+/* piece x of all layers' k and v of a sequence's rows; moves(k) is row k's */
+template <typename F>
+__device__ __forceinline__ void pg_move(const PgKeep &a, int64_t x, int keep, F moves) {
+    const int es = a.c.dtype == QMOE_BF16 ? 2 : 4, lv = (int)(x / a.cols.d);
+    const uint32_t col = (uint32_t)(x - (int64_t)lv * a.cols.d), hd = pg_div_of(a.heads, col), ch = col - hd * a.heads.d;
+    char *base = (char *)(lv & 1 ? a.c.v : a.c.k) + ((lv >> 1) * a.c.layer_stride + hd * a.c.head_stride) * es + 16 * ch;
+    for (int k0 = 0; k0 < keep; k0 += 8) {
+        float4 y[8];
+        longlong2 m[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) m[k] = moves(min(k0 + k, keep - 1));
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k0 + k < keep && m[k].x != m[k].y) y[k] = qk_ld((const float4 *)(base + m[k].x * es));
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k0 + k < keep && m[k].x != m[k].y) qk_st((float4 *)(base + m[k].y * es), y[k]);
+    }
+}
+/* the slot's length, and the pages behind it, by `threads` */
+__device__ __forceinline__ void pg_cut(const PgKeep &a, int slot, int was, int now, int tid, int threads) {
+    const int R = (int)a.c.page_rows.d;
+    int32_t *row = a.c.table + slot * a.c.table_stride;
+    for (int e = (now + R - 1) / R + tid; e < (was + R - 1) / R; e += threads) {
+        const int p = qk_ld(row + e);
+        if (p >= 0 && p < a.c.n_pages) atomicSub(a.c.refs + p, 1);
+        row[e] = -1;
+    }
+    if (tid == 0) a.c.lens[slot] = now;
+}
+
 __global__ __launch_bounds__(256) void k_pg_keep_find(PgKeep a) {
     const int i = blockIdx.x, tid = threadIdx.x;
-    const int from = qk_ld(a.starts + i), to = qk_ld(a.starts + i + 1), count = to - from;
-    const int slot = a.slots ? qk_ld(a.slots + i) : i, keep = qk_ld(a.counts + i);
-    bool bad = from < 0 || to < from || to > a.n || slot < 0 || slot >= a.c.n_slots || keep < 0 || keep > count;
-    if (a.slots)
-        for (int j = tid; j < a.n_seqs; j += 256) bad |= j != i && qk_ld(a.slots + j) == slot;
-    bad = __syncthreads_or(bad);
-    int len = 0;
-    if (!bad) {
-        len = qk_ld(a.c.lens + slot);
-        bad = len < count || len > a.c.cap;
-        const int first = len - count;
-        const int32_t *row = a.c.table + slot * a.c.table_stride;
-        for (int k = tid; !bad && k < keep; k += 256) {
-            const int r = qk_ld(a.rows + from + k), before = k ? qk_ld(a.rows + from + k - 1) : -1;
-            bad = r <= before || r >= count;
-            longlong2 m = {0, 0};
-            if (!bad && r != k) {
-                m.x = pg_row_at(&a.c, row, first + r);
-                m.y = pg_row_at(&a.c, row, first + k);
-                bad = m.x < 0 || m.y < 0 ||
-                      qk_ld(a.c.refs + qk_ld(row + pg_div_of(a.c.page_rows, (uint32_t)(first + k)))) > 1;
-            }
-            a.moves[from + k] = m;
-        }
-        bad = __syncthreads_or(bad);
-        len -= count;
-    }
     const int refused = a.status ? qk_ld(a.status) : 0;
-    if (tid == 0) a.head[i] = make_int4(refused ? refused : bad ? -1 : 0, slot, keep, len + keep);
+    PgKept q;
+    bool bad = pg_kept(a, i, q);
+    if (a.slots)
+        for (int j = tid; j < a.n_seqs; j += 256) bad |= j != i && qk_ld(a.slots + j) == q.slot;
+    for (int k = tid; !bad && k < q.keep; k += 256) {
+        longlong2 m;
+        bad = pg_move_of(a, q, k, m);
+        qk_st((float4 *)(a.moves + q.from + k), __builtin_bit_cast(float4, m));
+    }
+    bad = __syncthreads_or(bad);
+    if (tid == 0) a.head[i] = make_int4(refused ? refused : bad ? -1 : 0, q.slot, q.keep, q.len - q.count + q.keep);
 }
 
 __global__ __launch_bounds__(256) void k_pg_keep_move(PgKeep a) {
     const int i = blockIdx.y, tid = threadIdx.x;
+    const int from = qk_ld(a.starts + i), count = qk_ld(a.starts + i + 1) - from;
+    const int4 h = qk_ld(a.head + i);
     int bad = 0;
     for (int j = tid; j < a.n_seqs; j += 256) bad |= qk_ld((const int *)(a.head + j)) != 0;
     if (__syncthreads_or(bad)) {
@@ -453,38 +497,49 @@ __global__ __launch_bounds__(256) void k_pg_keep_move(PgKeep a) {
         }
         return;
     }
-    const int4 h = qk_ld(a.head + i);
-    const int es = a.c.dtype == QMOE_BF16 ? 2 : 4;
-    if (blockIdx.x == 0) { /* the slot's length, and the pages behind it */
-        const int R = (int)a.c.page_rows.d;
-        int32_t *row = a.c.table + h.y * a.c.table_stride;
-        const int count = qk_ld(a.starts + i + 1) - qk_ld(a.starts + i), was = h.w - h.z + count;
-        for (int e = (h.w + R - 1) / R + tid; e < (was + R - 1) / R; e += 256) {
-            const int p = qk_ld(row + e);
-            if (p >= 0 && p < a.c.n_pages) atomicSub(a.c.refs + p, 1);
-            row[e] = -1;
-        }
-        if (tid == 0) a.c.lens[h.y] = h.w;
+    if (blockIdx.x == 0) {
+        pg_cut(a, h.y, h.w - h.z + count, h.w, tid, 256);
         if (i == 0 && tid == 0) *a.result = 0;
     }
-    const longlong2 *mv = a.moves + qk_ld(a.starts + i);
+    const longlong2 *mv = a.moves + from;
     const int64_t pieces = (int64_t)2 * a.c.n_layers * a.cols.d;
-    for (int64_t x = (int64_t)blockIdx.x * 256 + tid; x < pieces; x += (int64_t)gridDim.x * 256) {
-        const int lv = (int)(x / a.cols.d);
-        const uint32_t col = (uint32_t)(x - (int64_t)lv * a.cols.d), hd = pg_div_of(a.heads, col), ch = col - hd * a.heads.d;
-        char *base = (char *)(lv & 1 ? a.c.v : a.c.k) + ((lv >> 1) * a.c.layer_stride + hd * a.c.head_stride) * es + 16 * ch;
-        for (int k0 = 0; k0 < h.z; k0 += 8) {
-            float4 y[8];
-            longlong2 m[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                m[k] = __builtin_bit_cast(longlong2, qk_ld((const float4 *)(mv + min(k0 + k, h.z - 1))));
-                y[k] = qk_ld((const float4 *)(base + m[k].x * es));
-            }
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (k0 + k < h.z && m[k].x != m[k].y) qk_st((float4 *)(base + m[k].y * es), y[k]);
+    for (int64_t x = (int64_t)blockIdx.x * 256 + tid; x < pieces; x += (int64_t)gridDim.x * 256)
+        pg_move(a, x, h.z, [&](int k) { return __builtin_bit_cast(longlong2, qk_ld((const float4 *)(mv + k))); });
+}
+
+/* The same by one workgroup, a wave per sequence up to the moves.  Up to
+ * PG_KEEP_SMALL pieces of all sequences' rows: one of one layer 4.9 us in two
+ * launches, so 2.9. */
+#define PG_KEEP_SEQS 16
+#define PG_KEEP_ROWS 1024
+#define PG_KEEP_SMALL 4096
+__global__ __launch_bounds__(1024) void k_pg_keep_small(PgKeep a) {
+    __shared__ longlong2 moves[PG_KEEP_ROWS];
+    __shared__ PgKept seq[PG_KEEP_SEQS];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int refused = a.status ? qk_ld(a.status) : 0;
+    bool bad = refused != 0;
+    if (wave < a.n_seqs) {
+        PgKept q;
+        bad |= pg_kept(a, wave, q);
+        if (a.slots) bad |= lane < a.n_seqs && lane != wave && qk_ld(a.slots + min(lane, a.n_seqs - 1)) == q.slot;
+        for (int k = lane; !bad && k < q.keep; k += 64) {
+            longlong2 m;
+            bad = pg_move_of(a, q, k, m);
+            moves[q.from + k] = m;
         }
+        if (lane == 0) seq[wave] = q;
+    }
+    if (__syncthreads_or(bad)) {
+        if (tid == 0) *a.result = refused ? refused : -1;
+        return;
+    }
+    if (wave < a.n_seqs) pg_cut(a, seq[wave].slot, seq[wave].len, seq[wave].len - seq[wave].count + seq[wave].keep, lane, 64);
+    if (tid == 0) *a.result = 0;
+    const int pieces = 2 * a.c.n_layers * (int)a.cols.d;
+    for (int x = tid; x < pieces * a.n_seqs; x += 1024) {
+        const int i = x / pieces;
+        pg_move(a, x - i * pieces, seq[i].keep, [&](int k) { return moves[seq[i].from + k]; });
     }
 }
 
@@ -508,6 +563,10 @@ extern "C" int qk_launch_pg_keep(const pg_cache *c, const int32_t *starts, const
     a.heads = pg_div_make((uint32_t)per_head);
     if (n_seqs == 0) {
         hipLaunchKernelGGL(k_pg_keep_none, dim3(1), dim3(1), 0, st, status, result);
+        return QK_CHECK_LAUNCH();
+    }
+    if (n_seqs <= PG_KEEP_SEQS && n <= PG_KEEP_ROWS && (int64_t)2 * c->n_layers * a.cols.d * n_seqs <= PG_KEEP_SMALL) {
+        hipLaunchKernelGGL(k_pg_keep_small, dim3(1), dim3(1024), 0, st, a);
         return QK_CHECK_LAUNCH();
     }
     hipLaunchKernelGGL(k_pg_keep_find, dim3(n_seqs), dim3(256), 0, st, a);

@@ -14,6 +14,7 @@ import ctypes
 import operator
 import os
 import struct
+import threading
 from dataclasses import dataclass
 from typing import Optional
 
@@ -141,7 +142,18 @@ class QmoePagedRotary(ctypes.Structure):
 
 
 # the same structs as bytes: a call fills one in 0.4 us, a ctypes one of 20 fields in 4
-_BATCH, _QUERY, _ROTARY = (struct.Struct(f) for f in ("@PPiiP", "@PP4q4if", "@4P8q2iP2iPPf"))
+_BATCH, _QUERY, _ROTARY, _TREE = (struct.Struct(f) for f in ("@PPiiP", "@PP4q4if", "@4P8q2iP2iPPf", "@PPi"))
+
+
+class _PagedErr(threading.local):
+    """a thread's message buffer for the paged calls"""
+
+    def __init__(self):
+        self.err = QmoeErr()
+        self.p = ctypes.byref(self.err)
+
+
+_paged_err = _PagedErr()
 
 PAGED_ATTN, PAGED_RESERVE, PAGED_FORK, PAGED_COMPACT, PAGED_KEEP, PAGED_ATTN_TREE = 0, 1, 2, 3, 4, 5
 _INT_END = 2 ** 31
@@ -207,14 +219,14 @@ SIGNATURES = {
                              ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_evict": (_I, [ctypes.POINTER(QmoePagedCache), _P, _I, _I, _I, _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_compact": (_I, [ctypes.POINTER(QmoePagedCache), _P, _P, ctypes.c_size_t, _P, ctypes.POINTER(QmoeErr)]),
-    "qmoe_paged_tree_build": (_I, [_P, _P, _I, _I, ctypes.POINTER(QmoePagedTree), _P, ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_tree_build": (_I, [_P, _P, _I, _I, _P, _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_attn_tree": (_I, [ctypes.POINTER(QmoePagedCache), _I, _P,
-                                  _P, ctypes.POINTER(QmoePagedTree), _P, ctypes.c_size_t, _P,
+                                  _P, _P, _P, ctypes.c_size_t, _P,
                                   ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_append_rotary": (_I, [ctypes.POINTER(QmoePagedCache), _I, _P,
-                                      _P, ctypes.POINTER(QmoePagedTree), _P,
+                                      _P, _P, _P,
                                       ctypes.POINTER(QmoeErr)]),
-    "qmoe_paged_follow": (_I, [ctypes.POINTER(QmoePagedTree), _P, _P, _P, _P, _I, _I, _P, _P, _P, _P,
+    "qmoe_paged_follow": (_I, [_P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P,
                                ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_keep": (_I, [ctypes.POINTER(QmoePagedCache), _P, _P, _P, _P, _P, ctypes.c_size_t,
                              _P, ctypes.POINTER(QmoeErr)]),
@@ -1072,8 +1084,7 @@ class DraftTree:
                     depths.get_device() != self.index:
                 raise QmoeError("depths [n] and seen [n, words] must be contiguous, of 32 bits and on one device")
             self.n, self.words = seen.shape
-        self._c = QmoePagedTree(at if depths is None else depths.data_ptr(), at + 4 * self.n if depths is None else at, self.words)
-        self._p = ctypes.byref(self._c)
+        self._p = _TREE.pack(at if depths is None else depths.data_ptr(), at + 4 * self.n if depths is None else at, self.words)
 
     @property
     def depths(self):
@@ -1253,11 +1264,11 @@ class PagedCache:
             raise QmoeError("k and v must have the same rows and type")
         if n >= _INT_END:
             self._fits("k", n)
-        (b, _), err = self._batch(n, starts, slots, status), QmoeErr()
+        (b, _), err = self._batch(n, starts, slots, status), _paged_err
 
         def call(st):
-            _check(lib().qmoe_paged_append(self._cp, layer, b, kp, vp, _dtype_code(k), kt, kh, vt, vh, st, ctypes.byref(err)),
-                   err, "qmoe_paged_append")
+            _check(lib().qmoe_paged_append(self._cp, layer, b, kp, vp, _dtype_code(k), kt, kh, vt, vh, st, err.p),
+                   err.err, "qmoe_paged_append")
         self._on(stream, call)
 
     def append_rotary(self, layer, k, v, starts, freqs, q=None, slots=None, tree=None, q_norm=None, k_norm=None, eps=1e-6,
@@ -1297,7 +1308,7 @@ class PagedCache:
         if f is None or not 1 <= freqs.numel() <= self.hd // 2:
             raise QmoeError(f"freqs must hold 1 to {self.hd // 2} numbers")
         qn, kn = self._floats(q_norm, self.hd, "q_norm"), self._floats(k_norm, self.hd, "k_norm")
-        (b, _), t, err = self._batch(n, starts, slots, status), self._tree(tree, n), QmoeErr()
+        (b, _), t, err = self._batch(n, starts, slots, status), self._tree(tree, n), _paged_err
         rot, code, eps = 2 * freqs.numel(), _dtype_code(k), ctypes.c_float(eps).value
 
         def call(st):
@@ -1307,7 +1318,7 @@ class PagedCache:
                 place = heads * self.hd, self.hd, o.data_ptr()
             a = _ROTARY.pack(qp, kp, vp, place[2], qt, qh, kt, kh, vt, vh, place[0], place[1], code, heads, f, rot,
                              1 if interleaved else 0, qn or 0, kn or 0, eps)
-            _check(lib().qmoe_paged_append_rotary(self._cp, layer, b, a, t, st, ctypes.byref(err)), err, "qmoe_paged_append_rotary")
+            _check(lib().qmoe_paged_append_rotary(self._cp, layer, b, a, t, st, err.p), err.err, "qmoe_paged_append_rotary")
             return o
         return self._on(stream, call)
 
@@ -1337,7 +1348,7 @@ class PagedCache:
         n, qt, qh, qp = self._rows(q, heads, self._own, "q")
         if n >= _INT_END or heads >= _INT_END:
             self._fits("q", n, heads)
-        (b, m), err = self._batch(n, starts, slots, status), QmoeErr()
+        (b, m), err = self._batch(n, starts, slots, status), _paged_err
         t = self._tree(tree, n)
         if out is not None:
             rows, ot, oh, op = self._rows(out, heads, self._own, "out")
@@ -1354,10 +1365,10 @@ class PagedCache:
             a = _QUERY.pack(qp, *place, heads, window, sinks, 1 if grouped else 0, scale)
             ws = self._work(PAGED_ATTN if t is None else PAGED_ATTN_TREE, n, m, heads)
             if t is None:
-                _check(lib().qmoe_paged_attn(self._cp, layer, b, a, ws.data_ptr(), ws.numel(), st, ctypes.byref(err)), err,
+                _check(lib().qmoe_paged_attn(self._cp, layer, b, a, ws.data_ptr(), ws.numel(), st, err.p), err.err,
                        "qmoe_paged_attn")
             else:
-                _check(lib().qmoe_paged_attn_tree(self._cp, layer, b, a, t, ws.data_ptr(), ws.numel(), st, ctypes.byref(err)), err,
+                _check(lib().qmoe_paged_attn_tree(self._cp, layer, b, a, t, ws.data_ptr(), ws.numel(), st, err.p), err.err,
                        "qmoe_paged_attn_tree")
             return o
         return self._on(stream, call)
@@ -1375,14 +1386,14 @@ class PagedCache:
         s = self._ints(starts, None, "starts")
         if p is None or s is None or starts.numel() < 1:
             raise QmoeError("parents must be given, and starts hold one number more than there are sequences")
-        n, m, err = parents.numel(), starts.numel() - 1, QmoeErr()
+        n, m, err = parents.numel(), starts.numel() - 1, _paged_err
         if most is not None and not 0 <= most < 2 ** 31:
             raise QmoeError(f"most {most} must be in [0, 2^31)")
         words = max(1, min(32, -(-min(n, n if most is None else most) // 32)))
 
         def call(st):
             t = DraftTree(parents, starts, None, self.lens.new_empty(n * (words + 1)), n, words)
-            _check(lib().qmoe_paged_tree_build(p, s, n, m, t._p, st, ctypes.byref(err)), err, "qmoe_paged_tree_build")
+            _check(lib().qmoe_paged_tree_build(p, s, n, m, t._p, st, err.p), err.err, "qmoe_paged_tree_build")
             return t
         return self._on(stream, call)
 
@@ -1411,7 +1422,7 @@ class PagedCache:
         sequence, -1 after them; counts [n_seqs]; next [n_seqs]: what was chosen
         after the last one, -1 for none)."""
         n = tree.n
-        t, m, err = self._tree(tree, n), tree.starts.numel() - 1, QmoeErr()
+        t, m, err = self._tree(tree, n), tree.starts.numel() - 1, _paged_err
         if tokens is None or chosen is None or tree.parents is None:
             raise QmoeError("tokens, chosen and the tree's parents must be given")
         a, b = self._ints(tokens, n, "tokens"), self._ints(chosen, n, "chosen")
@@ -1419,7 +1430,7 @@ class PagedCache:
         def call(st):
             rows, counts, last = self.lens.new_empty(n), self.lens.new_empty(m), self.lens.new_empty(m)
             _check(lib().qmoe_paged_follow(t, tree.parents.data_ptr(), a, b, tree.starts.data_ptr(), n, m, rows.data_ptr(),
-                                           counts.data_ptr(), last.data_ptr(), st, ctypes.byref(err)), err, "qmoe_paged_follow")
+                                           counts.data_ptr(), last.data_ptr(), st, err.p), err.err, "qmoe_paged_follow")
             return rows, counts, last
         return self._on(stream, call)
 
@@ -1432,13 +1443,13 @@ class PagedCache:
         if rows is None or counts is None:
             raise QmoeError("rows and counts must be given")
         r, n = self._ints(rows, None, "rows"), rows.numel()
-        (b, m), err = self._batch(n, starts, slots, status), QmoeErr()
+        (b, m), err = self._batch(n, starts, slots, status), _paged_err
         c = self._ints(counts, m, "counts")
 
         def call(st):
             result, ws = self._status(), self._work(PAGED_KEEP, n, m)
             _check(lib().qmoe_paged_keep(self._cp, b, r, c, result.data_ptr(), ws.data_ptr(), ws.numel(), st,
-                                         ctypes.byref(err)), err, "qmoe_paged_keep")
+                                         err.p), err.err, "qmoe_paged_keep")
             return result
         return self._on(stream, call)
 
@@ -1451,12 +1462,12 @@ class PagedCache:
         if n_new is None:
             raise QmoeError("n_new must be given")
         p, m = self._ints(n_new, None, "n_new"), n_new.shape[0]
-        sl, err = self._ints(slots, m, "slots"), QmoeErr()
+        sl, err = self._ints(slots, m, "slots"), _paged_err
 
         def call(st):
             status, ws = self._status(), self._work(PAGED_RESERVE, 0, m)
             _check(lib().qmoe_paged_reserve(self._cp, sl, p, m, status.data_ptr(), ws.data_ptr(), ws.numel(), st,
-                                            ctypes.byref(err)), err, "qmoe_paged_reserve")
+                                            err.p), err.err, "qmoe_paged_reserve")
             return status
         return self._on(stream, call)
 
@@ -1467,12 +1478,12 @@ class PagedCache:
         if src is None or dst is None:
             raise QmoeError("src and dst must be given")
         s, m = self._ints(src, None, "src"), src.shape[0]
-        d, r, err = self._ints(dst, m, "dst"), self._ints(rows, m, "rows"), QmoeErr()
+        d, r, err = self._ints(dst, m, "dst"), self._ints(rows, m, "rows"), _paged_err
 
         def call(st):
             status, ws = self._status(), self._work(PAGED_FORK, 0, m)
             _check(lib().qmoe_paged_fork(self._cp, s, d, r, m, status.data_ptr(), ws.data_ptr(), ws.numel(), st,
-                                         ctypes.byref(err)), err, "qmoe_paged_fork")
+                                         err.p), err.err, "qmoe_paged_fork")
             return status
         return self._on(stream, call)
 
@@ -1491,20 +1502,20 @@ class PagedCache:
             raise QmoeError(f"ahead {ahead} must be in [0, 2^31)")
         if window:  # 0 is refused below; past any table nothing lies behind the window
             window = min(window + ahead, 2 ** 31 - 1)
-        sl, err = self._ints(slots, None, "slots"), QmoeErr()
+        sl, err = self._ints(slots, None, "slots"), _paged_err
         m = self.table.shape[0] if slots is None else slots.shape[0]
 
         def call(st):
-            _check(lib().qmoe_paged_evict(self._cp, sl, m, window, sinks, st, ctypes.byref(err)), err, "qmoe_paged_evict")
+            _check(lib().qmoe_paged_evict(self._cp, sl, m, window, sinks, st, err.p), err.err, "qmoe_paged_evict")
         self._on(stream, call)
 
     def compact(self, stream=None):
         """moves the used pages to the front of the pool; returns their number, an int32 [1] on the device"""
-        err = QmoeErr()
+        err = _paged_err
 
         def call(st):
             used, ws = self._status(), self._work(PAGED_COMPACT)
-            _check(lib().qmoe_paged_compact(self._cp, used.data_ptr(), ws.data_ptr(), ws.numel(), st, ctypes.byref(err)), err,
+            _check(lib().qmoe_paged_compact(self._cp, used.data_ptr(), ws.data_ptr(), ws.numel(), st, err.p), err.err,
                    "qmoe_paged_compact")
             return used
         return self._on(stream, call)

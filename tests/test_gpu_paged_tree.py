@@ -701,6 +701,18 @@ def test_keep_some_slots(dev, dtype):
     x.check([180, 210], [list(range(0, 180, 2)), list(range(5, 205))])
 
 
+@DTYPES
+def test_keep_of_small_batches(dev, dtype):
+    """one workgroup's and two launches' sizes: sequences, rows and layers around the limits"""
+    r = random.Random(37)
+    for n, rows, layers, page in ((1, 3, 1, 16), (3, 40, 2, 5), (16, 64, 1, 16), (16, 65, 1, 16), (17, 5, 1, 8), (2, 512, 4, 32), (16, 4, 9, 4)):
+        counts = [r.randint(1, rows) for _ in range(n - 1)] + [rows]
+        x = Kept(dev, dtype, page, [c + r.randrange(40) for c in counts], layers=layers, seed=n)
+        slots = r.sample(range(n), n)
+        counts = [counts[sl] for sl in slots]
+        x.check(counts, [sorted(r.sample(range(c), r.randint(0, c))) for c in counts], slots=slots)
+
+
 def test_keep_of_many_sequences(dev):
     r = random.Random(34)
     counts = [r.randrange(0, 6) for _ in range(1024)]
