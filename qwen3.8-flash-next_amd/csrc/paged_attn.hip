@@ -813,9 +813,13 @@ __device__ __forceinline__ void pa_store(const PaArgs &p, const PaUnit &u, const
  * once or fewer, the shortest length at which every task, cut into parts of
  * that length or less, still gets a unit for each of them.  Parts of about the
  * mean length, as in pa_find, are up to half longer and leave units without
- * work: 16 nodes of 64 sequences of 4000 rows 93 us, so 75; up to 16 of 64 of
- * 64 to 32768 105, so 85 (of each layer).  Parts are not made for less than
- * PA_JOIN tiles that they save. */
+ * work: 16 nodes of 64 sequences of 4000 rows 93 us, so 79; up to 16 of 64 of
+ * 64 to 32768 104, so 85 (two groups of four waves a CU both; one workgroup of
+ * two groups 100 and 120).  Parts are not made for less than PA_JOIN tiles that
+ * they save (two parts of 9 tiles for 256 tasks of 17: 63 us, whole 56).  Equal
+ * runs over all tasks' tiles, several tasks a unit, leave no unit without work,
+ * but their loop took the registers of the tiles' (256 nodes of 2 sequences of
+ * 16000 131 us, so 107). */
 #define PA_JOIN 10
 
 struct PaNeed {
@@ -1653,22 +1657,26 @@ static int pa_rows(const pg_cache *c, const pg_attn *a) {
     if (later == 32) most /= 2;
     return units <= 8 || units * keys <= most ? 16 : later;
 }
-/* The same for trees, whose units of PM_RT rows start sooner and are cut by
- * their longest part: they take over at a quarter of the limits (64 nodes of a
- * sequence of 4000 rows 33 us with 16 rows and 25, 32 of 8 sequences at head
- * dim 256 58 and 43, f32 16 of one of 8000 41 and 35; 32 of 4 of 1000 rows 23
- * and 25), and, where there is one for every fourth CU, from units of 32 rows
- * of bf16 (4 nodes of 64 sequences of 4000 rows 72 and 64, of 32 47 and 41; of
- * 16 33 and 38; f32 163 and 187). */
-static int pa_tree_rows_long(const pg_cache *c, int64_t rows, int n_seqs) {
-    const int rt = pa_rows_long(c, rows, n_seqs);
-    return rt == 16 && rows <= (int64_t)16 * n_seqs ? 16 : c->dtype == QMOE_BF16 && (int64_t)n_seqs * c->kvh >= 64 ? PM_RT : rt;
+/* The same for trees, whose units of PM_RT rows start sooner and are joined
+ * sooner: those of bf16 take over wherever the table's keys (or the window's)
+ * are enough to be cut (with fewer rows, and with more: 8 nodes of a sequence
+ * of 300 rows 13.6 us and 17.8, of 1000 17.8 and 14.9, of 32000 38 and 26; 4 of
+ * 16 of 4000 33 and 26; one of 64 of 6000 89 and 84), past head dim 128 from 17
+ * rows of a sequence on (24 of 16 of 4000 at 256 41 and 39, at 192 41 and 35; 8
+ * of 64 73 and 91).  With fewer keys, and in f32, they come after units of 16
+ * or 32 rows, in f32 at a quarter of a prompt's limit (16 nodes of a sequence of
+ * 8000 41 and 35, 4 of 64 of 2000 94 and 104). */
+#define PA_TREE_KEYS ((PA_JOIN + 1) * 64)
+static bool pa_tree_many(const pg_cache *c, int64_t rows, int n_seqs) {
+    return c->dtype == QMOE_BF16 && (c->hd <= 128 || rows > (int64_t)16 * n_seqs);
 }
 static int pa_tree_rows(const pg_cache *c, const pg_attn *a) {
     const int64_t rows = (int64_t)a->n * (a->h / c->kvh), units = rows * c->kvh / 16;
-    int64_t keys = c->cap, most = c->dtype == QMOE_BF16 || c->hd == 64 ? 1 << 16 : c->hd < 256 ? 1 << 15 : 1 << 17;
+    int64_t keys = c->cap;
     if (a->window > 0 && (int64_t)a->window + a->sinks < keys) keys = (int64_t)a->window + a->sinks;
-    const int later = pa_tree_rows_long(c, rows, a->n_seqs);
+    int64_t most = c->dtype == QMOE_BF16 ? 1 << 18 : c->hd == 64 ? 1 << 16 : c->hd < 256 ? 1 << 15 : 1 << 17;
+    if (keys >= PA_TREE_KEYS && pa_tree_many(c, rows, a->n_seqs)) return PM_RT;
+    const int later = pa_rows_long(c, rows, a->n_seqs);
     if (later == 32) most /= 2;
     return units <= 8 || units * keys <= most ? 16 : later;
 }
@@ -1769,7 +1777,8 @@ static size_t pa_tree_ws(const pg_cache *c, int n, int n_seqs, int h) {
     return rows * c->hd * 4 + rows * 8 + pa_up((size_t)q.joins * 32) + pa_up(index);
 }
 extern "C" size_t qk_pg_attn_tree_ws(const pg_cache *c, int n, int n_seqs, int h) {
-    const int rt = pa_tree_rows_long(c, (int64_t)n * (h / c->kvh), n_seqs);
+    const int64_t rows = (int64_t)n * (h / c->kvh);
+    const int rt = pa_tree_many(c, rows, n_seqs) ? PM_RT : pa_rows_long(c, rows, n_seqs);
     const int64_t grid = rt == PM_RT ? 2 * pa_tree_plan(c, n, n_seqs, h).grid : pa_plan_of(c, n, n_seqs, h, rt).grid;
     if (grid * 256 > 0xFFFFFFFFll) return 0;
     const size_t a = pa_ws(c, n, n_seqs, h, 16), b = rt == PM_RT ? pa_tree_ws(c, n, n_seqs, h) : pa_ws(c, n, n_seqs, h, rt);
