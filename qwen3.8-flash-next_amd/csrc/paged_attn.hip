@@ -476,6 +476,21 @@ __device__ __forceinline__ qm_bf16x8 pa_pack(const qm_f32x16 &st, int s, float &
     return __builtin_bit_cast(qm_bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
 }
 
+/* the same in two bf16 parts, 16 bits; l takes the sum of the weights themselves */
+__device__ __forceinline__ void pa_pack2(const qm_f32x16 &st, int s, float &l, qm_bf16x8 &w, qm_bf16x8 &rest) {
+    uint32_t a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float x = st[8 * s + 2 * i], y = st[8 * s + 2 * i + 1];
+        a[i] = qk_cvt_pk_bf16(x, y);
+        b[i] = qk_cvt_pk_bf16(x - qk_bf16_lo(a[i]), y - qk_bf16_hi(a[i]));
+        l += x;
+        l += y;
+    }
+    w = __builtin_bit_cast(qm_bf16x8, make_uint4(a[0], a[1], a[2], a[3]));
+    rest = __builtin_bit_cast(qm_bf16x8, make_uint4(b[0], b[1], b[2], b[3]));
+}
+
 /* Where piece pc (16 bytes) of row rr of a tile lies in LDS: the pieces of a
  * row are exchanged by an xor, so that the 16 rows of K that a quarter of a
  * wave reads at once lie on all 64 banks (rows of 128 and 384 bytes start on
@@ -1069,7 +1084,7 @@ __device__ __forceinline__ bool pa_merge(qm_f32x16 (&o)[E], float &m, float &l, 
     return group == 0;
 }
 
-template <int HD, int NG, bool TREE>
+template <int HD, int NG, bool TREE, bool FINE>
 __global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
     typedef uint16_t T;
     constexpr int KT = pm_kt(HD), CR = HD / 8, NB = KT * CR / 256, NS = KT / 32, E = HD / 32, KS = HD / 16;
@@ -1205,7 +1220,9 @@ __global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
         for (int n = 0; n < NS; n++)
 #pragma unroll
             for (int s = 0; s < 2; s++) {
-                const qm_bf16x8 pw = pa_pack(st[n], s, l);
+                qm_bf16x8 pw, rest;
+                if constexpr (FINE) pa_pack2(st[n], s, l, pw, rest);
+                else pw = pa_pack(st[n], s, l);
                 const int key = 32 * n + 16 * s + 4 * h + (j >> 2);
 #pragma unroll
                 for (int d = 0; d < E; d++) {
@@ -1213,7 +1230,9 @@ __global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
                     const pa_s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_tptr)((const short *)(vb + key * CR + pc) + 4 * (j & 1)));
                     const pa_s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_tptr)((const short *)(vb + (key + 8) * CR + pc) + 4 * (j & 1)));
                     const uint2 aw = __builtin_bit_cast(uint2, a), bw = __builtin_bit_cast(uint2, b);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(qm_bf16x8, make_uint4(aw.x, aw.y, bw.x, bw.y)), pw, o[d], 0, 0, 0);
+                    const qm_bf16x8 vt = __builtin_bit_cast(qm_bf16x8, make_uint4(aw.x, aw.y, bw.x, bw.y));
+                    if constexpr (FINE) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, rest, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, pw, o[d], 0, 0, 0);
                 }
             }
     }
@@ -1791,6 +1810,15 @@ static unsigned pa_tree_join_rows(int joins) {
     return (unsigned)(r < 4 ? 4 : r > PM_RT ? PM_RT : r);
 }
 
+/* Trees of up to PM_RT rows a sequence take the softmax weights in two bf16
+ * parts, as single tokens do: the pages' loads hide most of the second product
+ * (4 nodes of 64 sequences of 4000 rows 64 us with one part and 67, 16 nodes 79
+ * and 85, 16 of 64 to 32768 85 and 96 a layer).  Larger ones are bound by the
+ * products (256 nodes of 8 sequences 360 and 463) and take them as prompts do. */
+static bool pa_tree_fine(const pg_cache *c, const pg_attn *a) {
+    return (int64_t)a->n * (a->h / c->kvh) <= (int64_t)PM_RT * a->n_seqs;
+}
+
 template <typename T, int HD, int KT>
 static int pa_launch_tree(PaArgs p, void (*kernel)(PaArgs), int threads, void *ws, hipStream_t st) {
     const PaTreePlan q = pa_tree_plan(&p.c, p.a.n, p.a.n_seqs, p.a.h);
@@ -1819,14 +1847,14 @@ static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
     if (TREE && rt == PM_RT) {
         if constexpr (sizeof(T) == 2) {
             constexpr int NG = HD <= 128 ? 1 : 2; /* pa_tree_groups */
-            return pa_launch_tree<T, HD, pm_kt(HD)>(p, k_pa_many<HD, NG, true>, 256 * NG, ws, st);
+            return pa_launch_tree<T, HD, pm_kt(HD)>(p, pa_tree_fine(&p.c, &p.a) ? k_pa_many<HD, NG, true, true> : k_pa_many<HD, NG, true, false>, 256 * NG, ws, st);
         } else return pa_launch_tree<T, HD, pm_kt(HD, true)>(p, k_pa_many32<HD, true>, 256 * pm_halves32(HD), ws, st);
     }
     if (rt == PM_RT) {
         if constexpr (sizeof(T) == 2) {
             if constexpr (HD <= 128)
-                if (pa_groups(&p.c, p.a.n, p.a.h) == 1) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 1, false>, ws, st);
-            return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 2, false>, ws, st);
+                if (pa_groups(&p.c, p.a.n, p.a.h) == 1) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 1, false, false>, ws, st);
+            return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 2, false, false>, ws, st);
         } else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD, false>, ws, st);
     }
     if constexpr (HD <= (sizeof(T) == 2 ? 192 : 128)) /* pa_two */

@@ -358,6 +358,28 @@ def test_released_pages_and_shared_slots(dev, dtype):
     run_trees(t, [grow(r, 5), grow(r, 12), grow(r, 5)], slots=[1, 0, 1], scale=-0.7)
 
 
+@pytest.mark.usefixtures("tables")
+@pytest.mark.parametrize("hd", [64, 128, 192, 256])
+def test_weights_of_small_trees_have_16_bits(dev, hd):
+    """up to 128 rows a sequence: bf16 outputs within the weights' 16 bits (2^-16 of A twice: a half step of the second
+    part, and of the sum that leaves it out) and their own rounding, far below one bf16 part's 2^-8"""
+    r = random.Random(hd)
+    lens, counts = [2000, 1500, 900], [16, 5, 11]
+    s = Setup(dev, (8, 1, hd), torch.bfloat16, 16, lens, seed=hd)
+    ups = [grow(r, c) for c in counts]
+    q, starts = s.queries(counts)
+    tree = s.cache.tree(i32([p for u in ups for p in u], dev), i32(starts, dev))
+    out = s.cache.attend_tree(0, q.to(dev), tree).double().cpu()
+    for i, up in enumerate(ups):
+        see = sight(lens[i] - counts[i], *plan(up), 0, 0)
+        want, A, B = masked(q[starts[i]:starts[i + 1]], s.hk[i], s.hv[i], see, False)
+        T = lens[i]
+        tol = A * (2 * (hd + 24) * U * (B + 1) + 2 * (T + 64) * U + 2 * 2.0 ** -16)
+        tol = tol + (want.abs() + tol) * 2.0 ** -8
+        err = (out[starts[i]:starts[i + 1]] - want).abs()
+        assert (err <= tol).all(), (i, float((err / tol).max()))
+
+
 @DTYPES
 def test_strides_and_repeats(dev, dtype):
     s = Setup(dev, HEADS[0], dtype, 16, [100, 33, 2000], seed=16, order="heads")
