@@ -872,7 +872,8 @@ int qmoe_paged_append_rotary(const qmoe_paged_cache *c, int layer, const qmoe_pa
  * its parent.  rows [n]: the path's rows at the first places of their
  * sequence, -1 after them; counts [n_seqs]: their number (0 for a sequence
  * without rows); next [n_seqs]: what was chosen after the last one, -1 for
- * none.  parents and t as qmoe_paged_tree_build's. */
+ * none.  parents and t as qmoe_paged_tree_build's; rows of no sequence are left
+ * alone. */
 int qmoe_paged_follow(const qmoe_paged_tree *t, const int32_t *parents, const int32_t *tokens, const int32_t *chosen,
                       const int32_t *starts, int n, int n_seqs, int32_t *rows, int32_t *counts, int32_t *next,
                       void *stream, qmoe_err *err);

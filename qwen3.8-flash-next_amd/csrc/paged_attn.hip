@@ -39,6 +39,8 @@ struct PaArgs {
     int4 *split;  /* [joins, 2], trees on units of PM_RT rows: of a task that is cut, rows (0: none), start, row tile,
                    * kv head; first slot, parts */
     int joins;
+    int twice;    /* the call may be cut into twice as many units (pa_length) */
+    int tasks;    /* at the most, of starts that ascend */
 };
 
 /* query head of member g of kv head kh's group: heads kh, kh + kvh, ... (the
@@ -856,20 +858,43 @@ __device__ __forceinline__ int pa_cuts(int len, int most) { return (int)(((uint3
  * (fp32, the same in every wave; its rounding is far below the factor's);
  * units_at(length) sums over the sequences.  More tasks than units: parts of
  * the units' mean, so that fewer tasks than units are cut, and at most twice
- * as many units belong to such. */
+ * as many units belong to such.  Where the tasks' lengths are far from a fit,
+ * twice as many units, of which the second half starts as the first ends: they
+ * take about the mean and a third of a part, PA_TWICE tiles in joins and
+ * starts, and the first choice its longest part (less where there is one to a
+ * CU): 700 nodes of 3 sequences of 20000 rows, 264 tasks, 692 us and 513, 256
+ * of 8 of 8000 to 24000 364 and 349, but 500 of 4 of 12000 280 and 296. */
+#define PA_TWICE 4
 template <typename F>
-__device__ __forceinline__ int pa_length(int tasks, int longest, float total, int units, F units_at) {
-    int lo = (int)(1.0001f * total / (float)units) + 1;
-    if (tasks <= units && lo < longest) {
-        int hi = min(longest, (int)(total / (float)(units - tasks + 1)) + 2);
-        if (units_at(hi) > units) hi = longest; /* of a rounded total */
+__device__ __forceinline__ int pa_length(const PaArgs &p, int tasks, int longest, float total, F units_at) {
+    const int units = p.units;
+    /* starts in no order, whose sequences have more rows than the call: slots and records are for
+     * those of the call, so nothing is cut (nor all of it computed) */
+    if (tasks > p.tasks) return max(longest, 1);
+    auto fit = [&](int most) {
+        int lo = (int)(1.0001f * total / (float)most) + 1;
+        if (lo >= longest) return lo;
+        int hi = min(longest, (int)(total / (float)(most - tasks + 1)) + 2);
+        if (units_at(hi) > most) hi = longest; /* of a rounded total */
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (units_at(mid) <= units) hi = mid;
+            if (units_at(mid) <= most) hi = mid;
             else lo = mid + 1;
         }
+        return lo;
+    };
+    const float mean = total / (float)units;
+    if (tasks > units) {
+        const int lo = (int)(1.0001f * mean) + 1;
+        return longest - lo < PA_JOIN ? max(longest, 1) : lo;
     }
-    return longest - lo < PA_JOIN ? max(longest, 1) : lo;
+    int most = fit(units);
+    if (p.twice && (float)most > mean + 3 * PA_TWICE) {
+        const int half = fit(2 * units);
+        const float alone = units_at(most) <= units / 2 + units / 16 ? 0.86f : 1.0f;
+        if (mean + (float)half / 3.0f + PA_TWICE < alone * (float)most) most = half;
+    }
+    return longest - most < PA_JOIN ? max(longest, 1) : most;
 }
 __device__ __forceinline__ int pa_sum(int v) { return __builtin_amdgcn_readlane(pa_scan(v), 63); }
 __device__ __forceinline__ int pa_most(int v) { return (int)qk_wave_max_u32((uint32_t)v); }
@@ -880,7 +905,7 @@ __device__ __forceinline__ int pa_most(int v) { return (int)qk_wave_max_u32((uin
 template <int KT>
 __global__ __launch_bounds__(1024) void k_pa_tree_index(PaArgs p) {
     __shared__ int part[4][16];
-    __shared__ float sums[16];
+    __shared__ float sums[2][16];
     const int tid = threadIdx.x, wave = tid >> 6, n = p.a.n_seqs, per = (n + 1023) >> 10;
     const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
     auto over = [&](int v, int k) { /* the workgroup's sum */
@@ -893,27 +918,32 @@ __global__ __launch_bounds__(1024) void k_pa_tree_index(PaArgs p) {
         return t;
     };
     int tasks = 0, longest = 0;
-    float total = 0.0f;
+    float total = 0.0f, rough = 0.0f; /* rough: the tasks of starts in no order may pass 32 bits */
     PaNeed last = {{-1, 0, 0, 0}, 0, 1};
     for (int i = i0; i < i1; i++) {
         last = pa_need<KT>(p, i);
         tasks += last.rows * p.c.kvh;
+        rough += (float)(last.rows * p.c.kvh);
         longest = max(longest, last.rows ? last.len : 0);
         total += (float)(last.rows * p.c.kvh) * (float)last.len;
     }
     total = qk_group_sum<64>(total);
+    rough = qk_group_sum<64>(rough);
     longest = pa_most(longest);
     if ((tid & 63) == 0) {
-        sums[wave] = total;
+        sums[0][wave] = total;
+        sums[1][wave] = rough;
         part[1][wave] = longest;
     }
     tasks = over(tasks, 0);
-    total = 0.0f;
+    total = rough = 0.0f;
     for (int w = 0; w < 16; w++) {
-        total += sums[w];
+        total += sums[0][w];
+        rough += sums[1][w];
         longest = max(longest, part[1][w]);
     }
-    const int most = pa_length(tasks, longest, total, p.units, [&](int length) {
+    if (rough > 1.01f * (float)p.tasks + 1.0f) tasks = 0x7FFFFFFF;
+    const int most = pa_length(p, tasks, longest, total, [&](int length) {
         int v = 0;
         for (int i = i0; i < i1; i++) {
             const PaNeed q = per == 1 ? last : pa_need<KT>(p, i);
@@ -964,7 +994,7 @@ __device__ __forceinline__ bool pa_tree_find(const PaArgs &p, PaUnit &u) {
         if (lane < n) q = pa_need<KT>(p, lane);
         const int mine = q.rows * p.c.kvh;
         const float total = qk_group_sum<64>((float)mine * (float)q.len);
-        const int most = pa_length(pa_sum(mine), pa_most(q.rows ? q.len : 0), total, p.units,
+        const int most = pa_length(p, pa_sum(mine), pa_most(q.rows ? q.len : 0), total,
                                    [&](int length) { return pa_sum(mine * pa_cuts(q.len, length)); });
         const int parts = pa_cuts(q.len, most), units = mine * parts, ue = pa_scan(units);
         const int cut = parts > 1 ? mine : 0, se = pa_scan(cut * parts), te = pa_scan(cut);
@@ -1005,7 +1035,9 @@ __device__ __forceinline__ bool pa_tree_find(const PaArgs &p, PaUnit &u) {
     }
     if (threadIdx.x == 0 && want < p.joins && (refused || want >= tasks))
         qk_st((float4 *)(p.split + 2 * want), make_float4(0.0f, 0.0f, 0.0f, 0.0f));
-    if (!is || refused) return false;
+    /* past the sequence's units: an index of sums that passed 32 bits */
+    const int rtiles = (u.s.count * p.G + PM_RT - 1) / PM_RT;
+    if (!is || refused || (uint32_t)want - (uint32_t)ubase >= (uint32_t)(rtiles * p.c.kvh * u.parts)) return false;
     /* row tile, part, kv head */
     const int q = (want - ubase) / p.c.kvh;
     u.kh = want - ubase - q * p.c.kvh;
@@ -1775,8 +1807,8 @@ static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), void *ws, hipStream_t 
  * where a unit is one group of four waves; the grid that holds the call's, the
  * slots of partial results and the tasks that may be cut. */
 struct PaTreePlan {
-    int units, slots, joins;
-    int64_t grid;
+    int units, slots, joins, twice;
+    int64_t tasks, grid;
 };
 static int pa_tree_groups(const pg_cache *c) { return c->dtype == QMOE_BF16 && c->hd <= 128 ? 1 : 2; }
 static PaTreePlan pa_tree_plan(const pg_cache *c, int n, int n_seqs, int h) {
@@ -1784,10 +1816,15 @@ static PaTreePlan pa_tree_plan(const pg_cache *c, int n, int n_seqs, int h) {
     q.units = pa_tree_groups(c) == 1 ? 512 : 256;
     const int64_t rows = (int64_t)n * (h / c->kvh), seqs = n_seqs < n ? n_seqs : n;
     const int64_t per_head = rows / PM_RT + seqs < rows ? rows / PM_RT + seqs : rows, tasks = per_head * c->kvh;
-    const bool cut = c->cap / pm_kt(c->hd, c->dtype == QMOE_F32) + 2 >= PA_JOIN + 1; /* the longest task may be cut at all */
-    q.grid = tasks <= q.units ? q.units : tasks + q.units;
-    q.slots = !cut ? 0 : (tasks <= q.units ? 1 : 2) * q.units;
-    q.joins = !cut ? 0 : (int)(tasks < q.units ? tasks : q.units);
+    const int64_t longest = c->cap / pm_kt(c->hd, c->dtype == QMOE_F32) + 2; /* tiles of a task */
+    const bool cut = longest >= PA_JOIN + 1, even = tasks <= q.units;
+    /* with 1024 units they may begin one after the other, 64 tiles each in the mean */
+    q.twice = even && q.units == 512 && tasks * longest >= 64 * q.units;
+    q.grid = even ? (q.twice ? 2 : 1) * q.units : tasks + q.units;
+    if (q.grid > tasks * longest) q.grid = tasks * longest;
+    q.tasks = tasks;
+    q.slots = !cut ? 0 : (even && !q.twice ? 1 : 2) * q.units;
+    q.joins = !cut ? 0 : (int)(even ? tasks : q.units);
     return q;
 }
 static size_t pa_tree_ws(const pg_cache *c, int n, int n_seqs, int h) {
@@ -1825,6 +1862,8 @@ static int pa_launch_tree(PaArgs p, void (*kernel)(PaArgs), int threads, void *w
     const size_t rows = (size_t)q.slots * PM_RT;
     p.units = q.units;
     p.joins = q.joins;
+    p.twice = q.twice;
+    p.tasks = (int)q.tasks;
     p.po = (float *)ws;
     p.pml = (float2 *)(p.po + rows * HD);
     p.split = (int4 *)(p.pml + rows);
@@ -1883,6 +1922,8 @@ extern "C" int qk_launch_pg_attn(const pg_cache *c, const pg_attn *a, void *ws, 
     p.index = NULL;
     p.split = NULL;
     p.joins = 0;
+    p.twice = 0;
+    p.tasks = 0;
     hipStream_t st = (hipStream_t)stream;
     if (a->depths) return c->dtype == QMOE_BF16 ? pa_launch_hd<uint16_t, true>(p, ws, st) : pa_launch_hd<float, true>(p, ws, st);
     return c->dtype == QMOE_BF16 ? pa_launch_hd<uint16_t, false>(p, ws, st) : pa_launch_hd<float, false>(p, ws, st);

@@ -1079,10 +1079,10 @@ class DraftTree:
         self.n, self.words, self.index = n, words, seen.get_device()
         at = seen.data_ptr()
         if depths is not None:
-            if seen.dim() != 2 or depths.dim() != 1 or seen.shape[0] != depths.shape[0] or seen.element_size() != 4 or \
-                    depths.element_size() != 4 or not seen.is_contiguous() or not depths.is_contiguous() or \
-                    depths.get_device() != self.index:
-                raise QmoeError("depths [n] and seen [n, words] must be contiguous, of 32 bits and on one device")
+            if seen.dim() != 2 or depths.dim() != 1 or seen.shape[0] != depths.shape[0] or not seen.is_contiguous() or \
+                    not depths.is_contiguous() or depths.get_device() != self.index or \
+                    {str(seen.dtype), str(depths.dtype)} - {"torch.int32", "torch.uint32"}:
+                raise QmoeError("depths [n] and seen [n, words] must be contiguous int32 on one device")
             self.n, self.words = seen.shape
         self._p = _TREE.pack(at if depths is None else depths.data_ptr(), at + 4 * self.n if depths is None else at, self.words)
 

@@ -204,6 +204,15 @@ def test_longer_trees(dev, lens, counts, dtype):
     run_trees(s, ups, window=300, sinks=2)
 
 
+@pytest.mark.usefixtures("tables")
+@pytest.mark.parametrize("lens,counts", [([6500] * 9, [1024] * 9), ([4000, 900, 12000, 300], [1000, 800, 1024, 256])], ids=["even", "uneven"])
+def test_more_units_than_run_at_once(dev, lens, counts):
+    """tasks that do not fit the card's units: parts in two turns, where the table is long enough for them"""
+    r = random.Random(50)
+    s = Setup(dev, HEADS[2], torch.bfloat16, 16, lens, seed=51)
+    run_trees(s, [grow(r, c) for c in counts])
+
+
 @DTYPES
 @pytest.mark.parametrize("shape", [(16, 2, 128), (4, 1, 256), (6, 2, 192), (8, 2, 64), (40, 1, 128)], ids=str)
 def test_trees_of_many_sequences(dev, shape, dtype):
@@ -333,6 +342,32 @@ def test_more_drafts_than_rows_and_bad_lengths(dev, dtype):
     guard.fill_(7)
     s.cache.attend_tree(0, q.to(dev), tree, out=guard[1:13], status=i32([4], dev))
     assert (guard == 7).all()
+
+
+@pytest.mark.usefixtures("tables")
+@DTYPES
+@pytest.mark.parametrize("n", [90, 400])
+def test_starts_in_no_order_stay_inside(dev, n, dtype):
+    """sequences that have more rows together than the call: nothing outside it is touched, by any of the calls"""
+    s = Setup(dev, HEADS[0], dtype, 16, [900] * 100, seed=19)
+    starts = i32([0 if i % 2 else n for i in range(99)] + [0, n], dev)
+    q = torch.randn(n, s.h, s.hd, generator=s.g).to(dtype).to(dev)
+    parents = i32([t - 1 if t % 7 else max(t - 2, -1) for t in range(n)], dev)
+    for st in (starts, starts.flip(0).contiguous(), starts[:40].contiguous()):
+        tree = s.cache.tree(parents, st)
+        guard = torch.full((n + 2, s.h, s.hd), 7.0, dtype=dtype, device=dev)
+        s.cache.attend_tree(0, q, tree, out=guard[1:n + 1])
+        assert (guard[0] == 7).all() and (guard[n + 1] == 7).all()
+        before = s.refs.clone(), s.full.clone(), s.len_t.clone()
+        rows, cnt, last = s.cache.follow(tree, torch.zeros_like(parents), torch.zeros_like(parents))
+        assert (cnt >= 0).all() and (cnt <= n).all()
+        assert int(s.cache.keep(rows, cnt, st)) == -1
+        for a, b in zip(before, (s.refs, s.full, s.len_t)):
+            assert torch.equal(a, b)
+    # the last sequence has rows 0 .. n in any case
+    kv = torch.randn(n, s.kvh, s.hd, generator=s.g).to(dtype).to(dev)
+    s.cache.append_rotary(0, kv, kv, starts, torch.rand(4, device=dev), q=q, tree=tree)
+    torch.cuda.synchronize()
 
 
 @pytest.mark.usefixtures("tables")

@@ -3,6 +3,7 @@ qmoe_paged_tree_build, _attn_tree, _append_rotary, _follow and _keep, which
 come back as -1 with a message before the device is touched (the pointers here
 are no memory at all)."""
 import ctypes
+import sys
 
 import pytest
 
@@ -166,3 +167,27 @@ def test_calls_with_nothing_to_do_touch_nothing():
         assert x.rotary() == 0 and x.attn(ws=None, size=0) == 0
         assert x.build(**kw) == 0
     assert Calls(pkg).follow(n_seqs=0) == 0
+
+
+def test_packed_structs_are_the_header_s():
+    """a call's structs as the binding packs them, field by field against the ctypes ones"""
+    pkg = load_pkg()
+    q = sys.modules["qmoe_amd.qmoe"]
+    for packed, cls, values in (
+            (q._BATCH, pkg.QmoePagedBatch, (1, 2, 3, 4, 5)),
+            (q._QUERY, pkg.QmoePagedQuery, (1, 2, 3, 4, 5, 6, 7, 8, 9, 1, 0.5)),
+            (q._ROTARY, pkg.QmoePagedRotary, tuple(range(1, 13)) + (13, 14, 15, 16, 1, 18, 19, 0.25)),
+            (q._TREE, pkg.QmoePagedTree, (1, 2, 3))):
+        raw = packed.pack(*values).ljust(ctypes.sizeof(cls), b"\0")
+        got = cls.from_buffer_copy(raw)
+        assert tuple(getattr(got, f) for f, _ in cls._fields_) == values
+
+
+def test_trees_of_other_tensors_are_refused():
+    import torch
+    pkg = load_pkg()
+    d, s = torch.zeros(5, dtype=torch.int32), torch.zeros(5, 2, dtype=torch.int32)
+    pkg.DraftTree(None, None, d, s)
+    for bad in ((d.float(), s), (d, s.float()), (d.long(), s), (d[:4], s), (d, s[0]), (d, s.t().contiguous().t()), (d[::2], s[::2])):
+        with pytest.raises(pkg.QmoeError, match="depths"):
+            pkg.DraftTree(None, None, *bad)
