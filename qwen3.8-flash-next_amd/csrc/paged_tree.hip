@@ -12,12 +12,18 @@
 #include "paged_parts.h"
 
 /* ------------------------------------------------------------ rotation
- * A workgroup per new row: cos and sin of its rot / 2 angles once, then its
- * heads of q, k and v, 8 elements a lane.  A head of q or k is normed first
- * where a weight is given: y = x / sqrt(mean x^2 + eps) * w, the sum in fp32
- * over the head's lanes.  Pairs (a, b) become (a cos - b sin, a sin + b cos);
- * in halves (i, i + rot / 2) a lane's partners lie with others and come
- * through LDS. */
+ * A workgroup per new row (of four in long calls): cos and sin of its rot / 2
+ * angles once, then its heads of q, k and v, 8 elements a lane.  A head of q or
+ * k is normed first where a weight is given: y = x / sqrt(mean x^2 + eps) * w,
+ * the sum in fp32 over the head's lanes.  Pairs (a, b) become (a cos - b sin, a
+ * sin + b cos); in halves (i, i + rot / 2) a lane's partners lie with others
+ * and come through LDS.  The heads' loads need no position and go out first;
+ * the sequence is found by a wave, 64 starts at a time.
+ * Bound: latency in short calls, 4.2 us for a row, 6.9 for 900 drafts of 64
+ * sequences (14 MB; of a wave of 256 threads for every row 5.0 and 7.4, found
+ * after the heads' loads by a search of one start at a time 5.8 and 9.6); HBM
+ * in long ones, prompts of 266 MB read and written 52 us, 5.1 TB/s (a row a
+ * workgroup 57), as much as a copy. */
 struct PgRotary {
     pg_cache c;
     const void *q, *k, *v;
@@ -29,7 +35,7 @@ struct PgRotary {
     int n, n_seqs, h, half, inter; /* half = rot / 2 */
     pg_div per_row;      /* heads of q, k and v of a token */
 };
-#define PG_ROTARY_MANY 2048
+#define PG_ROTARY_MANY 2048 /* rows from which a workgroup has four: as many as the card holds workgroups */
 
 /* cos and sin of position * freq, whose fp32 value is off by a radian at far
  * positions: x = position * freq in 64 bits (exact up to position 2^29: 29 and
@@ -97,15 +103,18 @@ __device__ __forceinline__ int pg_find_wave(const int32_t *starts, int n_seqs, i
     }
 }
 
+/* lanes of a head; of 192, 24 of them hold elements */
+constexpr int pg_head_lanes(int hd) { return hd <= 64 ? 8 : hd <= 128 ? 16 : 32; }
+
 template <typename S, typename D, int HD, int TOK>
-__global__ __launch_bounds__(256) void k_pg_rotary(PgRotary a) {
-    constexpr int LP = HD <= 64 ? 8 : HD <= 128 ? 16 : 32; /* lanes of a head; of 192, 24 of them hold elements */
-    constexpr int RP = 256 / LP;
+__global__ __launch_bounds__(512) void k_pg_rotary(PgRotary a) {
+    constexpr int LP = pg_head_lanes(HD);
+    const int threads = blockDim.x, RP = threads / LP;
     struct Row {
         int64_t at;   /* of its place in the pages, or -1 */
         int pos;      /* -1: nothing of it is written */
     };
-    __shared__ __attribute__((aligned(16))) float cs[TOK][HD / 2], sn[TOK][HD / 2], buf[RP][HD + 4];
+    __shared__ __attribute__((aligned(16))) float cs[TOK][HD / 2], sn[TOK][HD / 2], buf[512 / LP][HD + 4];
     __shared__ Row rows[TOK];
     const int tid = threadIdx.x, wave = tid >> 6, slot = tid / LP, e0 = 8 * (tid % LP), rot = 2 * a.half;
     const bool on = HD != 192 || e0 < HD;
@@ -134,7 +143,7 @@ __global__ __launch_bounds__(256) void k_pg_rotary(PgRotary a) {
     load(slot, next);
     const float freq = qk_ld(a.freqs + (tid < TOK * a.half ? tid % a.half : 0));
     const int refused = a.status ? qk_ld(a.status) : 0;
-    for (int k = wave; k < TOK; k += 4) {
+    for (int k = wave; k < TOK; k += threads >> 6) {
         const int t = t0 + k, s = t < a.n ? pg_find_wave(a.starts, a.n_seqs, t) : a.n_seqs;
         Row w = {-1, -1};
         if (s < a.n_seqs && !refused) {
@@ -149,7 +158,7 @@ __global__ __launch_bounds__(256) void k_pg_rotary(PgRotary a) {
         if ((tid & 63) == 0) rows[k] = w;
     }
     __syncthreads();
-    for (int i = tid; i < TOK * a.half; i += 256) {
+    for (int i = tid; i < TOK * a.half; i += threads) {
         const int k = i / a.half, f = i - k * a.half;
         const float2 c = pg_turn(max(rows[k].pos, 0), i == tid ? freq : qk_ld(a.freqs + f));
         cs[k][f] = c.x;
@@ -229,7 +238,8 @@ __global__ __launch_bounds__(256) void k_pg_rotary(PgRotary a) {
 
 template <typename S, typename D, int TOK>
 static int pg_rotary_hd(const PgRotary &a, hipStream_t st) {
-    const dim3 grid((unsigned)(((int64_t)a.n + TOK - 1) / TOK)), wg(256);
+    const int64_t lanes = (int64_t)a.per_row.d * pg_head_lanes(a.c.hd); /* of a row: one round of them where 512 threads hold it */
+    const dim3 grid((unsigned)(((int64_t)a.n + TOK - 1) / TOK)), wg(TOK > 1 ? 256 : lanes >= 512 ? 512 : (unsigned)(lanes + 63) / 64 * 64);
     switch (a.c.hd) {
     case 64: hipLaunchKernelGGL((k_pg_rotary<S, D, 64, TOK>), grid, wg, 0, st, a); break;
     case 128: hipLaunchKernelGGL((k_pg_rotary<S, D, 128, TOK>), grid, wg, 0, st, a); break;
