@@ -10,6 +10,10 @@
  * unit of work is (sequence, row tile, part, kv head), numbered on the device
  * from the lengths it finds (pa_find), and a second launch joins the parts.
  *
+ * The rows of a call are in causal order or, TREE, the nodes of trees of
+ * drafted tokens: another mask on the same tiles (pa_row_mask), and other units
+ * of the many-row kernels (pa_tree_find).
+ *
  * Products are transposed: S^T = K Q^T leaves each lane the scores of one
  * row, for keys 8 a + 4 (lane / 32) + b of a tile of 32, and those registers
  * are the B operand of O^T = V^T P^T as they are, if V^T's operand takes its
@@ -1070,7 +1074,14 @@ __device__ __forceinline__ bool pa_tree_find(const PaArgs &p, PaUnit &u) {
  * waiting at the barrier 100 to 970; the matrix cores work 40 % of it.  Without gain: a
  * raised wave priority in either half, two groups half a step apart (360 us),
  * scores of the next tile beside the softmax (337 to 348), three groups (326),
- * units of 64 rows (short prompts 10 % better, long contexts 40 % worse). */
+ * units of 64 rows (short prompts 10 % better, long contexts 40 % worse).
+ * Trees of drafted tokens have few rows, so their bound is HBM: up to 16 nodes
+ * of 64 sequences of 64 to 32768 rows (343 MB) 78 us, in two bf16 parts of the
+ * weights 87, of which 12 are the unit's start (its place 2.5, pages 2, first
+ * tile 3) and end; while tiles are read it is 6.5 TB/s.  256 nodes of 8
+ * sequences (251 GFLOP) 345 us, 730 TFLOP/s: parts of 118 to 150 tiles.  Without
+ * gain: waves past the last row that only copy (5 to 10 % slower: their copies
+ * go out at once). */
 #define PM_CHUNK 1024 /* keys of a look-up of two groups */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pa_s16x4 *pa_tptr;
@@ -1569,7 +1580,10 @@ __global__ __launch_bounds__(64 * W) void k_pa_join(PaArgs p) {
 /* The same of trees on units of PM_RT rows, whose units leave a record of every
  * task that is cut.  A row has HD / 4 lanes, which load up to PT_FEW parts at
  * once; of more parts the groups of the workgroup's lanes take runs of a row's,
- * which are added in their order. */
+ * which are added in their order.  Bound: latency of two loads in a row, then
+ * the parts read once (33 MB after 16 nodes of 64 sequences of 4000 rows 8.5 us,
+ * 15.2 where every workgroup searches its task; 64 parts of 8 tasks 7.5, 30
+ * with a row's parts in turn). */
 #define PT_FEW 8
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void k_pa_tree_join(PaArgs p) {

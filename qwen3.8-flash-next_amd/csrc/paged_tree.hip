@@ -278,7 +278,9 @@ extern "C" int qk_launch_pg_rotary(const pg_cache *c, const qmoe_paged_rotary *r
  * Depth and ancestors of every drafted row, a workgroup per sequence, a thread
  * per (row, word of 32 of its bits).  A thread walks from its row to the root;
  * a run of rows whose parents are the rows before them is one step, so a
- * chain, however long, is one. */
+ * chain, however long, is one.  Bound: latency, of the loads of starts and
+ * parents and of the walk in LDS: 1.8 us for 8 nodes, 3.1 to 5 for up to 24 of
+ * 64 sequences, 5.7 for 256 of 8. */
 #define PG_TREE_ROWS 1024
 
 struct PgTree {
@@ -344,7 +346,8 @@ extern "C" int qk_launch_pg_tree(const int32_t *parents, const int32_t *starts, 
  * is taken where its token is the one chosen after its parent and no lower
  * child of that parent has it too; a row is on the path where it and all its
  * ancestors are taken (row 0 always), so its place is its depth and no walk is
- * needed. */
+ * needed.  Bound: latency, 2.5 us for 12 nodes, 4.2 for up to 32 of 256
+ * sequences. */
 struct PgFollow {
     const int32_t *parents, *tokens, *chosen, *starts, *depths;
     const uint32_t *seen;
@@ -409,7 +412,8 @@ extern "C" int qk_launch_pg_follow(const int32_t *parents, const int32_t *tokens
  * of one workgroup.  Kept rows ascend, so row k goes to a place at or before
  * its own and behind those of the rows before it: a thread that moves its 16
  * bytes of every row of a sequence, in order, 8 loads before their stores,
- * never reads what it has written. */
+ * never reads what it has written.  Bound: latency, 4.8 and 5.6 us for 256
+ * sequences of 12 layers (about two rows of each move, 5.8 MB). */
 struct PgKeep {
     pg_cache c;
     const int32_t *starts, *slots, *status, *rows, *counts;
@@ -519,7 +523,7 @@ __global__ __launch_bounds__(256) void k_pg_keep_move(PgKeep a) {
 
 /* The same by one workgroup, a wave per sequence up to the moves.  Up to
  * PG_KEEP_SMALL pieces of all sequences' rows: one of one layer 4.9 us in two
- * launches, so 2.9. */
+ * launches, so 3.7; four of three 7.5 and 5.1. */
 #define PG_KEEP_SEQS 16
 #define PG_KEEP_ROWS 1024
 #define PG_KEEP_SMALL 4096

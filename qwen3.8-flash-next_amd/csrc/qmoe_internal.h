@@ -447,7 +447,7 @@ uint64_t qk_tensor_key(uint64_t seed, uint32_t layer, uint32_t tag);
 int qk_noalloc_scratch(void **ptr);
 
 /* ------------------------------------------------------------ paged cache
- * (paged_pages.hip, paged_attn.hip, qmoe_paged.c) */
+ * (paged_pages.hip, paged_attn.hip, paged_tree.hip, qmoe_paged.c) */
 
 /* division by a fixed d (paged_parts.h) */
 typedef struct {

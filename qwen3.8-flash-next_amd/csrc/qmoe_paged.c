@@ -1,6 +1,6 @@
 /*
  * qmoe_paged.c -- C11 host side of the paged cache: argument checks and the
- * launches of paged_pages.hip and paged_attn.hip.  Holds no state: the cache
+ * launches of paged_pages.hip, paged_attn.hip and paged_tree.hip.  Holds no state: the cache
  * and the workspaces are the caller's.
  */
 #include <limits.h>
