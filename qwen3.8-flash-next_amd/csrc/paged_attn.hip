@@ -1730,7 +1730,9 @@ static int pa_rows(const pg_cache *c, const pg_attn *a) {
  * rows of a sequence on (24 of 16 of 4000 at 256 41 and 39, at 192 41 and 35; 8
  * of 64 73 and 91).  With fewer keys, and in f32, they come after units of 16
  * or 32 rows, in f32 at a quarter of a prompt's limit (16 nodes of a sequence of
- * 8000 41 and 35, 4 of 64 of 2000 94 and 104). */
+ * 8000 41 and 35, 4 of 64 of 2000 94 and 104); at f32's head dim 256, whose many
+ * rows spill, later up to 256 rows a sequence (20 nodes of 16 of 2000 88 and
+ * 123, 60 of 4 of 3000 82 and 102, 150 of 4 of 2000 190 and 145). */
 #define PA_TREE_KEYS ((PA_JOIN + 1) * 64)
 static bool pa_tree_many(const pg_cache *c, int64_t rows, int n_seqs) {
     return c->dtype == QMOE_BF16 && (c->hd <= 128 || rows > (int64_t)16 * n_seqs);
@@ -1739,7 +1741,7 @@ static int pa_tree_rows(const pg_cache *c, const pg_attn *a) {
     const int64_t rows = (int64_t)a->n * (a->h / c->kvh), units = rows * c->kvh / 16;
     int64_t keys = c->cap;
     if (a->window > 0 && (int64_t)a->window + a->sinks < keys) keys = (int64_t)a->window + a->sinks;
-    int64_t most = c->dtype == QMOE_BF16 ? 1 << 18 : c->hd == 64 ? 1 << 16 : c->hd < 256 ? 1 << 15 : 1 << 17;
+    int64_t most = c->dtype == QMOE_BF16 ? 1 << 18 : c->hd == 64 ? 1 << 16 : c->hd < 256 ? 1 << 15 : rows <= (int64_t)256 * a->n_seqs ? 1 << 21 : 1 << 17;
     if (keys >= PA_TREE_KEYS && pa_tree_many(c, rows, a->n_seqs)) return PM_RT;
     const int later = pa_rows_long(c, rows, a->n_seqs);
     if (later == 32) most /= 2;
