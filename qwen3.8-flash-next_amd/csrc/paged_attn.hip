@@ -1726,16 +1726,18 @@ static int pa_rows(const pg_cache *c, const pg_attn *a) {
  * sooner: those of bf16 take over wherever the table's keys (or the window's)
  * are enough to be cut (with fewer rows, and with more: 8 nodes of a sequence
  * of 300 rows 13.6 us and 17.8, of 1000 17.8 and 14.9, of 32000 38 and 26; 4 of
- * 16 of 4000 33 and 26; one of 64 of 6000 89 and 84), past head dim 128 from 17
- * rows of a sequence on (24 of 16 of 4000 at 256 41 and 39, at 192 41 and 35; 8
- * of 64 73 and 91).  With fewer keys, and in f32, they come after units of 16
+ * 16 of 4000 33 and 26; one of 64 of 6000 89 and 84), at head dim 192 from 17
+ * rows of a sequence on (24 of 16 of 4000 41 and 38; 6 of 64 85 and 86), at 256
+ * from 33 rows and 40 units of 16 (32 of 48 of 2000 49 and 59, 64 of 16 of 4000
+ * 58 and 49; 96 of 4 of 3000 34 and 36).  With fewer keys, and in f32, they come after units of 16
  * or 32 rows, in f32 at a quarter of a prompt's limit (16 nodes of a sequence of
  * 8000 41 and 35, 4 of 64 of 2000 94 and 104); at f32's head dim 256, whose many
  * rows spill, later up to 256 rows a sequence (20 nodes of 16 of 2000 88 and
  * 123, 60 of 4 of 3000 82 and 102, 150 of 4 of 2000 190 and 145). */
 #define PA_TREE_KEYS ((PA_JOIN + 1) * 64)
 static bool pa_tree_many(const pg_cache *c, int64_t rows, int n_seqs) {
-    return c->dtype == QMOE_BF16 && (c->hd <= 128 || rows > (int64_t)16 * n_seqs);
+    if (c->dtype != QMOE_BF16) return false;
+    return c->hd <= 128 || (c->hd == 192 ? rows > (int64_t)16 * n_seqs : rows > (int64_t)32 * n_seqs && rows * c->kvh > 640);
 }
 static int pa_tree_rows(const pg_cache *c, const pg_attn *a) {
     const int64_t rows = (int64_t)a->n * (a->h / c->kvh), units = rows * c->kvh / 16;
