@@ -21,11 +21,9 @@
  */
 #include "qk_device.h"
 #include "mfma_parts.h"
-#include "paged_parts.h"
+#include "paged_plan.h"
 
 typedef float qm_f32x16 __attribute__((ext_vector_type(16)));
-
-#define PM_RT 128 /* rows of a unit of the many-row kernels */
 
 __device__ const uint4 pa_zero[64] = {}; /* a row of zeros, up to 1 KB */
 
@@ -133,9 +131,8 @@ __device__ __forceinline__ pg_seq pa_seq(const PaArgs &p, int i) { return pg_seq
  * of 1000 rows, 198 with the index; of 100 sequences of 200 rows 11.7 and
  * 13.0 (the launch), of 1000 rows 38 and 35.  So the two meet between 64 and some
  * hundred sequences, by their lengths, which the host does not know: the limit
- * is where a lane per sequence ends and the other way would need a loop.  The
- * total is summed in fp32, in a fixed order. */
-#define PA_INDEX 64
+ * (PA_INDEX) is where a lane per sequence ends and the other way would need a
+ * loop.  The total is summed in fp32, in a fixed order. */
 __global__ __launch_bounds__(1024) void k_pa_index(PaArgs p, int rt, int kt) {
     __shared__ float sum[16];
     __shared__ int before[16][3];
@@ -549,7 +546,6 @@ __device__ __forceinline__ bool pa_again(const V (&o)[N], float l, bool seen) {
  * sequences of 1000 rows 204 us, 5.2 TB/s, in f32 405; a kernel that only reads
  * reaches 5.9.  Short calls: latency, f32 under a window of 1024 of 32
  * sequences (68 MB) 25 us, a token on 333 rows 10, a prompt of 64 8. */
-#define PD_KT 32
 typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
 
 template <typename T, int HD, int NC>
@@ -841,7 +837,6 @@ __device__ __forceinline__ void pa_store(const PaArgs &p, const PaUnit &u, const
  * runs over all tasks' tiles, several tasks a unit, leave no unit without work,
  * but their loop took the registers of the tiles' (256 nodes of 2 sequences of
  * 16000 131 us, so 107). */
-#define PA_JOIN 10
 
 struct PaNeed {
     pg_seq s;
@@ -1085,9 +1080,6 @@ __device__ __forceinline__ bool pa_tree_find(const PaArgs &p, PaUnit &u) {
 #define PM_CHUNK 1024 /* keys of a look-up of two groups */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pa_s16x4 *pa_tptr;
-
-/* keys of a tile */
-constexpr int pm_kt(int hd, bool f32 = false) { return hd <= 128 && !f32 ? 64 : 32; }
 
 /* the rows' results of the other groups of four waves into the first one's,
  * through `ex` (HD / 8 pieces of 64 float4 per wave) and `ml`, in order; true
@@ -1338,9 +1330,6 @@ __device__ __forceinline__ qm_f32x16 pa_mfma6(const uint4 a[3], const uint4 b[3]
         c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(qm_bf16x8, a[ia[i]]), __builtin_bit_cast(qm_bf16x8, b[ib[i]]), c, 0, 0, 0);
     return c;
 }
-
-/* head dims past 128: four waves, whose registers and LDS are full */
-constexpr int pm_halves32(int hd) { return hd <= 128 ? 2 : 1; }
 
 template <int HD, bool TREE>
 __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p) {
@@ -1662,31 +1651,8 @@ __global__ __launch_bounds__(256) void k_pa_tree_join(PaArgs p) {
 
 /* ------------------------------------------------------------ host side */
 
-/* how a call is cut: units asked for, the grid that holds them whatever the
- * lengths, tasks that can need a join, and the slots of partial results */
-struct PaPlan {
-    int units, extra, one;
-    int64_t grid, join, slots;
-};
-
-static PaPlan pa_plan(const pg_cache *c, int n, int n_seqs, int h, int rt, int kt, int units, int extra, int one) {
-    PaPlan q;
-    const int G = h / c->kvh;
-    q.units = units;
-    q.extra = extra;
-    q.one = one;
-    /* sum of ceil(rows / rt) over the sequences that have rows */
-    const int64_t rows = (int64_t)n * G, seqs = n_seqs < n ? n_seqs : n;
-    const int64_t per_head = rows / rt + seqs < rows ? rows / rt + seqs : rows;
-    const int64_t tasks = per_head * c->kvh;
-    /* parts of the longest task, then the bounds that pg_share gives */
-    const int longest = c->cap / kt + 2;
-    const int64_t parts = pg_cuts(longest, extra) ? pg_parts(longest, one + 1) : 1, most = tasks * parts;
-    q.grid = most < 2 * (int64_t)units + tasks ? most : 2 * (int64_t)units + tasks;
-    q.slots = parts == 1 ? 0 : most < 3 * (int64_t)units ? most : 3 * (int64_t)units;
-    q.join = parts == 1 ? 0 : tasks < 3 * (int64_t)units / 2 ? tasks : 3 * (int64_t)units / 2; /* two parts at least */
-    return q;
-}
+extern "C" size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h) { return pa_ws(c, n, n_seqs, h, false); }
+extern "C" size_t qk_pg_attn_tree_ws(const pg_cache *c, int n, int n_seqs, int h) { return pa_ws(c, n, n_seqs, h, true); }
 
 /* workgroups that share a task's rows: about 2048 in all, where the tasks are
  * few every row has its own */
@@ -1695,103 +1661,14 @@ static unsigned pa_join_rows(int64_t tasks, int rt) {
     return (unsigned)(r < 1 ? 1 : r > rt ? rt : r);
 }
 
-/* Rows of a unit: 16 or 32 of the few-row kernel, or PM_RT of the many-row
- * one.  Units of 16 rows read a page once per 16 rows, but start at once and
- * have a short step: they are better as long as the call is short, measured by
- * their number times the rows of a table (or the window): 32 tokens on 1000
- * rows 27 us with 128 rows and 14.5 with 16, on 4000 rows of 4 sequences 30
- * and 39; f32 31 and 20, 52 and 73.  The limits are where the two meet, over 1
- * to 16 sequences, 1000 to 16000 rows and all head dims; f32 kernels past head
- * dim 128 lack registers for more rows (8 tokens of 16 sequences on 4000 rows
- * at 256: 151 and 71), and units of 32 rows take over at half the limit (4
- * tokens of 16 sequences on 4000 rows 29 and 34).  Up to 8 units are 16 rows
- * each whatever the table holds, which may be much more than the sequences
- * have (8 tokens on 1000 rows 23 and 15, on 16000 22 and 23).  Past the limit,
- * by the rows that a sequence has on average; 32 where the registers hold
- * them. */
-static bool pa_two(const pg_cache *c) { return c->dtype == QMOE_BF16 ? c->hd <= 192 : c->hd <= 128; }
-static int pa_rows_long(const pg_cache *c, int64_t rows, int n_seqs) {
-    if (rows <= (int64_t)16 * n_seqs) return 16;
-    return rows > (int64_t)32 * n_seqs ? PM_RT : pa_two(c) ? 32 : 16;
-}
-static int pa_rows(const pg_cache *c, const pg_attn *a) {
-    const int64_t rows = (int64_t)a->n * (a->h / c->kvh), units = rows * c->kvh / 16;
-    const int later = pa_rows_long(c, rows, a->n_seqs);
-    int64_t keys = c->cap, most = c->dtype == QMOE_BF16 || c->hd == 64 ? 1 << 18 : c->hd < 256 ? 1 << 17 : 1 << 19;
-    if (a->window > 0 && (int64_t)a->window + a->sinks < keys) keys = (int64_t)a->window + a->sinks;
-    if (later == 32) most /= 2;
-    return units <= 8 || units * keys <= most ? 16 : later;
-}
-/* The same for trees, whose units of PM_RT rows start sooner and are joined
- * sooner: those of bf16 take over wherever the table's keys (or the window's)
- * are enough to be cut (with fewer rows, and with more: 8 nodes of a sequence
- * of 300 rows 13.6 us and 17.8, of 1000 17.8 and 14.9, of 32000 38 and 26; 4 of
- * 16 of 4000 33 and 26; one of 64 of 6000 89 and 84), at head dim 192 from 17
- * rows of a sequence on (24 of 16 of 4000 41 and 38; 6 of 64 85 and 86), at 256
- * from 33 rows and 40 units of 16 (32 of 48 of 2000 49 and 59, 64 of 16 of 4000
- * 58 and 49; 96 of 4 of 3000 34 and 36).  With fewer keys, and in f32, they come
- * after units of 16 or 32 rows, in f32 at a quarter of a prompt's limit (16 nodes
- * of a sequence of 8000 41 and 35, 4 of 64 of 2000 94 and 104); at f32's head dim
- * 256, whose many rows spill, later up to 256 rows a sequence (20 nodes of 16 of
- * 2000 88 and 123, 60 of 4 of 3000 82 and 102, 150 of 4 of 2000 190 and 145). */
-#define PA_TREE_KEYS ((PA_JOIN + 1) * 64)
-static bool pa_tree_many(const pg_cache *c, int64_t rows, int n_seqs) {
-    if (c->dtype != QMOE_BF16) return false;
-    return c->hd <= 128 || (c->hd == 192 ? rows > (int64_t)16 * n_seqs : rows > (int64_t)32 * n_seqs && rows * c->kvh > 640);
-}
-static int pa_tree_rows(const pg_cache *c, const pg_attn *a) {
-    const int64_t rows = (int64_t)a->n * (a->h / c->kvh), units = rows * c->kvh / 16;
-    int64_t keys = c->cap;
-    if (a->window > 0 && (int64_t)a->window + a->sinks < keys) keys = (int64_t)a->window + a->sinks;
-    int64_t most = c->dtype == QMOE_BF16 ? 1 << 18 : c->hd == 64 ? 1 << 16 : c->hd < 256 ? 1 << 15 : rows <= (int64_t)256 * a->n_seqs ? 1 << 21 : 1 << 17;
-    if (keys >= PA_TREE_KEYS && pa_tree_many(c, rows, a->n_seqs)) return PM_RT;
-    const int later = pa_rows_long(c, rows, a->n_seqs);
-    if (later == 32) most /= 2;
-    return units <= 8 || units * keys <= most ? 16 : later;
-}
-/* Groups of four waves in a bf16 unit of the many-row kernel.  Two take the
- * unit's tiles in turn and halve its time; where there are units enough for
- * several rounds, two workgroups of one group per CU do better, since one
- * starts and ends under the other's products (two and one: a prompt of 1000 27
- * and 30 us, of 8192 320 and 308, of 16000 1249 and 1151, three of 4000 300 and
- * 264). */
-static int pa_groups(const pg_cache *c, int n, int h) {
-    return (int64_t)n * (h / c->kvh) / PM_RT * c->kvh >= 1000 && c->hd <= 128 ? 1 : 2;
-}
-static PaPlan pa_plan_of(const pg_cache *c, int n, int n_seqs, int h, int rt) {
-    /* A join costs about 12 bf16 tiles in time, or 2 f32 ones.  Where all units
-     * run at once it costs 3, since the others fill CUs that had nothing to do:
-     * 64 tokens on 3000 rows 40 us with 12, so 33, on 4000 rows in 16 sequences
-     * 81 and 70; but a prompt of 2000 (256 tasks) 46 with 12 and 59 with 3. */
-    if (rt == PM_RT && c->dtype == QMOE_BF16) return pa_plan(c, n, n_seqs, h, PM_RT, pm_kt(c->hd), 256, 12, 3);
-    if (rt == PM_RT) return pa_plan(c, n, n_seqs, h, PM_RT, pm_kt(c->hd, true), 256, 2, 2);
-    /* tables of up to 16 tiles (512 rows) are not cut: the join's launch costs
-     * more than the shorter run of tiles gives */
-    const int bytes = c->hd * (c->dtype == QMOE_BF16 ? 2 : 4) * (rt / 16); /* of a row's registers, as pd_occ */
-    const int wgs = bytes <= 128 ? 4 : bytes <= 256 ? 3 : bytes <= 512 ? 2 : 1; /* workgroups that a CU holds */
-    const int extra = c->cap <= 16 * PD_KT ? 17 : 2;
-    return pa_plan(c, n, n_seqs, h, rt, PD_KT, 256 * wgs, extra, extra);
-}
-
-static size_t pa_up(size_t v) { return (v + 255) / 256 * 256; }
-static size_t pa_ws(const pg_cache *c, int n, int n_seqs, int h, int rt) {
-    const PaPlan q = pa_plan_of(c, n, n_seqs, h, rt);
-    const size_t index = n_seqs > PA_INDEX ? pa_up((size_t)n_seqs * 16) : 0;
-    return 256 + index + pa_up((size_t)q.slots * rt * 8) + pa_up((size_t)q.slots * rt * c->hd * 4);
-}
-static int pa_threads(const pg_cache *c, int n, int h, int rt) {
-    if (rt != PM_RT) return 256;
-    return 256 * (c->dtype == QMOE_BF16 ? pa_groups(c, n, h) : pm_halves32(c->hd));
-}
-/* of either choice of rows: the window is not known here.  0 where a launch
- * would have 2^32 threads or more, which HIP does not take; units of 16 rows
- * that are chosen because the call is short (pa_rows) are below 2^24, and more
- * than the longer ones would be. */
-extern "C" size_t qk_pg_attn_ws(const pg_cache *c, int n, int n_seqs, int h) {
-    const int rt = pa_rows_long(c, (int64_t)n * (h / c->kvh), n_seqs);
-    if (pa_plan_of(c, n, n_seqs, h, rt).grid * pa_threads(c, n, h, rt) > 0xFFFFFFFFll) return 0;
-    const size_t a = pa_ws(c, n, n_seqs, h, 16), b = pa_ws(c, n, n_seqs, h, rt);
-    return a > b ? a : b;
+/* the call's places in its workspace */
+static void pa_place(PaArgs &p, int rt, bool tree, void *ws) {
+    const PaLayout l = pa_layout(&p.c, p.a.n, p.a.n_seqs, p.a.h, rt, tree);
+    char *at = (char *)ws;
+    p.pml = (float2 *)(at + l.pml);
+    p.po = (float *)(at + l.po);
+    p.split = (int4 *)(at + l.split);
+    p.index = (int4 *)(at + l.index);
 }
 
 template <typename T, int HD, int RT, int KT>
@@ -1801,9 +1678,7 @@ static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), void *ws, hipStream_t 
     p.extra = q.extra;
     p.one = q.one;
     p.units = q.units;
-    p.pml = (float2 *)ws;
-    p.po = (float *)((char *)ws + pa_up((size_t)q.slots * RT * 8));
-    p.index = (int4 *)((char *)p.po + pa_up((size_t)q.slots * RT * HD * 4));
+    pa_place(p, RT, false, ws); /* of trees too: their own places are those of units of PM_RT rows */
     if (p.a.n_seqs > PA_INDEX) {
         hipLaunchKernelGGL(k_pa_index, dim3(1), dim3(1024), 0, st, p, RT, KT);
         const int rc = QK_CHECK_LAUNCH();
@@ -1819,44 +1694,6 @@ static int pa_launch_rt(PaArgs p, void (*kernel)(PaArgs), void *ws, hipStream_t 
     if (q.join <= 16) hipLaunchKernelGGL((k_pa_join<T, HD, RT, KT, 16>), grid, dim3(1024), 0, st, p);
     else hipLaunchKernelGGL((k_pa_join<T, HD, RT, KT, 4>), grid, dim3(256), 0, st, p);
     return QK_CHECK_LAUNCH();
-}
-
-/* Trees on units of PM_RT rows: as many units as run at once, two to a CU
- * where a unit is one group of four waves; the grid that holds the call's, the
- * slots of partial results and the tasks that may be cut. */
-struct PaTreePlan {
-    int units, slots, joins, twice;
-    int64_t tasks, grid;
-};
-static int pa_tree_groups(const pg_cache *c) { return c->dtype == QMOE_BF16 && c->hd <= 128 ? 1 : 2; }
-static PaTreePlan pa_tree_plan(const pg_cache *c, int n, int n_seqs, int h) {
-    PaTreePlan q;
-    q.units = pa_tree_groups(c) == 1 ? 512 : 256;
-    const int64_t rows = (int64_t)n * (h / c->kvh), seqs = n_seqs < n ? n_seqs : n;
-    const int64_t per_head = rows / PM_RT + seqs < rows ? rows / PM_RT + seqs : rows, tasks = per_head * c->kvh;
-    const int64_t longest = c->cap / pm_kt(c->hd, c->dtype == QMOE_F32) + 2; /* tiles of a task */
-    const bool cut = longest >= PA_JOIN + 1, even = tasks <= q.units;
-    /* with 1024 units they may begin one after the other, 64 tiles each in the mean */
-    q.twice = even && q.units == 512 && tasks * longest >= 64 * q.units;
-    q.grid = even ? (q.twice ? 2 : 1) * q.units : tasks + q.units;
-    if (q.grid > tasks * longest) q.grid = tasks * longest;
-    q.tasks = tasks;
-    q.slots = !cut ? 0 : (even && !q.twice ? 1 : 2) * q.units;
-    q.joins = !cut ? 0 : (int)(even ? tasks : q.units);
-    return q;
-}
-static size_t pa_tree_ws(const pg_cache *c, int n, int n_seqs, int h) {
-    const PaTreePlan q = pa_tree_plan(c, n, n_seqs, h);
-    const size_t rows = (size_t)q.slots * PM_RT, index = n_seqs > PA_INDEX ? ((size_t)n_seqs + 1) * 16 : 0;
-    return rows * c->hd * 4 + rows * 8 + pa_up((size_t)q.joins * 32) + pa_up(index);
-}
-extern "C" size_t qk_pg_attn_tree_ws(const pg_cache *c, int n, int n_seqs, int h) {
-    const int64_t rows = (int64_t)n * (h / c->kvh);
-    const int rt = pa_tree_many(c, rows, n_seqs) ? PM_RT : pa_rows_long(c, rows, n_seqs);
-    const int64_t grid = rt == PM_RT ? 2 * pa_tree_plan(c, n, n_seqs, h).grid : pa_plan_of(c, n, n_seqs, h, rt).grid;
-    if (grid * 256 > 0xFFFFFFFFll) return 0;
-    const size_t a = pa_ws(c, n, n_seqs, h, 16), b = rt == PM_RT ? pa_tree_ws(c, n, n_seqs, h) : pa_ws(c, n, n_seqs, h, rt);
-    return a > b ? a : b;
 }
 
 /* workgroups of a task: of a few long ones, in a hundred parts, a row each */
@@ -1877,15 +1714,11 @@ static bool pa_tree_fine(const pg_cache *c, const pg_attn *a) {
 template <typename T, int HD, int KT>
 static int pa_launch_tree(PaArgs p, void (*kernel)(PaArgs), int threads, void *ws, hipStream_t st) {
     const PaTreePlan q = pa_tree_plan(&p.c, p.a.n, p.a.n_seqs, p.a.h);
-    const size_t rows = (size_t)q.slots * PM_RT;
     p.units = q.units;
     p.joins = q.joins;
     p.twice = q.twice;
     p.tasks = (int)q.tasks;
-    p.po = (float *)ws;
-    p.pml = (float2 *)(p.po + rows * HD);
-    p.split = (int4 *)(p.pml + rows);
-    p.index = (int4 *)((char *)p.split + pa_up((size_t)q.joins * 32));
+    pa_place(p, PM_RT, true, ws);
     if (p.a.n_seqs > PA_INDEX) {
         hipLaunchKernelGGL((k_pa_tree_index<KT>), dim3(1), dim3(1024), 0, st, p);
         const int rc = QK_CHECK_LAUNCH();
@@ -1900,7 +1733,7 @@ static int pa_launch_tree(PaArgs p, void (*kernel)(PaArgs), int threads, void *w
 
 template <typename T, int HD, bool TREE>
 static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
-    const int rt = TREE ? pa_tree_rows(&p.c, &p.a) : pa_rows(&p.c, &p.a);
+    const int rt = pa_rows(&p.c, p.a.n, p.a.n_seqs, p.a.h, p.a.window, p.a.sinks, TREE);
     if (TREE && rt == PM_RT) {
         if constexpr (sizeof(T) == 2) {
             constexpr int NG = HD <= 128 ? 1 : 2; /* pa_tree_groups */

@@ -1,0 +1,59 @@
+"""Trees of drafted tokens at sizes where units, places in the workspace and
+precision change over, on the GPU against the restatement in 64 bits of
+test_gpu_paged_tree (whose bars these are)."""
+import ctypes
+import random
+
+import pytest
+import torch
+
+from conftest import load_pkg
+from test_gpu_paged import Setup, check, i32
+from test_gpu_paged_tree import DTYPES, dev, grow, masked, plan, sight  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def guarded(s, layer, q, tree, starts, window, sinks, slack=1 << 22):
+    """qmoe_paged_attn_tree on a workspace of the size that it asks for, between bytes that have to stay"""
+    pkg, h, hd = load_pkg(), s.h, s.hd
+    n, m = q.shape[0], starts.shape[0] - 1
+    need = pkg.lib().qmoe_paged_ws_bytes(s.cache._cp, pkg.PAGED_ATTN_TREE, n, m, h)
+    ws = torch.full((256 + need + slack,), 0x5A, dtype=torch.uint8, device=s.dev)
+    out = torch.full((n + 2, h, hd), 7.0, dtype=s.dtype, device=s.dev)
+    b = pkg.QmoePagedBatch(starts=starts.data_ptr(), slots=None, n=n, n_seqs=m, status=None)
+    a = pkg.QmoePagedQuery(q=q.data_ptr(), out=out[1].data_ptr(), q_token_stride=h * hd, q_head_stride=hd, out_token_stride=h * hd,
+                           out_head_stride=hd, n_heads=h, window=window, sinks=sinks, grouped=0, scale=0.0)
+    t = pkg.QmoePagedTree(depths=tree.depths.data_ptr(), seen=tree.seen.data_ptr(), words=tree.words)
+    e = pkg.QmoeErr()
+    torch.cuda.synchronize()
+    rc = pkg.lib().qmoe_paged_attn_tree(s.cache._cp, layer, ctypes.byref(b), ctypes.byref(a), ctypes.byref(t), ws[256:].data_ptr(), need,
+                                        torch.cuda.current_stream().cuda_stream, ctypes.byref(e))
+    assert rc == 0, e.msg
+    torch.cuda.synchronize()
+    assert (ws[:256] == 0x5A).all() and (ws[256 + need:] == 0x5A).all()
+    assert (out[0] == 7).all() and (out[n + 1] == 7).all()
+    return out[1:n + 1]
+
+
+@DTYPES
+@pytest.mark.parametrize("m", [64, 65, 100])
+@pytest.mark.parametrize("shape,rows,nodes,window,sinks", [((16, 2, 128), 496, 4, 0, 0), ((4, 2, 64), 640, 16, 0, 0),
+                                                           ((4, 2, 64), 3968, 12, 700, 3), ((6, 2, 192), 656, 8, 0, 0),
+                                                           ((16, 2, 128), 2000, 3, 600, 0)], ids=str)
+def test_units_of_32_rows_stay_in_their_workspace(dev, shape, rows, nodes, window, sinks, m, dtype):  # noqa: F811
+    """17 to 32 rows a sequence on tables or windows of few keys, with and without an index of the sequences"""
+    r = random.Random(m * 1000 + rows + nodes)
+    lens = [rows] + [r.randrange(nodes, rows + 1) for _ in range(m - 1)]
+    s = Setup(dev, shape, dtype, 16, lens, seed=m + rows)
+    counts = [nodes - (1 if i % 7 == 3 else 0) for i in range(m)]
+    ups = [grow(r, c) for c in counts]
+    q, starts = s.queries(counts)
+    q, st = q.to(dev), i32(starts, dev)
+    tree = s.cache.tree(i32([p for u in ups for p in u], dev), st, most=nodes)
+    out = guarded(s, 0, q, tree, st, window, sinks)
+    for i, up in enumerate(ups):
+        a, b = starts[i], starts[i + 1]
+        want, A, B = masked(q[a:b].cpu(), s.hk[i], s.hv[i], sight(lens[i] - counts[i], *plan(up), window, sinks), False)
+        check(out[a:b], want, A, B, s.hd, lens[i], dtype, i)
+    assert torch.equal(s.cache.attend_tree(0, q, tree, window=window, sinks=sinks), out)

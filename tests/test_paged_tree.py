@@ -3,12 +3,15 @@ qmoe_paged_tree_build, _attn_tree, _append_rotary, _follow and _keep, which
 come back as -1 with a message before the device is touched (the pointers here
 are no memory at all)."""
 import ctypes
+import os
+import shutil
+import subprocess
 import sys
 
 import pytest
 
-from conftest import load_pkg
-from test_paged import A, BAD_ATTN, BAD_CACHE, batch, cache, query
+from conftest import ROOT, load_pkg
+from test_paged import A, BAD_ATTN, BAD_CACHE, CSRC, batch, cache, query
 
 BIG = 1 << 40
 
@@ -191,3 +194,29 @@ def test_trees_of_other_tensors_are_refused():
     for bad in ((d.float(), s), (d, s.float()), (d.long(), s), (d[:4], s), (d, s[0]), (d, s.t().contiguous().t()), (d[::2], s[::2])):
         with pytest.raises(pkg.QmoeError, match="depths"):
             pkg.DraftTree(None, None, *bad)
+
+
+def test_workspaces_hold_what_their_launches_take(tmp_path):
+    """every call's places in its workspace, of trees and in causal order, over types, head shapes, tables, windows, sequences
+    and rows (tests/c/paged_plan.cpp)"""
+    gxx = shutil.which("g++")
+    if not gxx:
+        pytest.skip("g++ is not available")
+    exe = str(tmp_path / "paged_plan")
+    r = subprocess.run([gxx, "-std=c++17", "-O2", "-Wall", "-Wextra", "-I" + os.path.join(ROOT, "include"), "-I" + CSRC,
+                        os.path.join(ROOT, "tests", "c", "paged_plan.cpp"), "-o", exe], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout
+
+
+@pytest.mark.parametrize("shape,pages,nodes,index", [((16, 2, 128), 33, 4, 25559040), ((4, 2, 64), 250, 12, 19464192)])
+def test_the_index_of_32_row_units_is_inside(shape, pages, nodes, index):
+    """65 sequences of 17 to 32 rows on few keys (of the table, or of a window of 700): units of 32 rows, whose index begins
+    at byte `index` (1536 slots of 32 rows of 8 + 4 * 128 bytes; 2304 of 8 + 4 * 64) and has 16 bytes a sequence"""
+    pkg = load_pkg()
+    h, kvh, hd = shape
+    c = cache(pkg, page_stride=16 * kvh * hd, row_stride=kvh * hd, head_stride=hd, n_kv_heads=kvh, head_dim=hd, table_stride=pages,
+              max_pages=pages, n_slots=65)
+    for call in (pkg.PAGED_ATTN_TREE, pkg.PAGED_ATTN):
+        assert pkg.lib().qmoe_paged_ws_bytes(ctypes.byref(c), call, 65 * nodes, 65, h) >= index + 16 * 65
