@@ -827,11 +827,9 @@ int qmoe_paged_tree_build(const int32_t *parents, const int32_t *starts, int n, 
  * first as a query at that position would, and of the new rows those in its
  * bits (up to its own), whose positions are first + their depths: the window
  * and the sinks count in positions.  A row that is no node gives zeros.  The
- * softmax weights of bf16 calls have 16 bits in calls of up to 128 rows (new rows
- * times n_heads / n_kv_heads) a sequence, else they may be rounded to bf16.  The
- * bits may be the caller's own, of any rows r <= t (bits past t do not count,
- * depths are brought into [-1, t], a seen row's into [0, r]).  Workspace:
- * QMOE_PAGED_ATTN_TREE. */
+ * softmax weights of bf16 calls have 16 bits.  The bits may be the caller's own,
+ * of any rows r <= t (bits past t do not count, depths are brought into [-1, t],
+ * a seen row's into [0, r]).  Workspace: QMOE_PAGED_ATTN_TREE. */
 int qmoe_paged_attn_tree(const qmoe_paged_cache *c, int layer, const qmoe_paged_batch *b, const qmoe_paged_query *q,
                          const qmoe_paged_tree *t, void *ws, size_t ws_bytes, void *stream, qmoe_err *err);
 

@@ -861,8 +861,8 @@ __device__ __forceinline__ int pa_cuts(int len, int most) { return (int)(((uint3
  * twice as many units, of which the second half starts as the first ends: they
  * take about the mean and a third of a part, PA_TWICE tiles in joins and
  * starts, and the first choice its longest part (less where there is one to a
- * CU): 700 nodes of 3 sequences of 20000 rows, 264 tasks, 692 us and 513, 256
- * of 8 of 8000 to 24000 364 and 349, but 500 of 4 of 12000 280 and 296. */
+ * CU): 700 nodes of 3 sequences of 20000 rows, 264 tasks, 865 us and 646, 256
+ * of 8 of 8000 to 24000 468 and 428, but 500 of 4 of 12000 321 and 319. */
 #define PA_TWICE 4
 template <typename F>
 __device__ __forceinline__ int pa_length(const PaArgs &p, int tasks, int longest, float total, F units_at) {
@@ -1070,13 +1070,17 @@ __device__ __forceinline__ bool pa_tree_find(const PaArgs &p, PaUnit &u) {
  * raised wave priority in either half, two groups half a step apart (360 us),
  * scores of the next tile beside the softmax (337 to 348), three groups (326),
  * units of 64 rows (short prompts 10 % better, long contexts 40 % worse).
- * Trees of drafted tokens have few rows, so their bound is HBM: up to 16 nodes
- * of 64 sequences of 64 to 32768 rows (343 MB) 78 us, in two bf16 parts of the
- * weights 87, of which 12 are the unit's start (its place 2.5, pages 2, first
- * tile 3) and end; while tiles are read it is 6.5 TB/s.  256 nodes of 8
- * sequences (251 GFLOP) 345 us, 730 TFLOP/s: parts of 118 to 150 tiles.  Without
- * gain: waves past the last row that only copy (5 to 10 % slower: their copies
- * go out at once). */
+ * Trees of drafted tokens take the softmax weights in two bf16 parts (16 bits),
+ * as units of few rows do: then every tree's output is within its own rounding
+ * (0.0017 from 64 bits; of one part 0.0023), whatever else is in its batch.  With
+ * few rows the bound is HBM, and the pages' loads hide most of the second
+ * product: up to 16 nodes of 64 sequences of 64 to 32768 rows (343 MB) 85 us,
+ * with one part 78, of which 12 are the unit's start (its place 2.5, pages 2,
+ * first tile 3) and end; while tiles are read it is 6.5 TB/s.  With many rows it
+ * is the step's chain: 256 nodes of 8 sequences of 8000 to 24000 rows (251 GFLOP,
+ * half as much again for the second part) 445 us, with one part 345: parts of 53
+ * to 66 tiles in two turns.  Without gain: waves past the last row that only copy
+ * (5 to 10 % slower: their copies go out at once). */
 #define PM_CHUNK 1024 /* keys of a look-up of two groups */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pa_s16x4 *pa_tptr;
@@ -1119,7 +1123,7 @@ __device__ __forceinline__ bool pa_merge(qm_f32x16 (&o)[E], float &m, float &l, 
     return group == 0;
 }
 
-template <int HD, int NG, bool TREE, bool FINE>
+template <int HD, int NG, bool TREE>
 __global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
     typedef uint16_t T;
     constexpr int KT = pm_kt(HD), CR = HD / 8, NB = KT * CR / 256, NS = KT / 32, E = HD / 32, KS = HD / 16;
@@ -1256,7 +1260,7 @@ __global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 qm_bf16x8 pw, rest;
-                if constexpr (FINE) pa_pack2(st[n], s, l, pw, rest);
+                if constexpr (TREE) pa_pack2(st[n], s, l, pw, rest);
                 else pw = pa_pack(st[n], s, l);
                 const int key = 32 * n + 16 * s + 4 * h + (j >> 2);
 #pragma unroll
@@ -1266,7 +1270,7 @@ __global__ __launch_bounds__(256 * NG, 2 / NG) void k_pa_many(PaArgs p) {
                     const pa_s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_tptr)((const short *)(vb + (key + 8) * CR + pc) + 4 * (j & 1)));
                     const uint2 aw = __builtin_bit_cast(uint2, a), bw = __builtin_bit_cast(uint2, b);
                     const qm_bf16x8 vt = __builtin_bit_cast(qm_bf16x8, make_uint4(aw.x, aw.y, bw.x, bw.y));
-                    if constexpr (FINE) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, rest, o[d], 0, 0, 0);
+                    if constexpr (TREE) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, rest, o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, pw, o[d], 0, 0, 0);
                 }
             }
@@ -1702,15 +1706,6 @@ static unsigned pa_tree_join_rows(int joins) {
     return (unsigned)(r < 4 ? 4 : r > PM_RT ? PM_RT : r);
 }
 
-/* Trees of up to PM_RT rows a sequence take the softmax weights in two bf16
- * parts, as single tokens do: the pages' loads hide most of the second product
- * (4 nodes of 64 sequences of 4000 rows 64 us with one part and 67, 16 nodes 79
- * and 85, 16 of 64 to 32768 85 and 96 a layer).  Larger ones are bound by the
- * products (256 nodes of 8 sequences 360 and 463) and take them as prompts do. */
-static bool pa_tree_fine(const pg_cache *c, const pg_attn *a) {
-    return (int64_t)a->n * (a->h / c->kvh) <= (int64_t)PM_RT * a->n_seqs;
-}
-
 template <typename T, int HD, int KT>
 static int pa_launch_tree(PaArgs p, void (*kernel)(PaArgs), int threads, void *ws, hipStream_t st) {
     const PaTreePlan q = pa_tree_plan(&p.c, p.a.n, p.a.n_seqs, p.a.h);
@@ -1737,14 +1732,14 @@ static int pa_launch(const PaArgs &p, void *ws, hipStream_t st) {
     if (TREE && rt == PM_RT) {
         if constexpr (sizeof(T) == 2) {
             constexpr int NG = HD <= 128 ? 1 : 2; /* pa_tree_groups */
-            return pa_launch_tree<T, HD, pm_kt(HD)>(p, pa_tree_fine(&p.c, &p.a) ? k_pa_many<HD, NG, true, true> : k_pa_many<HD, NG, true, false>, 256 * NG, ws, st);
+            return pa_launch_tree<T, HD, pm_kt(HD)>(p, k_pa_many<HD, NG, true>, 256 * NG, ws, st);
         } else return pa_launch_tree<T, HD, pm_kt(HD, true)>(p, k_pa_many32<HD, true>, 256 * pm_halves32(HD), ws, st);
     }
     if (rt == PM_RT) {
         if constexpr (sizeof(T) == 2) {
             if constexpr (HD <= 128)
-                if (pa_groups(&p.c, p.a.n, p.a.h) == 1) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 1, false, false>, ws, st);
-            return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 2, false, false>, ws, st);
+                if (pa_groups(&p.c, p.a.n, p.a.h) == 1) return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 1, false>, ws, st);
+            return pa_launch_rt<T, HD, PM_RT, pm_kt(HD)>(p, k_pa_many<HD, 2, false>, ws, st);
         } else return pa_launch_rt<T, HD, PM_RT, pm_kt(HD, true)>(p, k_pa_many32<HD, false>, ws, st);
     }
     if constexpr (HD <= (sizeof(T) == 2 ? 192 : 128)) /* pa_two */

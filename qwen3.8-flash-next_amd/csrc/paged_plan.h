@@ -72,7 +72,7 @@ static int pa_rows_long(const pg_cache *c, int64_t rows, int n_seqs) {
  * 16 of 4000 33 and 26; one of 64 of 6000 89 and 84), at head dim 192 from 17
  * rows of a sequence on (24 of 16 of 4000 41 and 38; 6 of 64 85 and 86), at 256
  * from 33 rows and 40 units of 16 (32 of 48 of 2000 49 and 59, 64 of 16 of 4000
- * 58 and 49; 96 of 4 of 3000 34 and 36).  With fewer keys, and in f32, they come
+ * 103 and 67; 96 of 4 of 3000 43 and 45).  With fewer keys, and in f32, they come
  * after units of 16 or 32 rows, in f32 at a quarter of a prompt's limit (16 nodes
  * of a sequence of 8000 41 and 35, 4 of 64 of 2000 94 and 104); at f32's head dim
  * 256, whose many rows spill, later up to 256 rows a sequence (20 nodes of 16 of

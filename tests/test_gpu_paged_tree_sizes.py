@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from conftest import load_pkg
-from test_gpu_paged import Setup, check, i32
+from test_gpu_paged import Setup, U, check, i32
 from test_gpu_paged_tree import DTYPES, dev, grow, masked, plan, sight  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -57,3 +57,25 @@ def test_units_of_32_rows_stay_in_their_workspace(dev, shape, rows, nodes, windo
         want, A, B = masked(q[a:b].cpu(), s.hk[i], s.hv[i], sight(lens[i] - counts[i], *plan(up), window, sinks), False)
         check(out[a:b], want, A, B, s.hd, lens[i], dtype, i)
     assert torch.equal(s.cache.attend_tree(0, q, tree, window=window, sinks=sinks), out)
+
+
+@pytest.mark.parametrize("lens,counts", [([90, 300, 150, 64], [60, 40, 20, 64]), ([260, 70, 100], [200, 3, 9])], ids=["large", "one_large"])
+@pytest.mark.parametrize("hd", [64, 128, 192, 256])
+def test_weights_of_all_trees_have_16_bits(dev, hd, lens, counts, monkeypatch):  # noqa: F811
+    """bf16 outputs of more than 128 rows a sequence, and of small trees beside a large one, within the weights' 16 bits
+    (2^-16 of A twice: a half step of the second part, and of the sum that leaves it out) and their own rounding.  Weights of
+    one bf16 part are off by 2^-9 of the heaviest: up to 7 times this bar on contexts as short as these"""
+    monkeypatch.setattr(Setup, "table_rows", 1024)
+    r = random.Random(hd + len(lens))
+    s = Setup(dev, (8, 1, hd), torch.bfloat16, 16, lens, seed=hd)
+    ups = [grow(r, c) for c in counts]
+    q, starts = s.queries(counts)
+    tree = s.cache.tree(i32([p for u in ups for p in u], dev), i32(starts, dev))
+    out = s.cache.attend_tree(0, q.to(dev), tree).double().cpu()
+    for i, up in enumerate(ups):
+        T = lens[i]
+        want, A, B = masked(q[starts[i]:starts[i + 1]], s.hk[i], s.hv[i], sight(T - counts[i], *plan(up), 0, 0), False)
+        tol = A * (2 * (hd + 24) * U * (B + 1) + 2 * (T + 64) * U + 2 * 2.0 ** -16)
+        tol = tol + (want.abs() + tol) * 2.0 ** -8
+        err = (out[starts[i]:starts[i + 1]] - want).abs()
+        assert (err <= tol).all(), (i, float((err / tol).max()))
