@@ -1421,16 +1421,19 @@ class PagedCache:
         Returns (rows [n]: the path's rows at the first places of their
         sequence, -1 after them; counts [n_seqs]; next [n_seqs]: what was chosen
         after the last one, -1 for none)."""
-        n = tree.n
-        t, m, err = self._tree(tree, n), tree.starts.numel() - 1, _paged_err
-        if tokens is None or chosen is None or tree.parents is None:
-            raise QmoeError("tokens, chosen and the tree's parents must be given")
+        if tree is None or tokens is None or chosen is None or tree.parents is None:
+            raise QmoeError("the tree with its parents, tokens and chosen must be given")
+        n, err = tree.n, _paged_err
+        t, p, s = self._tree(tree, n), self._ints(tree.parents, n, "parents"), self._ints(tree.starts, None, "starts")
+        if s is None or tree.starts.numel() < 1:
+            raise QmoeError("starts must hold one number more than there are sequences")
+        m = tree.starts.numel() - 1
         a, b = self._ints(tokens, n, "tokens"), self._ints(chosen, n, "chosen")
 
         def call(st):
             rows, counts, last = self.lens.new_empty(n), self.lens.new_empty(m), self.lens.new_empty(m)
-            _check(lib().qmoe_paged_follow(t, tree.parents.data_ptr(), a, b, tree.starts.data_ptr(), n, m, rows.data_ptr(),
-                                           counts.data_ptr(), last.data_ptr(), st, err.p), err.err, "qmoe_paged_follow")
+            _check(lib().qmoe_paged_follow(t, p, a, b, s, n, m, rows.data_ptr(), counts.data_ptr(), last.data_ptr(), st, err.p),
+                   err.err, "qmoe_paged_follow")
             return rows, counts, last
         return self._on(stream, call)
 

@@ -220,3 +220,30 @@ def test_the_index_of_32_row_units_is_inside(shape, pages, nodes, index):
               max_pages=pages, n_slots=65)
     for call in (pkg.PAGED_ATTN_TREE, pkg.PAGED_ATTN):
         assert pkg.lib().qmoe_paged_ws_bytes(ctypes.byref(c), call, 65 * nodes, 65, h) >= index + 16 * 65
+
+
+def hosted(pkg):
+    """a PagedCache whose tensors would lie on the host: its checks, which come before any call"""
+    import torch
+    c = object.__new__(pkg.PagedCache)
+    c._torch, c._index, c.device, c._i32, c._f32 = torch, -1, torch.device("cpu"), torch.int32, torch.float32
+    c.n_layers, c.kvh, c.hd, c.dtype = 1, 2, 64, torch.bfloat16
+    c._own, c._src = (torch.bfloat16,), (torch.bfloat16, torch.float32)
+    return c
+
+
+def test_follow_checks_the_tree_s_own_tensors():
+    """a DraftTree of the caller's: parents and starts are read as int32 vectors of n and m + 1 entries"""
+    import torch
+    pkg = load_pkg()
+    c = hosted(pkg)
+    d, seen, parents, starts = (torch.zeros(n, dtype=torch.int32) for n in (5, 5, 5, 3))
+    tree = lambda p=parents, s=starts: pkg.DraftTree(p, s, d, seen.view(5, 1))
+    tokens = torch.zeros(5, dtype=torch.int32)
+    wide = torch.zeros(10, dtype=torch.int32)
+    for bad, msg in ((tree(p=None), "parents"), (tree(p=parents.long()), "parents"), (tree(p=parents[:4]), "parents"),
+                     (tree(p=wide[::2]), "parents"), (tree(p=parents.float()), "parents"),
+                     (tree(s=None), "starts"), (tree(s=starts[:0]), "starts"), (tree(s=starts.long()), "starts"),
+                     (tree(s=wide[:6:2]), "starts"), (tree(s=starts.view(3, 1)), "starts"), (None, "tree")):
+        with pytest.raises(pkg.QmoeError, match=msg):
+            c.follow(bad, tokens, tokens)
