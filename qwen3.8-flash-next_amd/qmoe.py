@@ -1340,11 +1340,9 @@ class PagedCache:
             raise QmoeError(f"layer {layer} out of range [0, {self.n_layers})")
         if scale is not None:
             self._scale(scale)
+        window, sinks = operator.index(window), operator.index(sinks)
         if window or sinks:
             self._span(window, sinks)
-            window, sinks = operator.index(window), operator.index(sinks)
-        else:
-            window = sinks = 0
         n, qt, qh, qp = self._rows(q, heads, self._own, "q")
         if n >= _INT_END or heads >= _INT_END:
             self._fits("q", n, heads)

@@ -247,3 +247,17 @@ def test_follow_checks_the_tree_s_own_tensors():
                      (tree(s=wide[:6:2]), "starts"), (tree(s=starts.view(3, 1)), "starts"), (None, "tree")):
         with pytest.raises(pkg.QmoeError, match=msg):
             c.follow(bad, tokens, tokens)
+
+
+@pytest.mark.parametrize("kw", [dict(window=None), dict(window=0.0), dict(window=""), dict(sinks=None), dict(sinks=[]),
+                                dict(window=3.0), dict(window=5, sinks=None)], ids=str)
+def test_windows_that_are_no_integers_are_refused(kw):
+    """also those that are false, which are no 0"""
+    import torch
+    pkg = load_pkg()
+    c, starts = hosted(pkg), torch.zeros(2, dtype=torch.int32)
+    q = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+    tree = pkg.DraftTree(None, starts, torch.zeros(1, dtype=torch.int32), torch.ones(1, 1, dtype=torch.int32))
+    for call in (lambda: c.attend(0, q, starts, **kw), lambda: c.attend_tree(0, q, tree, **kw)):
+        with pytest.raises(TypeError):
+            call()
