@@ -208,11 +208,11 @@ SIGNATURES = {
     "qmoe_gr_mix": (_I, [_P, _I, _P, _I, _P, _P, _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_gr_inject": (_I, [_P, _P, _P, _I, _P, _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_ws_bytes": (ctypes.c_size_t, [ctypes.POINTER(QmoePagedCache), _I, _I, _I, _I]),
-    "qmoe_paged_append": (_I, [ctypes.POINTER(QmoePagedCache), _I, _P, _P, _P, _I,
+    "qmoe_paged_append": (_I, [ctypes.POINTER(QmoePagedCache), _I, ctypes.POINTER(QmoePagedBatch), _P, _P, _I,
                                ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _P,
                                ctypes.POINTER(QmoeErr)]),
-    "qmoe_paged_attn": (_I, [ctypes.POINTER(QmoePagedCache), _I, _P,
-                             _P, _P, ctypes.c_size_t, _P, ctypes.POINTER(QmoeErr)]),
+    "qmoe_paged_attn": (_I, [ctypes.POINTER(QmoePagedCache), _I, ctypes.POINTER(QmoePagedBatch),
+                             ctypes.POINTER(QmoePagedQuery), _P, ctypes.c_size_t, _P, ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_reserve": (_I, [ctypes.POINTER(QmoePagedCache), _P, _P, _I, _P, _P, ctypes.c_size_t, _P,
                                 ctypes.POINTER(QmoeErr)]),
     "qmoe_paged_fork": (_I, [ctypes.POINTER(QmoePagedCache), _P, _P, _P, _I, _P, _P, ctypes.c_size_t, _P,
@@ -293,6 +293,20 @@ def lib() -> ctypes.CDLL:
     if _lib is None:
         _lib = load_library()
     return _lib
+
+
+_packed_calls = {}
+
+
+def _packed(name):
+    """the library's function for a batch and query packed as bytes, where lib()'s own takes them typed"""
+    fn = _packed_calls.get(name)
+    if fn is None:
+        fn = lib()[name]  # a function object of its own
+        fn.restype, args = SIGNATURES[name]
+        fn.argtypes = [_P if a in (ctypes.POINTER(QmoePagedBatch), ctypes.POINTER(QmoePagedQuery)) else a for a in args]
+        _packed_calls[name] = fn
+    return fn
 
 
 def _ptr(t) -> Optional[int]:
@@ -1267,7 +1281,7 @@ class PagedCache:
         (b, _), err = self._batch(n, starts, slots, status), _paged_err
 
         def call(st):
-            _check(lib().qmoe_paged_append(self._cp, layer, b, kp, vp, _dtype_code(k), kt, kh, vt, vh, st, err.p),
+            _check(_packed("qmoe_paged_append")(self._cp, layer, b, kp, vp, _dtype_code(k), kt, kh, vt, vh, st, err.p),
                    err.err, "qmoe_paged_append")
         self._on(stream, call)
 
@@ -1363,7 +1377,7 @@ class PagedCache:
             a = _QUERY.pack(qp, *place, heads, window, sinks, 1 if grouped else 0, scale)
             ws = self._work(PAGED_ATTN if t is None else PAGED_ATTN_TREE, n, m, heads)
             if t is None:
-                _check(lib().qmoe_paged_attn(self._cp, layer, b, a, ws.data_ptr(), ws.numel(), st, err.p), err.err,
+                _check(_packed("qmoe_paged_attn")(self._cp, layer, b, a, ws.data_ptr(), ws.numel(), st, err.p), err.err,
                        "qmoe_paged_attn")
             else:
                 _check(lib().qmoe_paged_attn_tree(self._cp, layer, b, a, t, ws.data_ptr(), ws.numel(), st, err.p), err.err,

@@ -261,3 +261,17 @@ def test_windows_that_are_no_integers_are_refused(kw):
     for call in (lambda: c.attend(0, q, starts, **kw), lambda: c.attend_tree(0, q, tree, **kw)):
         with pytest.raises(TypeError):
             call()
+
+
+def test_structs_of_the_binding_are_typed():
+    """lib()'s paged calls take a struct as it is or by reference, and no other struct in its place"""
+    pkg = load_pkg()
+    L, e = pkg.lib(), pkg.QmoeErr()
+    c, b, q = cache(pkg), batch(pkg, n=0), query(pkg)
+    for r in (lambda x: x, ctypes.byref):
+        assert L.qmoe_paged_append(r(c), 0, r(b), A, A, pkg.BF16, 256, 128, 256, 128, None, r(e)) == 0, e.msg
+        assert L.qmoe_paged_attn(r(c), 0, r(b), r(q), A, BIG, None, r(e)) == 0, e.msg
+        with pytest.raises(ctypes.ArgumentError):
+            L.qmoe_paged_append(r(c), 0, r(q), A, A, pkg.BF16, 256, 128, 256, 128, None, r(e))
+        with pytest.raises(ctypes.ArgumentError):
+            L.qmoe_paged_attn(r(c), 0, r(q), r(b), A, BIG, None, r(e))
