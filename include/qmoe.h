@@ -840,7 +840,7 @@ int qmoe_paged_attn_tree(const qmoe_paged_cache *c, int layer, const qmoe_paged_
  * k_norm), then of its first rot elements the pairs (a, b) at position p
  * become (a cos - b sin, a sin + b cos), angle p * freqs[i] for pair i: (i, i
  * + rot / 2), the mixer's order, or (2i, 2i + 1) where interleaved.  Angles
- * are exact to fp32 up to position 2^29, whatever their size; norms and
+ * of up to 2^77 radians are exact to fp32 up to position 2^29; norms and
  * rotation are fp32, and each result is rounded once.  v is copied.  Rows of
  * q go to out, k and v to the pages.
  *

@@ -40,9 +40,11 @@ struct PgRotary {
 /* cos and sin of position * freq, whose fp32 value is off by a radian at far
  * positions: x = position * freq in 64 bits (exact up to position 2^29: 29 and
  * 24 bits), x / 2 pi in two parts, so that no bit of it is lost with the whole
- * turns, and the nearest quarter turn taken off.  What is left, at most 1/8, is
- * rounded to fp32, and sin and cos of 2 pi r are their Taylor series (the first
- * term left out is below 2e-9, the sums are off by about one step of fp32). */
+ * turns (up to 2^77 radians, where the second part's own rounding reaches a
+ * tenth of a step of fp32), and the nearest quarter turn taken off.  What is
+ * left, at most 1/8, is rounded to fp32, and sin and cos of 2 pi r are their
+ * Taylor series (the first term left out is below 2e-9, the sums are off by
+ * about one step of fp32). */
 __device__ __forceinline__ float2 pg_turn(int pos, float freq) {
     const double x = (double)pos * (double)freq;
     const double t = x * 0x1.45f306dc9c883p-3, e = fma(x, 0x1.45f306dc9c883p-3, -t) + x * -0x1.6b01ec5417056p-57;

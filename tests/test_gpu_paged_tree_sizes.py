@@ -1,6 +1,6 @@
-"""Trees of drafted tokens at sizes where units, places in the workspace and
-precision change over, on the GPU against the restatement in 64 bits of
-test_gpu_paged_tree (whose bars these are)."""
+"""Drafted tokens at sizes where units, places in the workspace and precision
+change over, and rotation by large angles, on the GPU against the restatements
+in 64 bits of test_gpu_paged_tree (whose bars these are)."""
 import ctypes
 import random
 
@@ -9,7 +9,7 @@ import torch
 
 from conftest import load_pkg
 from test_gpu_paged import Setup, U, check, i32
-from test_gpu_paged_tree import DTYPES, dev, grow, masked, plan, sight  # noqa: F401
+from test_gpu_paged_tree import DTYPES, dev, grow, masked, near, plan, sight, turned  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +79,23 @@ def test_weights_of_all_trees_have_16_bits(dev, hd, lens, counts, monkeypatch): 
         tol = tol + (want.abs() + tol) * 2.0 ** -8
         err = (out[starts[i]:starts[i + 1]] - want).abs()
         assert (err <= tol).all(), (i, float((err / tol).max()))
+
+
+def test_rotary_of_large_angles(dev):  # noqa: F811
+    """freqs up to 2^48 - 2^24 at positions up to 2^29: up to 2^77 radians"""
+    kvh, hd, page = 2, 128, 4096
+    lens = [2 ** 29, 2 ** 29 - 1, 2 ** 28 + 12345, 1000003, 4097, 2]
+    table = torch.full((len(lens), 2 ** 29 // page), -1, dtype=torch.int32, device=dev)
+    for i, n in enumerate(lens):
+        table[i, (n - 1) // page] = i
+    k, v = (torch.zeros(1, len(lens), page, kvh, hd, device=dev) for _ in range(2))
+    cache = load_pkg().PagedCache(k, v, table, i32(lens, dev), torch.ones(len(lens), dtype=torch.int32, device=dev))
+    g = torch.Generator().manual_seed(61)
+    n = len(lens)
+    for low, high in ((0, 8), (8, 32), (32, 47)):
+        freqs = torch.exp2(low + (high - low) * torch.rand(64, generator=g, dtype=torch.float64)).float()
+        freqs[0] = 2.0 ** high * (1 if high < 47 else 2 - 2.0 ** -23)
+        q, kn, vn = (torch.randn(n, m, hd, generator=g) for m in (3, kvh, kvh))
+        got = cache.append_rotary(0, kn.to(dev), vn.to(dev), i32(list(range(n + 1)), dev), freqs.to(dev), q=q.to(dev))
+        want, mag = turned(q, torch.tensor(lens) - 1, freqs, False, None, 0)
+        near(got, want, mag, torch.float32, (low, high))
