@@ -895,7 +895,7 @@ __device__ __forceinline__ int pa_length(const PaArgs &p, int tasks, int longest
     }
     return longest - most < PA_JOIN ? max(longest, 1) : most;
 }
-__device__ __forceinline__ int pa_sum(int v) { return __builtin_amdgcn_readlane(pa_scan(v), 63); }
+__device__ __forceinline__ int pa_wave_sum(int v) { return __builtin_amdgcn_readlane(pa_scan(v), 63); }
 __device__ __forceinline__ int pa_most(int v) { return (int)qk_wave_max_u32((uint32_t)v); }
 
 /* Calls of more sequences than a wave has lanes: what precedes each one (units,
@@ -908,7 +908,7 @@ __global__ __launch_bounds__(1024) void k_pa_tree_index(PaArgs p) {
     const int tid = threadIdx.x, wave = tid >> 6, n = p.a.n_seqs, per = (n + 1023) >> 10;
     const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
     auto over = [&](int v, int k) { /* the workgroup's sum */
-        v = pa_sum(v);
+        v = pa_wave_sum(v);
         __syncthreads();
         if ((tid & 63) == 0) part[k][wave] = v;
         __syncthreads();
@@ -993,8 +993,8 @@ __device__ __forceinline__ bool pa_tree_find(const PaArgs &p, PaUnit &u) {
         if (lane < n) q = pa_need<KT>(p, lane);
         const int mine = q.rows * p.c.kvh;
         const float total = qk_group_sum<64>((float)mine * (float)q.len);
-        const int most = pa_length(p, pa_sum(mine), pa_most(q.rows ? q.len : 0), total,
-                                   [&](int length) { return pa_sum(mine * pa_cuts(q.len, length)); });
+        const int most = pa_length(p, pa_wave_sum(mine), pa_most(q.rows ? q.len : 0), total,
+                                   [&](int length) { return pa_wave_sum(mine * pa_cuts(q.len, length)); });
         const int parts = pa_cuts(q.len, most), units = mine * parts, ue = pa_scan(units);
         const int cut = parts > 1 ? mine : 0, se = pa_scan(cut * parts), te = pa_scan(cut);
         tasks = __builtin_amdgcn_readlane(te, 63);
@@ -1372,7 +1372,7 @@ __global__ __launch_bounds__(256 * pm_halves32(HD), 1) void k_pa_many32(PaArgs p
         }
         __syncthreads();
     };
-    float4 kx[NB], vx[NB]; /* this threadIdx.x's pieces of four of the next step's tile */
+    float4 kx[NB], vx[NB]; /* this thread's pieces of four of the next step's tile */
     auto rows_of = [&](int i) { return where + (NG * (i % CH) + odd) * KT; };
     auto load_k = [&](int i, int x) {
         const int L = x * 256 + tid, rr = L / (HD / 4);

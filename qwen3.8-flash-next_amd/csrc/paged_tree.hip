@@ -282,7 +282,10 @@ extern "C" int qk_launch_pg_rotary(const pg_cache *c, const qmoe_paged_rotary *r
  * a run of rows whose parents are the rows before them is one step, so a
  * chain, however long, is one.  Bound: latency, of the loads of starts and
  * parents and of the walk in LDS: 1.8 us for 8 nodes, 3.1 to 5 for up to 24 of
- * 64 sequences, 5.7 for 256 of 8. */
+ * 64 sequences, 5.7 for 256 of 8.  Large trees are bound by the walks, one for
+ * each word of a row: 1024 nodes of a star or a chain 24 to 37 us a call, drawn
+ * at random 60 to 70, but of two chains row by row, 512 steps each and none of
+ * them a run, 1600 (256 nodes 33 to 110). */
 #define PG_TREE_ROWS 1024
 
 struct PgTree {

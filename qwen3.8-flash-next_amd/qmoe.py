@@ -1392,8 +1392,9 @@ class PagedCache:
         row's parent among its sequence's rows, -1 for a root, which follows
         the rows before the drafts.  A parent lies before its children; a row
         for which it does not is no node, nor are its descendants, nor the
-        rows past the first `most` of a sequence (None: all) or past 1024.
-        Returns a DraftTree for append_rotary, attend_tree, follow and keep."""
+        rows past the first 1024 of a sequence.  `most` is the largest tree's
+        rows (None: as many as the call has): rows past it, rounded up to a
+        multiple of 32, are no nodes either.  Returns a DraftTree for append_rotary, attend_tree, follow and keep."""
         p = self._ints(parents, None, "parents")
         s = self._ints(starts, None, "starts")
         if p is None or s is None or starts.numel() < 1:
